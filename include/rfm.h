@@ -385,6 +385,83 @@ int rfm_msda_backward(const float* value, const int64_t* spatial_shapes, const i
                       float* grad_value, float* grad_locations, float* grad_weights, void* stream);
 
 /*
+ * ---- Operators of the decoder layers around the matcher ---------------------
+ *
+ * What a training step on these predictions runs next to the matcher, the
+ * losses and deformable attention: layer norm, the optimiser's step and the
+ * layers' matrix products.  No counterpart kernels in the reference, which
+ * leaves these to torch.  Element types of their tensors: */
+#define RFM_DTYPE_F32 0
+#define RFM_DTYPE_BF16 1
+#define RFM_DTYPE_F16 2
+
+/*
+ * Layer norm over the last dimension:
+ *   out = (x - mean(x)) / sqrt(var(x) + eps) * weight + bias   (var: mean of squared deviations)
+ *
+ *   x            [rows, dim] of `dtype`, row r at x + r * ld_x (ld_x >= dim when rows > 1)
+ *   weight, bias [dim] of `param_dtype`; NULL: ones / zeros
+ *   out          [rows, dim] of `dtype`, contiguous
+ *   mean, rstd   [rows] float32, what the backward needs; both NULL: not written
+ *
+ * rfm_layer_norm_backward, given grad_out [rows, dim] (row stride ld_grad) and
+ * the forward's mean and rstd, writes grad_x [rows, dim] (`dtype`, contiguous)
+ * and the sums over the rows grad_weight, grad_bias [dim] (`param_dtype`); each
+ * may be NULL.  The sums are taken in float32 in a fixed order (deterministic)
+ * through `workspace`, rfm_layer_norm_workspace_bytes(rows, dim) bytes on the
+ * current device, needed when grad_weight or grad_bias is given.  All
+ * arithmetic is float32.  With rows = 0 the sums are zero.
+ */
+int rfm_layer_norm_forward(const void* x, int64_t ld_x, const void* weight, const void* bias, void* out,
+                           float* mean, float* rstd, int64_t rows, int dim, float eps, int dtype, int param_dtype,
+                           void* stream);
+int64_t rfm_layer_norm_workspace_bytes(int64_t rows, int dim);
+int rfm_layer_norm_backward(const void* x, int64_t ld_x, const void* weight, const float* mean, const float* rstd,
+                            const void* grad_out, int64_t ld_grad, void* grad_x, void* grad_weight, void* grad_bias,
+                            int64_t rows, int dim, int dtype, int param_dtype, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
+/*
+ * One AdamW step (decoupled weight decay) over many tensors, in place:
+ *   g = grad * grad_scale,  m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps)
+ *
+ *   tensors      [count] HOST array; every tensor contiguous, param and grad of `dtype`, all of them
+ *                disjoint (a tensor given twice would be updated twice at once)
+ *   moment_bits  32: exp_avg, exp_avg_sq float32 [numel]; the scales are not read
+ *                8: exp_avg int8 [numel], exp_avg_sq uint8 [numel], and per block of RFM_MOMENT_BLOCK
+ *                consecutive elements one float32 scale each ([ceil(numel / RFM_MOMENT_BLOCK)]):
+ *                m = scale c|c| / 127^2, v = scale (c / 255)^4.  Scales are the blocks' largest values;
+ *                codes are rounded at random by a hash of (t, the tensor's number, the element's index).
+ *                A NaN or infinite gradient leaves no finite value in its block.
+ *   step         t >= 1 of this update; device_step (int64, not NULL) replaces it, device_lr (float32)
+ *                replaces lr, for steps captured in a graph.  With either, `workspace` is 16 bytes,
+ *                16-byte aligned, used by this call's kernels alone.
+ *   grad_scale   float32 on the device, or NULL for 1 (a clipping or loss-scaling factor)
+ *
+ * The table travels in the kernels' parameters: one launch for up to 508 tensors.
+ */
+#define RFM_MOMENT_BLOCK 256
+typedef struct rfm_adamw_tensor {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;
+  float* exp_avg_sq_scale;
+  int64_t numel;
+  int64_t reserved; /* must be 0 */
+} rfm_adamw_tensor;
+
+int rfm_adamw(const rfm_adamw_tensor* tensors, int count, int dtype, int moment_bits, double lr, double beta1,
+              double beta2, double eps, double weight_decay, int64_t step, const float* device_lr,
+              const int64_t* device_step, const float* grad_scale, void* workspace, void* stream);
+
+/* The values that 8-bit moments of one tensor stand for, float32 [numel] each. */
+int rfm_adamw_moments(const void* exp_avg, const void* exp_avg_sq, const float* exp_avg_scale,
+                      const float* exp_avg_sq_scale, int64_t numel, float* out_avg, float* out_avg_sq, void* stream);
+
+/*
  * ---- The sharded sweep's exchange: pairs pushed into every rank's memory ----
  *
  * No counterpart in the reference, which matches on one GPU.  A batch split by

@@ -54,7 +54,22 @@ EXPORTS = (
     "rfm_peer_close",
     "rfm_peer_free",
     "rfm_peer_sync",
+    "rfm_layer_norm_forward",
+    "rfm_layer_norm_workspace_bytes",
+    "rfm_layer_norm_backward",
+    "rfm_adamw",
+    "rfm_adamw_moments",
 )
+
+#: RFM_DTYPE_*: element types of the layer operators.
+DTYPE_F32 = 0
+DTYPE_BF16 = 1
+DTYPE_F16 = 2
+
+#: RFM_MOMENT_BLOCK: elements that share one scale of the 8-bit moments.
+MOMENT_BLOCK = 256
+#: int64 words of one ``struct rfm_adamw_tensor``.
+ADAMW_TENSOR_WORDS = 8
 
 #: RFM_MAX_PUSH: destinations of one pushed solve, ranks of one pushed exchange.
 MAX_PUSH = 8
@@ -151,6 +166,7 @@ _p = ctypes.c_void_p
 _i32 = ctypes.c_int
 _i64 = ctypes.c_int64
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 
 
 def load() -> ctypes.CDLL:
@@ -221,6 +237,17 @@ def load() -> ctypes.CDLL:
     lib.rfm_peer_free.argtypes = [_p]
     lib.rfm_peer_sync.restype = _i32
     lib.rfm_peer_sync.argtypes = [ctypes.POINTER(PeerSyncArgs), _p]
+    lib.rfm_layer_norm_forward.restype = _i32
+    lib.rfm_layer_norm_forward.argtypes = [_p, _i64, _p, _p, _p, _p, _p, _i64, _i32, _f32, _i32, _i32, _p]
+    lib.rfm_layer_norm_workspace_bytes.restype = _i64
+    lib.rfm_layer_norm_workspace_bytes.argtypes = [_i64, _i32]
+    lib.rfm_layer_norm_backward.restype = _i32
+    lib.rfm_layer_norm_backward.argtypes = [_p, _i64, _p, _p, _p, _p, _i64, _p, _p, _p, _i64, _i32, _i32, _i32, _p,
+                                            _i64, _p]
+    lib.rfm_adamw.restype = _i32
+    lib.rfm_adamw.argtypes = [_p, _i32, _i32, _i32, _f64, _f64, _f64, _f64, _f64, _i64, _p, _p, _p, _p, _p]
+    lib.rfm_adamw_moments.restype = _i32
+    lib.rfm_adamw_moments.argtypes = [_p, _p, _p, _p, _i64, _p, _p, _p]
     _lib = lib
     return lib
 

@@ -1,0 +1,538 @@
+// Layer norm over the last dimension, forward and backward, fp32 / bf16 / fp16.
+//
+//   mean = sum x / D,  rstd = 1 / sqrt(sum (x - mean)^2 / D + eps)
+//   y    = (x - mean) rstd w + b
+//   with u = (x - mean) rstd and t = dy w:
+//   dx   = rstd (t - mean(t) - u mean(t u)),  dw = sum_rows dy u,  db = sum_rows dy
+//
+// All arithmetic is fp32; the only rounding to the tensors' type is the store
+// of y, dx, dw and db.  The variance is the mean of squared deviations from the
+// mean (two sums over registers, not E[x^2] - E[x]^2, which cancels for rows
+// whose mean is large).
+//
+// HBM-bound: the forward moves 2 and the backward 3 arrays of rows x D.  A team
+// of TEAM threads keeps one row in registers (TEAM * VEC * CH >= D), so every
+// element is read once; the next row's loads are issued before the current row
+// is reduced.  Teams of 8 lanes for short rows, a warp (no barrier) up to 512
+// columns, a CTA of 128 to 512 threads up to 8192; longer rows are re-read from L2.
+// The weight and bias gradients are summed in registers over a team's rows (a
+// thread always owns the same columns), then over the CTA's teams in shared
+// memory, then over the CTAs by a second kernel, all in a fixed order: no
+// atomics, and the same bits on every run.
+#include <math.h>
+
+#include "rfm_types.cuh"
+
+namespace rfm {
+namespace {
+
+constexpr int kThreads = 256;  // of a CTA of several teams, and of the kernels without teams
+constexpr int kWarps = kThreads / 32;
+constexpr int kMostWarps = 16;  // of a team
+
+// Threads of a CTA: a team of more than a warp has a CTA to itself.
+__host__ __device__ constexpr int cta_threads(int team) { return team > 32 ? team : kThreads; }
+constexpr int kWideDim = 8192;  // longest row held in registers
+constexpr int kWideSlabs = 64;  // row slabs of the wide rows' parameter gradients
+
+struct NormArgs {
+  const void* x;
+  const void* dy;
+  const void* weight;
+  const void* bias;
+  void* out;  // y or dx
+  const float* mean_in;
+  const float* rstd_in;
+  float* mean_out;
+  float* rstd_out;
+  float* partial;  // [CTAs][2][D]
+  int64_t rows;
+  int64_t ld_x;
+  int64_t ld_dy;
+  int dim;
+  int param_dtype;
+  float eps;
+  float inv_dim;
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_row(Pack<T, VEC>& r, const T* row, int col, int dim, bool valid) {
+  if (valid && col < dim) {
+    r = *reinterpret_cast<const Pack<T, VEC>*>(row + col);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) r.v[j] = from_float<T>(0.f);
+  }
+}
+
+// Sum of (a, b) over a team; every thread of the team gets it.  Teams of a CTA
+// use the slot pair `parity` of `slots`, so that two sums in a row need one
+// barrier each.
+template <int TEAM>
+__device__ __forceinline__ float2 team_sum(float2 s, float2 (*slots)[kMostWarps], int parity) {
+#pragma unroll
+  for (int o = (TEAM < 32 ? TEAM : 32) / 2; o > 0; o >>= 1) {
+    s.x += __shfl_xor_sync(kFullMask, s.x, o);
+    s.y += __shfl_xor_sync(kFullMask, s.y, o);
+  }
+  if (TEAM > 32) {
+    if ((threadIdx.x & 31) == 0) slots[parity][threadIdx.x >> 5] = s;
+    __syncthreads();
+    s = slots[parity][0];
+#pragma unroll
+    for (int w = 1; w < TEAM / 32; ++w) {
+      s.x += slots[parity][w].x;
+      s.y += slots[parity][w].y;
+    }
+  }
+  return s;
+}
+
+template <typename T, int VEC, int TEAM, int CH>
+__global__ void __launch_bounds__(cta_threads(TEAM)) norm_fwd_kernel(const NormArgs a) {
+  __shared__ float2 slots[2][kMostWarps];
+  constexpr int kTeams = cta_threads(TEAM) / TEAM;
+  constexpr int kStep = TEAM * VEC;
+  const int lane = static_cast<int>(threadIdx.x) % TEAM;
+  const int team = static_cast<int>(threadIdx.x) / TEAM;
+  const T* x = static_cast<const T*>(a.x);
+  T* out = static_cast<T*>(a.out);
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kTeams;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kTeams + team;
+  // the loop runs on the row of the warp's first team, so that a warp stays whole
+  int64_t lead = TEAM >= 32 ? row : static_cast<int64_t>(blockIdx.x) * kTeams + (threadIdx.x & ~31u) / TEAM;
+
+  Pack<T, VEC> next[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+    load_row<T, VEC>(next[c], x + row * a.ld_x, c * kStep + lane * VEC, a.dim, row < a.rows);
+  float w[CH * VEC], b[CH * VEC];
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const int col = c * kStep + lane * VEC + j;
+      w[c * VEC + j] = col < a.dim && a.weight != nullptr ? load_param(a.weight, a.param_dtype, col) : 1.f;
+      b[c * VEC + j] = col < a.dim && a.bias != nullptr ? load_param(a.bias, a.param_dtype, col) : 0.f;
+    }
+
+  for (; lead < a.rows; row += stride, lead += stride) {
+    float v[CH * VEC];
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        v[c * VEC + j] = to_float(next[c].v[j]);
+        s.x += v[c * VEC + j];
+      }
+    const int64_t after = row + stride;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+      load_row<T, VEC>(next[c], x + after * a.ld_x, c * kStep + lane * VEC, a.dim, after < a.rows);
+    const float mean = team_sum<TEAM>(s, slots, 0).x * a.inv_dim;
+    s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const bool in = c * kStep + lane * VEC + j < a.dim;
+        v[c * VEC + j] = in ? v[c * VEC + j] - mean : 0.f;
+        s.x = fmaf(v[c * VEC + j], v[c * VEC + j], s.x);
+      }
+    const float rstd = 1.f / sqrtf(fmaf(team_sum<TEAM>(s, slots, 1).x, a.inv_dim, a.eps));
+    if (row < a.rows) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int col = c * kStep + lane * VEC;
+        if (col >= a.dim) continue;
+        Pack<T, VEC> y;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          y.v[j] = from_float<T>(fmaf(v[c * VEC + j] * rstd, w[c * VEC + j], b[c * VEC + j]));
+        *reinterpret_cast<Pack<T, VEC>*>(out + row * a.dim + col) = y;
+      }
+      if (lane == 0 && a.mean_out != nullptr) {
+        a.mean_out[row] = mean;
+        a.rstd_out[row] = rstd;
+      }
+    }
+  }
+}
+
+// PARAMS: also the sums of dy u and dy per column, one partial pair per CTA.
+template <typename T, int VEC, int TEAM, int CH, bool PARAMS>
+__global__ void __launch_bounds__(cta_threads(TEAM)) norm_bwd_kernel(const NormArgs a) {
+  __shared__ float2 slots[2][kMostWarps];
+  constexpr int kTeams = cta_threads(TEAM) / TEAM;
+  constexpr int kStep = TEAM * VEC;
+  constexpr int kCols = CH * VEC;
+  const int lane = static_cast<int>(threadIdx.x) % TEAM;
+  const int team = static_cast<int>(threadIdx.x) / TEAM;
+  const T* x = static_cast<const T*>(a.x);
+  const T* dy = static_cast<const T*>(a.dy);
+  T* out = static_cast<T*>(a.out);
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kTeams;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kTeams + team;
+  int64_t lead = TEAM >= 32 ? row : static_cast<int64_t>(blockIdx.x) * kTeams + (threadIdx.x & ~31u) / TEAM;
+
+  Pack<T, VEC> next_x[CH], next_dy[CH];
+  float next_mean = 0.f, next_rstd = 0.f;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    load_row<T, VEC>(next_x[c], x + row * a.ld_x, c * kStep + lane * VEC, a.dim, row < a.rows);
+    load_row<T, VEC>(next_dy[c], dy + row * a.ld_dy, c * kStep + lane * VEC, a.dim, row < a.rows);
+  }
+  if (row < a.rows) {
+    next_mean = a.mean_in[row];
+    next_rstd = a.rstd_in[row];
+  }
+  float w[kCols];
+  float dw[PARAMS ? kCols : 1], db[PARAMS ? kCols : 1];
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const int col = c * kStep + lane * VEC + j;
+      w[c * VEC + j] = col < a.dim && a.weight != nullptr ? load_param(a.weight, a.param_dtype, col) : 1.f;
+      if (PARAMS) dw[c * VEC + j] = db[c * VEC + j] = 0.f;
+    }
+
+  int parity = 0;
+  for (; lead < a.rows; row += stride, lead += stride, parity ^= 1) {
+    const float mean = next_mean, rstd = next_rstd;
+    float u[kCols], t[kCols];
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const int i = c * VEC + j;
+        const bool in = c * kStep + lane * VEC + j < a.dim;
+        const float g = to_float(next_dy[c].v[j]);  // 0 outside the row
+        u[i] = in ? (to_float(next_x[c].v[j]) - mean) * rstd : 0.f;
+        t[i] = g * w[i];
+        s.x += t[i];
+        s.y = fmaf(t[i], u[i], s.y);
+        if (PARAMS) {
+          dw[i] = fmaf(g, u[i], dw[i]);
+          db[i] += g;
+        }
+      }
+    const int64_t after = row + stride;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      load_row<T, VEC>(next_x[c], x + after * a.ld_x, c * kStep + lane * VEC, a.dim, after < a.rows);
+      load_row<T, VEC>(next_dy[c], dy + after * a.ld_dy, c * kStep + lane * VEC, a.dim, after < a.rows);
+    }
+    next_mean = next_rstd = 0.f;
+    if (after < a.rows) {
+      next_mean = a.mean_in[after];
+      next_rstd = a.rstd_in[after];
+    }
+    s = team_sum<TEAM>(s, slots, parity);
+    if (out != nullptr && row < a.rows) {
+      const float m1 = s.x * a.inv_dim, m2 = s.y * a.inv_dim;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int col = c * kStep + lane * VEC;
+        if (col >= a.dim) continue;
+        Pack<T, VEC> g;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const int i = c * VEC + j;
+          g.v[j] = from_float<T>(rstd * (t[i] - fmaf(u[i], m2, m1)));
+        }
+        *reinterpret_cast<Pack<T, VEC>*>(out + row * a.dim + col) = g;
+      }
+    }
+  }
+
+  if (!PARAMS) return;
+  float* pw = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * a.dim;
+  if (TEAM > 32) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const int col = c * kStep + lane * VEC + j;
+        if (col < a.dim) {
+          pw[col] = dw[c * VEC + j];
+          pw[a.dim + col] = db[c * VEC + j];
+        }
+      }
+    return;
+  }
+  // the CTA's teams, summed in a fixed order, 32 columns' worth of registers of
+  // every team at a time: slab[team][lane] holds one register of each thread
+  __shared__ float slab[2][kThreads + 1];
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) {
+    __syncthreads();
+    slab[0][threadIdx.x] = dw[i];
+    slab[1][threadIdx.x] = db[i];
+    __syncthreads();
+    if (threadIdx.x < 2 * TEAM) {
+      const int which = static_cast<int>(threadIdx.x) / TEAM;
+      const int col = (i / VEC) * kStep + lane * VEC + i % VEC;
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < kTeams; ++k) sum += slab[which][k * TEAM + lane];
+      if (col < a.dim) pw[which * a.dim + col] = sum;
+    }
+  }
+}
+
+// Rows longer than the registers hold: one CTA per row, the row re-read (from
+// L2) for each sum.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) norm_fwd_wide_kernel(const NormArgs a) {
+  __shared__ float2 slots[2][kMostWarps];
+  T* out = static_cast<T*>(a.out);
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
+    float2 s = make_float2(0.f, 0.f);
+    for (int c = threadIdx.x; c < a.dim; c += kThreads) s.x += to_float(x[c]);
+    const float mean = team_sum<kThreads>(s, slots, 0).x * a.inv_dim;
+    s = make_float2(0.f, 0.f);
+    for (int c = threadIdx.x; c < a.dim; c += kThreads) {
+      const float d = to_float(x[c]) - mean;
+      s.x = fmaf(d, d, s.x);
+    }
+    const float rstd = 1.f / sqrtf(fmaf(team_sum<kThreads>(s, slots, 1).x, a.inv_dim, a.eps));
+    for (int c = threadIdx.x; c < a.dim; c += kThreads) {
+      const float w = a.weight != nullptr ? load_param(a.weight, a.param_dtype, c) : 1.f;
+      const float b = a.bias != nullptr ? load_param(a.bias, a.param_dtype, c) : 0.f;
+      out[row * a.dim + c] = from_float<T>(fmaf((to_float(x[c]) - mean) * rstd, w, b));
+    }
+    if (threadIdx.x == 0 && a.mean_out != nullptr) {
+      a.mean_out[row] = mean;
+      a.rstd_out[row] = rstd;
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) norm_bwd_wide_kernel(const NormArgs a) {
+  __shared__ float2 slots[2][kMostWarps];
+  T* out = static_cast<T*>(a.out);
+  int parity = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, parity ^= 1) {
+    const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
+    const T* dy = static_cast<const T*>(a.dy) + row * a.ld_dy;
+    const float mean = a.mean_in[row], rstd = a.rstd_in[row];
+    float2 s = make_float2(0.f, 0.f);
+    for (int c = threadIdx.x; c < a.dim; c += kThreads) {
+      const float w = a.weight != nullptr ? load_param(a.weight, a.param_dtype, c) : 1.f;
+      const float t = to_float(dy[c]) * w;
+      s.x += t;
+      s.y = fmaf(t, (to_float(x[c]) - mean) * rstd, s.y);
+    }
+    s = team_sum<kThreads>(s, slots, parity);
+    const float m1 = s.x * a.inv_dim, m2 = s.y * a.inv_dim;
+    for (int c = threadIdx.x; c < a.dim; c += kThreads) {
+      const float w = a.weight != nullptr ? load_param(a.weight, a.param_dtype, c) : 1.f;
+      const float u = (to_float(x[c]) - mean) * rstd;
+      out[row * a.dim + c] = from_float<T>(rstd * (to_float(dy[c]) * w - fmaf(u, m2, m1)));
+    }
+  }
+}
+
+// Parameter gradients of wide rows: a thread owns one column over one slab of
+// rows (blockIdx.y).
+template <typename T>
+__global__ void __launch_bounds__(kThreads) norm_wide_params_kernel(const NormArgs a) {
+  const int col = static_cast<int>(blockIdx.x) * kThreads + static_cast<int>(threadIdx.x);
+  if (col >= a.dim) return;
+  float dw = 0.f, db = 0.f;
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    const float g = to_float((static_cast<const T*>(a.dy) + row * a.ld_dy)[col]);
+    const float u = (to_float((static_cast<const T*>(a.x) + row * a.ld_x)[col]) - a.mean_in[row]) * a.rstd_in[row];
+    dw = fmaf(g, u, dw);
+    db += g;
+  }
+  float* p = a.partial + static_cast<int64_t>(blockIdx.y) * 2 * a.dim;
+  p[col] = dw;
+  p[a.dim + col] = db;
+}
+
+// Sums the CTAs' partials per column in a fixed order: 32 columns per CTA, each
+// of 8 warps every 8th partial, then the 8 sums.  blockIdx.y picks dw or db.
+__global__ void __launch_bounds__(kThreads) norm_param_sum_kernel(const float* partial, int parts, int dim,
+                                                                 void* dweight, void* dbias, int param_dtype) {
+  __shared__ float sums[kWarps][33];
+  void* out = blockIdx.y == 0 ? dweight : dbias;
+  if (out == nullptr) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col = static_cast<int>(blockIdx.x) * 32 + lane;
+  float s = 0.f;
+  if (col < dim) {
+    const float* p = partial + static_cast<int64_t>(blockIdx.y) * dim + col;
+#pragma unroll 4
+    for (int k = warp; k < parts; k += kWarps) s += p[static_cast<int64_t>(k) * 2 * dim];
+  }
+  sums[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && col < dim) {
+#pragma unroll
+    for (int k = 1; k < kWarps; ++k) s += sums[k][lane];
+    store_param(out, param_dtype, col, s);
+  }
+}
+
+// CTAs of a grid that walks `rows` in steps of `teams` rows: what is needed, at
+// most `per_sm` a SM.
+int norm_ctas(int64_t rows, int teams, int per_sm) {
+  const int64_t need = (rows + teams - 1) / teams;
+  const int64_t most = static_cast<int64_t>(device_sm_count()) * per_sm;
+  return static_cast<int>(need < most ? need : most);
+}
+
+// CTAs of the backward on one SM: 1,024 threads; kBwdPerSm, the most of them,
+// bounds the workspace.
+constexpr int bwd_per_sm(int threads) { return 1024 / threads; }
+constexpr int kBwdPerSm = 8;
+
+template <typename T, int VEC, int TEAM, int CH>
+int launch_norm(const NormArgs& a, bool backward, int* ctas, cudaStream_t stream) {
+  constexpr int threads = cta_threads(TEAM);
+  constexpr int teams = threads / TEAM;
+  if (!backward) {
+    // the SM's 2,048 threads where registers allow; more CTAs only queue
+    norm_fwd_kernel<T, VEC, TEAM, CH><<<norm_ctas(a.rows, teams, 2048 / threads), threads, 0, stream>>>(a);
+  } else if (a.partial != nullptr) {
+    *ctas = norm_ctas(a.rows, teams, bwd_per_sm(threads));
+    norm_bwd_kernel<T, VEC, TEAM, CH, true><<<*ctas, threads, 0, stream>>>(a);
+  } else {
+    norm_bwd_kernel<T, VEC, TEAM, CH, false>
+        <<<norm_ctas(a.rows, teams, bwd_per_sm(threads)), threads, 0, stream>>>(a);
+  }
+  return launch_status();
+}
+
+// The smallest team and register count that hold a row.
+template <typename T>
+int dispatch_norm(const NormArgs& a, bool vectors, bool backward, int* ctas, cudaStream_t s) {
+  constexpr int V = 16 / static_cast<int>(sizeof(T));
+  const int d = a.dim;
+  if (d > kWideDim) {
+    const int grid = norm_ctas(a.rows, 1, 8);
+    if (!backward) {
+      norm_fwd_wide_kernel<T><<<grid, kThreads, 0, s>>>(a);
+      return launch_status();
+    }
+    if (a.out != nullptr) norm_bwd_wide_kernel<T><<<grid, kThreads, 0, s>>>(a);
+    if (a.partial != nullptr) {
+      *ctas = static_cast<int>(a.rows < kWideSlabs ? a.rows : kWideSlabs);
+      norm_wide_params_kernel<T><<<dim3((d + kThreads - 1) / kThreads, *ctas), kThreads, 0, s>>>(a);
+    }
+    return launch_status();
+  }
+  // at most 16 columns a thread: the backward keeps five values for each
+  if (vectors) {
+    if (d <= 8 * V) return launch_norm<T, V, 8, 1>(a, backward, ctas, s);
+    if (d <= 32 * V) return launch_norm<T, V, 32, 1>(a, backward, ctas, s);
+    if (d <= 64 * V) return launch_norm<T, V, 32, 2>(a, backward, ctas, s);
+    if (d <= 128 * V) return launch_norm<T, V, 128, 1>(a, backward, ctas, s);
+    if (d <= 256 * V) return launch_norm<T, V, 128, 2>(a, backward, ctas, s);
+    if (d <= 512 * V) return launch_norm<T, V, 256, 2>(a, backward, ctas, s);
+    if (d <= 1024 * V) return launch_norm<T, V, 512, 2>(a, backward, ctas, s);
+    if constexpr (V == 4) return launch_norm<T, V, 512, 4>(a, backward, ctas, s);
+  }
+  if (d <= 32) return launch_norm<T, 1, 8, 4>(a, backward, ctas, s);
+  if (d <= 128) return launch_norm<T, 1, 32, 4>(a, backward, ctas, s);
+  if (d <= 512) return launch_norm<T, 1, 32, 16>(a, backward, ctas, s);
+  if (d <= 2048) return launch_norm<T, 1, 128, 16>(a, backward, ctas, s);
+  return launch_norm<T, 1, 512, 16>(a, backward, ctas, s);
+}
+
+int run_norm(const NormArgs& a, int dtype, bool backward, int* ctas, cudaStream_t s) {
+  const int v = 16 / dtype_bytes(dtype);
+  const bool vectors = a.dim % v == 0 && a.ld_x % v == 0 && a.ld_dy % v == 0 && aligned16(a.x) && aligned16(a.dy) &&
+                       aligned16(a.out);
+  if (dtype == RFM_DTYPE_F32) return dispatch_norm<float>(a, vectors, backward, ctas, s);
+  if (dtype == RFM_DTYPE_BF16) return dispatch_norm<__nv_bfloat16>(a, vectors, backward, ctas, s);
+  return dispatch_norm<__half>(a, vectors, backward, ctas, s);
+}
+
+int norm_args(NormArgs& a, const void* x, int64_t ld_x, const void* weight, int64_t rows, int dim, int dtype,
+              int param_dtype) {
+  if (rows < 0 || dim < 1 || !dtype_known(dtype) || !dtype_known(param_dtype) ||
+      (ld_x < dim && rows > 1) || ld_x < 0) {
+    return RFM_ERR_INVALID_ARGUMENT;
+  }
+  if (rows > (int64_t(1) << 40) || ld_x > (int64_t(1) << 40)) return RFM_ERR_UNSUPPORTED;
+  if (rows > 0 && x == nullptr) return RFM_ERR_INVALID_ARGUMENT;
+  a = NormArgs{};
+  a.x = x;
+  a.ld_x = ld_x;
+  a.weight = weight;
+  a.rows = rows;
+  a.dim = dim;
+  a.param_dtype = param_dtype;
+  a.inv_dim = 1.f / static_cast<float>(dim);
+  return RFM_OK;
+}
+
+}  // namespace
+}  // namespace rfm
+
+extern "C" int rfm_layer_norm_forward(const void* x, int64_t ld_x, const void* weight, const void* bias, void* out,
+                                      float* mean, float* rstd, int64_t rows, int dim, float eps, int dtype,
+                                      int param_dtype, void* stream) {
+  using namespace rfm;
+  NormArgs a;
+  const int rc = norm_args(a, x, ld_x, weight, rows, dim, dtype, param_dtype);
+  if (rc != RFM_OK) return rc;
+  if ((mean == nullptr) != (rstd == nullptr) || !(eps >= 0.f)) return RFM_ERR_INVALID_ARGUMENT;
+  if (rows == 0) return RFM_OK;
+  if (out == nullptr) return RFM_ERR_INVALID_ARGUMENT;
+  a.bias = bias;
+  a.out = out;
+  a.mean_out = mean;
+  a.rstd_out = rstd;
+  a.eps = eps;
+  return run_norm(a, dtype, false, nullptr, as_stream(stream));
+}
+
+extern "C" int64_t rfm_layer_norm_workspace_bytes(int64_t rows, int dim) {
+  using namespace rfm;
+  if (rows < 0 || dim < 1) return -RFM_ERR_INVALID_ARGUMENT;
+  const int64_t most = static_cast<int64_t>(device_sm_count()) * kBwdPerSm;
+  const int64_t parts = dim > kWideDim ? kWideSlabs : (rows < most ? rows : most);
+  return parts * 2 * dim * static_cast<int64_t>(sizeof(float));
+}
+
+extern "C" int rfm_layer_norm_backward(const void* x, int64_t ld_x, const void* weight, const float* mean,
+                                       const float* rstd, const void* grad_out, int64_t ld_grad, void* grad_x,
+                                       void* grad_weight, void* grad_bias, int64_t rows, int dim, int dtype,
+                                       int param_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace rfm;
+  NormArgs a;
+  const int rc = norm_args(a, x, ld_x, weight, rows, dim, dtype, param_dtype);
+  if (rc != RFM_OK) return rc;
+  if ((ld_grad < dim && rows > 1) || ld_grad < 0) return RFM_ERR_INVALID_ARGUMENT;
+  const bool params = grad_weight != nullptr || grad_bias != nullptr;
+  if (rows > 0 && (mean == nullptr || rstd == nullptr || grad_out == nullptr)) return RFM_ERR_INVALID_ARGUMENT;
+  if (params && rows > 0 &&
+      (workspace == nullptr || workspace_bytes < rfm_layer_norm_workspace_bytes(rows, dim))) {
+    return RFM_ERR_INVALID_ARGUMENT;
+  }
+  if (grad_x == nullptr && !params) return RFM_OK;
+  a.dy = grad_out;
+  a.ld_dy = ld_grad;
+  a.out = grad_x;
+  a.mean_in = mean;
+  a.rstd_in = rstd;
+  a.partial = params ? static_cast<float*>(workspace) : nullptr;
+  int ctas = 0;
+  if (rows > 0) {
+    const int done = run_norm(a, dtype, true, &ctas, as_stream(stream));
+    if (done != RFM_OK) return done;
+  }
+  if (!params) return RFM_OK;
+  // with no rows the sums are empty: zeros
+  norm_param_sum_kernel<<<dim3((dim + 31) / 32, 2), kThreads, 0, as_stream(stream)>>>(
+      a.partial, ctas, dim, grad_weight, grad_bias, param_dtype);
+  return launch_status();
+}

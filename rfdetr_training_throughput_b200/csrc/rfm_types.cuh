@@ -1,0 +1,60 @@
+// Element types of the layer operators (RFM_DTYPE_*): loads, stores and the
+// one rounding on the way out.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "rfm_common.cuh"
+
+namespace rfm {
+
+inline int dtype_bytes(int dtype) { return dtype == RFM_DTYPE_F32 ? 4 : 2; }
+inline bool dtype_known(int dtype) {
+  return dtype == RFM_DTYPE_F32 || dtype == RFM_DTYPE_BF16 || dtype == RFM_DTYPE_F16;
+}
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) {
+  return __float2half_rn(v);
+}
+
+// VEC consecutive elements moved as one access (16 bytes for the full vectors).
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+  T v[VEC];
+};
+
+// Element i of a parameter array whose type is known at run time only (read
+// once per thread, outside the row loops).
+__device__ __forceinline__ float load_param(const void* p, int dtype, int64_t i) {
+  if (dtype == RFM_DTYPE_F32) return static_cast<const float*>(p)[i];
+  if (dtype == RFM_DTYPE_BF16) return to_float(static_cast<const __nv_bfloat16*>(p)[i]);
+  return to_float(static_cast<const __half*>(p)[i]);
+}
+
+__device__ __forceinline__ void store_param(void* p, int dtype, int64_t i, float v) {
+  if (dtype == RFM_DTYPE_F32) {
+    static_cast<float*>(p)[i] = v;
+  } else if (dtype == RFM_DTYPE_BF16) {
+    static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  } else {
+    static_cast<__half*>(p)[i] = __float2half_rn(v);
+  }
+}
+
+}  // namespace rfm

@@ -1,0 +1,311 @@
+"""AdamW on the device: one launch over all tensors, moments in 32 bits or in 8 (``rfm_adamw``).
+
+``adamw_step`` is the step on lists of tensors; ``AdamW`` is a ``torch.optim.Optimizer`` on top of it
+with torch's arguments.  With ``moment_bits=8`` a parameter's two moments take one byte each, plus one
+float32 scale per moment and 256 elements: a quarter of the memory, and 16 instead of 28 bytes moved
+per float32 parameter and step.  The codes are rounded at random (a hash of the step, the tensor's
+number and the element's index, so a run is reproducible): with nearest rounding a moment that moves by
+less than half a code a step would stand still.
+"""
+
+from __future__ import annotations
+
+from typing import Any, Iterable, Sequence
+
+import numpy as np
+import torch
+
+from . import _lib
+from ._launch import DTYPES, on_device, raw_stream, require_cuda
+
+#: Elements that share one scale of the 8-bit moments.
+MOMENT_BLOCK = _lib.MOMENT_BLOCK
+
+
+def moment_scales(numel: int) -> int:
+    """Scales of one 8-bit moment of ``numel`` elements."""
+    return -(-numel // MOMENT_BLOCK)
+
+
+def _pointers(tensors: Sequence[torch.Tensor]) -> list[int]:
+    return list(map(torch.Tensor.data_ptr, tensors))
+
+
+def _check_list(name: str, tensors, dtype: torch.dtype, index: int, sizes: list[int]) -> None:
+    if len(tensors) != len(sizes):
+        raise ValueError(f"{name} has {len(tensors)} tensors, params has {len(sizes)}")
+    kind = torch.Tensor
+    if (list(map(kind.numel, tensors)) == sizes and {t.dtype for t in tensors} == {dtype}
+            and set(map(kind.get_device, tensors)) == {index} and all(map(kind.is_contiguous, tensors))):
+        return
+    for t, n in zip(tensors, sizes):
+        if t.dtype != dtype or t.get_device() != index or t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"{name} must hold contiguous {dtype} tensors on the params' device; one that needs {n} "
+                             f"elements is {t.dtype} with {t.numel()} on {t.device}")
+
+
+def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avg: Sequence[torch.Tensor],
+               exp_avg_sq: Sequence[torch.Tensor], step: int | torch.Tensor, *,
+               scales: tuple[Sequence[torch.Tensor], Sequence[torch.Tensor]] | None = None,
+               lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+               weight_decay: float = 1e-2, grad_scale: torch.Tensor | None = None) -> None:
+    """One AdamW step in place on ``params`` and their moments.
+
+    ``params`` and ``grads`` contiguous CUDA tensors of one type (float32, bfloat16 or float16) on one
+    device, pairwise of one size and all distinct.  Without ``scales``, ``exp_avg`` and ``exp_avg_sq`` are
+    float32 tensors of the params' sizes.  With ``scales`` (two lists of float32 tensors, of
+    ``moment_scales(numel)`` elements each) they hold int8 and uint8 codes (see ``rfm_adamw``).
+
+    ``step`` is the number of this update, from 1; an int64 tensor of one element on the device, and for
+    ``lr`` a float32 one, are read by the kernels, so that a captured step follows them.  ``grad_scale``
+    (float32, one element, on the device) multiplies the gradients: a clipping factor or the inverse of a
+    loss scale, without a host synchronisation.
+    """
+    if not len(params):
+        if len(grads) or len(exp_avg) or len(exp_avg_sq):
+            raise ValueError("params is empty, the other lists are not")
+        return
+    index = require_cuda(params[0], "params", "adamw_step")
+    dtype = params[0].dtype
+    if dtype not in DTYPES:
+        raise ValueError(f"params must be float32, bfloat16 or float16, got {dtype}")
+    eight = scales is not None
+    sizes = list(map(torch.Tensor.numel, params))
+    _check_list("params", params, dtype, index, sizes)
+    _check_list("grads", grads, dtype, index, sizes)
+    _check_list("exp_avg", exp_avg, torch.int8 if eight else torch.float32, index, sizes)
+    _check_list("exp_avg_sq", exp_avg_sq, torch.uint8 if eight else torch.float32, index, sizes)
+    table = np.zeros((len(sizes), _lib.ADAMW_TENSOR_WORDS), dtype=np.int64)
+    where = table.T
+    where[0], where[1] = _pointers(params), _pointers(grads)
+    where[2], where[3] = _pointers(exp_avg), _pointers(exp_avg_sq)
+    if eight:
+        counts = [moment_scales(n) for n in sizes]
+        for row, one in zip((4, 5), scales):
+            _check_list("scales", one, torch.float32, index, counts)
+            where[row] = _pointers(one)
+    where[6] = sizes
+    filled = [p for p, n in zip(where[0].tolist(), sizes) if n]
+    if len(set(filled)) != len(filled):
+        raise ValueError("params holds a tensor twice")
+    _launch(table, index, dtype, 8 if eight else 32, step, lr, betas, eps, weight_decay, grad_scale)
+
+
+def _scalar_pointer(name: str, t: torch.Tensor, dtype: torch.dtype, index: int) -> int:
+    if t.dtype != dtype or t.numel() != 1 or t.get_device() != index:
+        raise ValueError(f"{name} must be one {dtype} element on the params' device")
+    return t.data_ptr()
+
+
+def _launch(table: np.ndarray, index: int, dtype: torch.dtype, bits: int, step, lr, betas, eps, weight_decay,
+            grad_scale) -> None:
+    device_step = device_lr = scale = work = None
+    if isinstance(step, torch.Tensor):
+        device_step, step = _scalar_pointer("step", step, torch.int64, index), 0
+    elif step < 1:
+        raise ValueError(f"step counts from 1, got {step}")
+    if isinstance(lr, torch.Tensor):
+        device_lr, lr = _scalar_pointer("lr", lr, torch.float32, index), 0.0
+    if grad_scale is not None:
+        scale = _scalar_pointer("grad_scale", grad_scale, torch.float32, index)
+    b1, b2 = betas
+    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and lr >= 0.0 and weight_decay >= 0.0):
+        raise ValueError("betas must be in [0, 1), eps, lr and weight_decay not negative")
+    with on_device(index):
+        if device_step is not None or device_lr is not None:
+            work = torch.empty(4, dtype=torch.float32, device=torch.device("cuda", index))
+        _lib.check("rfm_adamw", _lib.load().rfm_adamw(
+            table.ctypes.data, len(table), DTYPES[dtype], bits, lr, b1, b2, eps, weight_decay, step, device_lr,
+            device_step, scale, work.data_ptr() if work is not None else None, raw_stream(index)))
+
+
+def dequantize_moments(exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, exp_avg_scale: torch.Tensor,
+                       exp_avg_sq_scale: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """The float32 values that one tensor's 8-bit moments stand for."""
+    index = require_cuda(exp_avg, "exp_avg", "dequantize_moments")
+    n = exp_avg.numel()
+    _check_list("exp_avg", [exp_avg], torch.int8, index, [n])
+    _check_list("exp_avg_sq", [exp_avg_sq], torch.uint8, index, [n])
+    _check_list("scales", [exp_avg_scale, exp_avg_sq_scale], torch.float32, index, [moment_scales(n)] * 2)
+    m, v = (torch.empty(exp_avg.shape, dtype=torch.float32, device=exp_avg.device) for _ in range(2))
+    with on_device(index):
+        _lib.check("rfm_adamw_moments", _lib.load().rfm_adamw_moments(
+            exp_avg.data_ptr(), exp_avg_sq.data_ptr(), exp_avg_scale.data_ptr(), exp_avg_sq_scale.data_ptr(), n,
+            m.data_ptr(), v.data_ptr(), raw_stream(index)))
+    return m, v
+
+
+def quantize_moments(exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor) -> tuple[torch.Tensor, ...]:
+    """8-bit codes and scales ``(exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale)`` nearest to one
+    tensor's float32 moments, for states that come from 32 bits.  Not part of a step."""
+    def blocks(t):
+        flat = t.detach().float().reshape(-1)
+        return torch.nn.functional.pad(flat, (0, -flat.numel() % MOMENT_BLOCK)).view(-1, MOMENT_BLOCK)
+
+    m, v = blocks(exp_avg), blocks(exp_avg_sq)
+    sm, sv = m.abs().amax(1), v.amax(1)
+    a = torch.nan_to_num((m.abs() / sm[:, None]).sqrt() * 127, nan=0.0).round().clamp(0, 127)
+    b = torch.nan_to_num((v / sv[:, None]).sqrt().sqrt() * 255, nan=0.0).round().clamp(0, 255)
+    b = torch.where(v > 0, b.clamp_min(1), b)
+
+    def codes(t, dtype):
+        return t.view(-1)[:exp_avg.numel()].to(dtype).view(exp_avg.shape)
+
+    return codes(torch.where(m < 0, -a, a), torch.int8), codes(b, torch.uint8), sm, sv
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW with torch's arguments, one launch per parameter group and type.
+
+    ``moment_bits`` 32 keeps float32 moments, 8 the codes and scales of ``adamw_step``.  With
+    ``capturable`` the step counter of a group lies on the device and advances inside ``step()``, so that
+    a captured step can be replayed; ``lr`` may then be a float32 device tensor.  ``amsgrad`` and
+    ``maximize`` are not offered and raise.  A parameter's state is ``exp_avg``, ``exp_avg_sq`` (and
+    ``exp_avg_scale``, ``exp_avg_sq_scale``) with ``step``; a float32 state dict loads into either form.
+    """
+
+    def __init__(self, params: Iterable, lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999),
+                 eps: float = 1e-8, weight_decay: float = 1e-2, amsgrad: bool = False, *, maximize: bool = False,
+                 foreach: bool | None = None, capturable: bool = False, differentiable: bool = False,
+                 fused: bool | None = None, moment_bits: int = 32):
+        if amsgrad or maximize or differentiable:
+            raise NotImplementedError("amsgrad, maximize and differentiable steps are not offered")
+        if moment_bits not in (8, 32):
+            raise ValueError(f"moment_bits must be 8 or 32, got {moment_bits}")
+        if isinstance(lr, torch.Tensor) and not capturable:
+            raise ValueError("a tensor lr needs capturable=True")
+        b1, b2 = betas
+        if not isinstance(lr, torch.Tensor) and not lr >= 0.0:
+            raise ValueError(f"lr must not be negative, got {lr}")
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and weight_decay >= 0.0):
+            raise ValueError("betas must be in [0, 1), eps and weight_decay not negative")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, capturable=capturable,
+                                      moment_bits=moment_bits))
+
+    def _new_state(self, p: torch.Tensor, group: dict) -> dict:
+        state: dict[str, Any] = {}
+        if group["capturable"]:
+            state["step"] = torch.zeros((), dtype=torch.int64, device=p.device)
+        else:
+            state["step"] = 0
+        if group["moment_bits"] == 32:  # with the parameter's strides
+            state["exp_avg"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+            state["exp_avg_sq"] = torch.zeros_like(state["exp_avg"])
+        else:
+            if not p.is_contiguous():
+                raise ValueError("8-bit moments need contiguous parameters")
+            state["exp_avg"] = torch.zeros(p.shape, dtype=torch.int8, device=p.device)
+            state["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device)
+            for k in ("exp_avg_scale", "exp_avg_sq_scale"):
+                state[k] = torch.zeros(moment_scales(p.numel()), dtype=torch.float32, device=p.device)
+        return state
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        """One update of every parameter that has a gradient."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            buckets: dict[tuple, list] = {}
+            fresh: dict[torch.device, torch.Tensor] = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise ValueError("AdamW does not take sparse gradients")
+                state = self.state[p]
+                if not state:
+                    state.update(self._new_state(p, group))
+                    if group["capturable"]:  # parameters that start together share one counter
+                        state["step"] = fresh.setdefault(p.device, state["step"])
+                if group["capturable"]:
+                    key = (p.dtype, p.device, id(state["step"]))
+                else:
+                    state["step"] += 1
+                    key = (p.dtype, p.device, state["step"])
+                buckets.setdefault(key, []).append(p)
+            for members in buckets.values():
+                self._step_bucket(group, members)
+        return loss
+
+    def _step_bucket(self, group: dict, members: list) -> None:
+        states = [self.state[p] for p in members]
+        eight = group["moment_bits"] == 8
+        step = states[0]["step"]
+        if group["capturable"]:
+            sharing = sum(1 for p in group["params"] if self.state.get(p, {}).get("step") is step)
+            if sharing != len(members):
+                raise ValueError("a capturable step needs a gradient for every parameter that shares a step counter")
+            step.add_(1)
+        params, grads, avg, avg_sq = [], [], [], []
+        for p, s in zip(members, states):
+            data, g, m, v = p.detach(), p.grad.detach(), s["exp_avg"], s["exp_avg_sq"]
+            if not data.is_contiguous():
+                data, g, m, v = _flat_alike(data, g, m, v)
+            elif not g.is_contiguous():
+                g = g.contiguous()
+            params.append(data)
+            grads.append(g)
+            avg.append(m)
+            avg_sq.append(v)
+        scales = tuple([s[k] for s in states] for k in ("exp_avg_scale", "exp_avg_sq_scale")) if eight else None
+        adamw_step(params, grads, avg, avg_sq, step, scales=scales, lr=group["lr"], betas=group["betas"],
+                   eps=group["eps"], weight_decay=group["weight_decay"])
+
+    def load_state_dict(self, state_dict: dict) -> None:
+        """Load a state dict of this class or of ``torch.optim.AdamW``.  ``moment_bits`` and ``capturable``
+        stay as constructed; moments are converted to the form they ask for."""
+        kept = [(g["moment_bits"], g["capturable"]) for g in self.param_groups]
+        for g in state_dict["param_groups"]:
+            if g.get("amsgrad") or g.get("maximize"):
+                raise NotImplementedError("amsgrad and maximize steps are not offered")
+        super().load_state_dict(state_dict)
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        raw = dict(zip((p for g in self.param_groups for p in g["params"]), ids))
+        for group, (bits, capturable) in zip(self.param_groups, kept):
+            group["moment_bits"], group["capturable"] = bits, capturable
+            shared: dict[tuple, torch.Tensor] = {}
+            for p in group["params"]:
+                saved = state_dict["state"].get(raw[p])
+                if not saved:
+                    continue
+                state = self._new_state(p, group)
+                _adopt(state, saved, bits)
+                count = int(saved["step"])
+                if capturable:
+                    state["step"] = shared.setdefault((p.device, count), state["step"].fill_(count))
+                else:
+                    state["step"] = count
+                self.state[p] = state
+
+
+def _flat_alike(data, g, m, v):
+    """The dense elements of a parameter with permuted strides as one contiguous view, and the
+    gradient and the moments in the same order."""
+    order = sorted(range(data.dim()), key=data.stride, reverse=True)
+    flat = data.permute(order)
+    if not flat.is_contiguous():
+        raise ValueError("parameters must be dense (no gaps or overlaps between their elements)")
+    g = g.permute(order).contiguous()
+    m, v = m.permute(order), v.permute(order)
+    if not (m.is_contiguous() and v.is_contiguous()):
+        raise ValueError("the moments must have their parameter's strides")
+    return flat, g, m, v
+
+
+@torch.no_grad()
+def _adopt(state: dict, saved: dict, bits: int) -> None:
+    """Copy saved moments, in either form, into ``state``'s."""
+    device = state["exp_avg"].device
+    m, v = saved["exp_avg"].to(device), saved["exp_avg_sq"].to(device)
+    names = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
+    if m.dtype == torch.int8:
+        values = [m, v, saved["exp_avg_scale"].to(device), saved["exp_avg_sq_scale"].to(device)]
+        if bits == 32:
+            values = dequantize_moments(*(t.contiguous() for t in values))
+    else:
+        values = (m, v) if bits == 32 else quantize_moments(m, v)
+    for name, value in zip(names, values):
+        state[name].copy_(value)
