@@ -1,0 +1,119 @@
+// adamw_step: checks of the tensor lists and the table that rfm_adamw takes.
+#include <algorithm>
+
+#include "host_adamw.h"
+
+namespace rfm_host {
+namespace {
+
+void check_list(const char* name, const TensorList& list, at::ScalarType type, const at::Device& device,
+                const TensorList& like, bool scales) {
+  RFM_REQUIRE(list.size() == like.size(), name, " has ", list.size(), " tensors, params has ", like.size());
+  for (size_t i = 0; i < list.size(); ++i) {
+    const Tensor& t = list[i];
+    const int64_t n = scales ? (like[i].numel() + RFM_MOMENT_BLOCK - 1) / RFM_MOMENT_BLOCK : like[i].numel();
+    RFM_REQUIRE(t.defined() && t.scalar_type() == type && t.device() == device && t.numel() == n &&
+                    t.layout() == at::kStrided && t.is_contiguous(),
+                name, " must hold contiguous ", type, " tensors on the params' device; number ", i, " needs ", n,
+                " elements and is ", t.defined() ? t.toString() : std::string("undefined"), " with ",
+                t.defined() ? t.numel() : 0, t.defined() && !t.is_contiguous() ? ", not contiguous" : "");
+  }
+}
+
+void* scalar_pointer(const char* name, const Tensor& t, at::ScalarType type, const at::Device& device) {
+  RFM_REQUIRE(t.scalar_type() == type && t.numel() == 1 && t.device() == device, name, " must be one ", type,
+              " element on the params' device");
+  return t.data_ptr();
+}
+
+}  // namespace
+
+void adamw_step(const TensorList& params, const TensorList& grads, const TensorList& exp_avg,
+                const TensorList& exp_avg_sq, const std::optional<TensorList>& exp_avg_scale,
+                const std::optional<TensorList>& exp_avg_sq_scale, int64_t step, const MaybeTensor& device_step,
+                double lr, const MaybeTensor& device_lr, double beta1, double beta2, double eps, double weight_decay,
+                const MaybeTensor& grad_scale) {
+  RFM_REQUIRE(device_step.has_value() || step >= 1, "step counts from 1, got ", step);
+  RFM_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0 && lr >= 0.0 &&
+                  weight_decay >= 0.0,
+              "betas must be in [0, 1), eps, lr and weight_decay not negative");
+  if (params.empty()) {
+    RFM_REQUIRE(grads.empty() && exp_avg.empty() && exp_avg_sq.empty(), "params is empty, the other lists are not");
+    return;
+  }
+  RFM_REQUIRE(params[0].is_cuda(), "params must be CUDA tensors (adamw_step has no CPU path)");
+  const at::Device device = params[0].device();
+  const at::ScalarType type = params[0].scalar_type();
+  RFM_REQUIRE(dtype_code(type) >= 0, "params must be float32, bfloat16 or float16, got ", type);
+  const bool eight = exp_avg_scale.has_value();
+  check_list("params", params, type, device, params, false);
+  check_list("grads", grads, type, device, params, false);
+  check_list("exp_avg", exp_avg, eight ? at::kChar : at::kFloat, device, params, false);
+  check_list("exp_avg_sq", exp_avg_sq, eight ? at::kByte : at::kFloat, device, params, false);
+  if (eight) {
+    check_list("scales", *exp_avg_scale, at::kFloat, device, params, true);
+    check_list("scales", *exp_avg_sq_scale, at::kFloat, device, params, true);
+  }
+  const size_t count = params.size();
+  std::vector<rfm_adamw_tensor> table(count);
+  std::vector<std::pair<uintptr_t, uintptr_t>> written;  // [first, past the last) byte of what the step writes
+  written.reserve(count * (eight ? 5 : 3));
+  const auto writes = [&written](void* p, int64_t bytes) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    if (bytes > 0) written.emplace_back(at, at + static_cast<uintptr_t>(bytes));
+    return p;
+  };
+  for (size_t i = 0; i < count; ++i) {
+    const int64_t n = params[i].numel();
+    rfm_adamw_tensor& t = table[i];
+    t = rfm_adamw_tensor{};
+    t.param = writes(params[i].data_ptr(), n * params[i].element_size());
+    t.grad = grads[i].data_ptr();
+    t.exp_avg = writes(exp_avg[i].data_ptr(), n * exp_avg[i].element_size());
+    t.exp_avg_sq = writes(exp_avg_sq[i].data_ptr(), n * exp_avg_sq[i].element_size());
+    if (eight) {
+      const Tensor &a = (*exp_avg_scale)[i], &b = (*exp_avg_sq_scale)[i];
+      t.exp_avg_scale = static_cast<float*>(writes(a.data_ptr(), a.numel() * 4));
+      t.exp_avg_sq_scale = static_cast<float*>(writes(b.data_ptr(), b.numel() * 4));
+    }
+    t.numel = n;
+  }
+  std::sort(written.begin(), written.end());
+  for (size_t i = 1; i < written.size(); ++i) {
+    RFM_REQUIRE(written[i].first >= written[i - 1].second,
+                "a tensor is given twice: params, moments and scales must not share memory");
+  }
+  void* at_step = device_step ? scalar_pointer("step", *device_step, at::kLong, device) : nullptr;
+  void* at_lr = device_lr ? scalar_pointer("lr", *device_lr, at::kFloat, device) : nullptr;
+  void* at_scale = grad_scale ? scalar_pointer("grad_scale", *grad_scale, at::kFloat, device) : nullptr;
+  const c10::cuda::CUDAGuard guard(device);
+  Tensor work;
+  if (at_step != nullptr || at_lr != nullptr) work = at::empty({4}, params[0].options().dtype(at::kFloat));
+  check_call("rfm_adamw",
+             rfm_adamw(table.data(), static_cast<int>(count), dtype_code(type), eight ? 8 : 32, lr, beta1, beta2, eps,
+                       weight_decay, step, static_cast<const float*>(at_lr), static_cast<const int64_t*>(at_step),
+                       static_cast<const float*>(at_scale), data_or_null(work), current_stream(device)));
+  // the in-place updates count as writes for autograd's saved tensors
+  for (const Tensor& p : params) p.unsafeGetTensorImpl()->bump_version();
+}
+
+std::tuple<Tensor, Tensor> dequantize_moments(const Tensor& exp_avg, const Tensor& exp_avg_sq,
+                                              const Tensor& exp_avg_scale, const Tensor& exp_avg_sq_scale) {
+  RFM_REQUIRE(exp_avg.is_cuda(), "exp_avg must be a CUDA tensor (dequantize_moments has no CPU path)");
+  const at::Device device = exp_avg.device();
+  const TensorList like{exp_avg};
+  check_list("exp_avg", {exp_avg}, at::kChar, device, like, false);
+  check_list("exp_avg_sq", {exp_avg_sq}, at::kByte, device, like, false);
+  check_list("scales", {exp_avg_scale}, at::kFloat, device, like, true);
+  check_list("scales", {exp_avg_sq_scale}, at::kFloat, device, like, true);
+  const c10::cuda::CUDAGuard guard(device);
+  const auto options = exp_avg.options().dtype(at::kFloat);
+  Tensor m = at::empty(exp_avg.sizes(), options), v = at::empty(exp_avg.sizes(), options);
+  check_call("rfm_adamw_moments",
+             rfm_adamw_moments(exp_avg.data_ptr(), exp_avg_sq.data_ptr(), exp_avg_scale.data_ptr<float>(),
+                               exp_avg_sq_scale.data_ptr<float>(), exp_avg.numel(), m.data_ptr<float>(),
+                               v.data_ptr<float>(), current_stream(device)));
+  return {m, v};
+}
+
+}  // namespace rfm_host

@@ -12,11 +12,10 @@ from __future__ import annotations
 
 from typing import Any, Iterable, Sequence
 
-import numpy as np
 import torch
 
 from . import _lib
-from ._launch import DTYPES, on_device, raw_stream, require_cuda
+from ._native import host
 
 #: Elements that share one scale of the 8-bit moments.
 MOMENT_BLOCK = _lib.MOMENT_BLOCK
@@ -25,23 +24,6 @@ MOMENT_BLOCK = _lib.MOMENT_BLOCK
 def moment_scales(numel: int) -> int:
     """Scales of one 8-bit moment of ``numel`` elements."""
     return -(-numel // MOMENT_BLOCK)
-
-
-def _pointers(tensors: Sequence[torch.Tensor]) -> list[int]:
-    return list(map(torch.Tensor.data_ptr, tensors))
-
-
-def _check_list(name: str, tensors, dtype: torch.dtype, index: int, sizes: list[int]) -> None:
-    if len(tensors) != len(sizes):
-        raise ValueError(f"{name} has {len(tensors)} tensors, params has {len(sizes)}")
-    kind = torch.Tensor
-    if (list(map(kind.numel, tensors)) == sizes and {t.dtype for t in tensors} == {dtype}
-            and set(map(kind.get_device, tensors)) == {index} and all(map(kind.is_contiguous, tensors))):
-        return
-    for t, n in zip(tensors, sizes):
-        if t.dtype != dtype or t.get_device() != index or t.numel() != n or not t.is_contiguous():
-            raise ValueError(f"{name} must hold contiguous {dtype} tensors on the params' device; one that needs {n} "
-                             f"elements is {t.dtype} with {t.numel()} on {t.device}")
 
 
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avg: Sequence[torch.Tensor],
@@ -61,78 +43,20 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     (float32, one element, on the device) multiplies the gradients: a clipping factor or the inverse of a
     loss scale, without a host synchronisation.
     """
-    if not len(params):
-        if len(grads) or len(exp_avg) or len(exp_avg_sq):
-            raise ValueError("params is empty, the other lists are not")
-        return
-    index = require_cuda(params[0], "params", "adamw_step")
-    dtype = params[0].dtype
-    if dtype not in DTYPES:
-        raise ValueError(f"params must be float32, bfloat16 or float16, got {dtype}")
-    eight = scales is not None
-    sizes = list(map(torch.Tensor.numel, params))
-    _check_list("params", params, dtype, index, sizes)
-    _check_list("grads", grads, dtype, index, sizes)
-    _check_list("exp_avg", exp_avg, torch.int8 if eight else torch.float32, index, sizes)
-    _check_list("exp_avg_sq", exp_avg_sq, torch.uint8 if eight else torch.float32, index, sizes)
-    table = np.zeros((len(sizes), _lib.ADAMW_TENSOR_WORDS), dtype=np.int64)
-    where = table.T
-    where[0], where[1] = _pointers(params), _pointers(grads)
-    where[2], where[3] = _pointers(exp_avg), _pointers(exp_avg_sq)
-    if eight:
-        counts = [moment_scales(n) for n in sizes]
-        for row, one in zip((4, 5), scales):
-            _check_list("scales", one, torch.float32, index, counts)
-            where[row] = _pointers(one)
-    where[6] = sizes
-    filled = [p for p, n in zip(where[0].tolist(), sizes) if n]
-    if len(set(filled)) != len(filled):
-        raise ValueError("params holds a tensor twice")
-    _launch(table, index, dtype, 8 if eight else 32, step, lr, betas, eps, weight_decay, grad_scale)
-
-
-def _scalar_pointer(name: str, t: torch.Tensor, dtype: torch.dtype, index: int) -> int:
-    if t.dtype != dtype or t.numel() != 1 or t.get_device() != index:
-        raise ValueError(f"{name} must be one {dtype} element on the params' device")
-    return t.data_ptr()
-
-
-def _launch(table: np.ndarray, index: int, dtype: torch.dtype, bits: int, step, lr, betas, eps, weight_decay,
-            grad_scale) -> None:
-    device_step = device_lr = scale = work = None
+    device_step = device_lr = None
     if isinstance(step, torch.Tensor):
-        device_step, step = _scalar_pointer("step", step, torch.int64, index), 0
-    elif step < 1:
-        raise ValueError(f"step counts from 1, got {step}")
+        device_step, step = step, 0
     if isinstance(lr, torch.Tensor):
-        device_lr, lr = _scalar_pointer("lr", lr, torch.float32, index), 0.0
-    if grad_scale is not None:
-        scale = _scalar_pointer("grad_scale", grad_scale, torch.float32, index)
-    b1, b2 = betas
-    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and lr >= 0.0 and weight_decay >= 0.0):
-        raise ValueError("betas must be in [0, 1), eps, lr and weight_decay not negative")
-    with on_device(index):
-        if device_step is not None or device_lr is not None:
-            work = torch.empty(4, dtype=torch.float32, device=torch.device("cuda", index))
-        _lib.check("rfm_adamw", _lib.load().rfm_adamw(
-            table.ctypes.data, len(table), DTYPES[dtype], bits, lr, b1, b2, eps, weight_decay, step, device_lr,
-            device_step, scale, work.data_ptr() if work is not None else None, raw_stream(index)))
+        device_lr, lr = lr, 0.0
+    avg_scales, avg_sq_scales = (None, None) if scales is None else scales
+    host().adamw_step(params, grads, exp_avg, exp_avg_sq, avg_scales, avg_sq_scales, step, device_step, lr, device_lr,
+                      betas[0], betas[1], eps, weight_decay, grad_scale)
 
 
 def dequantize_moments(exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, exp_avg_scale: torch.Tensor,
                        exp_avg_sq_scale: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """The float32 values that one tensor's 8-bit moments stand for."""
-    index = require_cuda(exp_avg, "exp_avg", "dequantize_moments")
-    n = exp_avg.numel()
-    _check_list("exp_avg", [exp_avg], torch.int8, index, [n])
-    _check_list("exp_avg_sq", [exp_avg_sq], torch.uint8, index, [n])
-    _check_list("scales", [exp_avg_scale, exp_avg_sq_scale], torch.float32, index, [moment_scales(n)] * 2)
-    m, v = (torch.empty(exp_avg.shape, dtype=torch.float32, device=exp_avg.device) for _ in range(2))
-    with on_device(index):
-        _lib.check("rfm_adamw_moments", _lib.load().rfm_adamw_moments(
-            exp_avg.data_ptr(), exp_avg_sq.data_ptr(), exp_avg_scale.data_ptr(), exp_avg_sq_scale.data_ptr(), n,
-            m.data_ptr(), v.data_ptr(), raw_stream(index)))
-    return m, v
+    return host().dequantize_moments(exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale)
 
 
 def quantize_moments(exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor) -> tuple[torch.Tensor, ...]:
