@@ -462,6 +462,86 @@ int rfm_adamw_moments(const void* exp_avg, const void* exp_avg_sq, const float* 
                       const float* exp_avg_sq_scale, int64_t numel, float* out_avg, float* out_avg_sq, void* stream);
 
 /*
+ * A layer's matrix product with its epilogue, on the tensor cores (fp32 sums):
+ *   out = act(x W^T + bias) + residual
+ *
+ *   x          [rows, in_features] of `dtype` (RFM_DTYPE_BF16 or _F16), row r at x + r * ld_x
+ *   weight     [out_features, in_features] of `dtype`, row stride ld_weight
+ *              both 16-byte aligned, their strides multiples of 8 elements and (with more than one row)
+ *              not below in_features
+ *   bias       [out_features] of bias_dtype (`dtype` or RFM_DTYPE_F32), or NULL
+ *   residual   [rows, out_features] of `dtype`, row stride ld_residual, any alignment, or NULL
+ *   out        [rows, out_features] of `dtype`, contiguous; not the residual's memory
+ *   pre        x W^T + bias rounded to `dtype`, contiguous, for the backward; or NULL
+ *   activation RFM_ACT_NONE, RFM_ACT_RELU, RFM_ACT_GELU (x times the normal distribution's cdf)
+ *   workspace  rfm_linear_forward_workspace_bytes(...) bytes on the current device, 16-byte aligned
+ *              (partial sums of a split contraction; 0 for most shapes), used by this call's kernels alone
+ *
+ * rfm_linear_backward, given grad_out (row stride ld_grad, any alignment), writes
+ *   dP = grad_out act'(saved),  grad_x = dP W,  grad_weight = dP^T x,  grad_bias = sum_rows dP
+ * (contiguous, `dtype`; grad_bias of bias_dtype; each may be NULL).  `saved` is the forward's `pre`; for
+ * RFM_ACT_RELU without a residual the forward's `out` does as well; NULL without an activation.
+ * grad_pre [rows, out_features] with stride ld_grad_pre (16-byte aligned, a multiple of 8) receives dP
+ * rounded to `dtype`, the products' operand; it is needed with an activation, and where grad_out is not
+ * 16-byte aligned with a stride that is a multiple of 8.  Sums over rows are in fixed order (deterministic).
+ */
+#define RFM_ACT_NONE 0
+#define RFM_ACT_RELU 1
+#define RFM_ACT_GELU 2
+typedef struct rfm_linear {
+  const void* x;
+  const void* weight;
+  const void* bias;
+  const void* residual;
+  void* out;
+  void* pre;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t rows;
+  int64_t ld_x;
+  int64_t ld_weight;
+  int64_t ld_residual;
+  int32_t in_features;
+  int32_t out_features;
+  int32_t dtype;
+  int32_t bias_dtype;
+  int32_t activation;
+  int32_t reserved; /* must be 0 */
+} rfm_linear;
+
+typedef struct rfm_linear_grad {
+  const void* x;
+  const void* weight;
+  const void* saved;
+  const void* grad_out;
+  void* grad_pre;
+  void* grad_x;
+  void* grad_weight;
+  void* grad_bias;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t rows;
+  int64_t ld_x;
+  int64_t ld_weight;
+  int64_t ld_grad;
+  int64_t ld_grad_pre;
+  int32_t in_features;
+  int32_t out_features;
+  int32_t dtype;
+  int32_t bias_dtype;
+  int32_t activation;
+  int32_t reserved; /* must be 0 */
+} rfm_linear_grad;
+
+int64_t rfm_linear_forward_workspace_bytes(int64_t rows, int in_features, int out_features);
+int rfm_linear_forward(const rfm_linear* args, void* stream);
+int64_t rfm_linear_backward_workspace_bytes(int64_t rows, int in_features, int out_features);
+int rfm_linear_backward(const rfm_linear_grad* args, void* stream);
+/* Whether a product on the current device ever gave up one of its bounded waits (never expected; its
+ * output is then incomplete): *faults 0 or 1.  Synchronises the device. */
+int rfm_linear_faults(int* faults);
+
+/*
  * ---- The sharded sweep's exchange: pairs pushed into every rank's memory ----
  *
  * No counterpart in the reference, which matches on one GPU.  A batch split by

@@ -59,12 +59,20 @@ EXPORTS = (
     "rfm_layer_norm_backward",
     "rfm_adamw",
     "rfm_adamw_moments",
+    "rfm_linear_forward_workspace_bytes",
+    "rfm_linear_forward",
+    "rfm_linear_backward_workspace_bytes",
+    "rfm_linear_backward",
+    "rfm_linear_faults",
 )
 
 #: RFM_DTYPE_*: element types of the layer operators.
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
 DTYPE_F16 = 2
+
+#: RFM_ACT_*: activations of the layers' products.
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2}
 
 #: RFM_MOMENT_BLOCK: elements that share one scale of the 8-bit moments.
 MOMENT_BLOCK = 256
@@ -150,6 +158,29 @@ class PeerSyncArgs(ctypes.Structure):
 
 
 assert ctypes.sizeof(PairPush) == 152 and ctypes.sizeof(PeerSyncArgs) == 104
+
+
+class Linear(ctypes.Structure):
+    """Mirror of ``struct rfm_linear``."""
+
+    _fields_ = [
+        *((k, ctypes.c_void_p) for k in ("x", "weight", "bias", "residual", "out", "pre", "workspace")),
+        *((k, ctypes.c_int64) for k in ("workspace_bytes", "rows", "ld_x", "ld_weight", "ld_residual")),
+        *((k, ctypes.c_int32) for k in ("in_features", "out_features", "dtype", "bias_dtype", "activation",
+                                        "reserved")),
+    ]
+
+
+class LinearGrad(ctypes.Structure):
+    """Mirror of ``struct rfm_linear_grad``."""
+
+    _fields_ = [
+        *((k, ctypes.c_void_p) for k in ("x", "weight", "saved", "grad_out", "grad_pre", "grad_x", "grad_weight",
+                                         "grad_bias", "workspace")),
+        *((k, ctypes.c_int64) for k in ("workspace_bytes", "rows", "ld_x", "ld_weight", "ld_grad", "ld_grad_pre")),
+        *((k, ctypes.c_int32) for k in ("in_features", "out_features", "dtype", "bias_dtype", "activation",
+                                        "reserved")),
+    ]
 
 
 class RfmError(RuntimeError):
@@ -246,6 +277,15 @@ def load() -> ctypes.CDLL:
                                             _i64, _p]
     lib.rfm_adamw.restype = _i32
     lib.rfm_adamw.argtypes = [_p, _i32, _i32, _i32, _f64, _f64, _f64, _f64, _f64, _i64, _p, _p, _p, _p, _p]
+    for name in ("rfm_linear_forward_workspace_bytes", "rfm_linear_backward_workspace_bytes"):
+        getattr(lib, name).restype = _i64
+        getattr(lib, name).argtypes = [_i64, _i32, _i32]
+    lib.rfm_linear_forward.restype = _i32
+    lib.rfm_linear_forward.argtypes = [ctypes.POINTER(Linear), _p]
+    lib.rfm_linear_backward.restype = _i32
+    lib.rfm_linear_backward.argtypes = [ctypes.POINTER(LinearGrad), _p]
+    lib.rfm_linear_faults.restype = _i32
+    lib.rfm_linear_faults.argtypes = [ctypes.POINTER(_i32)]
     lib.rfm_adamw_moments.restype = _i32
     lib.rfm_adamw_moments.argtypes = [_p, _p, _p, _p, _i64, _p, _p, _p]
     _lib = lib

@@ -43,6 +43,8 @@ inline void* current_stream(const at::Device& device) {
 inline void* data_or_null(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 inline Tensor or_undefined(const MaybeTensor& t) { return t.has_value() ? *t : Tensor(); }
 
+inline MaybeTensor maybe(const Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); }
+
 inline bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
 // `x` as [rows, last] with a unit stride along the rows' elements and rows that
@@ -77,5 +79,7 @@ inline variable_list once(variable_list grads, const char* op) {
 }
 
 Tensor layer_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, double eps);
+Tensor linear(const Tensor& x, const Tensor& weight, const MaybeTensor& bias, int64_t activation,
+              const MaybeTensor& residual);
 
 }  // namespace rfm_host

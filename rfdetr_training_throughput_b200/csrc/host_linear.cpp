@@ -1,0 +1,198 @@
+// linear: checks, allocation and autograd around rfm_linear_*.
+#include <ATen/autocast_mode.h>
+
+#include "host_common.h"
+
+namespace rfm_host {
+namespace {
+
+int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+
+bool tma_rows(const Tensor& y) {
+  return reinterpret_cast<uintptr_t>(y.data_ptr()) % 16 == 0 && (y.size(0) <= 1 || y.stride(0) % 8 == 0);
+}
+
+// `x` as a matrix that TMA can read: rows of adjacent elements, 16-byte aligned,
+// their stride a multiple of 8 elements.  A view where the layout allows, else a
+// copy with padded rows.
+Tensor operand(const Tensor& x) {
+  const Tensor y = rows_of(x);
+  if (y.numel() == 0 || tma_rows(y)) return y;
+  const Tensor copy = at::empty({y.size(0), pad8(y.size(1))}, y.options()).narrow(1, 0, y.size(1));
+  copy.copy_(y);
+  return copy;
+}
+
+int64_t operand_stride(const Tensor& y) { return y.size(0) > 1 ? y.stride(0) : pad8(y.size(1)); }
+
+struct Outputs {
+  Tensor out, pre;
+};
+
+Outputs forward_rows(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t activation,
+                     const Tensor& residual, bool keep_pre) {
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = weight.size(0);
+  Outputs o;
+  o.out = at::empty(shape, x.options().memory_format(at::MemoryFormat::Contiguous));
+  const Tensor xs = operand(x), ws = operand(weight);
+  const int64_t rows = xs.size(0);
+  if (keep_pre) o.pre = at::empty({rows, weight.size(0)}, x.options().memory_format(at::MemoryFormat::Contiguous));
+  if (rows == 0) return o;
+  const Tensor res = residual.defined() ? rows_of(residual) : Tensor();
+  rfm_linear a{};
+  a.x = xs.data_ptr();
+  a.weight = ws.data_ptr();
+  a.bias = data_or_null(bias);
+  a.residual = data_or_null(res);
+  a.out = o.out.data_ptr();
+  a.pre = data_or_null(o.pre);
+  a.rows = rows;
+  a.ld_x = operand_stride(xs);
+  a.ld_weight = operand_stride(ws);
+  a.ld_residual = res.defined() ? row_stride(res) : 0;
+  a.in_features = static_cast<int32_t>(weight.size(1));
+  a.out_features = static_cast<int32_t>(weight.size(0));
+  a.dtype = dtype_code(x.scalar_type());
+  a.bias_dtype = bias.defined() ? dtype_code(bias.scalar_type()) : a.dtype;
+  a.activation = static_cast<int32_t>(activation);
+  const int64_t size = rfm_linear_forward_workspace_bytes(rows, a.in_features, a.out_features);
+  Tensor work;
+  if (size > 0) {
+    work = at::empty({size}, x.options().dtype(at::kByte));
+    a.workspace = work.data_ptr();
+    a.workspace_bytes = size;
+  }
+  check_call("rfm_linear_forward", rfm_linear_forward(&a, current_stream(x.device())));
+  return o;
+}
+
+struct Linear : torch::autograd::Function<Linear> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const MaybeTensor& maybe_bias,
+                        int64_t activation, const MaybeTensor& maybe_residual) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    const Tensor bias = or_undefined(maybe_bias), residual = or_undefined(maybe_residual);
+    // relu's gradient only asks for the sign, which the output has where nothing was added to it
+    const bool from_out = activation == RFM_ACT_RELU && !residual.defined();
+    const Outputs o =
+        forward_rows(x, weight, bias, activation, residual, activation != RFM_ACT_NONE && !from_out);
+    ctx->save_for_backward({x, weight, from_out ? o.out : o.pre});
+    ctx->saved_data["activation"] = activation;
+    // places among the tensors given (-1: not given), which number the gradients asked for
+    ctx->saved_data["bias"] = static_cast<int64_t>(bias.defined() ? 2 : -1);
+    ctx->saved_data["residual"] = static_cast<int64_t>(residual.defined() ? (bias.defined() ? 3 : 2) : -1);
+    ctx->saved_data["bias_type"] = static_cast<int64_t>(bias.defined() ? bias.scalar_type() : x.scalar_type());
+    return o.out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    variable_list result(5);
+    if (!grads[0].defined()) return result;
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &weight = saved[1], &kept = saved[2];
+    const c10::cuda::CUDAGuard guard(x.device());
+    {
+      at::AutoGradMode off(false);
+      const int64_t at_bias = ctx->saved_data["bias"].toInt(), at_res = ctx->saved_data["residual"].toInt();
+      const bool need_bias = at_bias > 0 && ctx->needs_input_grad(at_bias);
+      const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+      const Tensor dy = grads[0].scalar_type() == x.scalar_type() ? grads[0] : grads[0].to(x.scalar_type());
+      if (at_res > 0 && ctx->needs_input_grad(at_res)) result[4] = dy;
+      if (need_x || need_w || need_bias) {
+        const Tensor g = rows_of(dy);
+        const Tensor xs = need_w ? operand(x) : rows_of(x), ws = operand(weight);
+        const auto options = x.options().memory_format(at::MemoryFormat::Contiguous);
+        rfm_linear_grad a{};
+        a.rows = xs.size(0);
+        a.in_features = static_cast<int32_t>(weight.size(1));
+        a.out_features = static_cast<int32_t>(weight.size(0));
+        a.dtype = dtype_code(x.scalar_type());
+        a.activation = static_cast<int32_t>(ctx->saved_data["activation"].toInt());
+        const auto bias_type = static_cast<at::ScalarType>(ctx->saved_data["bias_type"].toInt());
+        a.bias_dtype = dtype_code(bias_type);
+        if (need_x) result[0] = at::empty(x.sizes(), options);
+        if (need_w) result[1] = at::empty(weight.sizes(), options);
+        if (need_bias) result[2] = at::empty({weight.size(0)}, options.dtype(bias_type));
+        a.x = xs.data_ptr();
+        a.weight = ws.data_ptr();
+        a.saved = data_or_null(kept);
+        a.grad_out = g.data_ptr();
+        a.ld_x = operand_stride(xs);
+        a.ld_weight = operand_stride(ws);
+        a.ld_grad = operand_stride(g);
+        a.grad_x = data_or_null(result[0]);
+        a.grad_weight = data_or_null(result[1]);
+        a.grad_bias = data_or_null(result[2]);
+        Tensor dp, work;
+        if ((need_x || need_w) && a.rows > 0 && (a.activation != RFM_ACT_NONE || !tma_rows(g))) {
+          a.ld_grad_pre = pad8(weight.size(0));
+          dp = at::empty({a.rows, a.ld_grad_pre}, options);
+          a.grad_pre = dp.data_ptr();
+        }
+        const int64_t size = rfm_linear_backward_workspace_bytes(a.rows, a.in_features, a.out_features);
+        if (size > 0) {
+          work = at::empty({size}, options.dtype(at::kByte));
+          a.workspace = work.data_ptr();
+          a.workspace_bytes = size;
+        }
+        check_call("rfm_linear_backward", rfm_linear_backward(&a, current_stream(x.device())));
+      }
+    }
+    return once(std::move(result), "linear");
+  }
+};
+
+// Under autocast the operands take its type, as torch's own linear does.
+Tensor lowered(const Tensor& t, at::ScalarType type) {
+  return t.defined() && t.is_floating_point() && t.scalar_type() != at::kDouble && t.scalar_type() != type
+             ? t.to(type)
+             : t;
+}
+
+}  // namespace
+
+Tensor linear(const Tensor& x_in, const Tensor& weight_in, const MaybeTensor& maybe_bias, int64_t activation,
+              const MaybeTensor& maybe_residual) {
+  Tensor x = x_in, weight = weight_in, bias = or_undefined(maybe_bias), residual = or_undefined(maybe_residual);
+  RFM_REQUIRE(x.is_cuda(), "x must be a CUDA tensor (linear has no CPU path)");
+  RFM_REQUIRE(activation >= RFM_ACT_NONE && activation <= RFM_ACT_GELU, "unknown activation ", activation);
+  RFM_REQUIRE(weight.dim() == 2 && weight.device() == x.device(), "weight must be a matrix on x's device");
+  const int64_t in = weight.size(1), out = weight.size(0);
+  RFM_REQUIRE(in >= 1 && out >= 1 && in <= (1 << 30) && out <= (1 << 30),
+              "weight must have at least one row and one column");
+  RFM_REQUIRE(x.dim() >= 1 && x.size(-1) == in, "x must end in a dimension of ", in, " like weight's rows, got ",
+              x.sizes());
+  if (at::autocast::is_autocast_enabled(at::kCUDA)) {
+    const at::ScalarType type = at::autocast::get_autocast_dtype(at::kCUDA);
+    x = lowered(x, type);
+    weight = lowered(weight, type);
+    residual = lowered(residual, type);
+    if (bias.defined() && bias.scalar_type() != at::kFloat) bias = lowered(bias, type);
+  }
+  RFM_REQUIRE(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf,
+              "x must be bfloat16 or float16 (the tensor cores' types), got ", x.scalar_type());
+  RFM_REQUIRE(weight.scalar_type() == x.scalar_type(), "weight must have x's type, got ", weight.scalar_type());
+  if (bias.defined()) {
+    RFM_REQUIRE(bias.device() == x.device() && bias.dim() == 1 && bias.size(0) == out, "bias must have shape [", out,
+                "] on x's device");
+    RFM_REQUIRE(bias.scalar_type() == x.scalar_type() || bias.scalar_type() == at::kFloat,
+                "bias must be float32 or of x's type, got ", bias.scalar_type());
+    if (!bias.is_contiguous()) bias = bias.contiguous();
+  }
+  if (residual.defined()) {
+    RFM_REQUIRE(residual.device() == x.device() && residual.scalar_type() == x.scalar_type(),
+                "residual must have x's type and device");
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = out;
+    RFM_REQUIRE(residual.sizes() == at::IntArrayRef(shape), "residual must have the output's shape ",
+                at::IntArrayRef(shape), ", got ", residual.sizes());
+  }
+  const c10::cuda::CUDAGuard guard(x.device());
+  if (at::GradMode::is_enabled() &&
+      (wants_grad(x) || wants_grad(weight) || wants_grad(bias) || wants_grad(residual))) {
+    return Linear::apply(x, weight, maybe(bias), activation, maybe(residual));
+  }
+  return forward_rows(x, weight, bias, activation, residual, false).out;
+}
+
+}  // namespace rfm_host

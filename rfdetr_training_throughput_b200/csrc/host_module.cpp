@@ -13,6 +13,7 @@ PYBIND11_MODULE(_host, m) {
   namespace py = pybind11;
   const auto release = py::call_guard<py::gil_scoped_release>();
   m.def("layer_norm", &rfm_host::layer_norm, release);
+  m.def("linear", &rfm_host::linear, release);
   m.def("adamw_step", &rfm_host::adamw_step, release);
   m.def("dequantize_moments", &rfm_host::dequantize_moments, release);
 }

@@ -5,7 +5,7 @@ namespace rfm_host {
 namespace {
 
 struct Outputs {
-  Tensor out, rows, stats;
+  Tensor out, stats;
 };
 
 int param_code(const Tensor& x, const Tensor& weight, const Tensor& bias) {
@@ -15,14 +15,14 @@ int param_code(const Tensor& x, const Tensor& weight, const Tensor& bias) {
 
 Outputs forward_rows(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps, bool stats) {
   Outputs o;
-  o.rows = rows_of(x);
-  const int64_t n = o.rows.size(0), dim = o.rows.size(1);
+  const Tensor rows = rows_of(x);
+  const int64_t n = rows.size(0), dim = rows.size(1);
   o.out = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
   if (stats) o.stats = at::empty({2, n}, x.options().dtype(at::kFloat));
   if (n > 0) {
     float* mean = stats ? o.stats.data_ptr<float>() : nullptr;
     check_call("rfm_layer_norm_forward",
-               rfm_layer_norm_forward(o.rows.data_ptr(), row_stride(o.rows), data_or_null(weight), data_or_null(bias),
+               rfm_layer_norm_forward(rows.data_ptr(), row_stride(rows), data_or_null(weight), data_or_null(bias),
                                       o.out.data_ptr(), mean, stats ? mean + n : nullptr, n, static_cast<int>(dim),
                                       static_cast<float>(eps), dtype_code(x.scalar_type()),
                                       param_code(x, weight, bias), current_stream(x.device())));
@@ -36,8 +36,8 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const Tensor weight = or_undefined(maybe_weight), bias = or_undefined(maybe_bias);
     at::AutoDispatchBelowADInplaceOrView guard;
     Outputs o = forward_rows(x, weight, bias, eps, true);
-    ctx->save_for_backward({o.rows, weight, o.stats});
-    ctx->saved_data["shape"] = x.sizes().vec();
+    // x itself, not a view made here: only it shares the version that an in-place change advances
+    ctx->save_for_backward({x, weight, o.stats});
     ctx->saved_data["param"] = static_cast<int64_t>(param_code(x, weight, bias));
     // places among the tensors given (-1: not given), which number the gradients asked for
     ctx->saved_data["weight"] = static_cast<int64_t>(weight.defined() ? 1 : -1);
@@ -47,19 +47,20 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &rows = saved[0], &weight = saved[1], &stats = saved[2];
+    const Tensor &x = saved[0], &weight = saved[1], &stats = saved[2];
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
-    const c10::cuda::CUDAGuard guard(rows.device());
+    const c10::cuda::CUDAGuard guard(x.device());
     variable_list result(4);
     {
       at::AutoGradMode off(false);
+      const Tensor rows = rows_of(x);
       const int64_t n = rows.size(0), dim = rows.size(1);
       const int64_t param = ctx->saved_data["param"].toInt();
       const auto kind = param == RFM_DTYPE_F32 ? at::kFloat : param == RFM_DTYPE_BF16 ? at::kBFloat16 : at::kHalf;
       const Tensor g = rows_of(grads[0].scalar_type() == rows.scalar_type() ? grads[0]
                                                                             : grads[0].to(rows.scalar_type()));
       if (ctx->needs_input_grad(0)) {
-        result[0] = at::empty(ctx->saved_data["shape"].toIntVector(), rows.options());
+        result[0] = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
       }
       const int64_t at_w = ctx->saved_data["weight"].toInt(), at_b = ctx->saved_data["bias"].toInt();
       if (at_w > 0 && ctx->needs_input_grad(at_w)) result[1] = at::empty({dim}, rows.options().dtype(kind));
@@ -105,8 +106,7 @@ Tensor layer_norm(const Tensor& x, const MaybeTensor& maybe_weight, const MaybeT
   if (bias.defined() && !bias.is_contiguous()) bias = bias.contiguous();
   const c10::cuda::CUDAGuard guard(x.device());
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias))) {
-    return LayerNorm::apply(x, weight.defined() ? MaybeTensor(weight) : MaybeTensor(),
-                            bias.defined() ? MaybeTensor(bias) : MaybeTensor(), eps);
+    return LayerNorm::apply(x, maybe(weight), maybe(bias), eps);
   }
   return forward_rows(x, weight, bias, eps, false).out;
 }

@@ -1,0 +1,970 @@
+// The layers' matrix products on the 5th-generation tensor cores, bf16 and fp16.
+//
+//   forward     out = act(x W^T + bias) + residual        [rows, out]
+//   backward    dP = dY act'(pre),  dX = dP W,  dW = dP^T X,  dbias = sum_rows dP
+//
+// One kernel computes D[M, N] = sum_k A[m, k] B[n, k] for all three products;
+// they differ in which dimension of an operand is contiguous in memory: k for
+// both (forward), k for A and n for B (dX), m and n (dW).  TMA reads all of them
+// as stored, so nothing is transposed.
+//
+// Structure.  A persistent CTA of ten warps walks 128 x BN tiles: one thread
+// issues the TMA loads of 64-deep operand slices into a ring of stages, one
+// issues tcgen05.mma (fp32 accumulators in tensor memory, two of them, so that a
+// tile's products overlap the previous tile's epilogue), and eight warps read the
+// accumulators back (a warp can only read its own quarter of the lanes, so two
+// warps share a quarter, each half of the columns), apply bias, activation and
+// residual in fp32, round once and store 32 x 32 boxes through shared memory by
+// TMA.  The residual is fetched by TMA into the box it is added in, one box ahead.
+//
+// Few tiles leave SMs idle while the contraction is long (dW: a layer's weight
+// is a handful of tiles over tens of thousands of rows; one row against a wide
+// layer): the contraction is then split, each part leaves fp32 sums in the
+// workspace, and a second kernel adds the parts in their order and applies the
+// epilogue.  No atomics: the same bits on every run.
+//
+// Every wait on a barrier is bounded.  One that runs out marks the call as
+// failed (rfm_linear_faults) and every role leaves its loop.
+#include <math.h>
+
+#include <type_traits>
+
+#include "rfm_tcgen05.cuh"
+#include "rfm_types.cuh"
+
+namespace rfm {
+namespace {
+
+constexpr int kBM = 128;
+constexpr int kBK = 64;  // one 128-byte row of 16-bit elements
+constexpr int kEpiWarps = 8;
+constexpr int kLoadWarp = kEpiWarps;
+constexpr int kMmaWarp = kEpiWarps + 1;
+constexpr int kGemmThreads = 32 * (kEpiWarps + 2);
+constexpr int kBoxBytes = 32 * 64;  // 32 rows of 32 16-bit elements
+constexpr int kMaxSplits = 32;
+constexpr uint32_t kWaitTries = 1u << 22;
+
+__device__ int g_linear_faults = 0;
+
+template <int BN>
+struct Shape {
+  static constexpr int kABytes = kBM * kBK * 2;
+  static constexpr int kBBytes = BN * kBK * 2;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = 196608 / kStageBytes;  // 4, 6, 8
+  static constexpr int kBoxes = kStages * kStageBytes;
+  static constexpr int kBias = kBoxes + kEpiWarps * 2 * kBoxBytes;
+  static constexpr int kBars = kBias + kEpiWarps * 32 * 4;
+  // full and empty per stage, full and empty per accumulator, residual per warp and box
+  static constexpr int kNumBars = 2 * kStages + 4 + 2 * kEpiWarps;
+  static constexpr int kBytes = kBars + kNumBars * 8 + 16 + 1024;  // and room to align the base
+};
+static_assert(Shape<256>::kBytes <= 232448 && Shape<64>::kBytes <= 232448, "shared memory of one CTA");
+
+struct GemmArgs {
+  int64_t m;
+  int32_t n;
+  int32_t tiles_m, tiles_n;
+  int32_t k_blocks;       // of the whole contraction
+  int32_t splits;
+  int32_t activation;
+  int32_t bias_dtype;
+  int32_t tma_out, tma_res;
+  const void* bias;
+  const void* residual;   // null: none
+  int64_t ld_res;
+  void* out;              // [m, n], contiguous
+  void* pre;              // null: not kept
+  float* partial;         // splits > 1: [splits][m][n]
+};
+
+struct GemmMaps {
+  CUtensorMap a, b, out, pre, res;
+};
+
+__device__ __forceinline__ float activate(float v, int act) {
+  if (act == RFM_ACT_RELU) return v < 0.f ? 0.f : v;  // a NaN stays one
+  if (act == RFM_ACT_GELU) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+  return v;
+}
+
+// act'(v): 0 at relu's border; gelu: cdf(v) + v pdf(v).
+__device__ __forceinline__ float activate_grad(float v, int act) {
+  if (act == RFM_ACT_RELU) return v > 0.f ? 1.f : 0.f;
+  if (act == RFM_ACT_GELU) {
+    return fmaf(0.5f, erff(v * 0.70710678118654752f), 0.5f) + v * 0.39894228040143268f * expf(-0.5f * v * v);
+  }
+  return 1.f;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return reinterpret_cast<const uint32_t&>(v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return reinterpret_cast<const uint32_t&>(v);
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t v);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
+  return __bfloat1622float2(reinterpret_cast<const __nv_bfloat162&>(v));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
+  return __half22float2(reinterpret_cast<const __half2&>(v));
+}
+
+// A wait that gives up after kWaitTries polls (each of which the hardware
+// suspends for a while), or as soon as another role has given up.
+__device__ __forceinline__ bool bounded_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
+  for (uint32_t i = 0; i < kWaitTries; ++i) {
+    if (mbar_try(bar, parity)) return true;
+    if ((i & 255u) == 255u && *dead) return false;
+  }
+  *dead = 1;
+  atomicExch(&g_linear_faults, 1);
+  return false;
+}
+
+// Work item `w` of the grid: a part of the contraction of one tile.  Tiles run
+// down 16 rows of tiles before the next column, so that a wave's operands
+// overlap in L2.
+struct Work {
+  int tile_m, tile_n, split, k0, k1;
+};
+
+__device__ __forceinline__ Work work_item(const GemmArgs& a, int64_t w) {
+  Work r;
+  r.split = static_cast<int>(w % a.splits);
+  const int64_t tile = w / a.splits;
+  constexpr int kGroup = 16;
+  const int64_t per_group = static_cast<int64_t>(kGroup) * a.tiles_n;
+  const int group = static_cast<int>(tile / per_group);
+  const int inside = static_cast<int>(tile % per_group);
+  const int height = min(kGroup, a.tiles_m - group * kGroup);
+  r.tile_m = group * kGroup + inside % height;
+  r.tile_n = inside / height;
+  r.k0 = static_cast<int>(static_cast<int64_t>(a.k_blocks) * r.split / a.splits);
+  r.k1 = static_cast<int>(static_cast<int64_t>(a.k_blocks) * (r.split + 1) / a.splits);
+  return r;
+}
+
+template <typename T, int BN, bool A_MN, bool B_MN>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+    gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ GemmArgs a) {
+  using S = Shape<BN>;
+  extern __shared__ uint8_t raw_smem[];
+  __shared__ volatile int dead;
+  __shared__ uint32_t tmem_base;
+  const uint32_t base = (smem_u32(raw_smem) + 1023u) & ~1023u;
+  uint8_t* smem = raw_smem + (base - smem_u32(raw_smem));
+  const uint32_t bars = base + S::kBars;
+  const uint32_t full = bars, empty = bars + 8 * S::kStages;
+  const uint32_t acc_full = empty + 8 * S::kStages, acc_empty = acc_full + 16, res_full = acc_empty + 16;
+  const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
+  constexpr uint32_t kTmemColumns = 2 * BN;
+
+  if (threadIdx.x == 0) {
+    dead = 0;
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(acc_full + 8 * i, 1);
+      mbar_init(acc_empty + 8 * i, kEpiWarps);
+    }
+    for (int i = 0; i < 2 * kEpiWarps; ++i) mbar_init(res_full + 8 * i, 1);
+    mbar_init_fence();
+    tma_prefetch_map(&maps.a);
+    tma_prefetch_map(&maps.b);
+  }
+  if (warp == kMmaWarp) tmem_alloc(smem_u32(&tmem_base), kTmemColumns);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base;
+  const int64_t items = static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.splits;
+
+  if (warp == kLoadWarp) {
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0, issued = 0;
+      bool ok = true;
+      for (int64_t w = blockIdx.x; ok && w < items; w += gridDim.x) {
+        const Work t = work_item(a, w);
+        const int m0 = t.tile_m * kBM, n0 = t.tile_n * BN;
+        for (int kb = t.k0; kb < t.k1; ++kb) {
+          if (!bounded_wait(empty + 8 * stage, phase ^ 1u, &dead)) {
+            ok = false;
+            break;
+          }
+          const uint32_t bar = full + 8 * stage;
+          const uint32_t sa = base + stage * S::kStageBytes, sb = sa + S::kABytes;
+          mbar_expect(bar, S::kStageBytes);
+          if (A_MN) {
+#pragma unroll
+            for (int j = 0; j < kBM / 64; ++j) tma_load_2d(sa + j * 8192, &maps.a, m0 + j * 64, kb * kBK, bar);
+          } else {
+            tma_load_2d(sa, &maps.a, kb * kBK, m0, bar);
+          }
+          if (B_MN) {
+#pragma unroll
+            for (int j = 0; j < BN / 64; ++j) tma_load_2d(sb + j * 8192, &maps.b, n0 + j * 64, kb * kBK, bar);
+          } else {
+            tma_load_2d(sb, &maps.b, kb * kBK, n0, bar);
+          }
+          if (issued < S::kStages) ++issued;
+          if (++stage == S::kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok) {
+        // the copies in flight land before the CTA's shared memory is given up
+        for (uint32_t i = 0; i < issued; ++i) {
+          if (stage == 0) {
+            stage = S::kStages;
+            phase ^= 1u;
+          }
+          --stage;
+          for (uint32_t k = 0; k < kWaitTries && !mbar_try(full + 8 * stage, phase); ++k) {
+          }
+        }
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    if (lane == 0) {
+      constexpr int kType = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+      constexpr uint32_t kInstr = mma_instr(kType, A_MN, B_MN, kBM, BN);
+      constexpr uint32_t kAStep = A_MN ? 2048 : 32, kBStep = B_MN ? 2048 : 32;  // bytes of 16 along k
+      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+      bool ok = true;
+      for (int64_t w = blockIdx.x; ok && w < items; w += gridDim.x) {
+        const Work t = work_item(a, w);
+        if (!bounded_wait(acc_empty + 8 * acc, acc_phase ^ 1u, &dead)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + acc * BN;
+        for (int kb = t.k0; kb < t.k1; ++kb) {
+          if (!bounded_wait(full + 8 * stage, phase, &dead)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = base + stage * S::kStageBytes, sb = sa + S::kABytes;
+#pragma unroll
+          for (int k = 0; k < kBK / 16; ++k) {
+            tc_mma_f16(d, operand_desc(sa + k * kAStep, A_MN ? 8192 : 16, 1024),
+                       operand_desc(sb + k * kBStep, B_MN ? 8192 : 16, 1024), kInstr, kb > t.k0 || k > 0);
+          }
+          tc_commit(empty + 8 * stage);
+          if (++stage == S::kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        tc_commit(acc_full + 8 * acc);
+        acc ^= 1u;
+        if (acc == 0) acc_phase ^= 1u;
+      }
+      // The products in flight end before the tensor memory is given up: the
+      // epilogue waits for the last accumulator's barrier, and a role that gave
+      // up waits here.
+      if (dead) {
+        tc_commit(acc_full + 8 * acc);
+        for (uint32_t k = 0; k < kWaitTries && !mbar_try(acc_full + 8 * acc, acc_phase); ++k) {
+        }
+      }
+    }
+  } else {
+    constexpr int kHalf = BN / 2;
+    constexpr int kChunks = kHalf / 32;
+    const int quarter = warp & 3, half = warp >> 2;
+    const uint32_t boxes = base + S::kBoxes + warp * 2 * kBoxBytes;
+    uint8_t* box_ptr = smem + S::kBoxes + warp * 2 * kBoxBytes;
+    float* bias_smem = reinterpret_cast<float*>(smem + S::kBias) + warp * 32;
+    const uint32_t res_bar = res_full + 16 * warp;
+    const bool whole = a.splits == 1;
+    const bool has_res = whole && a.residual != nullptr, has_pre = whole && a.pre != nullptr;
+    const bool tma_res = has_res && a.tma_res;
+    uint32_t acc = 0, acc_phase = 0, box = 0, res_phase = 0;
+    // where a lane's 16-byte pieces of its row go in a box (64-byte swizzle)
+    const int row_off = lane * 64, swz = (lane >> 1) & 3;
+
+    for (int64_t w = blockIdx.x; w < items; w += gridDim.x) {
+      const Work t = work_item(a, w);
+      const int64_t row0 = static_cast<int64_t>(t.tile_m) * kBM + quarter * 32;
+      const int col_base = t.tile_n * BN + half * kHalf;
+      bool live = true;
+      for (int c = 0; c < kChunks; ++c) {
+        const int col0 = col_base + c * 32;
+        const bool inside = row0 < a.m && col0 < a.n;
+        // the box this chunk goes through: alternating, or the first beside `pre`'s
+        const uint32_t b = has_pre ? 0u : box;
+        if (inside && tma_res) {
+          if (lane == 0) {
+            tma_wait_read<0>();
+            proxy_fence();
+            mbar_expect(res_bar + 8 * b, kBoxBytes);
+            tma_load_2d(boxes + b * kBoxBytes, &maps.res, col0, static_cast<int>(row0), res_bar + 8 * b);
+          }
+          __syncwarp();
+        }
+        if (inside && whole && a.bias != nullptr) {
+          __syncwarp();
+          bias_smem[lane] = col0 + lane < a.n ? load_param(a.bias, a.bias_dtype, col0 + lane) : 0.f;
+          __syncwarp();
+        }
+        if (c == 0) {
+          live = __all_sync(kFullMask, bounded_wait(acc_full + 8 * acc, acc_phase, &dead));
+          tc_fence_after();
+        }
+        uint32_t v[32];
+        tmem_load_32(v, tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * BN + half * kHalf + c * 32);
+        if (c == kChunks - 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(acc_empty + 8 * acc);
+        }
+        if (!inside) continue;
+        if (!whole) {
+          const int64_t row = row0 + lane;
+          if (row < a.m && live) {
+            float* dst = a.partial + (static_cast<int64_t>(t.split) * a.m + row) * a.n + col0;
+            if ((a.n & 3) == 0 && col0 + 32 <= a.n) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                reinterpret_cast<uint4*>(dst)[j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (col0 + j < a.n) dst[j] = __uint_as_float(v[j]);
+            }
+          }
+          continue;
+        }
+        float f[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
+        if (a.bias != nullptr) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float4 q = reinterpret_cast<const float4*>(bias_smem)[j];
+            f[4 * j] += q.x;
+            f[4 * j + 1] += q.y;
+            f[4 * j + 2] += q.z;
+            f[4 * j + 3] += q.w;
+          }
+        }
+        if (!tma_res) {
+          // the box's last store must have been read before it is overwritten
+          if (lane == 0) {
+            if (has_pre) {
+              tma_wait_read<0>();
+            } else {
+              tma_wait_read<1>();
+            }
+          }
+          __syncwarp();
+        }
+        if (has_pre) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            *reinterpret_cast<uint4*>(box_ptr + kBoxBytes + row_off + ((j ^ swz) << 4)) =
+                make_uint4(pack2<T>(f[8 * j], f[8 * j + 1]), pack2<T>(f[8 * j + 2], f[8 * j + 3]),
+                           pack2<T>(f[8 * j + 4], f[8 * j + 5]), pack2<T>(f[8 * j + 6], f[8 * j + 7]));
+          }
+        }
+        if (a.activation != RFM_ACT_NONE) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) f[j] = activate(f[j], a.activation);
+        }
+        if (has_res) {
+          if (tma_res) {
+            live = __all_sync(kFullMask, bounded_wait(res_bar + 8 * b, (res_phase >> b) & 1u, &dead) && live);
+            res_phase ^= 1u << b;
+          } else {
+            // rows whose start is not a multiple of 16 bytes: element by element, a lane a column
+            T* cells = reinterpret_cast<T*>(box_ptr + b * kBoxBytes);
+            const T* res = static_cast<const T*>(a.residual);
+            for (int r = 0; r < 32; ++r) {
+              const int64_t row = row0 + r;
+              const int at = r * 32 + (((lane >> 3) ^ ((r >> 1) & 3)) << 3) + (lane & 7);
+              cells[at] = row < a.m && col0 + lane < a.n ? res[row * a.ld_res + col0 + lane] : from_float<T>(0.f);
+            }
+            __syncwarp();
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint4 q =
+                *reinterpret_cast<const uint4*>(box_ptr + b * kBoxBytes + row_off + ((j ^ swz) << 4));
+            const uint32_t words[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 two = unpack2<T>(words[i]);
+              f[8 * j + 2 * i] += two.x;
+              f[8 * j + 2 * i + 1] += two.y;
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          *reinterpret_cast<uint4*>(box_ptr + b * kBoxBytes + row_off + ((j ^ swz) << 4)) =
+              make_uint4(pack2<T>(f[8 * j], f[8 * j + 1]), pack2<T>(f[8 * j + 2], f[8 * j + 3]),
+                         pack2<T>(f[8 * j + 4], f[8 * j + 5]), pack2<T>(f[8 * j + 6], f[8 * j + 7]));
+        }
+        if (a.tma_out) {
+          proxy_fence();
+          __syncwarp();
+          if (lane == 0 && live) {
+            tma_store_2d(&maps.out, col0, static_cast<int>(row0), boxes + b * kBoxBytes);
+            if (has_pre) tma_store_2d(&maps.pre, col0, static_cast<int>(row0), boxes + kBoxBytes);
+            tma_commit();
+          }
+        } else {
+          __syncwarp();
+          if (live) {
+            for (int r = 0; r < 32; ++r) {
+              const int64_t row = row0 + r;
+              if (row >= a.m || col0 + lane >= a.n) continue;
+              const int at = r * 32 + (((lane >> 3) ^ ((r >> 1) & 3)) << 3) + (lane & 7);
+              static_cast<T*>(a.out)[row * a.n + col0 + lane] =
+                  reinterpret_cast<const T*>(box_ptr + b * kBoxBytes)[at];
+              if (has_pre) {
+                static_cast<T*>(a.pre)[row * a.n + col0 + lane] =
+                    reinterpret_cast<const T*>(box_ptr + kBoxBytes)[at];
+              }
+            }
+          }
+          __syncwarp();
+        }
+        box ^= 1u;
+      }
+      if (!live) break;
+      acc ^= 1u;
+      if (acc == 0) acc_phase ^= 1u;
+    }
+    if (lane == 0) tma_wait_read<0>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_free(tmem, kTmemColumns);
+  }
+}
+
+// ---- the parts of a split contraction, added in their order, and the epilogue
+
+struct FinishArgs {
+  const float* partial;
+  const void* bias;
+  const void* residual;
+  void* out;
+  void* pre;
+  int64_t m;
+  int64_t ld_res;
+  int32_t n;
+  int32_t splits;
+  int32_t activation;
+  int32_t bias_dtype;
+};
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) finish_kernel(const FinishArgs a) {
+  const int64_t per_row = a.n / VEC;
+  const int64_t total = a.m * per_row;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = i / per_row;
+    const int col = static_cast<int>(i % per_row) * VEC;
+    float v[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+      const Pack<float, VEC> q =
+          *reinterpret_cast<const Pack<float, VEC>*>(a.partial + (static_cast<int64_t>(s) * a.m + row) * a.n + col);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[j] += q.v[j];
+    }
+    Pack<T, VEC> o;
+    if (a.bias != nullptr) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[j] += load_param(a.bias, a.bias_dtype, col + j);
+    }
+    if (a.pre != nullptr) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) o.v[j] = from_float<T>(v[j]);
+      *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.pre) + row * a.n + col) = o;
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      float x = activate(v[j], a.activation);
+      if (a.residual != nullptr) x += to_float(static_cast<const T*>(a.residual)[row * a.ld_res + col + j]);
+      o.v[j] = from_float<T>(x);
+    }
+    *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.out) + row * a.n + col) = o;
+  }
+}
+
+// ---- dP = dY act'(saved) and its column sums
+
+struct GradPreArgs {
+  const void* dy;
+  const void* saved;  // pre, or (relu without a residual) out; null: no activation
+  void* dp;           // null: not stored
+  float* partial;     // [slabs][n] column sums, null: not wanted
+  int64_t rows;
+  int64_t ld_dy;
+  int64_t ld_dp;
+  int32_t n;
+  int32_t activation;
+};
+
+constexpr int kPreWarps = 8;
+
+// A CTA owns 32 * VEC columns and every gridDim.y-th group of 8 rows (a row a
+// warp); the sums of its warps are added in their order at the end.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(32 * kPreWarps) grad_pre_kernel(const GradPreArgs a) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col = (static_cast<int>(blockIdx.x) * 32 + lane) * VEC;
+  const bool in = col < a.n;
+  float sum[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
+  const int64_t stride = static_cast<int64_t>(gridDim.y) * kPreWarps;
+  if (in) {
+#pragma unroll 4
+    for (int64_t row = static_cast<int64_t>(blockIdx.y) * kPreWarps + warp; row < a.rows; row += stride) {
+      const Pack<T, VEC> g = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.dy) + row * a.ld_dy + col);
+      float v[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[j] = to_float(g.v[j]);
+      if (a.saved != nullptr) {
+        const Pack<T, VEC> p =
+            *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.saved) + row * a.n + col);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] *= activate_grad(to_float(p.v[j]), a.activation);
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) sum[j] += v[j];
+      if (a.dp != nullptr) {
+        Pack<T, VEC> o;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) o.v[j] = from_float<T>(v[j]);
+        *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.dp) + row * a.ld_dp + col) = o;
+      }
+    }
+  }
+  if (a.partial == nullptr) return;
+  __shared__ float sums[kPreWarps][32 * VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) sums[warp][j * 32 + lane] = sum[j];
+  __syncthreads();
+  if (warp == 0 && in) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      float s = sums[0][j * 32 + lane];
+#pragma unroll
+      for (int k = 1; k < kPreWarps; ++k) s += sums[k][j * 32 + lane];
+      a.partial[static_cast<int64_t>(blockIdx.y) * a.n + col + j] = s;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) bias_sum_kernel(const float* partial, int slabs, int n, void* out, int dtype) {
+  __shared__ float sums[8][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col = static_cast<int>(blockIdx.x) * 32 + lane;
+  float s = 0.f;
+  if (col < n) {
+#pragma unroll 4
+    for (int k = warp; k < slabs; k += 8) s += partial[static_cast<int64_t>(k) * n + col];
+  }
+  sums[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && col < n) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += sums[k][lane];
+    store_param(out, dtype, col, s);
+  }
+}
+
+// ---- host side
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      return static_cast<EncodeTiled>(nullptr);
+    }
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+// A matrix of `outer` rows of `inner` elements, `ld` apart, moved in boxes of
+// box_inner x box_outer.
+bool make_map(CUtensorMap* map, int dtype, const void* p, int64_t inner, int64_t outer, int64_t ld, int box_inner,
+              int box_outer, CUtensorMapSwizzle swizzle) {
+  const EncodeTiled encode = encode_tiled();
+  if (encode == nullptr) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_inner), static_cast<cuuint32_t>(box_outer)};
+  const cuuint32_t ones[2] = {1, 1};
+  return encode(map, dtype == RFM_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                const_cast<void*>(p), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool tma_rows(const void* p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
+
+// How a product is cut: the tile's columns and the parts of the contraction.
+struct Cut {
+  int bn = 64;
+  int splits = 1;
+};
+
+// Estimated cycles of the busiest SM for each cut.  A 64-deep slice of a
+// 128 x BN tile takes the tensor cores 2 BN cycles and brings (128 + BN) * 128
+// bytes, which an SM takes in at about 80 a cycle; a tile's epilogue, hidden
+// behind the next tile's products but for the last, 11 cycles a column (measured
+// range: 8 to 14); a part's fp32 sums are written and read once, and the second
+// kernel costs about 5000 cycles.
+Cut choose_cut(int64_t m, int n, int k_blocks) {
+  const int sms = device_sm_count();
+  Cut best;
+  double least = 1e30;
+  for (int bn = 256; bn >= 64; bn /= 2) {
+    const int64_t tiles = ((m + kBM - 1) / kBM) * ((n + bn - 1) / bn);
+    const double slice = fmax(2.0 * bn, (128.0 + bn) * 128.0 / 80.0);
+    for (int splits = 1; splits <= kMaxSplits && splits <= k_blocks; ++splits) {
+      if (splits > 1 && (k_blocks / splits < 2 || tiles * (splits - 1) >= 4 * sms)) break;
+      const int64_t waves = (tiles * splits + sms - 1) / sms;
+      const double depth = static_cast<double>((k_blocks + splits - 1) / splits);
+      const double epilogue = 11.0 * bn;
+      double cycles = 1500.0 + waves * fmax(depth * slice, epilogue) + epilogue;
+      if (splits > 1) {
+        cycles += 5000.0 + 8.0 * splits * static_cast<double>(m) * n / 3000.0;  // about 3 KB a cycle to L2
+      }
+      if (cycles < least) {
+        least = cycles;
+        best.bn = bn;
+        best.splits = splits;
+      }
+    }
+  }
+  return best;
+}
+
+struct Product {
+  const void* a;
+  const void* b;
+  int64_t ld_a, ld_b;
+  int64_t m;
+  int n;
+  int64_t k;
+  int dtype;
+  GemmArgs args;  // epilogue fields filled in by the caller
+};
+
+template <typename T, int BN, bool A_MN, bool B_MN>
+int launch_gemm(const Product& p, GemmArgs& g, float* partial, cudaStream_t stream) {
+  using S = Shape<BN>;
+  GemmMaps maps;
+  const bool ok_a = A_MN ? make_map(&maps.a, p.dtype, p.a, p.m, p.k, p.ld_a, 64, kBK, CU_TENSOR_MAP_SWIZZLE_128B)
+                         : make_map(&maps.a, p.dtype, p.a, p.k, p.m, p.ld_a, kBK, kBM, CU_TENSOR_MAP_SWIZZLE_128B);
+  const bool ok_b = B_MN ? make_map(&maps.b, p.dtype, p.b, p.n, p.k, p.ld_b, 64, kBK, CU_TENSOR_MAP_SWIZZLE_128B)
+                         : make_map(&maps.b, p.dtype, p.b, p.k, p.n, p.ld_b, kBK, BN, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (!ok_a || !ok_b) return RFM_ERR_LAUNCH;
+  g.tiles_m = static_cast<int>((p.m + kBM - 1) / kBM);
+  g.tiles_n = (p.n + BN - 1) / BN;
+  g.partial = partial;
+  g.tma_out = g.splits == 1 && tma_rows(g.out, p.n) && (g.pre == nullptr || tma_rows(g.pre, p.n));
+  g.tma_res = g.splits == 1 && g.residual != nullptr && tma_rows(g.residual, g.ld_res);
+  maps.out = maps.pre = maps.res = maps.a;
+  if (g.tma_out) {
+    if (!make_map(&maps.out, p.dtype, g.out, p.n, p.m, p.n, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B)) return RFM_ERR_LAUNCH;
+    if (g.pre != nullptr &&
+        !make_map(&maps.pre, p.dtype, g.pre, p.n, p.m, p.n, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B)) {
+      return RFM_ERR_LAUNCH;
+    }
+  }
+  if (g.tma_res &&
+      !make_map(&maps.res, p.dtype, g.residual, p.n, p.m, g.ld_res, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B)) {
+    return RFM_ERR_LAUNCH;
+  }
+  static thread_local unsigned long long ready = 0;  // the context whose shared-memory limit is raised
+  const auto kernel = gemm_kernel<T, BN, A_MN, B_MN>;
+  const unsigned long long context = current_context_id();
+  if (ready != context || context == 0) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess) {
+      cudaGetLastError();
+      return RFM_ERR_LAUNCH;
+    }
+    ready = context;
+  }
+  const int64_t items = static_cast<int64_t>(g.tiles_m) * g.tiles_n * g.splits;
+  const int sms = device_sm_count();
+  kernel<<<static_cast<unsigned>(items < sms ? items : sms), kGemmThreads, S::kBytes, stream>>>(maps, g);
+  return launch_status();
+}
+
+template <typename T, bool A_MN, bool B_MN>
+int run_product(const Product& p, void* workspace, cudaStream_t stream) {
+  const Cut cut = choose_cut(p.m, p.n, static_cast<int>((p.k + kBK - 1) / kBK));
+  GemmArgs g = p.args;
+  g.m = p.m;
+  g.n = p.n;
+  g.k_blocks = static_cast<int>((p.k + kBK - 1) / kBK);
+  g.splits = cut.splits;
+  float* partial = static_cast<float*>(workspace);
+  int rc;
+  if (cut.bn == 256) {
+    rc = launch_gemm<T, 256, A_MN, B_MN>(p, g, partial, stream);
+  } else if (cut.bn == 128) {
+    rc = launch_gemm<T, 128, A_MN, B_MN>(p, g, partial, stream);
+  } else {
+    rc = launch_gemm<T, 64, A_MN, B_MN>(p, g, partial, stream);
+  }
+  if (rc != RFM_OK || cut.splits == 1) return rc;
+  FinishArgs f{partial, g.bias, g.residual, g.out, g.pre, p.m, g.ld_res, p.n, cut.splits, g.activation, g.bias_dtype};
+  const bool quads = p.n % 4 == 0 && (reinterpret_cast<uintptr_t>(g.out) & 7) == 0 &&
+                     (reinterpret_cast<uintptr_t>(g.pre) & 7) == 0;
+  const int64_t cells = p.m * (p.n / (quads ? 4 : 1));
+  const int64_t most = static_cast<int64_t>(device_sm_count()) * 8;
+  const int64_t ctas = (cells + 255) / 256;
+  const unsigned grid = static_cast<unsigned>(ctas < most ? ctas : most);
+  if (quads) {
+    finish_kernel<T, 4><<<grid, 256, 0, stream>>>(f);
+  } else {
+    finish_kernel<T, 1><<<grid, 256, 0, stream>>>(f);
+  }
+  return launch_status();
+}
+
+template <bool A_MN, bool B_MN>
+int run_typed(const Product& p, void* workspace, cudaStream_t stream) {
+  return p.dtype == RFM_DTYPE_BF16 ? run_product<__nv_bfloat16, A_MN, B_MN>(p, workspace, stream)
+                                   : run_product<__half, A_MN, B_MN>(p, workspace, stream);
+}
+
+// fp32 sums of a split product, 16-byte multiples.
+int64_t partial_bytes(int64_t m, int64_t n, int64_t k) {
+  if (m == 0) return 0;
+  const Cut cut = choose_cut(m, static_cast<int>(n), static_cast<int>((k + kBK - 1) / kBK));
+  return cut.splits == 1 ? 0 : ((cut.splits * m * n * 4 + 15) & ~int64_t(15));
+}
+
+// Row slabs of the bias sums: about eight CTAs an SM, no less than 32 rows each.
+int bias_slabs(int64_t rows, int n, int vec) {
+  const int64_t strips = (n + 32 * vec - 1) / (32 * vec);
+  const int64_t want = static_cast<int64_t>(device_sm_count()) * 8 / strips + 1;
+  const int64_t most = (rows + 31) / 32;
+  const int64_t slabs = want < most ? want : most;
+  return static_cast<int>(slabs < 1 ? 1 : (slabs > 4096 ? 4096 : slabs));
+}
+
+int check_sizes(int64_t rows, int in_features, int out_features, int dtype) {
+  if (rows < 0 || in_features < 1 || out_features < 1 || (dtype != RFM_DTYPE_BF16 && dtype != RFM_DTYPE_F16)) {
+    return RFM_ERR_INVALID_ARGUMENT;
+  }
+  // TMA coordinates are 32-bit
+  if (rows > (int64_t(1) << 31) - 512 || in_features > (1 << 30) || out_features > (1 << 30)) {
+    return RFM_ERR_UNSUPPORTED;
+  }
+  return RFM_OK;
+}
+
+bool operand_rows(const void* p, int64_t ld, int64_t rows, int64_t cols) {
+  return p != nullptr && tma_rows(p, ld) && (rows <= 1 || ld >= cols) && ld > 0 && ld < (int64_t(1) << 38);
+}
+
+}  // namespace
+}  // namespace rfm
+
+extern "C" int64_t rfm_linear_forward_workspace_bytes(int64_t rows, int in_features, int out_features) {
+  using namespace rfm;
+  const int rc = check_sizes(rows, in_features, out_features, RFM_DTYPE_BF16);
+  if (rc != RFM_OK) return -rc;
+  return partial_bytes(rows, out_features, in_features);
+}
+
+extern "C" int rfm_linear_forward(const rfm_linear* p, void* stream) {
+  using namespace rfm;
+  if (p == nullptr || p->reserved != 0) return RFM_ERR_INVALID_ARGUMENT;
+  const int rc = check_sizes(p->rows, p->in_features, p->out_features, p->dtype);
+  if (rc != RFM_OK) return rc;
+  if (p->activation < RFM_ACT_NONE || p->activation > RFM_ACT_GELU) return RFM_ERR_INVALID_ARGUMENT;
+  if (p->rows == 0) return RFM_OK;
+  const bool bias_ok = p->bias == nullptr || p->bias_dtype == p->dtype || p->bias_dtype == RFM_DTYPE_F32;
+  if (!operand_rows(p->x, p->ld_x, p->rows, p->in_features) ||
+      !operand_rows(p->weight, p->ld_weight, p->out_features, p->in_features) || p->out == nullptr || !bias_ok) {
+    return RFM_ERR_INVALID_ARGUMENT;
+  }
+  if (p->residual != nullptr && p->rows > 1 && p->ld_residual < p->out_features) return RFM_ERR_INVALID_ARGUMENT;
+  const int64_t need = partial_bytes(p->rows, p->out_features, p->in_features);
+  if (need > 0 && (p->workspace == nullptr || !aligned16(p->workspace) || p->workspace_bytes < need)) {
+    return RFM_ERR_INVALID_ARGUMENT;
+  }
+  Product g{};
+  g.a = p->x;
+  g.ld_a = p->ld_x;
+  g.b = p->weight;
+  g.ld_b = p->ld_weight;
+  g.m = p->rows;
+  g.n = p->out_features;
+  g.k = p->in_features;
+  g.dtype = p->dtype;
+  g.args.activation = p->activation;
+  g.args.bias = p->bias;
+  g.args.bias_dtype = p->bias_dtype;
+  g.args.residual = p->residual;
+  g.args.ld_res = p->ld_residual;
+  g.args.out = p->out;
+  g.args.pre = p->pre;
+  return run_typed<false, false>(g, p->workspace, as_stream(stream));
+}
+
+extern "C" int64_t rfm_linear_backward_workspace_bytes(int64_t rows, int in_features, int out_features) {
+  using namespace rfm;
+  const int rc = check_sizes(rows, in_features, out_features, RFM_DTYPE_BF16);
+  if (rc != RFM_OK) return -rc;
+  // the products run one after the other and share the space; the bias sums come first
+  int64_t most = partial_bytes(rows, in_features, out_features);
+  const int64_t dw = rows == 0 ? 0 : partial_bytes(out_features, in_features, rows);
+  most = dw > most ? dw : most;
+  const int64_t bias = (static_cast<int64_t>(bias_slabs(rows, out_features, 1)) * out_features * 4 + 15) & ~int64_t(15);
+  return bias > most ? bias : most;
+}
+
+extern "C" int rfm_linear_backward(const rfm_linear_grad* p, void* stream) {
+  using namespace rfm;
+  if (p == nullptr || p->reserved != 0) return RFM_ERR_INVALID_ARGUMENT;
+  const int rc = check_sizes(p->rows, p->in_features, p->out_features, p->dtype);
+  if (rc != RFM_OK) return rc;
+  if (p->activation < RFM_ACT_NONE || p->activation > RFM_ACT_GELU) return RFM_ERR_INVALID_ARGUMENT;
+  if (p->grad_x == nullptr && p->grad_weight == nullptr && p->grad_bias == nullptr) return RFM_OK;
+  const int64_t rows = p->rows;
+  const int in = p->in_features, out = p->out_features;
+  cudaStream_t s = as_stream(stream);
+  if (p->grad_bias != nullptr && p->bias_dtype != p->dtype && p->bias_dtype != RFM_DTYPE_F32) {
+    return RFM_ERR_INVALID_ARGUMENT;
+  }
+  if (rows == 0) {  // empty sums
+    if (p->grad_weight != nullptr &&
+        cudaMemsetAsync(p->grad_weight, 0, static_cast<size_t>(in) * out * 2, s) != cudaSuccess) {
+      cudaGetLastError();
+      return RFM_ERR_LAUNCH;
+    }
+    if (p->grad_bias != nullptr) {
+      bias_sum_kernel<<<(out + 31) / 32, 256, 0, s>>>(nullptr, 0, out, p->grad_bias, p->bias_dtype);
+    }
+    return launch_status();
+  }
+  const bool acts = p->activation != RFM_ACT_NONE;
+  if (p->grad_out == nullptr || (rows > 1 && p->ld_grad < out) || (acts && p->saved == nullptr)) {
+    return RFM_ERR_INVALID_ARGUMENT;
+  }
+  const bool products = p->grad_x != nullptr || p->grad_weight != nullptr;
+  // dP is dY itself without an activation, where TMA can read it
+  const bool own = products && (acts || !tma_rows(p->grad_out, p->ld_grad));
+  if (own && !operand_rows(p->grad_pre, p->ld_grad_pre, rows, out)) return RFM_ERR_INVALID_ARGUMENT;
+  if (p->grad_x != nullptr && !operand_rows(p->weight, p->ld_weight, out, in)) return RFM_ERR_INVALID_ARGUMENT;
+  if (p->grad_weight != nullptr && !operand_rows(p->x, p->ld_x, rows, in)) return RFM_ERR_INVALID_ARGUMENT;
+  const int64_t need = rfm_linear_backward_workspace_bytes(rows, in, out);
+  if (need > 0 && (p->workspace == nullptr || !aligned16(p->workspace) || p->workspace_bytes < need)) {
+    return RFM_ERR_INVALID_ARGUMENT;
+  }
+
+  if (own || p->grad_bias != nullptr) {
+    GradPreArgs a{};
+    a.dy = p->grad_out;
+    a.ld_dy = rows > 1 ? p->ld_grad : out;
+    a.saved = acts ? p->saved : nullptr;
+    a.dp = own ? p->grad_pre : nullptr;
+    a.ld_dp = p->ld_grad_pre;
+    a.partial = p->grad_bias != nullptr ? static_cast<float*>(p->workspace) : nullptr;
+    a.rows = rows;
+    a.n = out;
+    a.activation = p->activation;
+    const bool vec = out % 8 == 0 && a.ld_dy % 8 == 0 && aligned16(a.dy) && aligned16(a.saved);
+    const int width = 32 * (vec ? 8 : 1);
+    const int slabs = bias_slabs(rows, out, vec ? 8 : 1);
+    const dim3 grid((out + width - 1) / width, slabs);
+    if (p->dtype == RFM_DTYPE_BF16) {
+      if (vec) {
+        grad_pre_kernel<__nv_bfloat16, 8><<<grid, 256, 0, s>>>(a);
+      } else {
+        grad_pre_kernel<__nv_bfloat16, 1><<<grid, 256, 0, s>>>(a);
+      }
+    } else if (vec) {
+      grad_pre_kernel<__half, 8><<<grid, 256, 0, s>>>(a);
+    } else {
+      grad_pre_kernel<__half, 1><<<grid, 256, 0, s>>>(a);
+    }
+    int done = launch_status();
+    if (done != RFM_OK) return done;
+    if (p->grad_bias != nullptr) {
+      bias_sum_kernel<<<(out + 31) / 32, 256, 0, s>>>(a.partial, slabs, out, p->grad_bias, p->bias_dtype);
+      done = launch_status();
+      if (done != RFM_OK) return done;
+    }
+  }
+  const void* dp = own ? p->grad_pre : p->grad_out;
+  const int64_t ld_dp = own ? p->ld_grad_pre : p->ld_grad;
+  if (p->grad_x != nullptr) {
+    Product g{};
+    g.a = dp;
+    g.ld_a = ld_dp;
+    g.b = p->weight;
+    g.ld_b = p->ld_weight;
+    g.m = rows;
+    g.n = in;
+    g.k = out;
+    g.dtype = p->dtype;
+    g.args.out = p->grad_x;
+    const int done = run_typed<false, true>(g, p->workspace, s);
+    if (done != RFM_OK) return done;
+  }
+  if (p->grad_weight != nullptr) {
+    Product g{};
+    g.a = dp;
+    g.ld_a = ld_dp;
+    g.b = p->x;
+    g.ld_b = p->ld_x;
+    g.m = out;
+    g.n = in;
+    g.k = rows;
+    g.dtype = p->dtype;
+    g.args.out = p->grad_weight;
+    return run_typed<true, true>(g, p->workspace, s);
+  }
+  return RFM_OK;
+}
+
+extern "C" int rfm_linear_faults(int* faults) {
+  using namespace rfm;
+  if (faults == nullptr) return RFM_ERR_INVALID_ARGUMENT;
+  const cudaError_t err = cudaMemcpyFromSymbol(faults, g_linear_faults, sizeof(int));
+  if (err == cudaSuccess) return RFM_OK;
+  const int rc = launch_status();
+  return rc == RFM_OK ? RFM_ERR_LAUNCH : rc;
+}

@@ -75,7 +75,7 @@ __device__ __forceinline__ float2 team_sum(float2 s, float2 (*slots)[kMostWarps]
     s.x += __shfl_xor_sync(kFullMask, s.x, o);
     s.y += __shfl_xor_sync(kFullMask, s.y, o);
   }
-  if (TEAM > 32) {
+  if constexpr (TEAM > 32) {
     if ((threadIdx.x & 31) == 0) slots[parity][threadIdx.x >> 5] = s;
     __syncthreads();
     s = slots[parity][0];

@@ -1,0 +1,45 @@
+"""A layer's matrix product with its epilogue, forward and backward, on the tensor cores
+(``rfm_linear_forward`` / ``rfm_linear_backward``).
+
+``linear`` computes ``act(x W^T + bias) + residual`` in one pass over the output: the projections and
+feed-forward products of the decoder's and encoder's layers.  bfloat16 and float16 operands, float32
+sums and epilogue, one rounding at the store; the backward's weight and bias gradients are summed in a
+fixed order (the same bits on every run).
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from ._native import host
+
+#: ``activation`` values.
+ACTIVATIONS = _lib.ACTIVATIONS
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, activation: str = "none",
+           residual: torch.Tensor | None = None) -> torch.Tensor:
+    """``act(x W^T + bias) + residual``, differentiable (once) in all four.
+
+    ``x`` ``[..., in]`` and ``weight`` ``[out, in]`` bfloat16 or float16 (under autocast they are cast to its
+    type first); ``bias`` ``[out]`` of that type or float32; ``residual`` ``[..., out]`` of that type.
+    ``activation`` is ``"none"``, ``"relu"`` or ``"gelu"`` (the exact one).  Any sizes and strides: operands
+    whose rows are not 16-byte aligned (an odd number of columns) are copied into padded rows first.
+    """
+    code = ACTIVATIONS.get(activation)
+    if code is None:
+        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
+    return host().linear(x, weight, bias, code, residual)
+
+
+def check_faults(device: torch.device | int | None = None) -> None:
+    """Raise if a product on ``device`` (the current one) ever gave up a bounded wait, which leaves its
+    output incomplete.  Never expected; synchronises the device."""
+    faults = ctypes.c_int(0)
+    with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
+        _lib.check("rfm_linear_faults", _lib.load().rfm_linear_faults(ctypes.byref(faults)))
+    if faults.value:
+        raise RuntimeError("a matrix product gave up a bounded wait: its output is incomplete")
