@@ -14,7 +14,7 @@
 // tile's products overlap the previous tile's epilogue), and eight warps read the
 // accumulators back (a warp can only read its own quarter of the lanes, so two
 // warps share a quarter, each half of the columns), apply bias, activation and
-// residual in fp32, round once and store 32 x 32 boxes through shared memory by
+// residual in fp32, round once and store boxes of 32 rows through shared memory by
 // TMA.  The residual is fetched by TMA into the box it is added in, one box ahead.
 //
 // Few tiles leave SMs idle while the contraction is long (dW: a layer's weight
@@ -41,7 +41,6 @@ constexpr int kEpiWarps = 8;
 constexpr int kLoadWarp = kEpiWarps;
 constexpr int kMmaWarp = kEpiWarps + 1;
 constexpr int kGemmThreads = 32 * (kEpiWarps + 2);
-constexpr int kBoxBytes = 32 * 64;  // 32 rows of 32 16-bit elements
 constexpr int kMaxSplits = 32;
 constexpr uint32_t kWaitTries = 1u << 22;
 
@@ -52,15 +51,22 @@ struct Shape {
   static constexpr int kABytes = kBM * kBK * 2;
   static constexpr int kBBytes = BN * kBK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = 196608 / kStageBytes;  // 4, 6, 8
+  // an epilogue warp's boxes: 32 rows of up to 64 columns (128 bytes), two of them
+  static constexpr int kHalf = BN / 2;
+  static constexpr int kBoxCols = kHalf < 64 ? kHalf : 64;
+  static constexpr int kBoxBytes = 32 * kBoxCols * 2;
+  static constexpr int kBoxesBytes = kEpiWarps * 2 * kBoxBytes;
+  static constexpr int kBiasBytes = kEpiWarps * kHalf * 4;
+  static constexpr int kSmem = 232448;  // of one CTA
+  static constexpr int kStages = (kSmem - 1024 - 16 - kBoxesBytes - kBiasBytes - 512) / kStageBytes;  // 3, 4, 8
   static constexpr int kBoxes = kStages * kStageBytes;
-  static constexpr int kBias = kBoxes + kEpiWarps * 2 * kBoxBytes;
-  static constexpr int kBars = kBias + kEpiWarps * 32 * 4;
+  static constexpr int kBias = kBoxes + kBoxesBytes;
+  static constexpr int kBars = kBias + kBiasBytes;
   // full and empty per stage, full and empty per accumulator, residual per warp and box
   static constexpr int kNumBars = 2 * kStages + 4 + 2 * kEpiWarps;
-  static constexpr int kBytes = kBars + kNumBars * 8 + 16 + 1024;  // and room to align the base
+  static constexpr int kBytes = kBars + kNumBars * 8 + 1024;  // and room to align the base
+  static_assert(kNumBars * 8 <= 512 && kBytes + 16 <= kSmem, "shared memory of one CTA");
 };
-static_assert(Shape<256>::kBytes <= 232448 && Shape<64>::kBytes <= 232448, "shared memory of one CTA");
 
 struct GemmArgs {
   int64_t m;
@@ -68,7 +74,7 @@ struct GemmArgs {
   int32_t tiles_m, tiles_n;
   int32_t k_blocks;       // of the whole contraction
   int32_t splits;
-  int32_t activation;
+  int32_t activation;     // of the second kernel; the product's own is a template argument
   int32_t bias_dtype;
   int32_t tma_out, tma_res;
   const void* bias;
@@ -156,7 +162,7 @@ __device__ __forceinline__ Work work_item(const GemmArgs& a, int64_t w) {
   return r;
 }
 
-template <typename T, int BN, bool A_MN, bool B_MN>
+template <typename T, int BN, bool A_MN, bool B_MN, int ACT>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ GemmArgs a) {
   using S = Shape<BN>;
@@ -285,51 +291,68 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       }
     }
   } else {
-    constexpr int kHalf = BN / 2;
-    constexpr int kChunks = kHalf / 32;
+    constexpr int kCols = S::kBoxCols;        // columns of a box
+    constexpr int kTurns = S::kHalf / kCols;  // boxes of this warp's half of a tile
+    constexpr int kPieces = kCols / 8;        // 16-byte pieces of a box's row
     const int quarter = warp & 3, half = warp >> 2;
-    const uint32_t boxes = base + S::kBoxes + warp * 2 * kBoxBytes;
-    uint8_t* box_ptr = smem + S::kBoxes + warp * 2 * kBoxBytes;
-    float* bias_smem = reinterpret_cast<float*>(smem + S::kBias) + warp * 32;
+    const uint32_t boxes = base + S::kBoxes + warp * 2 * S::kBoxBytes;
+    uint8_t* box_ptr = smem + S::kBoxes + warp * 2 * S::kBoxBytes;
+    float* bias_smem = reinterpret_cast<float*>(smem + S::kBias) + warp * S::kHalf;
     const uint32_t res_bar = res_full + 16 * warp;
     const bool whole = a.splits == 1;
+    const bool has_bias = whole && a.bias != nullptr;
     const bool has_res = whole && a.residual != nullptr, has_pre = whole && a.pre != nullptr;
     const bool tma_res = has_res && a.tma_res;
     uint32_t acc = 0, acc_phase = 0, box = 0, res_phase = 0;
-    // where a lane's 16-byte pieces of its row go in a box (64-byte swizzle)
-    const int row_off = lane * 64, swz = (lane >> 1) & 3;
+    // where a lane's 16-byte pieces of its row go in a box: the TMA swizzle of
+    // its row length, which also spreads the lanes' accesses over the banks
+    const int row_off = lane * kCols * 2, swz = kCols == 64 ? lane & 7 : (lane >> 1) & 3;
 
     for (int64_t w = blockIdx.x; w < items; w += gridDim.x) {
       const Work t = work_item(a, w);
       const int64_t row0 = static_cast<int64_t>(t.tile_m) * kBM + quarter * 32;
-      const int col_base = t.tile_n * BN + half * kHalf;
+      const int col_base = t.tile_n * BN + half * S::kHalf;
+      const bool rows_in = row0 < a.m;
       bool live = true;
-      for (int c = 0; c < kChunks; ++c) {
-        const int col0 = col_base + c * 32;
-        const bool inside = row0 < a.m && col0 < a.n;
-        // the box this chunk goes through: alternating, or the first beside `pre`'s
+      if (has_bias) {
+        __syncwarp();
+#pragma unroll
+        for (int j = lane; j < S::kHalf; j += 32)
+          bias_smem[j] = col_base + j < a.n ? load_param(a.bias, a.bias_dtype, col_base + j) : 0.f;
+        __syncwarp();
+      }
+      // the first box's residual travels while the products are still running
+      const auto fetch = [&](int turn, uint32_t b) {
+        const int col0 = col_base + turn * kCols;
+        if (lane == 0 && rows_in && col0 < a.n) {
+          tma_wait_read<0>();
+          proxy_fence();
+          mbar_expect(res_bar + 8 * b, S::kBoxBytes);
+          tma_load_2d(boxes + b * S::kBoxBytes, &maps.res, col0, static_cast<int>(row0), res_bar + 8 * b);
+        }
+        __syncwarp();
+      };
+      if (tma_res) fetch(0, has_pre ? 0u : box);
+      live = __all_sync(kFullMask, bounded_wait(acc_full + 8 * acc, acc_phase, &dead));
+      tc_fence_after();
+#pragma unroll 1
+      for (int turn = 0; turn < kTurns; ++turn) {
+        const int col0 = col_base + turn * kCols;
+        const bool inside = rows_in && col0 < a.n;
+        // boxes alternate, or the first is the output's and the second `pre`'s
         const uint32_t b = has_pre ? 0u : box;
-        if (inside && tma_res) {
-          if (lane == 0) {
-            tma_wait_read<0>();
-            proxy_fence();
-            mbar_expect(res_bar + 8 * b, kBoxBytes);
-            tma_load_2d(boxes + b * kBoxBytes, &maps.res, col0, static_cast<int>(row0), res_bar + 8 * b);
-          }
-          __syncwarp();
+        uint32_t v[kCols];
+        {
+          const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * BN + half * S::kHalf +
+                                turn * kCols;
+          uint32_t(&low)[32] = *reinterpret_cast<uint32_t(*)[32]>(&v[0]);
+          uint32_t(&high)[32] = *reinterpret_cast<uint32_t(*)[32]>(&v[kCols - 32]);
+          tmem_load_32(low, from);
+          if (kCols == 64) tmem_load_32(high, from + kCols - 32);
+          tmem_wait_load(low);
+          if (kCols == 64) tmem_wait_load(high);
         }
-        if (inside && whole && a.bias != nullptr) {
-          __syncwarp();
-          bias_smem[lane] = col0 + lane < a.n ? load_param(a.bias, a.bias_dtype, col0 + lane) : 0.f;
-          __syncwarp();
-        }
-        if (c == 0) {
-          live = __all_sync(kFullMask, bounded_wait(acc_full + 8 * acc, acc_phase, &dead));
-          tc_fence_after();
-        }
-        uint32_t v[32];
-        tmem_load_32(v, tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * BN + half * kHalf + c * 32);
-        if (c == kChunks - 1) {
+        if (turn == kTurns - 1) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(acc_empty + 8 * acc);
@@ -339,32 +362,22 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           const int64_t row = row0 + lane;
           if (row < a.m && live) {
             float* dst = a.partial + (static_cast<int64_t>(t.split) * a.m + row) * a.n + col0;
-            if ((a.n & 3) == 0 && col0 + 32 <= a.n) {
+            if ((a.n & 3) == 0 && col0 + kCols <= a.n) {
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
+              for (int j = 0; j < kCols / 4; ++j)
                 reinterpret_cast<uint4*>(dst)[j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
             } else {
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
+              for (int j = 0; j < kCols; ++j)
                 if (col0 + j < a.n) dst[j] = __uint_as_float(v[j]);
             }
           }
           continue;
         }
-        float f[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
-        if (a.bias != nullptr) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float4 q = reinterpret_cast<const float4*>(bias_smem)[j];
-            f[4 * j] += q.x;
-            f[4 * j + 1] += q.y;
-            f[4 * j + 2] += q.z;
-            f[4 * j + 3] += q.w;
-          }
-        }
-        if (!tma_res) {
+        if (tma_res) {
+          // the next box's residual, into the box that the store before last has left
+          if (!has_pre && turn + 1 < kTurns) fetch(turn + 1, box ^ 1u);
+        } else {
           // the box's last store must have been read before it is overwritten
           if (lane == 0) {
             if (has_pre) {
@@ -375,58 +388,73 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           }
           __syncwarp();
         }
-        if (has_pre) {
+        if (has_bias) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            *reinterpret_cast<uint4*>(box_ptr + kBoxBytes + row_off + ((j ^ swz) << 4)) =
-                make_uint4(pack2<T>(f[8 * j], f[8 * j + 1]), pack2<T>(f[8 * j + 2], f[8 * j + 3]),
-                           pack2<T>(f[8 * j + 4], f[8 * j + 5]), pack2<T>(f[8 * j + 6], f[8 * j + 7]));
+          for (int j = 0; j < kCols / 4; ++j) {
+            const float4 q = reinterpret_cast<const float4*>(bias_smem + turn * kCols)[j];
+            v[4 * j] = __float_as_uint(__uint_as_float(v[4 * j]) + q.x);
+            v[4 * j + 1] = __float_as_uint(__uint_as_float(v[4 * j + 1]) + q.y);
+            v[4 * j + 2] = __float_as_uint(__uint_as_float(v[4 * j + 2]) + q.z);
+            v[4 * j + 3] = __float_as_uint(__uint_as_float(v[4 * j + 3]) + q.w);
           }
         }
-        if (a.activation != RFM_ACT_NONE) {
+        const auto put = [&](uint32_t which) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) f[j] = activate(f[j], a.activation);
+          for (int j = 0; j < kPieces; ++j) {
+            uint32_t p[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              p[i] = pack2<T>(__uint_as_float(v[8 * j + 2 * i]), __uint_as_float(v[8 * j + 2 * i + 1]));
+            *reinterpret_cast<uint4*>(box_ptr + which * S::kBoxBytes + row_off + ((j ^ swz) << 4)) =
+                make_uint4(p[0], p[1], p[2], p[3]);
+          }
+        };
+        if (has_pre) put(1);
+        if (ACT != RFM_ACT_NONE) {
+#pragma unroll
+          for (int j = 0; j < kCols; ++j) v[j] = __float_as_uint(activate(__uint_as_float(v[j]), ACT));
         }
+        // element (r, c) of a box lies at cell r * kCols + (piece ^ swizzle) * 8 + c % 8
+        const auto cell = [](int r, int c) {
+          return r * kCols + (((c >> 3) ^ (kCols == 64 ? r & 7 : (r >> 1) & 3)) << 3) + (c & 7);
+        };
         if (has_res) {
           if (tma_res) {
             live = __all_sync(kFullMask, bounded_wait(res_bar + 8 * b, (res_phase >> b) & 1u, &dead) && live);
             res_phase ^= 1u << b;
           } else {
             // rows whose start is not a multiple of 16 bytes: element by element, a lane a column
-            T* cells = reinterpret_cast<T*>(box_ptr + b * kBoxBytes);
+            T* cells = reinterpret_cast<T*>(box_ptr + b * S::kBoxBytes);
             const T* res = static_cast<const T*>(a.residual);
             for (int r = 0; r < 32; ++r) {
               const int64_t row = row0 + r;
-              const int at = r * 32 + (((lane >> 3) ^ ((r >> 1) & 3)) << 3) + (lane & 7);
-              cells[at] = row < a.m && col0 + lane < a.n ? res[row * a.ld_res + col0 + lane] : from_float<T>(0.f);
+#pragma unroll
+              for (int c = lane; c < kCols; c += 32)
+                cells[cell(r, c)] =
+                    row < a.m && col0 + c < a.n ? res[row * a.ld_res + col0 + c] : from_float<T>(0.f);
             }
             __syncwarp();
           }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < kPieces; ++j) {
             const uint4 q =
-                *reinterpret_cast<const uint4*>(box_ptr + b * kBoxBytes + row_off + ((j ^ swz) << 4));
+                *reinterpret_cast<const uint4*>(box_ptr + b * S::kBoxBytes + row_off + ((j ^ swz) << 4));
             const uint32_t words[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const float2 two = unpack2<T>(words[i]);
-              f[8 * j + 2 * i] += two.x;
-              f[8 * j + 2 * i + 1] += two.y;
+              v[8 * j + 2 * i] = __float_as_uint(__uint_as_float(v[8 * j + 2 * i]) + two.x);
+              v[8 * j + 2 * i + 1] = __float_as_uint(__uint_as_float(v[8 * j + 2 * i + 1]) + two.y);
             }
           }
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          *reinterpret_cast<uint4*>(box_ptr + b * kBoxBytes + row_off + ((j ^ swz) << 4)) =
-              make_uint4(pack2<T>(f[8 * j], f[8 * j + 1]), pack2<T>(f[8 * j + 2], f[8 * j + 3]),
-                         pack2<T>(f[8 * j + 4], f[8 * j + 5]), pack2<T>(f[8 * j + 6], f[8 * j + 7]));
-        }
+        put(b);
         if (a.tma_out) {
           proxy_fence();
           __syncwarp();
           if (lane == 0 && live) {
-            tma_store_2d(&maps.out, col0, static_cast<int>(row0), boxes + b * kBoxBytes);
-            if (has_pre) tma_store_2d(&maps.pre, col0, static_cast<int>(row0), boxes + kBoxBytes);
+            tma_store_2d(&maps.out, col0, static_cast<int>(row0), boxes + b * S::kBoxBytes);
+            if (has_pre) tma_store_2d(&maps.pre, col0, static_cast<int>(row0), boxes + S::kBoxBytes);
             tma_commit();
           }
         } else {
@@ -434,18 +462,21 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           if (live) {
             for (int r = 0; r < 32; ++r) {
               const int64_t row = row0 + r;
-              if (row >= a.m || col0 + lane >= a.n) continue;
-              const int at = r * 32 + (((lane >> 3) ^ ((r >> 1) & 3)) << 3) + (lane & 7);
-              static_cast<T*>(a.out)[row * a.n + col0 + lane] =
-                  reinterpret_cast<const T*>(box_ptr + b * kBoxBytes)[at];
-              if (has_pre) {
-                static_cast<T*>(a.pre)[row * a.n + col0 + lane] =
-                    reinterpret_cast<const T*>(box_ptr + kBoxBytes)[at];
+#pragma unroll
+              for (int c = lane; c < kCols; c += 32) {
+                if (row >= a.m || col0 + c >= a.n) continue;
+                const int64_t at = row * a.n + col0 + c;
+                static_cast<T*>(a.out)[at] = reinterpret_cast<const T*>(box_ptr + b * S::kBoxBytes)[cell(r, c)];
+                if (has_pre) {
+                  static_cast<T*>(a.pre)[at] = reinterpret_cast<const T*>(box_ptr + S::kBoxBytes)[cell(r, c)];
+                }
               }
             }
           }
           __syncwarp();
         }
+        // one box for residual and output: the next residual follows this store
+        if (tma_res && has_pre && turn + 1 < kTurns) fetch(turn + 1, 0);
         box ^= 1u;
       }
       if (!live) break;
@@ -685,7 +716,7 @@ struct Product {
   GemmArgs args;  // epilogue fields filled in by the caller
 };
 
-template <typename T, int BN, bool A_MN, bool B_MN>
+template <typename T, int BN, bool A_MN, bool B_MN, int ACT>
 int launch_gemm(const Product& p, GemmArgs& g, float* partial, cudaStream_t stream) {
   using S = Shape<BN>;
   GemmMaps maps;
@@ -700,19 +731,20 @@ int launch_gemm(const Product& p, GemmArgs& g, float* partial, cudaStream_t stre
   g.tma_out = g.splits == 1 && tma_rows(g.out, p.n) && (g.pre == nullptr || tma_rows(g.pre, p.n));
   g.tma_res = g.splits == 1 && g.residual != nullptr && tma_rows(g.residual, g.ld_res);
   maps.out = maps.pre = maps.res = maps.a;
+  constexpr CUtensorMapSwizzle swizzle = S::kBoxCols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
   if (g.tma_out) {
-    if (!make_map(&maps.out, p.dtype, g.out, p.n, p.m, p.n, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B)) return RFM_ERR_LAUNCH;
+    if (!make_map(&maps.out, p.dtype, g.out, p.n, p.m, p.n, S::kBoxCols, 32, swizzle)) return RFM_ERR_LAUNCH;
     if (g.pre != nullptr &&
-        !make_map(&maps.pre, p.dtype, g.pre, p.n, p.m, p.n, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B)) {
+        !make_map(&maps.pre, p.dtype, g.pre, p.n, p.m, p.n, S::kBoxCols, 32, swizzle)) {
       return RFM_ERR_LAUNCH;
     }
   }
   if (g.tma_res &&
-      !make_map(&maps.res, p.dtype, g.residual, p.n, p.m, g.ld_res, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B)) {
+      !make_map(&maps.res, p.dtype, g.residual, p.n, p.m, g.ld_res, S::kBoxCols, 32, swizzle)) {
     return RFM_ERR_LAUNCH;
   }
   static thread_local unsigned long long ready = 0;  // the context whose shared-memory limit is raised
-  const auto kernel = gemm_kernel<T, BN, A_MN, B_MN>;
+  const auto kernel = gemm_kernel<T, BN, A_MN, B_MN, ACT>;
   const unsigned long long context = current_context_id();
   if (ready != context || context == 0) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess) {
@@ -727,6 +759,26 @@ int launch_gemm(const Product& p, GemmArgs& g, float* partial, cudaStream_t stre
   return launch_status();
 }
 
+template <typename T, int BN, bool A_MN, bool B_MN>
+int launch_act(const Product& p, GemmArgs& g, float* partial, cudaStream_t stream) {
+  if constexpr (!A_MN && !B_MN) {  // the forward; a split product's activation comes in the second kernel
+    if (g.splits == 1 && g.activation == RFM_ACT_RELU) {
+      return launch_gemm<T, BN, A_MN, B_MN, RFM_ACT_RELU>(p, g, partial, stream);
+    }
+    if (g.splits == 1 && g.activation == RFM_ACT_GELU) {
+      return launch_gemm<T, BN, A_MN, B_MN, RFM_ACT_GELU>(p, g, partial, stream);
+    }
+  }
+  return launch_gemm<T, BN, A_MN, B_MN, RFM_ACT_NONE>(p, g, partial, stream);
+}
+
+template <typename T, bool A_MN, bool B_MN>
+int launch_cut(const Product& p, GemmArgs& g, const Cut& cut, float* partial, cudaStream_t stream) {
+  if (cut.bn == 256) return launch_act<T, 256, A_MN, B_MN>(p, g, partial, stream);
+  if (cut.bn == 128) return launch_act<T, 128, A_MN, B_MN>(p, g, partial, stream);
+  return launch_act<T, 64, A_MN, B_MN>(p, g, partial, stream);
+}
+
 template <typename T, bool A_MN, bool B_MN>
 int run_product(const Product& p, void* workspace, cudaStream_t stream) {
   const Cut cut = choose_cut(p.m, p.n, static_cast<int>((p.k + kBK - 1) / kBK));
@@ -736,14 +788,7 @@ int run_product(const Product& p, void* workspace, cudaStream_t stream) {
   g.k_blocks = static_cast<int>((p.k + kBK - 1) / kBK);
   g.splits = cut.splits;
   float* partial = static_cast<float*>(workspace);
-  int rc;
-  if (cut.bn == 256) {
-    rc = launch_gemm<T, 256, A_MN, B_MN>(p, g, partial, stream);
-  } else if (cut.bn == 128) {
-    rc = launch_gemm<T, 128, A_MN, B_MN>(p, g, partial, stream);
-  } else {
-    rc = launch_gemm<T, 64, A_MN, B_MN>(p, g, partial, stream);
-  }
+  const int rc = launch_cut<T, A_MN, B_MN>(p, g, cut, partial, stream);
   if (rc != RFM_OK || cut.splits == 1) return rc;
   FinishArgs f{partial, g.bias, g.residual, g.out, g.pre, p.m, g.ld_res, p.n, cut.splits, g.activation, g.bias_dtype};
   const bool quads = p.n % 4 == 0 && (reinterpret_cast<uintptr_t>(g.out) & 7) == 0 &&
