@@ -46,26 +46,30 @@ constexpr uint32_t kWaitTries = 1u << 22;
 
 __device__ int g_linear_faults = 0;
 
-template <int BN>
+// Shared memory of one CTA.  CG 2: two CTAs share a tile of 256 rows; each holds
+// its own 128 rows of A and half of B's.
+template <int BN, int CG>
 struct Shape {
+  static constexpr int kBRows = BN / CG;
   static constexpr int kABytes = kBM * kBK * 2;
-  static constexpr int kBBytes = BN * kBK * 2;
+  static constexpr int kBBytes = kBRows * kBK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
   // an epilogue warp's boxes: 32 rows of up to 64 columns (128 bytes), two of them
   static constexpr int kHalf = BN / 2;
   static constexpr int kBoxCols = kHalf < 64 ? kHalf : 64;
   static constexpr int kBoxBytes = 32 * kBoxCols * 2;
   static constexpr int kBoxesBytes = kEpiWarps * 2 * kBoxBytes;
-  static constexpr int kBiasBytes = kEpiWarps * kHalf * 4;
-  static constexpr int kSmem = 232448;  // of one CTA
-  static constexpr int kStages = (kSmem - 1024 - 16 - kBoxesBytes - kBiasBytes - 512) / kStageBytes;  // 3, 4, 8
+  static constexpr int kBiasBytes = kEpiWarps * kBoxCols * 4;  // of the box in work
+  static constexpr int kSmem = 232448;                         // of one CTA
+  static constexpr int kStages = (kSmem - kBoxesBytes - kBiasBytes - 512) / kStageBytes;  // pair: 5; 3, 5, 8
   static constexpr int kBoxes = kStages * kStageBytes;
   static constexpr int kBias = kBoxes + kBoxesBytes;
   static constexpr int kBars = kBias + kBiasBytes;
   // full and empty per stage, full and empty per accumulator, residual per warp and box
   static constexpr int kNumBars = 2 * kStages + 4 + 2 * kEpiWarps;
-  static constexpr int kBytes = kBars + kNumBars * 8 + 1024;  // and room to align the base
-  static_assert(kNumBars * 8 <= 512 && kBytes + 16 <= kSmem, "shared memory of one CTA");
+  static constexpr int kFlags = kBars + kNumBars * 8;
+  static constexpr int kBytes = kFlags + 16;
+  static_assert(kBytes <= kSmem, "shared memory of one CTA");
 };
 
 struct GemmArgs {
@@ -162,69 +166,87 @@ __device__ __forceinline__ Work work_item(const GemmArgs& a, int64_t w) {
   return r;
 }
 
-template <typename T, int BN, bool A_MN, bool B_MN, int ACT>
+template <typename T, int BN, int CG, bool A_MN, bool B_MN, int ACT>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ GemmArgs a) {
-  using S = Shape<BN>;
-  extern __shared__ uint8_t raw_smem[];
-  __shared__ volatile int dead;
-  __shared__ uint32_t tmem_base;
-  const uint32_t base = (smem_u32(raw_smem) + 1023u) & ~1023u;
-  uint8_t* smem = raw_smem + (base - smem_u32(raw_smem));
+  using S = Shape<BN, CG>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = smem_u32(smem);
   const uint32_t bars = base + S::kBars;
   const uint32_t full = bars, empty = bars + 8 * S::kStages;
   const uint32_t acc_full = empty + 8 * S::kStages, acc_empty = acc_full + 16, res_full = acc_empty + 16;
+  volatile int* dead = reinterpret_cast<volatile int*>(smem + S::kFlags);
   const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
   constexpr uint32_t kTmemColumns = 2 * BN;
+  // of a pair, CTA 0 issues the products and counts both CTAs' loads
+  const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
 
   if (threadIdx.x == 0) {
-    dead = 0;
+    *dead = 0;
+    if ((base & 1023u) != 0) {  // the swizzles count on it; never expected
+      *dead = 1;
+      atomicExch(&g_linear_faults, 1);
+    }
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(full + 8 * i, 1);
       mbar_init(empty + 8 * i, 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(acc_full + 8 * i, 1);
-      mbar_init(acc_empty + 8 * i, kEpiWarps);
+      mbar_init(acc_empty + 8 * i, kEpiWarps * CG);
     }
     for (int i = 0; i < 2 * kEpiWarps; ++i) mbar_init(res_full + 8 * i, 1);
     mbar_init_fence();
     tma_prefetch_map(&maps.a);
     tma_prefetch_map(&maps.b);
   }
-  if (warp == kMmaWarp) tmem_alloc(smem_u32(&tmem_base), kTmemColumns);
+  if (warp == kMmaWarp) tmem_alloc<CG>(base + S::kFlags + 4, kTmemColumns);
   tc_fence_before();
-  __syncthreads();
+  if (CG == 2) {
+    cluster_sync();
+  } else {
+    __syncthreads();
+  }
   tc_fence_after();
-  const uint32_t tmem = tmem_base;
+  const uint32_t tmem = *reinterpret_cast<const volatile uint32_t*>(smem + S::kFlags + 4);
   const int64_t items = static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.splits;
+  const int64_t first = blockIdx.x / CG, stride = gridDim.x / CG;
 
   if (warp == kLoadWarp) {
     if (lane == 0) {
       uint32_t stage = 0, phase = 0, issued = 0;
       bool ok = true;
-      for (int64_t w = blockIdx.x; ok && w < items; w += gridDim.x) {
+      for (int64_t w = first; ok && w < items; w += stride) {
         const Work t = work_item(a, w);
-        const int m0 = t.tile_m * kBM, n0 = t.tile_n * BN;
+        const int m0 = (t.tile_m * CG + static_cast<int>(rank)) * kBM;
+        const int n0 = t.tile_n * BN + static_cast<int>(rank) * S::kBRows;
         for (int kb = t.k0; kb < t.k1; ++kb) {
-          if (!bounded_wait(empty + 8 * stage, phase ^ 1u, &dead)) {
+          if (!bounded_wait(empty + 8 * stage, phase ^ 1u, dead)) {
             ok = false;
             break;
           }
-          const uint32_t bar = full + 8 * stage;
+          uint32_t bar = full + 8 * stage;
           const uint32_t sa = base + stage * S::kStageBytes, sb = sa + S::kABytes;
-          mbar_expect(bar, S::kStageBytes);
+          if (rank == 0) mbar_expect(bar, CG * S::kStageBytes);
+          if (CG == 2) bar = map_rank(bar, 0);
+          const auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
+            if (CG == 2) {
+              tma_load_2d_pair(dst, map, x, y, bar);
+            } else {
+              tma_load_2d(dst, map, x, y, bar);
+            }
+          };
           if (A_MN) {
 #pragma unroll
-            for (int j = 0; j < kBM / 64; ++j) tma_load_2d(sa + j * 8192, &maps.a, m0 + j * 64, kb * kBK, bar);
+            for (int j = 0; j < kBM / 64; ++j) load(sa + j * 8192, &maps.a, m0 + j * 64, kb * kBK);
           } else {
-            tma_load_2d(sa, &maps.a, kb * kBK, m0, bar);
+            load(sa, &maps.a, kb * kBK, m0);
           }
           if (B_MN) {
 #pragma unroll
-            for (int j = 0; j < BN / 64; ++j) tma_load_2d(sb + j * 8192, &maps.b, n0 + j * 64, kb * kBK, bar);
+            for (int j = 0; j < S::kBRows / 64; ++j) load(sb + j * 8192, &maps.b, n0 + j * 64, kb * kBK);
           } else {
-            tma_load_2d(sb, &maps.b, kb * kBK, n0, bar);
+            load(sb, &maps.b, kb * kBK, n0);
           }
           if (issued < S::kStages) ++issued;
           if (++stage == S::kStages) {
@@ -233,8 +255,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           }
         }
       }
-      if (!ok) {
-        // the copies in flight land before the CTA's shared memory is given up
+      if (!ok && rank == 0) {
+        // the copies in flight (a pair's: of both) land before the shared memory is given up
         for (uint32_t i = 0; i < issued; ++i) {
           if (stage == 0) {
             stage = S::kStages;
@@ -247,19 +269,19 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       }
     }
   } else if (warp == kMmaWarp) {
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       constexpr int kType = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
-      constexpr uint32_t kInstr = mma_instr(kType, A_MN, B_MN, kBM, BN);
+      constexpr uint32_t kInstr = mma_instr(kType, A_MN, B_MN, kBM * CG, BN);
       constexpr uint32_t kAStep = A_MN ? 2048 : 32, kBStep = B_MN ? 2048 : 32;  // bytes of 16 along k
       uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
       bool ok = true;
-      for (int64_t w = blockIdx.x; ok && w < items; w += gridDim.x) {
+      for (int64_t w = first; ok && w < items; w += stride) {
         const Work t = work_item(a, w);
-        if (!bounded_wait(acc_empty + 8 * acc, acc_phase ^ 1u, &dead)) break;
+        if (!bounded_wait(acc_empty + 8 * acc, acc_phase ^ 1u, dead)) break;
         tc_fence_after();
         const uint32_t d = tmem + acc * BN;
         for (int kb = t.k0; kb < t.k1; ++kb) {
-          if (!bounded_wait(full + 8 * stage, phase, &dead)) {
+          if (!bounded_wait(full + 8 * stage, phase, dead)) {
             ok = false;
             break;
           }
@@ -267,25 +289,25 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           const uint32_t sa = base + stage * S::kStageBytes, sb = sa + S::kABytes;
 #pragma unroll
           for (int k = 0; k < kBK / 16; ++k) {
-            tc_mma_f16(d, operand_desc(sa + k * kAStep, A_MN ? 8192 : 16, 1024),
-                       operand_desc(sb + k * kBStep, B_MN ? 8192 : 16, 1024), kInstr, kb > t.k0 || k > 0);
+            tc_mma_f16<CG>(d, operand_desc(sa + k * kAStep, A_MN ? 8192 : 16, 1024),
+                           operand_desc(sb + k * kBStep, B_MN ? 8192 : 16, 1024), kInstr, kb > t.k0 || k > 0);
           }
-          tc_commit(empty + 8 * stage);
+          tc_commit<CG>(empty + 8 * stage);
           if (++stage == S::kStages) {
             stage = 0;
             phase ^= 1u;
           }
         }
         if (!ok) break;
-        tc_commit(acc_full + 8 * acc);
+        tc_commit<CG>(acc_full + 8 * acc);
         acc ^= 1u;
         if (acc == 0) acc_phase ^= 1u;
       }
       // The products in flight end before the tensor memory is given up: the
       // epilogue waits for the last accumulator's barrier, and a role that gave
       // up waits here.
-      if (dead) {
-        tc_commit(acc_full + 8 * acc);
+      if (*dead) {
+        tc_commit<CG>(acc_full + 8 * acc);
         for (uint32_t k = 0; k < kWaitTries && !mbar_try(acc_full + 8 * acc, acc_phase); ++k) {
         }
       }
@@ -297,7 +319,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     const int quarter = warp & 3, half = warp >> 2;
     const uint32_t boxes = base + S::kBoxes + warp * 2 * S::kBoxBytes;
     uint8_t* box_ptr = smem + S::kBoxes + warp * 2 * S::kBoxBytes;
-    float* bias_smem = reinterpret_cast<float*>(smem + S::kBias) + warp * S::kHalf;
+    float* bias_smem = reinterpret_cast<float*>(smem + S::kBias) + warp * kCols;
     const uint32_t res_bar = res_full + 16 * warp;
     const bool whole = a.splits == 1;
     const bool has_bias = whole && a.bias != nullptr;
@@ -308,19 +330,25 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     // its row length, which also spreads the lanes' accesses over the banks
     const int row_off = lane * kCols * 2, swz = kCols == 64 ? lane & 7 : (lane >> 1) & 3;
 
-    for (int64_t w = blockIdx.x; w < items; w += gridDim.x) {
+    constexpr int kBiasRegs = kCols / 32;
+    const uint32_t released = CG == 2 ? map_rank(acc_empty, 0) : acc_empty;
+
+    for (int64_t w = first; w < items; w += stride) {
       const Work t = work_item(a, w);
-      const int64_t row0 = static_cast<int64_t>(t.tile_m) * kBM + quarter * 32;
+      const int64_t row0 = (static_cast<int64_t>(t.tile_m) * CG + rank) * kBM + quarter * 32;
       const int col_base = t.tile_n * BN + half * S::kHalf;
       const bool rows_in = row0 < a.m;
       bool live = true;
-      if (has_bias) {
-        __syncwarp();
+      // the bias of a box, read one box ahead: lane l holds columns l, l + 32
+      float bias[kBiasRegs];
+      const auto read_bias = [&](int turn) {
 #pragma unroll
-        for (int j = lane; j < S::kHalf; j += 32)
-          bias_smem[j] = col_base + j < a.n ? load_param(a.bias, a.bias_dtype, col_base + j) : 0.f;
-        __syncwarp();
-      }
+        for (int j = 0; j < kBiasRegs; ++j) {
+          const int col = col_base + turn * kCols + j * 32 + lane;
+          bias[j] = col < a.n ? load_param(a.bias, a.bias_dtype, col) : 0.f;
+        }
+      };
+      if (has_bias) read_bias(0);
       // the first box's residual travels while the products are still running
       const auto fetch = [&](int turn, uint32_t b) {
         const int col0 = col_base + turn * kCols;
@@ -333,7 +361,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         __syncwarp();
       };
       if (tma_res) fetch(0, has_pre ? 0u : box);
-      live = __all_sync(kFullMask, bounded_wait(acc_full + 8 * acc, acc_phase, &dead));
+      live = __all_sync(kFullMask, bounded_wait(acc_full + 8 * acc, acc_phase, dead));
       tc_fence_after();
 #pragma unroll 1
       for (int turn = 0; turn < kTurns; ++turn) {
@@ -355,7 +383,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         if (turn == kTurns - 1) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(acc_empty + 8 * acc);
+          if (lane == 0) {
+            if (CG == 2) {
+              mbar_arrive_cluster(released + 8 * acc);
+            } else {
+              mbar_arrive(released + 8 * acc);
+            }
+          }
         }
         if (!inside) continue;
         if (!whole) {
@@ -389,9 +423,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           __syncwarp();
         }
         if (has_bias) {
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < kBiasRegs; ++j) bias_smem[j * 32 + lane] = bias[j];
+          __syncwarp();
+          if (turn + 1 < kTurns) read_bias(turn + 1);
 #pragma unroll
           for (int j = 0; j < kCols / 4; ++j) {
-            const float4 q = reinterpret_cast<const float4*>(bias_smem + turn * kCols)[j];
+            const float4 q = reinterpret_cast<const float4*>(bias_smem)[j];
             v[4 * j] = __float_as_uint(__uint_as_float(v[4 * j]) + q.x);
             v[4 * j + 1] = __float_as_uint(__uint_as_float(v[4 * j + 1]) + q.y);
             v[4 * j + 2] = __float_as_uint(__uint_as_float(v[4 * j + 2]) + q.z);
@@ -420,7 +459,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         };
         if (has_res) {
           if (tma_res) {
-            live = __all_sync(kFullMask, bounded_wait(res_bar + 8 * b, (res_phase >> b) & 1u, &dead) && live);
+            live = __all_sync(kFullMask, bounded_wait(res_bar + 8 * b, (res_phase >> b) & 1u, dead) && live);
             res_phase ^= 1u << b;
           } else {
             // rows whose start is not a multiple of 16 bytes: element by element, a lane a column
@@ -485,11 +524,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     }
     if (lane == 0) tma_wait_read<0>();
   }
+  __syncwarp();
   tc_fence_before();
-  __syncthreads();
+  if (CG == 2) {
+    cluster_sync();  // neither CTA leaves while the other's products read its memory
+  } else {
+    __syncthreads();
+  }
   if (warp == kMmaWarp) {
     tc_fence_after();
-    tmem_free(tmem, kTmemColumns);
+    tmem_free<CG>(tmem, kTmemColumns);
   }
 }
 
@@ -667,28 +711,33 @@ bool make_map(CUtensorMap* map, int dtype, const void* p, int64_t inner, int64_t
 
 bool tma_rows(const void* p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
 
-// How a product is cut: the tile's columns and the parts of the contraction.
+// How a product is cut: the tile's columns, one CTA or a pair to a tile, and the
+// parts of the contraction.
 struct Cut {
   int bn = 64;
+  int pair = 0;
   int splits = 1;
 };
 
 // Estimated cycles of the busiest SM for each cut.  A 64-deep slice of a
 // 128 x BN tile takes the tensor cores 2 BN cycles and brings (128 + BN) * 128
-// bytes, which an SM takes in at about 80 a cycle; a tile's epilogue, hidden
-// behind the next tile's products but for the last, 11 cycles a column (measured
-// range: 8 to 14); a part's fp32 sums are written and read once, and the second
-// kernel costs about 5000 cycles.
+// bytes (a pair of CTAs: each half of B's), which an SM takes in at about 80 a
+// cycle; a tile's epilogue, hidden behind the next tile's products but for the
+// last, 11 cycles a column (measured range: 8 to 14); a part's fp32 sums are
+// written and read once, and the second kernel costs about 5000 cycles.
 Cut choose_cut(int64_t m, int n, int k_blocks) {
   const int sms = device_sm_count();
   Cut best;
   double least = 1e30;
-  for (int bn = 256; bn >= 64; bn /= 2) {
-    const int64_t tiles = ((m + kBM - 1) / kBM) * ((n + bn - 1) / bn);
-    const double slice = fmax(2.0 * bn, (128.0 + bn) * 128.0 / 80.0);
+  for (int shape = 0; shape < 4; ++shape) {
+    const int pair = shape == 0, bn = shape < 2 ? 256 : shape == 2 ? 128 : 64;
+    const int64_t rows = pair ? 2 * kBM : kBM;
+    const int64_t tiles = ((m + rows - 1) / rows) * ((n + bn - 1) / bn);
+    const int64_t workers = pair ? sms / 2 : sms;
+    const double slice = fmax(2.0 * bn, (128.0 + (pair ? bn / 2 : bn)) * 128.0 / 80.0);
     for (int splits = 1; splits <= kMaxSplits && splits <= k_blocks; ++splits) {
-      if (splits > 1 && (k_blocks / splits < 2 || tiles * (splits - 1) >= 4 * sms)) break;
-      const int64_t waves = (tiles * splits + sms - 1) / sms;
+      if (splits > 1 && (k_blocks / splits < 2 || tiles * (splits - 1) >= 4 * workers)) break;
+      const int64_t waves = (tiles * splits + workers - 1) / workers;
       const double depth = static_cast<double>((k_blocks + splits - 1) / splits);
       const double epilogue = 11.0 * bn;
       double cycles = 1500.0 + waves * fmax(depth * slice, epilogue) + epilogue;
@@ -697,8 +746,7 @@ Cut choose_cut(int64_t m, int n, int k_blocks) {
       }
       if (cycles < least) {
         least = cycles;
-        best.bn = bn;
-        best.splits = splits;
+        best = Cut{bn, pair, splits};
       }
     }
   }
@@ -716,16 +764,16 @@ struct Product {
   GemmArgs args;  // epilogue fields filled in by the caller
 };
 
-template <typename T, int BN, bool A_MN, bool B_MN, int ACT>
+template <typename T, int BN, int CG, bool A_MN, bool B_MN, int ACT>
 int launch_gemm(const Product& p, GemmArgs& g, float* partial, cudaStream_t stream) {
-  using S = Shape<BN>;
+  using S = Shape<BN, CG>;
   GemmMaps maps;
   const bool ok_a = A_MN ? make_map(&maps.a, p.dtype, p.a, p.m, p.k, p.ld_a, 64, kBK, CU_TENSOR_MAP_SWIZZLE_128B)
                          : make_map(&maps.a, p.dtype, p.a, p.k, p.m, p.ld_a, kBK, kBM, CU_TENSOR_MAP_SWIZZLE_128B);
   const bool ok_b = B_MN ? make_map(&maps.b, p.dtype, p.b, p.n, p.k, p.ld_b, 64, kBK, CU_TENSOR_MAP_SWIZZLE_128B)
-                         : make_map(&maps.b, p.dtype, p.b, p.k, p.n, p.ld_b, kBK, BN, CU_TENSOR_MAP_SWIZZLE_128B);
+                         : make_map(&maps.b, p.dtype, p.b, p.k, p.n, p.ld_b, kBK, S::kBRows, CU_TENSOR_MAP_SWIZZLE_128B);
   if (!ok_a || !ok_b) return RFM_ERR_LAUNCH;
-  g.tiles_m = static_cast<int>((p.m + kBM - 1) / kBM);
+  g.tiles_m = static_cast<int>((p.m + kBM * CG - 1) / (kBM * CG));
   g.tiles_n = (p.n + BN - 1) / BN;
   g.partial = partial;
   g.tma_out = g.splits == 1 && tma_rows(g.out, p.n) && (g.pre == nullptr || tma_rows(g.pre, p.n));
@@ -744,7 +792,7 @@ int launch_gemm(const Product& p, GemmArgs& g, float* partial, cudaStream_t stre
     return RFM_ERR_LAUNCH;
   }
   static thread_local unsigned long long ready = 0;  // the context whose shared-memory limit is raised
-  const auto kernel = gemm_kernel<T, BN, A_MN, B_MN, ACT>;
+  const auto kernel = gemm_kernel<T, BN, CG, A_MN, B_MN, ACT>;
   const unsigned long long context = current_context_id();
   if (ready != context || context == 0) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess) {
@@ -755,28 +803,44 @@ int launch_gemm(const Product& p, GemmArgs& g, float* partial, cudaStream_t stre
   }
   const int64_t items = static_cast<int64_t>(g.tiles_m) * g.tiles_n * g.splits;
   const int sms = device_sm_count();
-  kernel<<<static_cast<unsigned>(items < sms ? items : sms), kGemmThreads, S::kBytes, stream>>>(maps, g);
+  const int64_t workers = sms / CG;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>((items < workers ? items : workers) * CG));
+  config.blockDim = dim3(kGemmThreads);
+  config.dynamicSmemBytes = S::kBytes;
+  config.stream = stream;
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = CG;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  config.attrs = &cluster;
+  config.numAttrs = CG == 2 ? 1 : 0;
+  if (cudaLaunchKernelEx(&config, kernel, maps, g) != cudaSuccess) {
+    cudaGetLastError();
+    return RFM_ERR_LAUNCH;
+  }
   return launch_status();
 }
 
-template <typename T, int BN, bool A_MN, bool B_MN>
+template <typename T, int BN, int CG, bool A_MN, bool B_MN>
 int launch_act(const Product& p, GemmArgs& g, float* partial, cudaStream_t stream) {
   if constexpr (!A_MN && !B_MN) {  // the forward; a split product's activation comes in the second kernel
     if (g.splits == 1 && g.activation == RFM_ACT_RELU) {
-      return launch_gemm<T, BN, A_MN, B_MN, RFM_ACT_RELU>(p, g, partial, stream);
+      return launch_gemm<T, BN, CG, A_MN, B_MN, RFM_ACT_RELU>(p, g, partial, stream);
     }
     if (g.splits == 1 && g.activation == RFM_ACT_GELU) {
-      return launch_gemm<T, BN, A_MN, B_MN, RFM_ACT_GELU>(p, g, partial, stream);
+      return launch_gemm<T, BN, CG, A_MN, B_MN, RFM_ACT_GELU>(p, g, partial, stream);
     }
   }
-  return launch_gemm<T, BN, A_MN, B_MN, RFM_ACT_NONE>(p, g, partial, stream);
+  return launch_gemm<T, BN, CG, A_MN, B_MN, RFM_ACT_NONE>(p, g, partial, stream);
 }
 
 template <typename T, bool A_MN, bool B_MN>
 int launch_cut(const Product& p, GemmArgs& g, const Cut& cut, float* partial, cudaStream_t stream) {
-  if (cut.bn == 256) return launch_act<T, 256, A_MN, B_MN>(p, g, partial, stream);
-  if (cut.bn == 128) return launch_act<T, 128, A_MN, B_MN>(p, g, partial, stream);
-  return launch_act<T, 64, A_MN, B_MN>(p, g, partial, stream);
+  if (cut.pair) return launch_act<T, 256, 2, A_MN, B_MN>(p, g, partial, stream);
+  if (cut.bn == 256) return launch_act<T, 256, 1, A_MN, B_MN>(p, g, partial, stream);
+  if (cut.bn == 128) return launch_act<T, 128, 1, A_MN, B_MN>(p, g, partial, stream);
+  return launch_act<T, 64, 1, A_MN, B_MN>(p, g, partial, stream);
 }
 
 template <typename T, bool A_MN, bool B_MN>
