@@ -8,14 +8,16 @@
 // both (forward), k for A and n for B (dX), m and n (dW).  TMA reads all of them
 // as stored, so nothing is transposed.
 //
-// Structure.  A persistent CTA of ten warps walks 128 x BN tiles: one thread
-// issues the TMA loads of 64-deep operand slices into a ring of stages, one
-// issues tcgen05.mma (fp32 accumulators in tensor memory, two of them, so that a
-// tile's products overlap the previous tile's epilogue), and eight warps read the
-// accumulators back (a warp can only read its own quarter of the lanes, so two
-// warps share a quarter, each half of the columns), apply bias, activation and
-// residual in fp32, round once and store boxes of 32 rows through shared memory by
-// TMA.  The residual is fetched by TMA into the box it is added in, one box ahead.
+// Structure.  A persistent CTA walks 128 x BN tiles: one thread issues the TMA
+// loads of 64-deep operand slices into a ring of stages, one issues tcgen05.mma
+// (fp32 accumulators in tensor memory, two of them, so that a tile's products
+// overlap the previous tile's epilogue), and 16 warps (8 for the narrow tile) read
+// the accumulators back, apply bias, activation and residual in fp32, round once
+// and store boxes of 32 rows through shared memory by TMA.  A warp can only read
+// its own quarter of the lanes; the four warps of a quarter share the columns, one
+// box a warp: shallow products are bound by the epilogue's latencies (tensor
+// memory, the proxy fence, the store's read), which more warps overlap.  The
+// residual is fetched by TMA into the box it is added in, while the products run.
 //
 // Few tiles leave SMs idle while the contraction is long (dW: a layer's weight
 // is a handful of tiles over tens of thousands of rows; one row against a wide
@@ -37,10 +39,6 @@ namespace {
 
 constexpr int kBM = 128;
 constexpr int kBK = 64;  // one 128-byte row of 16-bit elements
-constexpr int kEpiWarps = 8;
-constexpr int kLoadWarp = kEpiWarps;
-constexpr int kMmaWarp = kEpiWarps + 1;
-constexpr int kGemmThreads = 32 * (kEpiWarps + 2);
 constexpr int kMaxSplits = 32;
 constexpr uint32_t kWaitTries = 1u << 22;
 
@@ -54,19 +52,22 @@ struct Shape {
   static constexpr int kABytes = kBM * kBK * 2;
   static constexpr int kBBytes = kBRows * kBK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  // an epilogue warp's boxes: 32 rows of up to 64 columns (128 bytes), two of them
-  static constexpr int kHalf = BN / 2;
-  static constexpr int kBoxCols = kHalf < 64 ? kHalf : 64;
+  // four warps a quarter of the lanes (two for 64 columns), each with one box of 32 rows
+  static constexpr int kEpiWarps = BN == 64 ? 8 : 16;
+  static constexpr int kLoadWarp = kEpiWarps;
+  static constexpr int kMmaWarp = kEpiWarps + 1;
+  static constexpr int kThreads = 32 * (kEpiWarps + 2);
+  static constexpr int kBoxCols = BN / (kEpiWarps / 4);  // 64, 32, 32
   static constexpr int kBoxBytes = 32 * kBoxCols * 2;
-  static constexpr int kBoxesBytes = kEpiWarps * 2 * kBoxBytes;
-  static constexpr int kBiasBytes = kEpiWarps * kBoxCols * 4;  // of the box in work
-  static constexpr int kSmem = 232448;                         // of one CTA
-  static constexpr int kStages = (kSmem - kBoxesBytes - kBiasBytes - 512) / kStageBytes;  // pair: 5; 3, 5, 8
+  static constexpr int kBoxesBytes = kEpiWarps * kBoxBytes;
+  static constexpr int kBiasBytes = kEpiWarps * 32 * 4;  // 32 columns a warp
+  static constexpr int kSmem = 232448;                   // of one CTA
+  static constexpr int kStages = (kSmem - kBoxesBytes - kBiasBytes - 512) / kStageBytes;  // pair: 5; 3, 6, 8
   static constexpr int kBoxes = kStages * kStageBytes;
   static constexpr int kBias = kBoxes + kBoxesBytes;
   static constexpr int kBars = kBias + kBiasBytes;
-  // full and empty per stage, full and empty per accumulator, residual per warp and box
-  static constexpr int kNumBars = 2 * kStages + 4 + 2 * kEpiWarps;
+  // full and empty per stage, full and empty per accumulator, residual per warp
+  static constexpr int kNumBars = 2 * kStages + 4 + kEpiWarps;
   static constexpr int kFlags = kBars + kNumBars * 8;
   static constexpr int kBytes = kFlags + 16;
   static_assert(kBytes <= kSmem, "shared memory of one CTA");
@@ -93,9 +94,41 @@ struct GemmMaps {
   CUtensorMap a, b, out, pre, res;
 };
 
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// The normal distribution's cdf at v: its tail q(|v|) as 2 to a polynomial.
+// log2 q is smooth where q itself falls over many orders; the coefficients are a
+// least-maximum fit of degree 8 on [0, 6]: q is off by at most 2.5e-6 of itself
+// up to 3 and 1.2e-5 up to 6 (below 2^-30 there), |v| q by 3e-7, far under half a
+// step of the 16-bit results (2^-12).  Beyond, the polynomial keeps falling and q
+// underflows to 0 (at an infinity too; a NaN stays one).  14 instructions, against
+// some 25 of erff and a division less than the usual rational forms.
+__device__ __forceinline__ float normal_cdf(float v) {
+  const float z = fabsf(v);
+  float p = -1.2245089919815655e-07f;
+  p = fmaf(p, z, 8.983980137600156e-07f);
+  p = fmaf(p, z, 3.7126268580323085e-05f);
+  p = fmaf(p, z, -8.181885350495577e-04f);
+  p = fmaf(p, z, 8.22749175131321e-03f);
+  p = fmaf(p, z, -5.3588107228279114e-02f);
+  p = fmaf(p, z, -4.587007761001587e-01f);
+  p = fmaf(p, z, -1.1511954069137573f);
+  p = fmaf(p, z, -9.999973773956299e-01f);
+  const float q = exp2_fast(p);
+  return v > 0.f ? 1.f - q : q;
+}
+
 __device__ __forceinline__ float activate(float v, int act) {
-  if (act == RFM_ACT_RELU) return v < 0.f ? 0.f : v;  // a NaN stays one
-  if (act == RFM_ACT_GELU) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+  if (act == RFM_ACT_RELU) {  // a NaN stays one
+    float r;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(v));
+    return r;
+  }
+  if (act == RFM_ACT_GELU) return v * normal_cdf(v);
   return v;
 }
 
@@ -103,9 +136,19 @@ __device__ __forceinline__ float activate(float v, int act) {
 __device__ __forceinline__ float activate_grad(float v, int act) {
   if (act == RFM_ACT_RELU) return v > 0.f ? 1.f : 0.f;
   if (act == RFM_ACT_GELU) {
-    return fmaf(0.5f, erff(v * 0.70710678118654752f), 0.5f) + v * 0.39894228040143268f * expf(-0.5f * v * v);
+    // pdf(v) = 2^(-v^2 log2(e) / 2) / sqrt(2 pi)
+    return fmaf(v * 0.39894228040143268f, exp2_fast(v * v * -0.72134752044448170f), normal_cdf(v));
   }
   return 1.f;
+}
+
+// Two fp32 sums in one instruction.
+__device__ __forceinline__ void add2(uint32_t& a, uint32_t& b, float x, float y) {
+  uint64_t s = static_cast<uint64_t>(b) << 32 | a;
+  const uint64_t t = static_cast<uint64_t>(__float_as_uint(y)) << 32 | __float_as_uint(x);
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s) : "l"(t));
+  a = static_cast<uint32_t>(s);
+  b = static_cast<uint32_t>(s >> 32);
 }
 
 template <typename T>
@@ -167,7 +210,7 @@ __device__ __forceinline__ Work work_item(const GemmArgs& a, int64_t w) {
 }
 
 template <typename T, int BN, int CG, bool A_MN, bool B_MN, int ACT>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __launch_bounds__(Shape<BN, CG>::kThreads, 1)
     gemm_kernel(const __grid_constant__ GemmMaps maps, const __grid_constant__ GemmArgs a) {
   using S = Shape<BN, CG>;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -193,14 +236,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(acc_full + 8 * i, 1);
-      mbar_init(acc_empty + 8 * i, kEpiWarps * CG);
+      mbar_init(acc_empty + 8 * i, S::kEpiWarps * CG);
     }
-    for (int i = 0; i < 2 * kEpiWarps; ++i) mbar_init(res_full + 8 * i, 1);
+    for (int i = 0; i < S::kEpiWarps; ++i) mbar_init(res_full + 8 * i, 1);
     mbar_init_fence();
     tma_prefetch_map(&maps.a);
     tma_prefetch_map(&maps.b);
   }
-  if (warp == kMmaWarp) tmem_alloc<CG>(base + S::kFlags + 4, kTmemColumns);
+  if (warp == S::kMmaWarp) tmem_alloc<CG>(base + S::kFlags + 4, kTmemColumns);
   tc_fence_before();
   if (CG == 2) {
     cluster_sync();
@@ -212,7 +255,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   const int64_t items = static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.splits;
   const int64_t first = blockIdx.x / CG, stride = gridDim.x / CG;
 
-  if (warp == kLoadWarp) {
+  if (warp == S::kLoadWarp) {
     if (lane == 0) {
       uint32_t stage = 0, phase = 0, issued = 0;
       bool ok = true;
@@ -268,7 +311,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
       }
     }
-  } else if (warp == kMmaWarp) {
+  } else if (warp == S::kMmaWarp) {
     if (lane == 0 && rank == 0) {
       constexpr int kType = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
       constexpr uint32_t kInstr = mma_instr(kType, A_MN, B_MN, kBM * CG, BN);
@@ -313,210 +356,207 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       }
     }
   } else {
-    constexpr int kCols = S::kBoxCols;        // columns of a box
-    constexpr int kTurns = S::kHalf / kCols;  // boxes of this warp's half of a tile
-    constexpr int kPieces = kCols / 8;        // 16-byte pieces of a box's row
-    const int quarter = warp & 3, half = warp >> 2;
-    const uint32_t boxes = base + S::kBoxes + warp * 2 * S::kBoxBytes;
-    uint8_t* box_ptr = smem + S::kBoxes + warp * 2 * S::kBoxBytes;
-    float* bias_smem = reinterpret_cast<float*>(smem + S::kBias) + warp * kCols;
-    const uint32_t res_bar = res_full + 16 * warp;
+    constexpr int kCols = S::kBoxCols;
+    constexpr int kTurns = kCols / 32;  // 32 columns at a time in registers
+    const int quarter = warp & 3, part = warp >> 2;
+    const uint32_t box = base + S::kBoxes + warp * S::kBoxBytes;
+    uint8_t* box_ptr = smem + S::kBoxes + warp * S::kBoxBytes;
+    float* bias_smem = reinterpret_cast<float*>(smem + S::kBias) + warp * 32;
+    const uint32_t res_bar = res_full + 8 * warp;
+    const uint32_t released = CG == 2 ? map_rank(acc_empty, 0) : acc_empty;
     const bool whole = a.splits == 1;
     const bool has_bias = whole && a.bias != nullptr;
     const bool has_res = whole && a.residual != nullptr, has_pre = whole && a.pre != nullptr;
-    const bool tma_res = has_res && a.tma_res;
-    uint32_t acc = 0, acc_phase = 0, box = 0, res_phase = 0;
-    // where a lane's 16-byte pieces of its row go in a box: the TMA swizzle of
+    // the box can only wait for the residual where `pre` does not pass through it first
+    const bool tma_res = has_res && a.tma_res && !has_pre;
+    // beside `pre`, the aligned residual comes straight from memory, 8 columns at a time
+    const bool straight = has_res && a.tma_res && has_pre && (a.n & 7) == 0;
+    uint32_t acc = 0, acc_phase = 0, res_phase = 0;
+    // where a lane's 16-byte pieces of its row go in the box: the TMA swizzle of
     // its row length, which also spreads the lanes' accesses over the banks
     const int row_off = lane * kCols * 2, swz = kCols == 64 ? lane & 7 : (lane >> 1) & 3;
-
-    constexpr int kBiasRegs = kCols / 32;
-    const uint32_t released = CG == 2 ? map_rank(acc_empty, 0) : acc_empty;
+    const auto piece = [&](int j) { return reinterpret_cast<uint4*>(box_ptr + row_off + ((j ^ swz) << 4)); };
+    // element (r, c) of the box
+    const auto cell = [&](int r, int c) {
+      return reinterpret_cast<T*>(box_ptr) + r * kCols +
+             (((c >> 3) ^ (kCols == 64 ? r & 7 : (r >> 1) & 3)) << 3) + (c & 7);
+    };
 
     for (int64_t w = first; w < items; w += stride) {
       const Work t = work_item(a, w);
       const int64_t row0 = (static_cast<int64_t>(t.tile_m) * CG + rank) * kBM + quarter * 32;
-      const int col_base = t.tile_n * BN + half * S::kHalf;
-      const bool rows_in = row0 < a.m;
-      bool live = true;
-      // the bias of a box, read one box ahead: lane l holds columns l, l + 32
-      float bias[kBiasRegs];
-      const auto read_bias = [&](int turn) {
+      const int col0 = t.tile_n * BN + part * kCols;
+      const bool inside = row0 < a.m && col0 < a.n;
+      float bias[kTurns];
+      if (inside && has_bias) {
 #pragma unroll
-        for (int j = 0; j < kBiasRegs; ++j) {
-          const int col = col_base + turn * kCols + j * 32 + lane;
-          bias[j] = col < a.n ? load_param(a.bias, a.bias_dtype, col) : 0.f;
+        for (int s = 0; s < kTurns; ++s) {
+          const int col = col0 + s * 32 + lane;
+          bias[s] = col < a.n ? load_param(a.bias, a.bias_dtype, col) : 0.f;
         }
-      };
-      if (has_bias) read_bias(0);
-      // the first box's residual travels while the products are still running
-      const auto fetch = [&](int turn, uint32_t b) {
-        const int col0 = col_base + turn * kCols;
-        if (lane == 0 && rows_in && col0 < a.n) {
+      }
+      if (inside && whole) {
+        // the box's last store has been read before anything is written to it
+        if (lane == 0) {
           tma_wait_read<0>();
-          proxy_fence();
-          mbar_expect(res_bar + 8 * b, S::kBoxBytes);
-          tma_load_2d(boxes + b * S::kBoxBytes, &maps.res, col0, static_cast<int>(row0), res_bar + 8 * b);
+          if (tma_res) {
+            proxy_fence();
+            mbar_expect(res_bar, S::kBoxBytes);
+            tma_load_2d(box, &maps.res, col0, static_cast<int>(row0), res_bar);
+          }
         }
         __syncwarp();
-      };
-      if (tma_res) fetch(0, has_pre ? 0u : box);
-      live = __all_sync(kFullMask, bounded_wait(acc_full + 8 * acc, acc_phase, dead));
+      }
+      bool live = __all_sync(kFullMask, bounded_wait(acc_full + 8 * acc, acc_phase, dead));
       tc_fence_after();
-#pragma unroll 1
-      for (int turn = 0; turn < kTurns; ++turn) {
-        const int col0 = col_base + turn * kCols;
-        const bool inside = rows_in && col0 < a.n;
-        // boxes alternate, or the first is the output's and the second `pre`'s
-        const uint32_t b = has_pre ? 0u : box;
-        uint32_t v[kCols];
-        {
-          const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * BN + half * S::kHalf +
-                                turn * kCols;
-          uint32_t(&low)[32] = *reinterpret_cast<uint32_t(*)[32]>(&v[0]);
-          uint32_t(&high)[32] = *reinterpret_cast<uint32_t(*)[32]>(&v[kCols - 32]);
-          tmem_load_32(low, from);
-          if (kCols == 64) tmem_load_32(high, from + kCols - 32);
-          tmem_wait_load(low);
-          if (kCols == 64) tmem_wait_load(high);
-        }
-        if (turn == kTurns - 1) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            if (CG == 2) {
-              mbar_arrive_cluster(released + 8 * acc);
-            } else {
-              mbar_arrive(released + 8 * acc);
-            }
+      const uint32_t from =
+          tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * BN + part * kCols;
+      const auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (CG == 2) {
+            mbar_arrive_cluster(released + 8 * acc);
+          } else {
+            mbar_arrive(released + 8 * acc);
           }
         }
-        if (!inside) continue;
-        if (!whole) {
-          const int64_t row = row0 + lane;
-          if (row < a.m && live) {
-            float* dst = a.partial + (static_cast<int64_t>(t.split) * a.m + row) * a.n + col0;
-            if ((a.n & 3) == 0 && col0 + kCols <= a.n) {
-#pragma unroll
-              for (int j = 0; j < kCols / 4; ++j)
-                reinterpret_cast<uint4*>(dst)[j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-            } else {
-#pragma unroll
-              for (int j = 0; j < kCols; ++j)
-                if (col0 + j < a.n) dst[j] = __uint_as_float(v[j]);
-            }
-          }
-          continue;
-        }
-        if (tma_res) {
-          // the next box's residual, into the box that the store before last has left
-          if (!has_pre && turn + 1 < kTurns) fetch(turn + 1, box ^ 1u);
-        } else {
-          // the box's last store must have been read before it is overwritten
-          if (lane == 0) {
-            if (has_pre) {
-              tma_wait_read<0>();
-            } else {
-              tma_wait_read<1>();
-            }
-          }
-          __syncwarp();
-        }
+      };
+      // columns s * 32 .. of this lane's row, with the bias
+      const auto take = [&](uint32_t(&v)[32], int s) {
+        tmem_load_32(v, from + s * 32);
         if (has_bias) {
           __syncwarp();
-#pragma unroll
-          for (int j = 0; j < kBiasRegs; ++j) bias_smem[j * 32 + lane] = bias[j];
+          bias_smem[lane] = bias[s];
           __syncwarp();
-          if (turn + 1 < kTurns) read_bias(turn + 1);
+        }
+        tmem_wait_load(v);
+        if (has_bias) {
 #pragma unroll
-          for (int j = 0; j < kCols / 4; ++j) {
+          for (int j = 0; j < 8; ++j) {
             const float4 q = reinterpret_cast<const float4*>(bias_smem)[j];
-            v[4 * j] = __float_as_uint(__uint_as_float(v[4 * j]) + q.x);
-            v[4 * j + 1] = __float_as_uint(__uint_as_float(v[4 * j + 1]) + q.y);
-            v[4 * j + 2] = __float_as_uint(__uint_as_float(v[4 * j + 2]) + q.z);
-            v[4 * j + 3] = __float_as_uint(__uint_as_float(v[4 * j + 3]) + q.w);
+            add2(v[4 * j], v[4 * j + 1], q.x, q.y);
+            add2(v[4 * j + 2], v[4 * j + 3], q.z, q.w);
           }
         }
-        const auto put = [&](uint32_t which) {
+      };
+      const auto put = [&](const uint32_t(&v)[32], int s) {
 #pragma unroll
-          for (int j = 0; j < kPieces; ++j) {
-            uint32_t p[4];
+        for (int j = 0; j < 4; ++j) {
+          uint32_t p[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              p[i] = pack2<T>(__uint_as_float(v[8 * j + 2 * i]), __uint_as_float(v[8 * j + 2 * i + 1]));
-            *reinterpret_cast<uint4*>(box_ptr + which * S::kBoxBytes + row_off + ((j ^ swz) << 4)) =
-                make_uint4(p[0], p[1], p[2], p[3]);
-          }
-        };
-        if (has_pre) put(1);
-        if (ACT != RFM_ACT_NONE) {
-#pragma unroll
-          for (int j = 0; j < kCols; ++j) v[j] = __float_as_uint(activate(__uint_as_float(v[j]), ACT));
+          for (int i = 0; i < 4; ++i)
+            p[i] = pack2<T>(__uint_as_float(v[8 * j + 2 * i]), __uint_as_float(v[8 * j + 2 * i + 1]));
+          *piece(s * 4 + j) = make_uint4(p[0], p[1], p[2], p[3]);
         }
-        // element (r, c) of a box lies at cell r * kCols + (piece ^ swizzle) * 8 + c % 8
-        const auto cell = [](int r, int c) {
-          return r * kCols + (((c >> 3) ^ (kCols == 64 ? r & 7 : (r >> 1) & 3)) << 3) + (c & 7);
-        };
-        if (has_res) {
-          if (tma_res) {
-            live = __all_sync(kFullMask, bounded_wait(res_bar + 8 * b, (res_phase >> b) & 1u, dead) && live);
-            res_phase ^= 1u << b;
-          } else {
-            // rows whose start is not a multiple of 16 bytes: element by element, a lane a column
-            T* cells = reinterpret_cast<T*>(box_ptr + b * S::kBoxBytes);
-            const T* res = static_cast<const T*>(a.residual);
-            for (int r = 0; r < 32; ++r) {
-              const int64_t row = row0 + r;
-#pragma unroll
-              for (int c = lane; c < kCols; c += 32)
-                cells[cell(r, c)] =
-                    row < a.m && col0 + c < a.n ? res[row * a.ld_res + col0 + c] : from_float<T>(0.f);
-            }
-            __syncwarp();
-          }
-#pragma unroll
-          for (int j = 0; j < kPieces; ++j) {
-            const uint4 q =
-                *reinterpret_cast<const uint4*>(box_ptr + b * S::kBoxBytes + row_off + ((j ^ swz) << 4));
-            const uint32_t words[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 two = unpack2<T>(words[i]);
-              v[8 * j + 2 * i] = __float_as_uint(__uint_as_float(v[8 * j + 2 * i]) + two.x);
-              v[8 * j + 2 * i + 1] = __float_as_uint(__uint_as_float(v[8 * j + 2 * i + 1]) + two.y);
-            }
-          }
-        }
-        put(b);
+      };
+      // the filled box goes out: by TMA, or a lane a column where rows do not start on 16 bytes
+      const auto send = [&](const CUtensorMap* map, void* to) {
         if (a.tma_out) {
           proxy_fence();
           __syncwarp();
           if (lane == 0 && live) {
-            tma_store_2d(&maps.out, col0, static_cast<int>(row0), boxes + b * S::kBoxBytes);
-            if (has_pre) tma_store_2d(&maps.pre, col0, static_cast<int>(row0), boxes + S::kBoxBytes);
+            tma_store_2d(map, col0, static_cast<int>(row0), box);
             tma_commit();
           }
         } else {
           __syncwarp();
-          if (live) {
-            for (int r = 0; r < 32; ++r) {
-              const int64_t row = row0 + r;
+          for (int r = 0; r < 32 && live; ++r) {
+            const int64_t row = row0 + r;
 #pragma unroll
-              for (int c = lane; c < kCols; c += 32) {
-                if (row >= a.m || col0 + c >= a.n) continue;
-                const int64_t at = row * a.n + col0 + c;
-                static_cast<T*>(a.out)[at] = reinterpret_cast<const T*>(box_ptr + b * S::kBoxBytes)[cell(r, c)];
-                if (has_pre) {
-                  static_cast<T*>(a.pre)[at] = reinterpret_cast<const T*>(box_ptr + S::kBoxBytes)[cell(r, c)];
-                }
-              }
-            }
+            for (int c = lane; c < kCols; c += 32)
+              if (row < a.m && col0 + c < a.n) static_cast<T*>(to)[row * a.n + col0 + c] = *cell(r, c);
           }
           __syncwarp();
         }
-        // one box for residual and output: the next residual follows this store
-        if (tma_res && has_pre && turn + 1 < kTurns) fetch(turn + 1, 0);
-        box ^= 1u;
+      };
+
+      if (!inside) {
+        release();
+      } else if (!whole) {
+        const int64_t row = row0 + lane;
+        float* dst = a.partial + (static_cast<int64_t>(t.split) * a.m + row) * a.n + col0;
+#pragma unroll
+        for (int s = 0; s < kTurns; ++s) {
+          uint32_t v[32];
+          tmem_load_32(v, from + s * 32);
+          tmem_wait_load(v);
+          if (s == kTurns - 1) release();
+          if (row >= a.m || !live) continue;
+          if ((a.n & 3) == 0 && col0 + s * 32 + 32 <= a.n) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              reinterpret_cast<uint4*>(dst + s * 32)[j] =
+                  make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (col0 + s * 32 + j < a.n) dst[s * 32 + j] = __uint_as_float(v[j]);
+          }
+        }
+      } else {
+        if (has_pre) {
+#pragma unroll
+          for (int s = 0; s < kTurns; ++s) {
+            uint32_t v[32];
+            take(v, s);
+            put(v, s);
+          }
+          send(&maps.pre, a.pre);
+        }
+        if (tma_res) {
+          live = __all_sync(kFullMask, bounded_wait(res_bar, res_phase, dead) && live);
+          res_phase ^= 1u;
+        } else if (has_res && !straight) {
+          // residual rows that do not start on 16 bytes: element by element, a lane a column
+          if (lane == 0) tma_wait_read<0>();
+          __syncwarp();
+          const T* res = static_cast<const T*>(a.residual);
+          for (int r = 0; r < 32; ++r) {
+            const int64_t row = row0 + r;
+#pragma unroll
+            for (int c = lane; c < kCols; c += 32)
+              *cell(r, c) = row < a.m && col0 + c < a.n ? res[row * a.ld_res + col0 + c] : from_float<T>(0.f);
+          }
+          __syncwarp();
+        }
+#pragma unroll
+        for (int s = 0; s < kTurns; ++s) {
+          uint4 direct[4];
+          if (straight) {
+            const int64_t row = row0 + lane;
+            const T* res = static_cast<const T*>(a.residual) + row * a.ld_res + col0 + s * 32;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              direct[j] = row < a.m && col0 + s * 32 + j * 8 < a.n ? reinterpret_cast<const uint4*>(res)[j]
+                                                                   : make_uint4(0, 0, 0, 0);
+          }
+          uint32_t v[32];
+          take(v, s);
+          if (s == kTurns - 1) release();
+          if (ACT != RFM_ACT_NONE) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(activate(__uint_as_float(v[j]), ACT));
+          }
+          if (has_res) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint4 q = straight ? direct[j] : *piece(s * 4 + j);
+              const uint32_t words[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float2 two = unpack2<T>(words[i]);
+                add2(v[8 * j + 2 * i], v[8 * j + 2 * i + 1], two.x, two.y);
+              }
+            }
+          }
+          if (has_pre && s == 0) {  // `pre` has been read out of the box
+            if (lane == 0) tma_wait_read<0>();
+            __syncwarp();
+          }
+          put(v, s);
+        }
+        send(&maps.out, a.out);
       }
       if (!live) break;
       acc ^= 1u;
@@ -531,7 +571,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   } else {
     __syncthreads();
   }
-  if (warp == kMmaWarp) {
+  if (warp == S::kMmaWarp) {
     tc_fence_after();
     tmem_free<CG>(tmem, kTmemColumns);
   }
@@ -806,7 +846,7 @@ int launch_gemm(const Product& p, GemmArgs& g, float* partial, cudaStream_t stre
   const int64_t workers = sms / CG;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>((items < workers ? items : workers) * CG));
-  config.blockDim = dim3(kGemmThreads);
+  config.blockDim = dim3(S::kThreads);
   config.dynamicSmemBytes = S::kBytes;
   config.stream = stream;
   cudaLaunchAttribute cluster{};
