@@ -154,30 +154,92 @@ __device__ __forceinline__ void store_codes(uint32_t w, void* base, int64_t i, i
 constexpr float kInv127 = static_cast<float>(1.0 / 127.0);
 constexpr float kInv255 = static_cast<float>(1.0 / 255.0);
 
-__device__ __forceinline__ float decode_m(uint32_t code, float scale) {
-  const float a = __fmul_rn(static_cast<float>(static_cast<int8_t>(code)), kInv127);
+// Byte j of a word as a float, through the mantissa of 2^23 (conversions run at
+// an eighth of the rate of additions).
+__device__ __forceinline__ float byte_float(uint32_t w, int j) {
+  return __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440u + j)) - 8388608.f;
+}
+
+// `flipped`: the word of codes with every byte's top bit inverted (c + 128).
+__device__ __forceinline__ float decode_m(uint32_t flipped, int j, float scale) {
+  const float a = __fmul_rn(byte_float(flipped, j) - 128.f, kInv127);
   return __fmul_rn(scale, __fmul_rn(a, fabsf(a)));
 }
 
-__device__ __forceinline__ float decode_v(uint32_t code, float scale) {
-  float b = __fmul_rn(static_cast<float>(code & 0xffu), kInv255);
+__device__ __forceinline__ float decode_v(uint32_t codes, int j, float scale) {
+  float b = __fmul_rn(byte_float(codes, j), kInv255);
   b = __fmul_rn(b, b);
   return __fmul_rn(scale, __fmul_rn(b, b));
 }
 
-// A NaN quotient (a block of zeros, or of infinities) converts to code 0.
-__device__ __forceinline__ uint32_t encode_m(float m, float scale, uint32_t h) {
+// The codes by definition.  A NaN quotient (a block of zeros, or of infinities)
+// converts to code 0.
+__device__ __noinline__ uint32_t exact_code_m(float m, float scale, uint32_t h) {
   const float u = __fmul_rn(static_cast<float>(h & 0xffffu), 1.f / 65536.f);
   const float x = __fadd_rn(__fmul_rn(__fsqrt_rn(__fdiv_rn(fabsf(m), scale)), 127.f), u);
-  const int q = min(__float2int_rz(x), 127);
-  return static_cast<uint32_t>(m < 0.f ? -q : q) & 0xffu;
+  return static_cast<uint32_t>(min(__float2int_rz(x), 127));
 }
 
-__device__ __forceinline__ uint32_t encode_v(float v, float scale, uint32_t h) {
+__device__ __noinline__ uint32_t exact_code_v(float v, float scale, uint32_t h) {
   const float u = __fmul_rn(static_cast<float>(h >> 16), 1.f / 65536.f);
   const float x = __fadd_rn(__fmul_rn(__fsqrt_rn(__fsqrt_rn(__fdiv_rn(v, scale))), 255.f), u);
-  const int q = min(__float2int_rz(x), 255);
-  return static_cast<uint32_t>(v > 0.f ? max(q, 1) : q);
+  return static_cast<uint32_t>(min(__float2int_rz(x), 255));
+}
+
+__device__ __forceinline__ float sqrt_fast(float x) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Codes the quick way: with the scale's reciprocal and the approximate root the
+// value x is off by at most 255 * 2^-21 = 1.2e-4 from the definition's (the root
+// and the reciprocal 2^-22 of themselves each, the roundings of both ways 2^-23
+// and less).  Where x lies further than kNear from a whole number both have the
+// same floor; `sure` says so, and false also for a NaN or an infinity.  About
+// one code in 2500 is computed again.
+constexpr float kNear = 2e-4f;
+
+__device__ __forceinline__ uint32_t quick_floor(float root, float top, uint32_t bits16, bool& sure) {
+  // 1 + the random fraction, exactly: its 16 bits at the top of the mantissa
+  const float one_u = __uint_as_float(0x3F800000u | (bits16 & 0x7fff80u));
+  const float x1 = fmaf(root, top, one_u);           // x + 1
+  const float low = __fadd_rd(x1, 8388607.f);        // 2^23 + floor(x)
+  const float part = x1 - (low - 8388607.f);         // x - floor(x)
+  sure = sure && fabsf(part - 0.5f) < 0.5f - kNear;
+  return __float_as_uint(low) & 0xffu;
+}
+
+// The codes of four elements, element j in byte j; `inv`: the scale's reciprocal
+//.
+__device__ __forceinline__ uint32_t encode_m(const float (&m)[4], float scale, float inv, const uint32_t (&h)[4]) {
+  uint32_t q[4];
+  bool sure = true;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) q[j] = quick_floor(sqrt_fast(fabsf(m[j]) * inv), 127.f, h[j] << 7, sure);
+  if (!sure) {  // a scale of 0 ends here too: its block is all zeros
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q[j] = scale == 0.f ? 0u : exact_code_m(m[j], scale, h[j]);
+  }
+  uint32_t w = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w |= ((m[j] < 0.f ? 0u - q[j] : q[j]) & 0xffu) << (8 * j);
+  return w;
+}
+
+__device__ __forceinline__ uint32_t encode_v(const float (&v)[4], float scale, float inv, const uint32_t (&h)[4]) {
+  uint32_t q[4];
+  bool sure = true;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) q[j] = quick_floor(sqrt_fast(sqrt_fast(v[j] * inv)), 255.f, h[j] >> 9, sure);
+  if (!sure) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q[j] = scale == 0.f ? 0u : exact_code_v(v[j], scale, h[j]);
+  }
+  uint32_t w = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w |= (v[j] > 0.f ? max(q[j], 1u) : q[j]) << (8 * j);
+  return w;
 }
 
 // Largest of a warp's non-negative values (their bit patterns order as the
@@ -247,14 +309,17 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
         float& mj = m[b][q][j];
         float& vj = v[b][q][j];
         if (EIGHT) {
-          mj = decode_m(cm[b][q] >> (8 * j), sm[b]);
-          vj = decode_v(cv[b][q] >> (8 * j), sv[b]);
+          mj = decode_m(cm[b][q] ^ 0x80808080u, j, sm[b]);
+          vj = decode_v(cv[b][q], j, sv[b]);
         }
         const float gj = __fmul_rn(g[b][q][j], grad_scale);
         mj = __fadd_rn(__fmul_rn(mj, a.c.b1), __fmul_rn(gj, a.c.one_b1));
         vj = __fadd_rn(__fmul_rn(vj, a.c.b2), __fmul_rn(__fmul_rn(gj, gj), a.c.one_b2));
-        const float denom = fmaf(sqrtf(vj), s.inv_sqrt_bc2, a.c.eps);
-        pj = fmaf(pj, s.keep, -s.step_size * (mj / denom));
+        // approximate root and quotient: 2^-22 of an update that is a small part of the parameter
+        float root;  // of subnormal values too: with eps 0 a root of 0 would be divided by
+        asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(vj));
+        const float denom = fmaf(root, s.inv_sqrt_bc2, a.c.eps);
+        pj = fmaf(pj, s.keep, -s.step_size * __fdividef(mj, denom));
         if (EIGHT) {
           // elements past the tensor's end count as zeros whatever their block's scale is
           const bool in = base + b * kBlock + q * 128 + lane * 4 + j < n;
@@ -272,18 +337,15 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     if (EIGHT) {
       const uint32_t key = mix(t.ordinal * 0x632BE5ABu + s.seed);
       const float new_sm = warp_max_bits(top_m), new_sv = warp_max_bits(top_v);
+      const float inv_m = __frcp_rn(new_sm), inv_v = __frcp_rn(new_sv);
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         const int64_t i = base + b * kBlock + q * 128 + lane * 4;
-        uint32_t wm = 0, wv = 0;
+        uint32_t h[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t h = mix(static_cast<uint32_t>(i + j) + key);
-          wm |= encode_m(m[b][q][j], new_sm, h) << (8 * j);
-          wv |= encode_v(v[b][q][j], new_sv, h) << (8 * j);
-        }
-        store_codes(wm, t.m, i, n, vec);
-        store_codes(wv, t.v, i, n, vec);
+        for (int j = 0; j < 4; ++j) h[j] = mix(static_cast<uint32_t>(i + j) + key);
+        store_codes(encode_m(m[b][q], new_sm, inv_m, h), t.m, i, n, vec);
+        store_codes(encode_v(v[b][q], new_sv, inv_v, h), t.v, i, n, vec);
       }
       const int64_t first = base + b * kBlock;
       if (lane == 0 && first < n) {
@@ -311,8 +373,8 @@ __global__ void __launch_bounds__(kThreads) adam_moments_kernel(const void* m, c
     float dm[4], dv[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      dm[j] = decode_m(cm >> (8 * j), sm);
-      dv[j] = decode_v(cv >> (8 * j), sv);
+      dm[j] = decode_m(cm ^ 0x80808080u, j, sm);
+      dv[j] = decode_v(cv, j, sv);
     }
     store_quad<float>(dm, out_m, i, n, vec);
     store_quad<float>(dv, out_v, i, n, vec);

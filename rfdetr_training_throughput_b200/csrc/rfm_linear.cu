@@ -193,19 +193,28 @@ struct Work {
   int tile_m, tile_n, split, k0, k1;
 };
 
-__device__ __forceinline__ Work work_item(const GemmArgs& a, int64_t w) {
+__device__ __forceinline__ Work work_item(const GemmArgs& a, uint32_t w) {
   Work r;
-  r.split = static_cast<int>(w % a.splits);
-  const int64_t tile = w / a.splits;
-  constexpr int kGroup = 16;
-  const int64_t per_group = static_cast<int64_t>(kGroup) * a.tiles_n;
-  const int group = static_cast<int>(tile / per_group);
-  const int inside = static_cast<int>(tile % per_group);
-  const int height = min(kGroup, a.tiles_m - group * kGroup);
-  r.tile_m = group * kGroup + inside % height;
-  r.tile_n = inside / height;
-  r.k0 = static_cast<int>(static_cast<int64_t>(a.k_blocks) * r.split / a.splits);
-  r.k1 = static_cast<int>(static_cast<int64_t>(a.k_blocks) * (r.split + 1) / a.splits);
+  uint32_t tile = w;
+  r.split = 0;
+  r.k0 = 0;
+  r.k1 = a.k_blocks;
+  if (a.splits > 1) {
+    const uint32_t splits = static_cast<uint32_t>(a.splits);
+    tile = w / splits;
+    r.split = static_cast<int>(w - tile * splits);
+    // whole slices to every part, one more to the first ones
+    const int each = a.k_blocks / a.splits, more = a.k_blocks - each * a.splits;
+    r.k0 = each * r.split + min(r.split, more);
+    r.k1 = r.k0 + each + (r.split < more ? 1 : 0);
+  }
+  constexpr uint32_t kGroup = 16;
+  const uint32_t per_group = kGroup * static_cast<uint32_t>(a.tiles_n);
+  const uint32_t group = tile / per_group, inside = tile - group * per_group;
+  const uint32_t height = min(kGroup, static_cast<uint32_t>(a.tiles_m) - group * kGroup);
+  const uint32_t column = height == kGroup ? inside / kGroup : inside / height;
+  r.tile_m = static_cast<int>(group * kGroup + inside - column * height);
+  r.tile_n = static_cast<int>(column);
   return r;
 }
 
@@ -252,14 +261,14 @@ __global__ void __launch_bounds__(Shape<BN, CG>::kThreads, 1)
   }
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<const volatile uint32_t*>(smem + S::kFlags + 4);
-  const int64_t items = static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.splits;
-  const int64_t first = blockIdx.x / CG, stride = gridDim.x / CG;
+  const uint32_t items = static_cast<uint32_t>(a.tiles_m) * a.tiles_n * a.splits;  // below 2^31
+  const uint32_t first = blockIdx.x / CG, stride = gridDim.x / CG;
 
   if (warp == S::kLoadWarp) {
     if (lane == 0) {
       uint32_t stage = 0, phase = 0, issued = 0;
       bool ok = true;
-      for (int64_t w = first; ok && w < items; w += stride) {
+      for (uint32_t w = first; ok && w < items; w += stride) {
         const Work t = work_item(a, w);
         const int m0 = (t.tile_m * CG + static_cast<int>(rank)) * kBM;
         const int n0 = t.tile_n * BN + static_cast<int>(rank) * S::kBRows;
@@ -318,7 +327,7 @@ __global__ void __launch_bounds__(Shape<BN, CG>::kThreads, 1)
       constexpr uint32_t kAStep = A_MN ? 2048 : 32, kBStep = B_MN ? 2048 : 32;  // bytes of 16 along k
       uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
       bool ok = true;
-      for (int64_t w = first; ok && w < items; w += stride) {
+      for (uint32_t w = first; ok && w < items; w += stride) {
         const Work t = work_item(a, w);
         if (!bounded_wait(acc_empty + 8 * acc, acc_phase ^ 1u, dead)) break;
         tc_fence_after();
@@ -382,28 +391,30 @@ __global__ void __launch_bounds__(Shape<BN, CG>::kThreads, 1)
              (((c >> 3) ^ (kCols == 64 ? r & 7 : (r >> 1) & 3)) << 3) + (c & 7);
     };
 
-    for (int64_t w = first; w < items; w += stride) {
-      const Work t = work_item(a, w);
+    // lane l holds the bias of its box's columns l and l + 32, read a tile ahead
+    float bias[kTurns];
+    const auto read_bias = [&](int tile_n) {
+#pragma unroll
+      for (int s = 0; s < kTurns; ++s) {
+        const int col = tile_n * BN + part * kCols + s * 32 + lane;
+        bias[s] = col < a.n ? load_param(a.bias, a.bias_dtype, col) : 0.f;
+      }
+    };
+    Work next = work_item(a, min(first, items - 1));
+    if (has_bias) read_bias(next.tile_n);
+
+    for (uint32_t w = first; w < items; w += stride) {
+      const Work t = next;
       const int64_t row0 = (static_cast<int64_t>(t.tile_m) * CG + rank) * kBM + quarter * 32;
       const int col0 = t.tile_n * BN + part * kCols;
       const bool inside = row0 < a.m && col0 < a.n;
-      float bias[kTurns];
-      if (inside && has_bias) {
-#pragma unroll
-        for (int s = 0; s < kTurns; ++s) {
-          const int col = col0 + s * 32 + lane;
-          bias[s] = col < a.n ? load_param(a.bias, a.bias_dtype, col) : 0.f;
-        }
-      }
-      if (inside && whole) {
-        // the box's last store has been read before anything is written to it
+      if (w + stride < items) next = work_item(a, w + stride);
+      if (inside && tma_res) {
         if (lane == 0) {
           tma_wait_read<0>();
-          if (tma_res) {
-            proxy_fence();
-            mbar_expect(res_bar, S::kBoxBytes);
-            tma_load_2d(box, &maps.res, col0, static_cast<int>(row0), res_bar);
-          }
+          proxy_fence();
+          mbar_expect(res_bar, S::kBoxBytes);
+          tma_load_2d(box, &maps.res, col0, static_cast<int>(row0), res_bar);
         }
         __syncwarp();
       }
@@ -440,6 +451,11 @@ __global__ void __launch_bounds__(Shape<BN, CG>::kThreads, 1)
           }
         }
       };
+      // the box's last store has been read before anything is written to it
+      const auto box_free = [&] {
+        if (lane == 0) tma_wait_read<0>();
+        __syncwarp();
+      };
       const auto put = [&](const uint32_t(&v)[32], int s) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -473,6 +489,7 @@ __global__ void __launch_bounds__(Shape<BN, CG>::kThreads, 1)
 
       if (!inside) {
         release();
+        if (has_bias) read_bias(next.tile_n);
       } else if (!whole) {
         const int64_t row = row0 + lane;
         float* dst = a.partial + (static_cast<int64_t>(t.split) * a.m + row) * a.n + col0;
@@ -500,6 +517,7 @@ __global__ void __launch_bounds__(Shape<BN, CG>::kThreads, 1)
           for (int s = 0; s < kTurns; ++s) {
             uint32_t v[32];
             take(v, s);
+            if (s == 0) box_free();
             put(v, s);
           }
           send(&maps.pre, a.pre);
@@ -509,8 +527,7 @@ __global__ void __launch_bounds__(Shape<BN, CG>::kThreads, 1)
           res_phase ^= 1u;
         } else if (has_res && !straight) {
           // residual rows that do not start on 16 bytes: element by element, a lane a column
-          if (lane == 0) tma_wait_read<0>();
-          __syncwarp();
+          box_free();
           const T* res = static_cast<const T*>(a.residual);
           for (int r = 0; r < 32; ++r) {
             const int64_t row = row0 + r;
@@ -533,7 +550,10 @@ __global__ void __launch_bounds__(Shape<BN, CG>::kThreads, 1)
           }
           uint32_t v[32];
           take(v, s);
-          if (s == kTurns - 1) release();
+          if (s == kTurns - 1) {
+            release();
+            if (has_bias) read_bias(next.tile_n);
+          }
           if (ACT != RFM_ACT_NONE) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(activate(__uint_as_float(v[j]), ACT));
@@ -550,10 +570,7 @@ __global__ void __launch_bounds__(Shape<BN, CG>::kThreads, 1)
               }
             }
           }
-          if (has_pre && s == 0) {  // `pre` has been read out of the box
-            if (lane == 0) tma_wait_read<0>();
-            __syncwarp();
-          }
+          if (s == 0 && (!has_res || straight)) box_free();  // a residual in the box has waited for it
           put(v, s);
         }
         send(&maps.out, a.out);
@@ -842,6 +859,7 @@ int launch_gemm(const Product& p, GemmArgs& g, float* partial, cudaStream_t stre
     ready = context;
   }
   const int64_t items = static_cast<int64_t>(g.tiles_m) * g.tiles_n * g.splits;
+  if (items >= (int64_t(1) << 31) - (1 << 16)) return RFM_ERR_UNSUPPORTED;
   const int sms = device_sm_count();
   const int64_t workers = sms / CG;
   cudaLaunchConfig_t config{};

@@ -12,9 +12,12 @@
 //
 // HBM-bound: the forward moves 2 and the backward 3 arrays of rows x D.  A team
 // of TEAM threads keeps one row in registers (TEAM * VEC * CH >= D), so every
-// element is read once; the next row's loads are issued before the current row
-// is reduced.  Teams of 8 lanes for short rows, a warp (no barrier) up to 512
-// columns, a CTA of 128 to 512 threads up to 8192; longer rows are re-read from L2.
+// element is read once.  Teams of 8 lanes for short rows, a warp (no barrier) up to
+// 512 columns, 128 to 512 threads up to 8192; longer rows are re-read from L2.
+// Each thread copies its own 16-byte pieces of the next DEPTH rows into shared
+// memory ahead of time (cp.async; nobody else reads them, so no barrier is
+// needed): bytes in flight, some 100 KB an SM, are what the bandwidth hangs on,
+// and registers could hold only one row more.
 // The weight and bias gradients are summed in registers over a team's rows (a
 // thread always owns the same columns), then over the CTA's teams in shared
 // memory, then over the CTAs by a second kernel, all in a fixed order: no
@@ -26,14 +29,15 @@
 namespace rfm {
 namespace {
 
-constexpr int kThreads = 256;  // of a CTA of several teams, and of the kernels without teams
+constexpr int kThreads = 256;  // of the kernels without teams
 constexpr int kWarps = kThreads / 32;
-constexpr int kMostWarps = 16;  // of a team
-
-// Threads of a CTA: a team of more than a warp has a CTA to itself.
-__host__ __device__ constexpr int cta_threads(int team) { return team > 32 ? team : kThreads; }
 constexpr int kWideDim = 8192;  // longest row held in registers
 constexpr int kWideSlabs = 64;  // row slabs of the wide rows' parameter gradients
+
+// Threads of a CTA of teams.
+__host__ __device__ constexpr int cta_threads(int team) { return team > 32 ? 512 : 256; }
+// Rows a thread copies ahead (0: element loads, one row ahead in registers).
+__host__ __device__ constexpr int ring_depth(int vec, int ch) { return vec == 1 ? 0 : ch == 1 ? 4 : 2; }
 
 struct NormArgs {
   const void* x;
@@ -55,34 +59,98 @@ struct NormArgs {
   float inv_dim;
 };
 
-template <typename T, int VEC>
-__device__ __forceinline__ void load_row(Pack<T, VEC>& r, const T* row, int col, int dim, bool valid) {
-  if (valid && col < dim) {
-    r = *reinterpret_cast<const Pack<T, VEC>*>(row + col);
-  } else {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) r.v[j] = from_float<T>(0.f);
+// One thread's pieces of rows to come: copied ahead into its own places of
+// shared memory, or (element loads) one row ahead in registers.
+template <typename T, int VEC, int TEAM, int CH>
+struct Ahead {
+  static constexpr int kDepth = ring_depth(VEC, CH);
+  static constexpr int kThreadsCta = cta_threads(TEAM);
+  static constexpr int kBytes = kDepth * CH * kThreadsCta * 16;  // of one array
+  static constexpr int kStep = TEAM * VEC;
+  const T* at;     // the array
+  int64_t ld;
+  int dim, lane;
+  uint8_t* smem;   // this array's ring
+  Pack<T, VEC> next[kDepth == 0 ? CH : 1];
+
+  __device__ __forceinline__ Ahead(const void* base, int64_t ld_, int dim_, int lane_, uint8_t* ring)
+      : at(static_cast<const T*>(base)), ld(ld_), dim(dim_), lane(lane_), smem(ring) {}
+
+  __device__ __forceinline__ uint8_t* place(int slot, int c) const {
+    return smem + ((slot * CH + c) * kThreadsCta + static_cast<int>(threadIdx.x)) * 16;
   }
+
+  __device__ __forceinline__ void request(int64_t row, bool valid, int slot) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int col = c * kStep + lane * VEC;
+      if constexpr (kDepth > 0) {
+        if (valid && col < dim) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                           static_cast<uint32_t>(__cvta_generic_to_shared(place(slot, c)))),
+                       "l"(at + row * ld + col)
+                       : "memory");
+        }
+      } else {
+        if (valid && col < dim) {
+          next[c] = *reinterpret_cast<const Pack<T, VEC>*>(at + row * ld + col);
+        } else {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) next[c].v[j] = from_float<T>(0.f);
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void take(Pack<T, VEC> (&r)[CH], bool valid, int slot) const {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      if constexpr (kDepth > 0) {
+        if (valid && c * kStep + lane * VEC < dim) {
+          r[c] = *reinterpret_cast<const Pack<T, VEC>*>(place(slot, c));
+        } else {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) r[c].v[j] = from_float<T>(0.f);
+        }
+      } else {
+        r[c] = next[c];
+      }
+    }
+  }
+};
+
+template <int DEPTH>
+__device__ __forceinline__ void ring_commit() {
+  if constexpr (DEPTH > 0) asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
-// Sum of (a, b) over a team; every thread of the team gets it.  Teams of a CTA
-// use the slot pair `parity` of `slots`, so that two sums in a row need one
-// barrier each.
+// All but the newest DEPTH - 1 requests of this thread have landed.
+template <int DEPTH>
+__device__ __forceinline__ void ring_wait() {
+  if constexpr (DEPTH > 0) asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+}
+
+// Sum of (a, b) over a team; every thread of the team gets it.  A team of more
+// than a warp meets at a barrier of its own and uses the slots `parity` of its
+// part of `slots`, so that two sums in a row need one barrier each.
 template <int TEAM>
-__device__ __forceinline__ float2 team_sum(float2 s, float2 (*slots)[kMostWarps], int parity) {
+__device__ __forceinline__ float2 team_sum(float2 s, float2* slots, int parity) {
 #pragma unroll
   for (int o = (TEAM < 32 ? TEAM : 32) / 2; o > 0; o >>= 1) {
     s.x += __shfl_xor_sync(kFullMask, s.x, o);
     s.y += __shfl_xor_sync(kFullMask, s.y, o);
   }
   if constexpr (TEAM > 32) {
-    if ((threadIdx.x & 31) == 0) slots[parity][threadIdx.x >> 5] = s;
-    __syncthreads();
-    s = slots[parity][0];
+    constexpr int kTeamWarps = TEAM / 32;
+    const int team = static_cast<int>(threadIdx.x) / TEAM;
+    float2* mine = slots + (team * 2 + parity) * kTeamWarps;
+    if ((threadIdx.x & 31) == 0) mine[(threadIdx.x % TEAM) >> 5] = s;
+    asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(TEAM) : "memory");
+    s = mine[0];
 #pragma unroll
-    for (int w = 1; w < TEAM / 32; ++w) {
-      s.x += slots[parity][w].x;
-      s.y += slots[parity][w].y;
+    for (int w = 1; w < kTeamWarps; ++w) {
+      s.x += mine[w].x;
+      s.y += mine[w].y;
     }
   }
   return s;
@@ -90,22 +158,26 @@ __device__ __forceinline__ float2 team_sum(float2 s, float2 (*slots)[kMostWarps]
 
 template <typename T, int VEC, int TEAM, int CH>
 __global__ void __launch_bounds__(cta_threads(TEAM)) norm_fwd_kernel(const NormArgs a) {
-  __shared__ float2 slots[2][kMostWarps];
+  using Rows = Ahead<T, VEC, TEAM, CH>;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ float2 slots[2 * cta_threads(TEAM) / 32];
   constexpr int kTeams = cta_threads(TEAM) / TEAM;
   constexpr int kStep = TEAM * VEC;
+  constexpr int kDepth = Rows::kDepth > 0 ? Rows::kDepth : 1;
   const int lane = static_cast<int>(threadIdx.x) % TEAM;
   const int team = static_cast<int>(threadIdx.x) / TEAM;
-  const T* x = static_cast<const T*>(a.x);
   T* out = static_cast<T*>(a.out);
   const int64_t stride = static_cast<int64_t>(gridDim.x) * kTeams;
   int64_t row = static_cast<int64_t>(blockIdx.x) * kTeams + team;
   // the loop runs on the row of the warp's first team, so that a warp stays whole
   int64_t lead = TEAM >= 32 ? row : static_cast<int64_t>(blockIdx.x) * kTeams + (threadIdx.x & ~31u) / TEAM;
 
-  Pack<T, VEC> next[CH];
+  Rows rows(a.x, a.ld_x, a.dim, lane, ring);
 #pragma unroll
-  for (int c = 0; c < CH; ++c)
-    load_row<T, VEC>(next[c], x + row * a.ld_x, c * kStep + lane * VEC, a.dim, row < a.rows);
+  for (int d = 0; d < kDepth; ++d) {
+    rows.request(row + d * stride, row + d * stride < a.rows, d);
+    ring_commit<Rows::kDepth>();
+  }
   float w[CH * VEC], b[CH * VEC];
 #pragma unroll
   for (int c = 0; c < CH; ++c)
@@ -116,20 +188,23 @@ __global__ void __launch_bounds__(cta_threads(TEAM)) norm_fwd_kernel(const NormA
       b[c * VEC + j] = col < a.dim && a.bias != nullptr ? load_param(a.bias, a.param_dtype, col) : 0.f;
     }
 
+  int slot = 0;
   for (; lead < a.rows; row += stride, lead += stride) {
+    Pack<T, VEC> x[CH];
+    ring_wait<Rows::kDepth>();
+    rows.take(x, row < a.rows, slot);
     float v[CH * VEC];
     float2 s = make_float2(0.f, 0.f);
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        v[c * VEC + j] = to_float(next[c].v[j]);
+        v[c * VEC + j] = to_float(x[c].v[j]);
         s.x += v[c * VEC + j];
       }
-    const int64_t after = row + stride;
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
-      load_row<T, VEC>(next[c], x + after * a.ld_x, c * kStep + lane * VEC, a.dim, after < a.rows);
+    rows.request(row + kDepth * stride, row + kDepth * stride < a.rows, slot);
+    ring_commit<Rows::kDepth>();
+    if (++slot == kDepth) slot = 0;
     const float mean = team_sum<TEAM>(s, slots, 0).x * a.inv_dim;
     s = make_float2(0.f, 0.f);
 #pragma unroll
@@ -163,30 +238,33 @@ __global__ void __launch_bounds__(cta_threads(TEAM)) norm_fwd_kernel(const NormA
 // PARAMS: also the sums of dy u and dy per column, one partial pair per CTA.
 template <typename T, int VEC, int TEAM, int CH, bool PARAMS>
 __global__ void __launch_bounds__(cta_threads(TEAM)) norm_bwd_kernel(const NormArgs a) {
-  __shared__ float2 slots[2][kMostWarps];
+  using Rows = Ahead<T, VEC, TEAM, CH>;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ float2 slots[2 * cta_threads(TEAM) / 32];
   constexpr int kTeams = cta_threads(TEAM) / TEAM;
   constexpr int kStep = TEAM * VEC;
   constexpr int kCols = CH * VEC;
+  constexpr int kDepth = Rows::kDepth > 0 ? Rows::kDepth : 1;
   const int lane = static_cast<int>(threadIdx.x) % TEAM;
   const int team = static_cast<int>(threadIdx.x) / TEAM;
-  const T* x = static_cast<const T*>(a.x);
-  const T* dy = static_cast<const T*>(a.dy);
   T* out = static_cast<T*>(a.out);
   const int64_t stride = static_cast<int64_t>(gridDim.x) * kTeams;
   int64_t row = static_cast<int64_t>(blockIdx.x) * kTeams + team;
   int64_t lead = TEAM >= 32 ? row : static_cast<int64_t>(blockIdx.x) * kTeams + (threadIdx.x & ~31u) / TEAM;
 
-  Pack<T, VEC> next_x[CH], next_dy[CH];
-  float next_mean = 0.f, next_rstd = 0.f;
+  Rows xs(a.x, a.ld_x, a.dim, lane, ring);
+  Rows dys(a.dy, a.ld_dy, a.dim, lane, ring + Rows::kBytes);
+  float mean_ahead[kDepth], rstd_ahead[kDepth];
+  const auto request = [&](int64_t r, int d) {
+    const bool valid = r < a.rows;
+    xs.request(r, valid, d);
+    dys.request(r, valid, d);
+    ring_commit<Rows::kDepth>();
+    mean_ahead[d] = valid ? a.mean_in[r] : 0.f;
+    rstd_ahead[d] = valid ? a.rstd_in[r] : 0.f;
+  };
 #pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    load_row<T, VEC>(next_x[c], x + row * a.ld_x, c * kStep + lane * VEC, a.dim, row < a.rows);
-    load_row<T, VEC>(next_dy[c], dy + row * a.ld_dy, c * kStep + lane * VEC, a.dim, row < a.rows);
-  }
-  if (row < a.rows) {
-    next_mean = a.mean_in[row];
-    next_rstd = a.rstd_in[row];
-  }
+  for (int d = 0; d < kDepth; ++d) request(row + d * stride, d);
   float w[kCols];
   float dw[PARAMS ? kCols : 1], db[PARAMS ? kCols : 1];
 #pragma unroll
@@ -199,86 +277,87 @@ __global__ void __launch_bounds__(cta_threads(TEAM)) norm_bwd_kernel(const NormA
     }
 
   int parity = 0;
-  for (; lead < a.rows; row += stride, lead += stride, parity ^= 1) {
-    const float mean = next_mean, rstd = next_rstd;
-    float u[kCols], t[kCols];
-    float2 s = make_float2(0.f, 0.f);
+  while (lead < a.rows) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+    for (int d = 0; d < kDepth; ++d) {
+      if (lead >= a.rows) break;
+      const float mean = mean_ahead[d], rstd = rstd_ahead[d];
+      Pack<T, VEC> x[CH], dy[CH];
+      ring_wait<Rows::kDepth>();
+      xs.take(x, row < a.rows, d);
+      dys.take(dy, row < a.rows, d);
+      float u[kCols], t[kCols];
+      float2 s = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const int i = c * VEC + j;
-        const bool in = c * kStep + lane * VEC + j < a.dim;
-        const float g = to_float(next_dy[c].v[j]);  // 0 outside the row
-        u[i] = in ? (to_float(next_x[c].v[j]) - mean) * rstd : 0.f;
-        t[i] = g * w[i];
-        s.x += t[i];
-        s.y = fmaf(t[i], u[i], s.y);
-        if (PARAMS) {
-          dw[i] = fmaf(g, u[i], dw[i]);
-          db[i] += g;
-        }
-      }
-    const int64_t after = row + stride;
-#pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      load_row<T, VEC>(next_x[c], x + after * a.ld_x, c * kStep + lane * VEC, a.dim, after < a.rows);
-      load_row<T, VEC>(next_dy[c], dy + after * a.ld_dy, c * kStep + lane * VEC, a.dim, after < a.rows);
-    }
-    next_mean = next_rstd = 0.f;
-    if (after < a.rows) {
-      next_mean = a.mean_in[after];
-      next_rstd = a.rstd_in[after];
-    }
-    s = team_sum<TEAM>(s, slots, parity);
-    if (out != nullptr && row < a.rows) {
-      const float m1 = s.x * a.inv_dim, m2 = s.y * a.inv_dim;
-#pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        const int col = c * kStep + lane * VEC;
-        if (col >= a.dim) continue;
-        Pack<T, VEC> g;
+      for (int c = 0; c < CH; ++c)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const int i = c * VEC + j;
-          g.v[j] = from_float<T>(rstd * (t[i] - fmaf(u[i], m2, m1)));
+          const bool in = c * kStep + lane * VEC + j < a.dim;
+          const float g = to_float(dy[c].v[j]);  // 0 outside the row
+          u[i] = in ? (to_float(x[c].v[j]) - mean) * rstd : 0.f;
+          t[i] = g * w[i];
+          s.x += t[i];
+          s.y = fmaf(t[i], u[i], s.y);
+          if (PARAMS) {
+            dw[i] = fmaf(g, u[i], dw[i]);
+            db[i] += g;
+          }
         }
-        *reinterpret_cast<Pack<T, VEC>*>(out + row * a.dim + col) = g;
+      request(row + kDepth * stride, d);
+      s = team_sum<TEAM>(s, slots, parity);
+      parity ^= 1;
+      if (out != nullptr && row < a.rows) {
+        const float m1 = s.x * a.inv_dim, m2 = s.y * a.inv_dim;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          const int col = c * kStep + lane * VEC;
+          if (col >= a.dim) continue;
+          Pack<T, VEC> g;
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            const int i = c * VEC + j;
+            g.v[j] = from_float<T>(rstd * (t[i] - fmaf(u[i], m2, m1)));
+          }
+          *reinterpret_cast<Pack<T, VEC>*>(out + row * a.dim + col) = g;
+        }
       }
+      row += stride;
+      lead += stride;
     }
   }
 
-  if (!PARAMS) return;
-  float* pw = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * a.dim;
-  if (TEAM > 32) {
+  if constexpr (PARAMS) {
+    float* pw = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * a.dim;
+    if constexpr (kTeams == 1) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+      for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const int col = c * kStep + lane * VEC + j;
-        if (col < a.dim) {
-          pw[col] = dw[c * VEC + j];
-          pw[a.dim + col] = db[c * VEC + j];
+        for (int j = 0; j < VEC; ++j) {
+          const int col = c * kStep + lane * VEC + j;
+          if (col < a.dim) {
+            pw[col] = dw[c * VEC + j];
+            pw[a.dim + col] = db[c * VEC + j];
+          }
+        }
+    } else {
+      // the CTA's teams, summed in a fixed order, one register of every thread at a time
+      __shared__ float slab[2][cta_threads(TEAM)];
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) {
+        __syncthreads();
+        slab[0][threadIdx.x] = dw[i];
+        slab[1][threadIdx.x] = db[i];
+        __syncthreads();
+        if (threadIdx.x < 2 * TEAM) {
+          const int which = static_cast<int>(threadIdx.x) / TEAM;
+          const int col = (i / VEC) * kStep + lane * VEC + i % VEC;
+          float sum = 0.f;
+#pragma unroll
+          for (int k = 0; k < kTeams; ++k) sum += slab[which][k * TEAM + lane];
+          if (col < a.dim) pw[which * a.dim + col] = sum;
         }
       }
-    return;
-  }
-  // the CTA's teams, summed in a fixed order, 32 columns' worth of registers of
-  // every team at a time: slab[team][lane] holds one register of each thread
-  __shared__ float slab[2][kThreads + 1];
-#pragma unroll
-  for (int i = 0; i < kCols; ++i) {
-    __syncthreads();
-    slab[0][threadIdx.x] = dw[i];
-    slab[1][threadIdx.x] = db[i];
-    __syncthreads();
-    if (threadIdx.x < 2 * TEAM) {
-      const int which = static_cast<int>(threadIdx.x) / TEAM;
-      const int col = (i / VEC) * kStep + lane * VEC + i % VEC;
-      float sum = 0.f;
-#pragma unroll
-      for (int k = 0; k < kTeams; ++k) sum += slab[which][k * TEAM + lane];
-      if (col < a.dim) pw[which * a.dim + col] = sum;
     }
   }
 }
@@ -287,7 +366,7 @@ __global__ void __launch_bounds__(cta_threads(TEAM)) norm_bwd_kernel(const NormA
 // L2) for each sum.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) norm_fwd_wide_kernel(const NormArgs a) {
-  __shared__ float2 slots[2][kMostWarps];
+  __shared__ float2 slots[2 * kWarps];
   T* out = static_cast<T*>(a.out);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
@@ -314,7 +393,7 @@ __global__ void __launch_bounds__(kThreads) norm_fwd_wide_kernel(const NormArgs 
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) norm_bwd_wide_kernel(const NormArgs a) {
-  __shared__ float2 slots[2][kMostWarps];
+  __shared__ float2 slots[2 * kWarps];
   T* out = static_cast<T*>(a.out);
   int parity = 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, parity ^= 1) {
@@ -357,10 +436,10 @@ __global__ void __launch_bounds__(kThreads) norm_wide_params_kernel(const NormAr
 }
 
 // Sums the CTAs' partials per column in a fixed order: 32 columns per CTA, each
-// of 8 warps every 8th partial, then the 8 sums.  blockIdx.y picks dw or db.
-__global__ void __launch_bounds__(kThreads) norm_param_sum_kernel(const float* partial, int parts, int dim,
-                                                                 void* dweight, void* dbias, int param_dtype) {
-  __shared__ float sums[kWarps][33];
+// of 32 warps every 32nd partial, then the 32 sums.  blockIdx.y picks dw or db.
+__global__ void __launch_bounds__(1024) norm_param_sum_kernel(const float* partial, int parts, int dim,
+                                                              void* dweight, void* dbias, int param_dtype) {
+  __shared__ float sums[32][33];
   void* out = blockIdx.y == 0 ? dweight : dbias;
   if (out == nullptr) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -368,16 +447,17 @@ __global__ void __launch_bounds__(kThreads) norm_param_sum_kernel(const float* p
   float s = 0.f;
   if (col < dim) {
     const float* p = partial + static_cast<int64_t>(blockIdx.y) * dim + col;
-#pragma unroll 4
-    for (int k = warp; k < parts; k += kWarps) s += p[static_cast<int64_t>(k) * 2 * dim];
+#pragma unroll 8
+    for (int k = warp; k < parts; k += 32) s += p[static_cast<int64_t>(k) * 2 * dim];
   }
   sums[warp][lane] = s;
   __syncthreads();
-  if (warp == 0 && col < dim) {
+  // warp w adds the 32 sums of column w
+  s = sums[lane][warp];
 #pragma unroll
-    for (int k = 1; k < kWarps; ++k) s += sums[k][lane];
-    store_param(out, param_dtype, col, s);
-  }
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kFullMask, s, o);
+  const int mine = static_cast<int>(blockIdx.x) * 32 + warp;
+  if (lane == 0 && mine < dim) store_param(out, param_dtype, mine, s);
 }
 
 // CTAs of a grid that walks `rows` in steps of `teams` rows: what is needed, at
@@ -388,25 +468,52 @@ int norm_ctas(int64_t rows, int teams, int per_sm) {
   return static_cast<int>(need < most ? need : most);
 }
 
-// CTAs of the backward on one SM: 1,024 threads; kBwdPerSm, the most of them,
-// bounds the workspace.
-constexpr int bwd_per_sm(int threads) { return 1024 / threads; }
-constexpr int kBwdPerSm = 8;
+// Most CTAs of the backward on one SM, which bounds its workspace.
+constexpr int kBwdPerSm = 4;
+
+// CTAs of `kernel` that one SM holds (asked once: the library runs on one kind
+// of GPU), after raising the kernel's shared-memory limit for this context.
+template <typename Kernel>
+int resident(Kernel kernel, int threads, int bytes, unsigned long long* ready, int* per_sm) {
+  const unsigned long long context = current_context_id();
+  if (*per_sm > 0 && *ready == context && context != 0) return *per_sm;
+  int n = 0;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, bytes) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    return 0;
+  }
+  *ready = context;
+  *per_sm = n;
+  return n;
+}
+
+template <typename T, int VEC, int TEAM, int CH, bool PARAMS>
+int launch_bwd(const NormArgs& a, int* ctas, cudaStream_t stream) {
+  constexpr int threads = cta_threads(TEAM), bytes = 2 * Ahead<T, VEC, TEAM, CH>::kBytes;
+  static thread_local unsigned long long ready = 0;
+  static thread_local int per_sm = 0;
+  const auto kernel = norm_bwd_kernel<T, VEC, TEAM, CH, PARAMS>;
+  const int fit = resident(kernel, threads, bytes, &ready, &per_sm);
+  if (fit == 0) return RFM_ERR_LAUNCH;
+  *ctas = norm_ctas(a.rows, threads / TEAM, fit < kBwdPerSm ? fit : kBwdPerSm);
+  kernel<<<*ctas, threads, bytes, stream>>>(a);
+  return launch_status();
+}
 
 template <typename T, int VEC, int TEAM, int CH>
 int launch_norm(const NormArgs& a, bool backward, int* ctas, cudaStream_t stream) {
-  constexpr int threads = cta_threads(TEAM);
-  constexpr int teams = threads / TEAM;
-  if (!backward) {
-    // the SM's 2,048 threads where registers allow; more CTAs only queue
-    norm_fwd_kernel<T, VEC, TEAM, CH><<<norm_ctas(a.rows, teams, 2048 / threads), threads, 0, stream>>>(a);
-  } else if (a.partial != nullptr) {
-    *ctas = norm_ctas(a.rows, teams, bwd_per_sm(threads));
-    norm_bwd_kernel<T, VEC, TEAM, CH, true><<<*ctas, threads, 0, stream>>>(a);
-  } else {
-    norm_bwd_kernel<T, VEC, TEAM, CH, false>
-        <<<norm_ctas(a.rows, teams, bwd_per_sm(threads)), threads, 0, stream>>>(a);
+  if (backward) {
+    return a.partial != nullptr ? launch_bwd<T, VEC, TEAM, CH, true>(a, ctas, stream)
+                                : launch_bwd<T, VEC, TEAM, CH, false>(a, ctas, stream);
   }
+  constexpr int threads = cta_threads(TEAM), bytes = Ahead<T, VEC, TEAM, CH>::kBytes;
+  static thread_local unsigned long long ready = 0;
+  static thread_local int per_sm = 0;
+  const auto kernel = norm_fwd_kernel<T, VEC, TEAM, CH>;
+  const int fit = resident(kernel, threads, bytes, &ready, &per_sm);
+  if (fit == 0) return RFM_ERR_LAUNCH;
+  kernel<<<norm_ctas(a.rows, threads / TEAM, fit), threads, bytes, stream>>>(a);
   return launch_status();
 }
 
@@ -532,7 +639,7 @@ extern "C" int rfm_layer_norm_backward(const void* x, int64_t ld_x, const void* 
   }
   if (!params) return RFM_OK;
   // with no rows the sums are empty: zeros
-  norm_param_sum_kernel<<<dim3((dim + 31) / 32, 2), kThreads, 0, as_stream(stream)>>>(
+  norm_param_sum_kernel<<<dim3((dim + 31) / 32, 2), 1024, 0, as_stream(stream)>>>(
       a.partial, ctas, dim, grad_weight, grad_bias, param_dtype);
   return launch_status();
 }
