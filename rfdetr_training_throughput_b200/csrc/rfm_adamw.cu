@@ -23,10 +23,9 @@
 //
 // HBM-bound: 28 bytes a parameter in fp32 with 32-bit moments, 16 with 8-bit
 // ones.  The tensors' table travels in the kernel's parameters (64 bytes a
-// tensor), so no upload precedes the launch.  One CTA takes 4096 consecutive
-// elements of one tensor, a warp two blocks of 256, a lane two quads of each, so
-// that every access of a warp is contiguous and 16 loads are in flight a thread
-// before the first is used.
+// tensor), so no upload precedes the launch.  One CTA takes 2048 consecutive
+// elements of one tensor, a warp a block of 256, a lane two quads of it, so that
+// every access of a warp is contiguous.
 #include <math.h>
 
 #include "rfm_types.cuh"
@@ -36,7 +35,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBlock = RFM_MOMENT_BLOCK;          // elements that share a scale
-constexpr int kChunk = 4096;                      // elements of one CTA
+constexpr int kChunk = 2048;                      // elements of one CTA
 constexpr int kWarpBlocks = kChunk / kBlock / 8;  // blocks of one warp
 static_assert(kBlock == 32 * 8, "a warp holds one block, eight elements a lane");
 static_assert(sizeof(rfm_adamw_tensor) == 64, "tensor entries are 64 bytes");
@@ -249,7 +248,7 @@ __device__ __forceinline__ float warp_max_bits(uint32_t bits) {
 }
 
 template <typename T, bool EIGHT, int N>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ AdamArgs<N> a) {
+__global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constant__ AdamArgs<N> a) {
   // the tensor of this CTA: the last whose first chunk is not after it
   int lo = 0, hi = a.c.count - 1;
   const int chunk = static_cast<int>(blockIdx.x);

@@ -34,10 +34,10 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kWideDim = 8192;  // longest row held in registers
 constexpr int kWideSlabs = 64;  // row slabs of the wide rows' parameter gradients
 
-// Threads of a CTA of teams.
-__host__ __device__ constexpr int cta_threads(int team) { return team > 32 ? 512 : 256; }
+// Threads of a CTA of teams; `cols`: columns a thread owns.
+__host__ __device__ constexpr int cta_threads(int team, int cols) { return team > 32 ? 512 : cols > 16 ? 128 : 256; }
 // Rows a thread copies ahead (0: element loads, one row ahead in registers).
-__host__ __device__ constexpr int ring_depth(int vec, int ch) { return vec == 1 ? 0 : ch == 1 ? 4 : 2; }
+__host__ __device__ constexpr int ring_depth(int vec, int ch) { return vec == 1 ? 0 : ch == 1 ? 4 : ch <= 4 ? 3 : 2; }
 
 struct NormArgs {
   const void* x;
@@ -64,7 +64,7 @@ struct NormArgs {
 template <typename T, int VEC, int TEAM, int CH>
 struct Ahead {
   static constexpr int kDepth = ring_depth(VEC, CH);
-  static constexpr int kThreadsCta = cta_threads(TEAM);
+  static constexpr int kThreadsCta = cta_threads(TEAM, CH * VEC);
   static constexpr int kBytes = kDepth * CH * kThreadsCta * 16;  // of one array
   static constexpr int kStep = TEAM * VEC;
   const T* at;     // the array
@@ -156,13 +156,69 @@ __device__ __forceinline__ float2 team_sum(float2 s, float2* slots, int parity) 
   return s;
 }
 
+// Weight (or bias) of a thread's columns as pairs: in registers up to 16 columns,
+// read from shared memory beyond (where every thread of a warp-team's lane needs
+// the same columns for each of its rows, and registers are short).
+template <int VEC, int TEAM, int CH>
+struct Params {
+  static constexpr int kCols = CH * VEC, kStep = TEAM * VEC;
+  static constexpr bool kShared = kCols > 16;
+  static constexpr int kFloats = kShared ? TEAM * kCols : 0;
+  Pair reg[kShared ? 1 : kCols / 2];
+  const float* smem;
+
+  __device__ __forceinline__ void load(const void* p, int dtype, int dim, float missing, int lane, float* shared) {
+    smem = shared;
+    if constexpr (kShared) {
+      for (int i = threadIdx.x; i < kFloats; i += blockDim.x)
+        shared[i] = i < dim && p != nullptr ? load_param(p, dtype, i) : missing;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kCols / 2; ++i) {
+        float v[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int c = (2 * i + k) / VEC, j = (2 * i + k) % VEC;
+          const int col = c * kStep + lane * VEC + j;
+          v[k] = col < dim && p != nullptr ? load_param(p, dtype, col) : missing;
+        }
+        reg[i] = pair(v[0], v[1]);
+      }
+    }
+  }
+
+  // columns 4 q .. 4 q + 3 of the thread (VEC >= 4) or 2 q, 2 q + 1
+  __device__ __forceinline__ Pair at(int i, int lane) const {
+    if constexpr (kShared) {
+      const int c = (2 * i) / VEC, j = (2 * i) % VEC;
+      const float2 f = *reinterpret_cast<const float2*>(smem + c * kStep + lane * VEC + j);
+      return pair(f.x, f.y);
+    } else {
+      return reg[i];
+    }
+  }
+};
+
+// The thread's elements 2 i, 2 i + 1 of a row (element loads: of two chunks).
+template <typename T, int VEC, int CH>
+__device__ __forceinline__ Pair element_pair(const Pack<T, VEC> (&r)[CH], int i) {
+  if constexpr (VEC == 1) {
+    return pair(to_float(r[2 * i].v[0]), to_float(r[2 * i + 1].v[0]));
+  } else {
+    return load_pair(r[2 * i / VEC], (2 * i % VEC) / 2);
+  }
+}
+
 template <typename T, int VEC, int TEAM, int CH>
-__global__ void __launch_bounds__(cta_threads(TEAM)) norm_fwd_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(cta_threads(TEAM, CH* VEC)) norm_fwd_kernel(const NormArgs a) {
   using Rows = Ahead<T, VEC, TEAM, CH>;
+  using P = Params<VEC, TEAM, CH>;
   extern __shared__ __align__(16) uint8_t ring[];
-  __shared__ float2 slots[2 * cta_threads(TEAM) / 32];
-  constexpr int kTeams = cta_threads(TEAM) / TEAM;
+  __shared__ float2 slots[2 * Rows::kThreadsCta / 32];
+  __shared__ __align__(16) float params[P::kShared ? 2 * P::kFloats : 1];
+  constexpr int kTeams = Rows::kThreadsCta / TEAM;
   constexpr int kStep = TEAM * VEC;
+  constexpr int kPairs = CH * VEC / 2;
   constexpr int kDepth = Rows::kDepth > 0 ? Rows::kDepth : 1;
   const int lane = static_cast<int>(threadIdx.x) % TEAM;
   const int team = static_cast<int>(threadIdx.x) / TEAM;
@@ -178,53 +234,63 @@ __global__ void __launch_bounds__(cta_threads(TEAM)) norm_fwd_kernel(const NormA
     rows.request(row + d * stride, row + d * stride < a.rows, d);
     ring_commit<Rows::kDepth>();
   }
-  float w[CH * VEC], b[CH * VEC];
-#pragma unroll
-  for (int c = 0; c < CH; ++c)
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const int col = c * kStep + lane * VEC + j;
-      w[c * VEC + j] = col < a.dim && a.weight != nullptr ? load_param(a.weight, a.param_dtype, col) : 1.f;
-      b[c * VEC + j] = col < a.dim && a.bias != nullptr ? load_param(a.bias, a.param_dtype, col) : 0.f;
-    }
+  P w, b;
+  w.load(a.weight, a.param_dtype, a.dim, 1.f, lane, params);
+  b.load(a.bias, a.param_dtype, a.dim, 0.f, lane, params + P::kFloats);
+  if (P::kShared) __syncthreads();
 
   int slot = 0;
   for (; lead < a.rows; row += stride, lead += stride) {
     Pack<T, VEC> x[CH];
     ring_wait<Rows::kDepth>();
     rows.take(x, row < a.rows, slot);
-    float v[CH * VEC];
-    float2 s = make_float2(0.f, 0.f);
+    Pair v[kPairs];
+    Pair s = pair(0.f, 0.f);
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        v[c * VEC + j] = to_float(x[c].v[j]);
-        s.x += v[c * VEC + j];
-      }
+    for (int i = 0; i < kPairs; ++i) {
+      v[i] = element_pair<T, VEC, CH>(x, i);
+      s = s + v[i];
+    }
     rows.request(row + kDepth * stride, row + kDepth * stride < a.rows, slot);
     ring_commit<Rows::kDepth>();
     if (++slot == kDepth) slot = 0;
-    const float mean = team_sum<TEAM>(s, slots, 0).x * a.inv_dim;
-    s = make_float2(0.f, 0.f);
+    float2 sums = split(s);
+    const float mean = team_sum<TEAM>(make_float2(sums.x + sums.y, 0.f), slots, 0).x * a.inv_dim;
+    const Pair minus = pair(-mean, -mean);
+    s = pair(0.f, 0.f);
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const bool in = c * kStep + lane * VEC + j < a.dim;
-        v[c * VEC + j] = in ? v[c * VEC + j] - mean : 0.f;
-        s.x = fmaf(v[c * VEC + j], v[c * VEC + j], s.x);
+    for (int i = 0; i < kPairs; ++i) {
+      v[i] = v[i] + minus;
+      if constexpr (VEC == 1) {  // columns past the row's end (a whole piece of a vector row) count nothing
+        float2 f = split(v[i]);
+        if (2 * i * kStep + lane >= a.dim) f.x = 0.f;
+        if ((2 * i + 1) * kStep + lane >= a.dim) f.y = 0.f;
+        v[i] = pair(f.x, f.y);
+      } else if ((2 * i / VEC) * kStep + lane * VEC >= a.dim) {
+        v[i] = pair(0.f, 0.f);
       }
-    const float rstd = 1.f / sqrtf(fmaf(team_sum<TEAM>(s, slots, 1).x, a.inv_dim, a.eps));
+      s = fma(v[i], v[i], s);
+    }
+    sums = split(s);
+    const float var = team_sum<TEAM>(make_float2(sums.x + sums.y, 0.f), slots, 1).x;
+    const float rstd = 1.f / sqrtf(fmaf(var, a.inv_dim, a.eps));
     if (row < a.rows) {
+      const Pair scale = pair(rstd, rstd);
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         const int col = c * kStep + lane * VEC;
         if (col >= a.dim) continue;
         Pack<T, VEC> y;
+        if constexpr (VEC == 1) {
+          const float2 f = split(fma(v[c / 2] * scale, w.at(c / 2, lane), b.at(c / 2, lane)));
+          y.v[0] = from_float<T>(c % 2 == 0 ? f.x : f.y);
+        } else {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j)
-          y.v[j] = from_float<T>(fmaf(v[c * VEC + j] * rstd, w[c * VEC + j], b[c * VEC + j]));
+          for (int j = 0; j < VEC / 2; ++j) {
+            const int i = c * VEC / 2 + j;
+            store_pair(y, j, fma(v[i] * scale, w.at(i, lane), b.at(i, lane)));
+          }
+        }
         *reinterpret_cast<Pack<T, VEC>*>(out + row * a.dim + col) = y;
       }
       if (lane == 0 && a.mean_out != nullptr) {
@@ -235,15 +301,19 @@ __global__ void __launch_bounds__(cta_threads(TEAM)) norm_fwd_kernel(const NormA
   }
 }
 
-// PARAMS: also the sums of dy u and dy per column, one partial pair per CTA.
+// PARAMS: also the sums of dy u and dy per column, one partial pair per CTA.  u
+// and t are computed twice, for the sums and for dx: cheaper than the registers
+// that would keep them.
 template <typename T, int VEC, int TEAM, int CH, bool PARAMS>
-__global__ void __launch_bounds__(cta_threads(TEAM)) norm_bwd_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(cta_threads(TEAM, CH* VEC)) norm_bwd_kernel(const NormArgs a) {
   using Rows = Ahead<T, VEC, TEAM, CH>;
+  using P = Params<VEC, TEAM, CH>;
   extern __shared__ __align__(16) uint8_t ring[];
-  __shared__ float2 slots[2 * cta_threads(TEAM) / 32];
-  constexpr int kTeams = cta_threads(TEAM) / TEAM;
+  __shared__ float2 slots[2 * Rows::kThreadsCta / 32];
+  __shared__ __align__(16) float params[P::kShared ? P::kFloats : 1];
+  constexpr int kTeams = Rows::kThreadsCta / TEAM;
   constexpr int kStep = TEAM * VEC;
-  constexpr int kCols = CH * VEC;
+  constexpr int kPairs = CH * VEC / 2;
   constexpr int kDepth = Rows::kDepth > 0 ? Rows::kDepth : 1;
   const int lane = static_cast<int>(threadIdx.x) % TEAM;
   const int team = static_cast<int>(threadIdx.x) / TEAM;
@@ -265,16 +335,12 @@ __global__ void __launch_bounds__(cta_threads(TEAM)) norm_bwd_kernel(const NormA
   };
 #pragma unroll
   for (int d = 0; d < kDepth; ++d) request(row + d * stride, d);
-  float w[kCols];
-  float dw[PARAMS ? kCols : 1], db[PARAMS ? kCols : 1];
+  P w;
+  w.load(a.weight, a.param_dtype, a.dim, 1.f, lane, params);
+  if (P::kShared) __syncthreads();
+  Pair dw[PARAMS ? kPairs : 1], db[PARAMS ? kPairs : 1];
 #pragma unroll
-  for (int c = 0; c < CH; ++c)
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const int col = c * kStep + lane * VEC + j;
-      w[c * VEC + j] = col < a.dim && a.weight != nullptr ? load_param(a.weight, a.param_dtype, col) : 1.f;
-      if (PARAMS) dw[c * VEC + j] = db[c * VEC + j] = 0.f;
-    }
+  for (int i = 0; i < (PARAMS ? kPairs : 1); ++i) dw[i] = db[i] = pair(0.f, 0.f);
 
   int parity = 0;
   while (lead < a.rows) {
@@ -284,44 +350,51 @@ __global__ void __launch_bounds__(cta_threads(TEAM)) norm_bwd_kernel(const NormA
       const float mean = mean_ahead[d], rstd = rstd_ahead[d];
       Pack<T, VEC> x[CH], dy[CH];
       ring_wait<Rows::kDepth>();
-      xs.take(x, row < a.rows, d);
+      xs.take(x, row < a.rows, d);  // zeros past the row's end and past the last row
       dys.take(dy, row < a.rows, d);
-      float u[kCols], t[kCols];
-      float2 s = make_float2(0.f, 0.f);
+      // u = x rstd - mean rstd would cancel for rows whose mean is large
+      const Pair minus = pair(-mean, -mean), scale = pair(rstd, rstd);
+      Pair s1 = pair(0.f, 0.f), s2 = pair(0.f, 0.f);
 #pragma unroll
-      for (int c = 0; c < CH; ++c)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const int i = c * VEC + j;
-          const bool in = c * kStep + lane * VEC + j < a.dim;
-          const float g = to_float(dy[c].v[j]);  // 0 outside the row
-          u[i] = in ? (to_float(x[c].v[j]) - mean) * rstd : 0.f;
-          t[i] = g * w[i];
-          s.x += t[i];
-          s.y = fmaf(t[i], u[i], s.y);
-          if (PARAMS) {
-            dw[i] = fmaf(g, u[i], dw[i]);
-            db[i] += g;
-          }
+      for (int i = 0; i < kPairs; ++i) {
+        const Pair g = element_pair<T, VEC, CH>(dy, i);
+        const Pair u = (element_pair<T, VEC, CH>(x, i) + minus) * scale;  // past the end: times dy, 0
+        const Pair t = g * w.at(i, lane);
+        s1 = s1 + t;
+        s2 = fma(t, u, s2);
+        if (PARAMS) {
+          dw[i] = fma(g, u, dw[i]);
+          db[i] = db[i] + g;
         }
-      request(row + kDepth * stride, d);
-      s = team_sum<TEAM>(s, slots, parity);
+      }
+      const float2 f1 = split(s1), f2 = split(s2);
+      const float2 s = team_sum<TEAM>(make_float2(f1.x + f1.y, f2.x + f2.y), slots, parity);
       parity ^= 1;
       if (out != nullptr && row < a.rows) {
+        // dx = rstd (t - m1 - u m2)
         const float m1 = s.x * a.inv_dim, m2 = s.y * a.inv_dim;
+        const Pair minus1 = pair(-m1, -m1), minus2 = pair(-m2, -m2);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
           const int col = c * kStep + lane * VEC;
           if (col >= a.dim) continue;
-          Pack<T, VEC> g;
+          Pack<T, VEC> o;
+          const auto dx = [&](int i) {
+            const Pair u = (element_pair<T, VEC, CH>(x, i) + minus) * scale;
+            const Pair t = fma(element_pair<T, VEC, CH>(dy, i), w.at(i, lane), minus1);
+            return fma(u, minus2, t) * scale;
+          };
+          if constexpr (VEC == 1) {
+            const float2 f = split(dx(c / 2));
+            o.v[0] = from_float<T>(c % 2 == 0 ? f.x : f.y);
+          } else {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const int i = c * VEC + j;
-            g.v[j] = from_float<T>(rstd * (t[i] - fmaf(u[i], m2, m1)));
+            for (int j = 0; j < VEC / 2; ++j) store_pair(o, j, dx(c * VEC / 2 + j));
           }
-          *reinterpret_cast<Pack<T, VEC>*>(out + row * a.dim + col) = g;
+          *reinterpret_cast<Pack<T, VEC>*>(out + row * a.dim + col) = o;
         }
       }
+      request(row + kDepth * stride, d);
       row += stride;
       lead += stride;
     }
@@ -329,33 +402,41 @@ __global__ void __launch_bounds__(cta_threads(TEAM)) norm_bwd_kernel(const NormA
 
   if constexpr (PARAMS) {
     float* pw = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * a.dim;
+    const auto column = [&](int e) { return (e / VEC) * kStep + lane * VEC + e % VEC; };
     if constexpr (kTeams == 1) {
 #pragma unroll
-      for (int c = 0; c < CH; ++c)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const int col = c * kStep + lane * VEC + j;
-          if (col < a.dim) {
-            pw[col] = dw[c * VEC + j];
-            pw[a.dim + col] = db[c * VEC + j];
-          }
+      for (int i = 0; i < kPairs; ++i) {
+        const float2 fw = split(dw[i]), fb = split(db[i]);
+        if (column(2 * i) < a.dim) {
+          pw[column(2 * i)] = fw.x;
+          pw[a.dim + column(2 * i)] = fb.x;
         }
+        if (column(2 * i + 1) < a.dim) {
+          pw[column(2 * i + 1)] = fw.y;
+          pw[a.dim + column(2 * i + 1)] = fb.y;
+        }
+      }
     } else {
-      // the CTA's teams, summed in a fixed order, one register of every thread at a time
-      __shared__ float slab[2][cta_threads(TEAM)];
+      // the CTA's teams, summed in a fixed order, one register pair of every thread at a time
+      __shared__ float2 slab[2][Rows::kThreadsCta];
 #pragma unroll
-      for (int i = 0; i < kCols; ++i) {
+      for (int i = 0; i < kPairs; ++i) {
         __syncthreads();
-        slab[0][threadIdx.x] = dw[i];
-        slab[1][threadIdx.x] = db[i];
+        slab[0][threadIdx.x] = split(dw[i]);
+        slab[1][threadIdx.x] = split(db[i]);
         __syncthreads();
-        if (threadIdx.x < 2 * TEAM) {
-          const int which = static_cast<int>(threadIdx.x) / TEAM;
-          const int col = (i / VEC) * kStep + lane * VEC + i % VEC;
-          float sum = 0.f;
+        for (int k = threadIdx.x; k < 2 * TEAM; k += Rows::kThreadsCta) {
+          const int which = k / TEAM, from = k % TEAM;
+          float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-          for (int k = 0; k < kTeams; ++k) sum += slab[which][k * TEAM + lane];
-          if (col < a.dim) pw[which * a.dim + col] = sum;
+          for (int m = 0; m < kTeams; ++m) {
+            sum.x += slab[which][m * TEAM + from].x;
+            sum.y += slab[which][m * TEAM + from].y;
+          }
+          const int c0 = (2 * i / VEC) * kStep + from * VEC + 2 * i % VEC;
+          const int c1 = ((2 * i + 1) / VEC) * kStep + from * VEC + (2 * i + 1) % VEC;
+          if (c0 < a.dim) pw[which * a.dim + c0] = sum.x;
+          if (c1 < a.dim) pw[which * a.dim + c1] = sum.y;
         }
       }
     }
@@ -469,7 +550,7 @@ int norm_ctas(int64_t rows, int teams, int per_sm) {
 }
 
 // Most CTAs of the backward on one SM, which bounds its workspace.
-constexpr int kBwdPerSm = 4;
+constexpr int kBwdPerSm = 6;
 
 // CTAs of `kernel` that one SM holds (asked once: the library runs on one kind
 // of GPU), after raising the kernel's shared-memory limit for this context.
@@ -490,7 +571,7 @@ int resident(Kernel kernel, int threads, int bytes, unsigned long long* ready, i
 
 template <typename T, int VEC, int TEAM, int CH, bool PARAMS>
 int launch_bwd(const NormArgs& a, int* ctas, cudaStream_t stream) {
-  constexpr int threads = cta_threads(TEAM), bytes = 2 * Ahead<T, VEC, TEAM, CH>::kBytes;
+  constexpr int threads = cta_threads(TEAM, CH * VEC), bytes = 2 * Ahead<T, VEC, TEAM, CH>::kBytes;
   static thread_local unsigned long long ready = 0;
   static thread_local int per_sm = 0;
   const auto kernel = norm_bwd_kernel<T, VEC, TEAM, CH, PARAMS>;
@@ -507,7 +588,7 @@ int launch_norm(const NormArgs& a, bool backward, int* ctas, cudaStream_t stream
     return a.partial != nullptr ? launch_bwd<T, VEC, TEAM, CH, true>(a, ctas, stream)
                                 : launch_bwd<T, VEC, TEAM, CH, false>(a, ctas, stream);
   }
-  constexpr int threads = cta_threads(TEAM), bytes = Ahead<T, VEC, TEAM, CH>::kBytes;
+  constexpr int threads = cta_threads(TEAM, CH * VEC), bytes = Ahead<T, VEC, TEAM, CH>::kBytes;
   static thread_local unsigned long long ready = 0;
   static thread_local int per_sm = 0;
   const auto kernel = norm_fwd_kernel<T, VEC, TEAM, CH>;
@@ -535,16 +616,21 @@ int dispatch_norm(const NormArgs& a, bool vectors, bool backward, int* ctas, cud
     }
     return launch_status();
   }
-  // at most 16 columns a thread: the backward keeps five values for each
+  // a warp a row up to 1024 columns (32 a lane): a team of several warps pays its
+  // shuffles in each of them and a barrier twice a row (16384 x 1024 and longer:
+  // four warps a row 67 and 98 us at 65536 rows of fp16, forward and backward,
+  // see the table beside launch_norm's callers for one warp)
   if (vectors) {
     if (d <= 8 * V) return launch_norm<T, V, 8, 1>(a, backward, ctas, s);
     if (d <= 32 * V) return launch_norm<T, V, 32, 1>(a, backward, ctas, s);
     if (d <= 64 * V) return launch_norm<T, V, 32, 2>(a, backward, ctas, s);
-    if (d <= 128 * V) return launch_norm<T, V, 128, 1>(a, backward, ctas, s);
-    if (d <= 256 * V) return launch_norm<T, V, 128, 2>(a, backward, ctas, s);
-    if (d <= 512 * V) return launch_norm<T, V, 256, 2>(a, backward, ctas, s);
-    if (d <= 1024 * V) return launch_norm<T, V, 512, 2>(a, backward, ctas, s);
-    if constexpr (V == 4) return launch_norm<T, V, 512, 4>(a, backward, ctas, s);
+    if (d <= 128 * V) return launch_norm<T, V, 32, 4>(a, backward, ctas, s);
+    if constexpr (V == 4) {
+      if (d <= 1024) return launch_norm<T, V, 32, 8>(a, backward, ctas, s);
+    }
+    if (d <= 2048) return launch_norm<T, V, 128, 16 / V>(a, backward, ctas, s);
+    if (d <= 4096) return launch_norm<T, V, 256, 16 / V>(a, backward, ctas, s);
+    return launch_norm<T, V, 512, 16 / V>(a, backward, ctas, s);
   }
   if (d <= 32) return launch_norm<T, 1, 8, 4>(a, backward, ctas, s);
   if (d <= 128) return launch_norm<T, 1, 32, 4>(a, backward, ctas, s);

@@ -39,6 +39,57 @@ struct alignas(sizeof(T) * VEC) Pack {
   T v[VEC];
 };
 
+// Two fp32 values in one register pair and one instruction (the sm_100 f32x2
+// operations; each half is rounded by itself).
+struct Pair {
+  uint64_t v;
+};
+__device__ __forceinline__ Pair pair(float x, float y) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 split(Pair p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p.v));
+  return r;
+}
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// Elements 2 i and 2 i + 1 of a pack.
+template <typename T, int VEC>
+__device__ __forceinline__ Pair load_pair(const Pack<T, VEC>& p, int i) {
+  return pair(to_float(p.v[2 * i]), to_float(p.v[2 * i + 1]));
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_pair(Pack<T, VEC>& p, int i, Pair v) {
+  const float2 f = split(v);
+  p.v[2 * i] = from_float<T>(f.x);
+  p.v[2 * i + 1] = from_float<T>(f.y);
+}
+template <>
+__device__ __forceinline__ void store_pair<__nv_bfloat16, 8>(Pack<__nv_bfloat16, 8>& p, int i, Pair v) {
+  reinterpret_cast<__nv_bfloat162*>(p.v)[i] = __float22bfloat162_rn(split(v));
+}
+template <>
+__device__ __forceinline__ void store_pair<__half, 8>(Pack<__half, 8>& p, int i, Pair v) {
+  reinterpret_cast<__half2*>(p.v)[i] = __float22half2_rn(split(v));
+}
+
 // Element i of a parameter array whose type is known at run time only (read
 // once per thread, outside the row loops).
 __device__ __forceinline__ float load_param(const void* p, int dtype, int64_t i) {
