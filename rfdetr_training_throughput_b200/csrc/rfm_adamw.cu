@@ -28,6 +28,8 @@
 // every access of a warp is contiguous.
 #include <math.h>
 
+#include <type_traits>
+
 #include "rfm_types.cuh"
 
 namespace rfm {
@@ -36,8 +38,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kBlock = RFM_MOMENT_BLOCK;          // elements that share a scale
 constexpr int kChunk = 2048;                      // elements of one CTA
-constexpr int kWarpBlocks = kChunk / kBlock / 8;  // blocks of one warp
-static_assert(kBlock == 32 * 8, "a warp holds one block, eight elements a lane");
+static_assert(kBlock == 32 * 8 && kChunk == 8 * kBlock, "a warp holds one block, eight elements a lane");
 static_assert(sizeof(rfm_adamw_tensor) == 64, "tensor entries are 64 bytes");
 
 struct AdamScalars {
@@ -102,77 +103,95 @@ __global__ void adam_scalars_kernel(const float* device_lr, const int64_t* devic
                       device_step != nullptr ? *device_step : step);
 }
 
-template <typename T>
-__device__ __forceinline__ void load_quad(float (&r)[4], const T* p, int64_t i, int64_t n, bool vec) {
-  if (vec && i + 4 <= n) {
-    const Pack<T, 4> q = *reinterpret_cast<const Pack<T, 4>*>(p + i);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = to_float(q.v[j]);
+// Four elements of a lane: those from `i` on, of `left` that the tensor has there.
+// WHOLE: all of the warp's block lies in the tensor, aligned.
+template <bool WHOLE, typename T>
+__device__ __forceinline__ void load_quad(Pair (&r)[2], const T* p, int64_t left) {
+  if (WHOLE) {
+    const Pack<T, 4> q = *reinterpret_cast<const Pack<T, 4>*>(p);
+    r[0] = load_pair(q, 0);
+    r[1] = load_pair(q, 1);
   } else {
+    float f[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = i + j < n ? to_float(p[i + j]) : 0.f;
+    for (int j = 0; j < 4; ++j) f[j] = j < left ? to_float(p[j]) : 0.f;
+    r[0] = pair(f[0], f[1]);
+    r[1] = pair(f[2], f[3]);
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void store_quad(const float (&r)[4], T* p, int64_t i, int64_t n, bool vec) {
-  if (vec && i + 4 <= n) {
+template <bool WHOLE, typename T>
+__device__ __forceinline__ void store_quad(const Pair (&r)[2], T* p, int64_t left) {
+  const float2 a = split(r[0]), b = split(r[1]);
+  const float f[4] = {a.x, a.y, b.x, b.y};
+  if (WHOLE) {
     Pack<T, 4> q;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) q.v[j] = from_float<T>(r[j]);
-    *reinterpret_cast<Pack<T, 4>*>(p + i) = q;
+    for (int j = 0; j < 4; ++j) q.v[j] = from_float<T>(f[j]);
+    *reinterpret_cast<Pack<T, 4>*>(p) = q;
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (i + j < n) p[i + j] = from_float<T>(r[j]);
+      if (j < left) p[j] = from_float<T>(f[j]);
   }
 }
 
 // Four codes as one word, element j in byte j.
-__device__ __forceinline__ uint32_t load_codes(const void* base, int64_t i, int64_t n, bool vec) {
-  const uint8_t* p = static_cast<const uint8_t*>(base) + i;
-  if (vec && i + 4 <= n) return *reinterpret_cast<const uint32_t*>(p);
+template <bool WHOLE>
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* p, int64_t left) {
+  if (WHOLE) return *reinterpret_cast<const uint32_t*>(p);
   uint32_t w = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
-    if (i + j < n) w |= static_cast<uint32_t>(p[j]) << (8 * j);
+    if (j < left) w |= static_cast<uint32_t>(p[j]) << (8 * j);
   return w;
 }
 
-__device__ __forceinline__ void store_codes(uint32_t w, void* base, int64_t i, int64_t n, bool vec) {
-  uint8_t* p = static_cast<uint8_t*>(base) + i;
-  if (vec && i + 4 <= n) {
+template <bool WHOLE>
+__device__ __forceinline__ void store_codes(uint32_t w, uint8_t* p, int64_t left) {
+  if constexpr (WHOLE) {
     *reinterpret_cast<uint32_t*>(p) = w;
-    return;
-  }
+  } else {
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (i + j < n) p[j] = static_cast<uint8_t>(w >> (8 * j));
+    for (int j = 0; j < 4; ++j)
+      if (j < left) p[j] = static_cast<uint8_t>(w >> (8 * j));
+  }
 }
 
 constexpr float kInv127 = static_cast<float>(1.0 / 127.0);
 constexpr float kInv255 = static_cast<float>(1.0 / 255.0);
 
-// Byte j of a word as a float, through the mantissa of 2^23 (conversions run at
-// an eighth of the rate of additions).
+__device__ __forceinline__ Pair both(float x) { return pair(x, x); }
+
+// a + b where both are products: ptxas contracts a packed product and a packed
+// sum into a multiply-add even with explicit rounding, which the codes'
+// definition does not have; scalar sums stay as they are.
+__device__ __forceinline__ Pair sum_of_products(Pair a, Pair b) {
+  const float2 x = split(a), y = split(b);
+  return pair(__fadd_rn(x.x, y.x), __fadd_rn(x.y, y.y));
+}
+
+// 2^23 + byte j of a word, as a float: conversions of integers run at an eighth
+// of the rate of additions, a byte moved under 2^23's mantissa at half of it.
 __device__ __forceinline__ float byte_float(uint32_t w, int j) {
-  return __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440u + j)) - 8388608.f;
+  return __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440u + j));
 }
 
-// `flipped`: the word of codes with every byte's top bit inverted (c + 128).
-__device__ __forceinline__ float decode_m(uint32_t flipped, int j, float scale) {
-  const float a = __fmul_rn(byte_float(flipped, j) - 128.f, kInv127);
-  return __fmul_rn(scale, __fmul_rn(a, fabsf(a)));
+// Codes j, j + 1 of a word; `flipped`: with every byte's top bit inverted (c + 128).
+__device__ __forceinline__ Pair decode_m(uint32_t flipped, int j, float scale) {
+  const Pair a = (pair(byte_float(flipped, j), byte_float(flipped, j + 1)) + both(-8388736.f)) * both(kInv127);
+  const float2 f = split(a);
+  return both(scale) * pair(__fmul_rn(f.x, fabsf(f.x)), __fmul_rn(f.y, fabsf(f.y)));
 }
 
-__device__ __forceinline__ float decode_v(uint32_t codes, int j, float scale) {
-  float b = __fmul_rn(byte_float(codes, j), kInv255);
-  b = __fmul_rn(b, b);
-  return __fmul_rn(scale, __fmul_rn(b, b));
+__device__ __forceinline__ Pair decode_v(uint32_t codes, int j, float scale) {
+  Pair b = (pair(byte_float(codes, j), byte_float(codes, j + 1)) + both(-8388608.f)) * both(kInv255);
+  b = b * b;
+  return both(scale) * (b * b);
 }
 
-// The codes by definition.  A NaN quotient (a block of zeros, or of infinities)
-// converts to code 0.
+// The codes by definition.  A NaN quotient (a block of infinities) converts to
+// code 0, as does a block of zeros.
 __device__ __noinline__ uint32_t exact_code_m(float m, float scale, uint32_t h) {
   const float u = __fmul_rn(static_cast<float>(h & 0xffffu), 1.f / 65536.f);
   const float x = __fadd_rn(__fmul_rn(__fsqrt_rn(__fdiv_rn(fabsf(m), scale)), 127.f), u);
@@ -199,52 +218,165 @@ __device__ __forceinline__ float sqrt_fast(float x) {
 // one code in 2500 is computed again.
 constexpr float kNear = 2e-4f;
 
-__device__ __forceinline__ uint32_t quick_floor(float root, float top, uint32_t bits16, bool& sure) {
-  // 1 + the random fraction, exactly: its 16 bits at the top of the mantissa
-  const float one_u = __uint_as_float(0x3F800000u | (bits16 & 0x7fff80u));
-  const float x1 = fmaf(root, top, one_u);           // x + 1
-  const float low = __fadd_rd(x1, 8388607.f);        // 2^23 + floor(x)
-  const float part = x1 - (low - 8388607.f);         // x - floor(x)
-  sure = sure && fabsf(part - 0.5f) < 0.5f - kNear;
-  return __float_as_uint(low) & 0xffu;
+// Two floors of root * top + u, each in the low byte of a word.  The random
+// fraction u is 16 bits at the top of the mantissa of 1 + u.
+__device__ __forceinline__ void quick_floor(Pair root, float top, uint32_t bits_a, uint32_t bits_b, uint32_t& a,
+                                            uint32_t& b, bool& sure) {
+  const Pair one_u = pair(__uint_as_float(0x3F800000u | (bits_a & 0x7fff80u)),
+                          __uint_as_float(0x3F800000u | (bits_b & 0x7fff80u)));
+  const Pair x1 = fma(root, both(top), one_u);  // x + 1
+  Pair low;                                     // 2^23 + floor(x)
+  asm("add.rm.f32x2 %0, %1, %2;" : "=l"(low.v) : "l"(x1.v), "l"(both(8388607.f).v));
+  // x - floor(x) - 1/2, exactly: floor(x) + 1.5 first
+  const Pair floor15 = low + both(-8388606.5f);
+  const float2 f = split(floor15), x = split(x1), l = split(low);
+  sure = sure && fabsf(x.x - f.x) < 0.5f - kNear && fabsf(x.y - f.y) < 0.5f - kNear;
+  a = __float_as_uint(l.x);
+  b = __float_as_uint(l.y);
 }
 
-// The codes of four elements, element j in byte j; `inv`: the scale's reciprocal
-//.
+// The low bytes of four words, in order.
+__device__ __forceinline__ uint32_t pack_bytes(const uint32_t (&q)[4]) {
+  return __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+}
+
+// The codes of four elements, element j in byte j; `inv`: the scale's reciprocal.
 __device__ __forceinline__ uint32_t encode_m(const float (&m)[4], float scale, float inv, const uint32_t (&h)[4]) {
   uint32_t q[4];
   bool sure = true;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) q[j] = quick_floor(sqrt_fast(fabsf(m[j]) * inv), 127.f, h[j] << 7, sure);
-  if (!sure) {  // a scale of 0 ends here too: its block is all zeros
+  for (int j = 0; j < 4; j += 2) {
+    quick_floor(pair(sqrt_fast(fabsf(m[j]) * inv), sqrt_fast(fabsf(m[j + 1]) * inv)), 127.f, h[j] << 7, h[j + 1] << 7,
+                q[j], q[j + 1], sure);
+  }
+  if (!sure) {  // a scale of 0 ends here too
 #pragma unroll
     for (int j = 0; j < 4; ++j) q[j] = scale == 0.f ? 0u : exact_code_m(m[j], scale, h[j]);
   }
-  uint32_t w = 0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) w |= ((m[j] < 0.f ? 0u - q[j] : q[j]) & 0xffu) << (8 * j);
-  return w;
+  for (int j = 0; j < 4; ++j) q[j] = m[j] < 0.f ? 0u - q[j] : q[j];  // 2^23 leaves the low byte as it is
+  return pack_bytes(q);
 }
 
 __device__ __forceinline__ uint32_t encode_v(const float (&v)[4], float scale, float inv, const uint32_t (&h)[4]) {
   uint32_t q[4];
   bool sure = true;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) q[j] = quick_floor(sqrt_fast(sqrt_fast(v[j] * inv)), 255.f, h[j] >> 9, sure);
+  for (int j = 0; j < 4; j += 2) {
+    const float2 t = split(pair(v[j], v[j + 1]) * both(inv));
+    quick_floor(pair(sqrt_fast(sqrt_fast(t.x)), sqrt_fast(sqrt_fast(t.y))), 255.f, h[j] >> 9, h[j + 1] >> 9, q[j],
+                q[j + 1], sure);
+  }
   if (!sure) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) q[j] = scale == 0.f ? 0u : exact_code_v(v[j], scale, h[j]);
+    for (int j = 0; j < 4; ++j) q[j] = 0x4B000000u | (scale == 0.f ? 0u : exact_code_v(v[j], scale, h[j]));
   }
-  uint32_t w = 0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) w |= (v[j] > 0.f ? max(q[j], 1u) : q[j]) << (8 * j);
-  return w;
+  for (int j = 0; j < 4; ++j) q[j] = v[j] > 0.f ? max(q[j], 0x4B000001u) : q[j];  // code 1 at least
+  return pack_bytes(q);
 }
 
 // Largest of a warp's non-negative values (their bit patterns order as the
 // values do, and a NaN's is above infinity's, so a NaN is kept).
 __device__ __forceinline__ float warp_max_bits(uint32_t bits) {
   return __uint_as_float(__reduce_max_sync(kFullMask, bits));
+}
+
+// One warp's block of 256 elements from `first` on: lane l holds the quads at 4 l
+// and 128 + 4 l.
+template <typename T, bool EIGHT, bool WHOLE>
+__device__ __forceinline__ void adam_block(const AdamTensor& t, const AdamCommon& c, const AdamScalars& s,
+                                           float grad_scale, int64_t first) {
+  const int lane = threadIdx.x & 31;
+  const int64_t place = first + lane * 4;
+  const int64_t left = WHOLE ? 256 : t.numel - place;  // elements from this lane's first on
+  T* param = static_cast<T*>(t.param) + place;
+  const T* grad = static_cast<const T*>(t.grad) + place;
+  using Moment = typename std::conditional<EIGHT, uint8_t, float>::type;
+  Moment* avg = static_cast<Moment*>(t.m) + place;
+  Moment* avg_sq = static_cast<Moment*>(t.v) + place;
+
+  Pair p[2][2], g[2][2], m[2][2], v[2][2];
+  uint32_t cm[2], cv[2];
+  float sm = 0.f, sv = 0.f;
+  if constexpr (EIGHT) {
+    sm = t.m_scale[first / kBlock];
+    sv = t.v_scale[first / kBlock];
+  }
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    load_quad<WHOLE>(g[q], grad + q * 128, left - q * 128);
+    load_quad<WHOLE>(p[q], param + q * 128, left - q * 128);
+    if constexpr (EIGHT) {
+      cm[q] = load_codes<WHOLE>(avg + q * 128, left - q * 128) ^ 0x80808080u;
+      cv[q] = load_codes<WHOLE>(avg_sq + q * 128, left - q * 128);
+    } else {
+      load_quad<WHOLE>(m[q], avg + q * 128, left - q * 128);
+      load_quad<WHOLE>(v[q], avg_sq + q * 128, left - q * 128);
+    }
+  }
+
+  float top_m = 0.f, top_v = 0.f;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (EIGHT) {
+        m[q][i] = decode_m(cm[q], 2 * i, sm);
+        v[q][i] = decode_v(cv[q], 2 * i, sv);
+      }
+      const Pair gi = g[q][i] * both(grad_scale);
+      m[q][i] = sum_of_products(m[q][i] * both(c.b1), gi * both(c.one_b1));
+      v[q][i] = sum_of_products(v[q][i] * both(c.b2), (gi * gi) * both(c.one_b2));
+      // Approximate root and reciprocal: 2^-21 of an update that is a small part
+      // of the parameter.  The root takes subnormal values too: with eps 0 one of
+      // 0 would be divided by.
+      const float2 fv = split(v[q][i]), fm = split(m[q][i]);
+      float r0, r1;
+      asm("sqrt.approx.f32 %0, %1;" : "=f"(r0) : "f"(fv.x));
+      asm("sqrt.approx.f32 %0, %1;" : "=f"(r1) : "f"(fv.y));
+      const float2 denom = split(fma(pair(r0, r1), both(s.inv_sqrt_bc2), both(c.eps)));
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(denom.x));
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r1) : "f"(denom.y));
+      p[q][i] = fma(m[q][i] * pair(r0, r1), both(-s.step_size), p[q][i] * both(s.keep));
+      if constexpr (EIGHT) {
+        // elements past the tensor's end count as zeros whatever their block's scale is
+        const bool in0 = WHOLE || q * 128 + 2 * i < left, in1 = WHOLE || q * 128 + 2 * i + 1 < left;
+        const auto raise = [](float& top, float x) {  // a NaN is kept
+          asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(x));
+        };
+        raise(top_m, in0 ? fabsf(fm.x) : 0.f);
+        raise(top_m, in1 ? fabsf(fm.y) : 0.f);
+        raise(top_v, in0 ? fv.x : 0.f);
+        raise(top_v, in1 ? fv.y : 0.f);
+      }
+    }
+    store_quad<WHOLE>(p[q], param + q * 128, left - q * 128);
+    if constexpr (!EIGHT) {
+      store_quad<WHOLE>(m[q], avg + q * 128, left - q * 128);
+      store_quad<WHOLE>(v[q], avg_sq + q * 128, left - q * 128);
+    }
+  }
+  if constexpr (EIGHT) {
+    const uint32_t key = mix(t.ordinal * 0x632BE5ABu + s.seed) + static_cast<uint32_t>(place);
+    const float new_sm = warp_max_bits(__float_as_uint(top_m) & 0x7fffffffu);
+    const float new_sv = warp_max_bits(__float_as_uint(top_v) & 0x7fffffffu);
+    const float inv_m = __frcp_rn(new_sm), inv_v = __frcp_rn(new_sv);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      uint32_t h[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h[j] = mix(key + (q * 128 + j));
+      const float2 m0 = split(m[q][0]), m1 = split(m[q][1]), v0 = split(v[q][0]), v1 = split(v[q][1]);
+      const float fm[4] = {m0.x, m0.y, m1.x, m1.y}, fv[4] = {v0.x, v0.y, v1.x, v1.y};
+      store_codes<WHOLE>(encode_m(fm, new_sm, inv_m, h), avg + q * 128, left - q * 128);
+      store_codes<WHOLE>(encode_v(fv, new_sv, inv_v, h), avg_sq + q * 128, left - q * 128);
+    }
+    if (lane == 0) {
+      t.m_scale[first / kBlock] = new_sm;
+      t.v_scale[first / kBlock] = new_sv;
+    }
+  }
 }
 
 template <typename T, bool EIGHT, int N>
@@ -263,120 +395,46 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constan
   const AdamTensor& t = a.t[lo];
   const AdamScalars s = a.c.device_s != nullptr ? *a.c.device_s : a.c.s;
   const float grad_scale = a.c.grad_scale != nullptr ? *a.c.grad_scale : 1.f;
-  const int64_t n = t.numel;
-  T* param = static_cast<T*>(t.param);
-  const T* grad = static_cast<const T*>(t.grad);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t base = static_cast<int64_t>(chunk - t.first_chunk) * kChunk + warp * (kWarpBlocks * kBlock);
+  const int64_t first = static_cast<int64_t>(chunk - t.first_chunk) * kChunk + (threadIdx.x >> 5) * kBlock;
+  if (first >= t.numel) return;
   const uintptr_t wide = reinterpret_cast<uintptr_t>(t.param) | reinterpret_cast<uintptr_t>(t.grad);
   const uintptr_t state = reinterpret_cast<uintptr_t>(t.m) | reinterpret_cast<uintptr_t>(t.v);
-  const bool vec = (wide & (4 * sizeof(T) - 1)) == 0 && (state & (EIGHT ? 3 : 15)) == 0;
-
-  float p[kWarpBlocks][2][4], g[kWarpBlocks][2][4], m[kWarpBlocks][2][4], v[kWarpBlocks][2][4];
-  uint32_t cm[kWarpBlocks][2], cv[kWarpBlocks][2];
-  float sm[kWarpBlocks], sv[kWarpBlocks];
-#pragma unroll
-  for (int b = 0; b < kWarpBlocks; ++b) {
-    const int64_t first = base + b * kBlock;
-    if (EIGHT) {
-      sm[b] = first < n ? t.m_scale[first / kBlock] : 0.f;
-      sv[b] = first < n ? t.v_scale[first / kBlock] : 0.f;
-    }
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int64_t i = first + q * 128 + lane * 4;
-      load_quad<T>(g[b][q], grad, i, n, vec);
-      load_quad<T>(p[b][q], param, i, n, vec);
-      if (EIGHT) {
-        cm[b][q] = load_codes(t.m, i, n, vec);
-        cv[b][q] = load_codes(t.v, i, n, vec);
-      } else {
-        load_quad<float>(m[b][q], static_cast<const float*>(t.m), i, n, vec);
-        load_quad<float>(v[b][q], static_cast<const float*>(t.v), i, n, vec);
-      }
-    }
-  }
-
-#pragma unroll
-  for (int b = 0; b < kWarpBlocks; ++b) {
-    uint32_t top_m = 0, top_v = 0;
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float& pj = p[b][q][j];
-        float& mj = m[b][q][j];
-        float& vj = v[b][q][j];
-        if (EIGHT) {
-          mj = decode_m(cm[b][q] ^ 0x80808080u, j, sm[b]);
-          vj = decode_v(cv[b][q], j, sv[b]);
-        }
-        const float gj = __fmul_rn(g[b][q][j], grad_scale);
-        mj = __fadd_rn(__fmul_rn(mj, a.c.b1), __fmul_rn(gj, a.c.one_b1));
-        vj = __fadd_rn(__fmul_rn(vj, a.c.b2), __fmul_rn(__fmul_rn(gj, gj), a.c.one_b2));
-        // approximate root and quotient: 2^-22 of an update that is a small part of the parameter
-        float root;  // of subnormal values too: with eps 0 a root of 0 would be divided by
-        asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(vj));
-        const float denom = fmaf(root, s.inv_sqrt_bc2, a.c.eps);
-        pj = fmaf(pj, s.keep, -s.step_size * __fdividef(mj, denom));
-        if (EIGHT) {
-          // elements past the tensor's end count as zeros whatever their block's scale is
-          const bool in = base + b * kBlock + q * 128 + lane * 4 + j < n;
-          top_m = max(top_m, in ? __float_as_uint(mj) & 0x7fffffffu : 0u);
-          top_v = max(top_v, in ? __float_as_uint(vj) & 0x7fffffffu : 0u);
-        }
-      }
-      const int64_t i = base + b * kBlock + q * 128 + lane * 4;
-      store_quad<T>(p[b][q], param, i, n, vec);
-      if (!EIGHT) {
-        store_quad<float>(m[b][q], static_cast<float*>(t.m), i, n, vec);
-        store_quad<float>(v[b][q], static_cast<float*>(t.v), i, n, vec);
-      }
-    }
-    if (EIGHT) {
-      const uint32_t key = mix(t.ordinal * 0x632BE5ABu + s.seed);
-      const float new_sm = warp_max_bits(top_m), new_sv = warp_max_bits(top_v);
-      const float inv_m = __frcp_rn(new_sm), inv_v = __frcp_rn(new_sv);
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int64_t i = base + b * kBlock + q * 128 + lane * 4;
-        uint32_t h[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) h[j] = mix(static_cast<uint32_t>(i + j) + key);
-        store_codes(encode_m(m[b][q], new_sm, inv_m, h), t.m, i, n, vec);
-        store_codes(encode_v(v[b][q], new_sv, inv_v, h), t.v, i, n, vec);
-      }
-      const int64_t first = base + b * kBlock;
-      if (lane == 0 && first < n) {
-        t.m_scale[first / kBlock] = new_sm;
-        t.v_scale[first / kBlock] = new_sv;
-      }
-    }
+  const bool aligned = (wide & (4 * sizeof(T) - 1)) == 0 && (state & (EIGHT ? 3 : 15)) == 0;
+  if (aligned && first + kBlock <= t.numel) {
+    adam_block<T, EIGHT, true>(t, a.c, s, grad_scale, first);
+  } else {
+    adam_block<T, EIGHT, false>(t, a.c, s, grad_scale, first);
   }
 }
 
 // The values that 8-bit moments stand for; a warp decodes one block.
-__global__ void __launch_bounds__(kThreads) adam_moments_kernel(const void* m, const void* v, const float* m_scale,
-                                                               const float* v_scale, int64_t n, float* out_m,
-                                                               float* out_v) {
-  const int lane = threadIdx.x & 31;
+template <bool WHOLE>
+__device__ __forceinline__ void decode_block(const uint8_t* m, const uint8_t* v, float sm, float sv, int64_t left,
+                                             float* out_m, float* out_v) {
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const uint32_t cm = load_codes<WHOLE>(m + q * 128, left - q * 128) ^ 0x80808080u;
+    const uint32_t cv = load_codes<WHOLE>(v + q * 128, left - q * 128);
+    const Pair dm[2] = {decode_m(cm, 0, sm), decode_m(cm, 2, sm)};
+    const Pair dv[2] = {decode_v(cv, 0, sv), decode_v(cv, 2, sv)};
+    store_quad<WHOLE>(dm, out_m + q * 128, left - q * 128);
+    store_quad<WHOLE>(dv, out_v + q * 128, left - q * 128);
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) adam_moments_kernel(const uint8_t* m, const uint8_t* v,
+                                                               const float* m_scale, const float* v_scale, int64_t n,
+                                                               float* out_m, float* out_v) {
   const int64_t block = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
   if (block * kBlock >= n) return;
   const uintptr_t at = reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v);
-  const bool vec = (at & 3) == 0 && aligned16(out_m) && aligned16(out_v);
+  const bool aligned = (at & 3) == 0 && aligned16(out_m) && aligned16(out_v);
   const float sm = m_scale[block], sv = v_scale[block];
-#pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const int64_t i = block * kBlock + q * 128 + lane * 4;
-    const uint32_t cm = load_codes(m, i, n, vec), cv = load_codes(v, i, n, vec);
-    float dm[4], dv[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      dm[j] = decode_m(cm ^ 0x80808080u, j, sm);
-      dv[j] = decode_v(cv, j, sv);
-    }
-    store_quad<float>(dm, out_m, i, n, vec);
-    store_quad<float>(dv, out_v, i, n, vec);
+  const int64_t place = block * kBlock + (threadIdx.x & 31) * 4;
+  if (aligned && (block + 1) * kBlock <= n) {
+    decode_block<true>(m + place, v + place, sm, sv, 0, out_m + place, out_v + place);
+  } else {
+    decode_block<false>(m + place, v + place, sm, sv, n - place, out_m + place, out_v + place);
   }
 }
 
@@ -496,6 +554,7 @@ extern "C" int rfm_adamw_moments(const void* exp_avg, const void* exp_avg_sq, co
   }
   const int64_t per = static_cast<int64_t>(kThreads / 32) * kBlock;
   adam_moments_kernel<<<static_cast<unsigned>((numel + per - 1) / per), kThreads, 0, as_stream(stream)>>>(
-      exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, numel, out_avg, out_avg_sq);
+      static_cast<const uint8_t*>(exp_avg), static_cast<const uint8_t*>(exp_avg_sq), exp_avg_scale, exp_avg_sq_scale,
+      numel, out_avg, out_avg_sq);
   return launch_status();
 }
