@@ -651,21 +651,20 @@ __global__ void __launch_bounds__(256) finish_kernel(const FinishArgs a) {
 
 struct GradPreArgs {
   const void* dy;
-  const void* saved;  // pre, or (relu without a residual) out; null: no activation
+  const void* saved;  // pre, or (relu without a residual) out; not read without an activation
   void* dp;           // null: not stored
   float* partial;     // [slabs][n] column sums, null: not wanted
   int64_t rows;
   int64_t ld_dy;
   int64_t ld_dp;
   int32_t n;
-  int32_t activation;
 };
 
 constexpr int kPreWarps = 8;
 
 // A CTA owns 32 * VEC columns and every gridDim.y-th group of 8 rows (a row a
 // warp); the sums of its warps are added in their order at the end.
-template <typename T, int VEC>
+template <typename T, int VEC, int ACT>
 __global__ void __launch_bounds__(32 * kPreWarps) grad_pre_kernel(const GradPreArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = (static_cast<int>(blockIdx.x) * 32 + lane) * VEC;
@@ -675,25 +674,36 @@ __global__ void __launch_bounds__(32 * kPreWarps) grad_pre_kernel(const GradPreA
   for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
   const int64_t stride = static_cast<int64_t>(gridDim.y) * kPreWarps;
   if (in) {
-#pragma unroll 4
-    for (int64_t row = static_cast<int64_t>(blockIdx.y) * kPreWarps + warp; row < a.rows; row += stride) {
-      const Pack<T, VEC> g = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.dy) + row * a.ld_dy + col);
-      float v[VEC];
+    // four rows' loads go out before the first row is used
+    constexpr int kRows = VEC > 1 ? 4 : 8;
+    for (int64_t row = static_cast<int64_t>(blockIdx.y) * kPreWarps + warp; row < a.rows; row += kRows * stride) {
+      Pack<T, VEC> g[kRows], p[kRows];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) v[j] = to_float(g.v[j]);
-      if (a.saved != nullptr) {
-        const Pack<T, VEC> p =
-            *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.saved) + row * a.n + col);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] *= activate_grad(to_float(p.v[j]), a.activation);
+      for (int r = 0; r < kRows; ++r) {
+        const int64_t at = row + r * stride;
+        if (at >= a.rows) continue;
+        g[r] = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.dy) + at * a.ld_dy + col);
+        if (ACT != RFM_ACT_NONE) {
+          p[r] = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.saved) + at * a.n + col);
+        }
       }
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) sum[j] += v[j];
-      if (a.dp != nullptr) {
-        Pack<T, VEC> o;
+      for (int r = 0; r < kRows; ++r) {
+        const int64_t at = row + r * stride;
+        if (at >= a.rows) continue;
+        float v[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) o.v[j] = from_float<T>(v[j]);
-        *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.dp) + row * a.ld_dp + col) = o;
+        for (int j = 0; j < VEC; ++j) {
+          v[j] = to_float(g[r].v[j]);
+          if (ACT != RFM_ACT_NONE) v[j] *= activate_grad(to_float(p[r].v[j]), ACT);
+          sum[j] += v[j];
+        }
+        if (a.dp != nullptr) {
+          Pack<T, VEC> o;
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) o.v[j] = from_float<T>(v[j]);
+          *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.dp) + at * a.ld_dp + col) = o;
+        }
       }
     }
   }
@@ -713,22 +723,137 @@ __global__ void __launch_bounds__(32 * kPreWarps) grad_pre_kernel(const GradPreA
   }
 }
 
-__global__ void __launch_bounds__(256) bias_sum_kernel(const float* partial, int slabs, int n, void* out, int dtype) {
-  __shared__ float sums[8][33];
+// The slabs' sums per column, in a fixed order: 32 columns per CTA, each of 32
+// warps every 32nd slab, then the 32 sums.
+__global__ void __launch_bounds__(1024) bias_sum_kernel(const float* partial, int slabs, int n, void* out, int dtype) {
+  __shared__ float sums[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = static_cast<int>(blockIdx.x) * 32 + lane;
   float s = 0.f;
   if (col < n) {
-#pragma unroll 4
-    for (int k = warp; k < slabs; k += 8) s += partial[static_cast<int64_t>(k) * n + col];
+#pragma unroll 8
+    for (int k = warp; k < slabs; k += 32) s += partial[static_cast<int64_t>(k) * n + col];
   }
   sums[warp][lane] = s;
   __syncthreads();
-  if (warp == 0 && col < n) {
+  // warp w adds the 32 sums of column w
+  s = sums[lane][warp];
 #pragma unroll
-    for (int k = 1; k < 8; ++k) s += sums[k][lane];
-    store_param(out, dtype, col, s);
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kFullMask, s, o);
+  const int mine = static_cast<int>(blockIdx.x) * 32 + warp;
+  if (lane == 0 && mine < n) store_param(out, dtype, mine, s);
+}
+
+template <typename T, int VEC>
+int launch_grad_pre(const GradPreArgs& a, int activation, const dim3& grid, cudaStream_t s) {
+  if (activation == RFM_ACT_RELU) {
+    grad_pre_kernel<T, VEC, RFM_ACT_RELU><<<grid, 32 * kPreWarps, 0, s>>>(a);
+  } else if (activation == RFM_ACT_GELU) {
+    grad_pre_kernel<T, VEC, RFM_ACT_GELU><<<grid, 32 * kPreWarps, 0, s>>>(a);
+  } else {
+    grad_pre_kernel<T, VEC, RFM_ACT_NONE><<<grid, 32 * kPreWarps, 0, s>>>(a);
   }
+  return launch_status();
+}
+
+// ---- a few rows: the weight is read once and nothing is tiled
+
+// One warp computes W columns of the output for R rows: lane l holds the 16-byte
+// pieces l, l + 32, .. of the weight's rows and of x's, products and sums in fp32,
+// one shuffle tree at the end.  With a tile of 128 rows the tensor cores would
+// work on zeros, and the contraction would be split to occupy the SMs: two
+// launches.  Here the weight's bytes in flight are all that counts.  Measured
+// (4096 -> 4096, fp16): 1 row 8.4 us (4.0 TB/s with its launch), tiles 20.6; 2
+// rows 10.4 and 23.9; 4 rows 18.6 and 16.5, so two rows are the most.
+struct FewArgs {
+  const void* x;
+  const void* weight;
+  const void* bias;
+  const void* residual;
+  void* out;
+  void* pre;
+  int64_t ld_x, ld_w, ld_res;
+  int32_t rows, n, k;
+  int32_t bias_dtype;
+  int32_t activation;
+};
+
+constexpr int kFewWarps = 4;
+
+template <typename T>
+__device__ __forceinline__ Pack<T, 8> load_piece(const T* row, int k, int depth) {
+  if (k + 8 <= depth) return *reinterpret_cast<const Pack<T, 8>*>(row + k);
+  Pack<T, 8> p;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) p.v[j] = k + j < depth ? row[k + j] : from_float<T>(0.f);
+  return p;
+}
+
+template <typename T, int R, int W, int UNROLL>
+__global__ void __launch_bounds__(32 * kFewWarps) few_rows_kernel(const FewArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int n0 = (static_cast<int>(blockIdx.x) * kFewWarps + (threadIdx.x >> 5)) * W;
+  if (n0 >= a.n) return;
+  const T* x = static_cast<const T*>(a.x);
+  const T* w = static_cast<const T*>(a.weight) + n0 * a.ld_w;
+  Pair acc[R][W];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int c = 0; c < W; ++c) acc[r][c] = pair(0.f, 0.f);
+  for (int k0 = lane * 8; k0 < a.k; k0 += 256 * UNROLL) {
+    Pack<T, 8> wp[UNROLL][W];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int c = 0; c < W; ++c)
+        wp[u][c] = load_piece(w + (n0 + c < a.n ? c : 0) * a.ld_w, k0 + u * 256, a.k);  // a column past the end: twice
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const Pack<T, 8> xp = load_piece(x + (r < a.rows ? r : 0) * a.ld_x, k0 + u * 256, a.k);
+#pragma unroll
+        for (int c = 0; c < W; ++c)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[r][c] = fma(load_pair(xp, j), load_pair(wp[u][c], j), acc[r][c]);
+      }
+    }
+  }
+  // element e = r * W + c of the warp's block ends up with lane e
+  float mine = 0.f;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int c = 0; c < W; ++c) {
+      const float2 f = split(acc[r][c]);
+      float s = f.x + f.y;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kFullMask, s, o);
+      if (lane == r * W + c) mine = s;
+    }
+  const int row = lane / W, col = n0 + lane % W;
+  if (lane >= R * W || row >= a.rows || col >= a.n) return;
+  if (a.bias != nullptr) mine += load_param(a.bias, a.bias_dtype, col);
+  const int64_t at = static_cast<int64_t>(row) * a.n + col;
+  if (a.pre != nullptr) static_cast<T*>(a.pre)[at] = from_float<T>(mine);
+  mine = activate(mine, a.activation);
+  if (a.residual != nullptr) mine += to_float(static_cast<const T*>(a.residual)[row * a.ld_res + col]);
+  static_cast<T*>(a.out)[at] = from_float<T>(mine);
+}
+
+constexpr int kFewRows = 2;  // most rows of this form
+
+template <typename T>
+int launch_few_rows(const FewArgs& a, cudaStream_t s) {
+  constexpr int kColumns = 2;  // of a warp
+  const unsigned grid = static_cast<unsigned>((a.n + kFewWarps * kColumns - 1) / (kFewWarps * kColumns));
+  if (a.rows == 1) {
+    few_rows_kernel<T, 1, kColumns, 4><<<grid, 32 * kFewWarps, 0, s>>>(a);
+  } else {
+    few_rows_kernel<T, 2, kColumns, 4><<<grid, 32 * kFewWarps, 0, s>>>(a);
+  }
+  return launch_status();
 }
 
 // ---- host side
@@ -776,34 +901,39 @@ struct Cut {
   int splits = 1;
 };
 
-// Estimated cycles of the busiest SM for each cut.  A 64-deep slice of a
-// 128 x BN tile takes the tensor cores 2 BN cycles and brings (128 + BN) * 128
-// bytes (a pair of CTAs: each half of B's), which an SM takes in at about 80 a
-// cycle; a tile's epilogue, hidden behind the next tile's products but for the
-// last, 11 cycles a column (measured range: 8 to 14); a part's fp32 sums are
-// written and read once, and the second kernel costs about 5000 cycles.
+// Estimated cycles of the busiest SM for each cut: a tile's fixed part (fill and
+// drain of its pipeline, its stores) and one part per 64-deep slice, fitted to
+// measurements of 38 products (rows 16 to 31200, 64 to 4096 deep, forward and both
+// backward products; the chosen cut is on average 2 % behind the best, 19 % at
+// worst).  Shallow products go to one CTA a tile (31200 x 256 -> 2048: 42.9 us,
+// pairs 49.2), deep ones to pairs, which bring a third less through L2 (16384 x
+// 4096 -> 4096: 371 us, single 427); narrower tiles only fill SMs (300 x 2048 ->
+// 256: 64 columns in 4 parts 12.4 us, 256 columns whole 16.5).  Splitting pays
+// the fp32 sums' way through L2 and a second launch.
 Cut choose_cut(int64_t m, int n, int k_blocks) {
+  struct Cost {
+    int bn, pair;
+    double start, tile, slice;
+  };
+  constexpr Cost kCosts[] = {
+      {256, 1, 7500, 4200, 650}, {256, 0, 5000, 3400, 820}, {128, 0, 5000, 1800, 590}, {64, 0, 5000, 1200, 550}};
+  constexpr double kSecondKernel = 9000.0, kPartBytesPerCycle = 1650.0;
+  constexpr int kLeastSlices = 5;  // of a part
   const int sms = device_sm_count();
   Cut best;
-  double least = 1e30;
-  for (int shape = 0; shape < 4; ++shape) {
-    const int pair = shape == 0, bn = shape < 2 ? 256 : shape == 2 ? 128 : 64;
-    const int64_t rows = pair ? 2 * kBM : kBM;
-    const int64_t tiles = ((m + rows - 1) / rows) * ((n + bn - 1) / bn);
-    const int64_t workers = pair ? sms / 2 : sms;
-    const double slice = fmax(2.0 * bn, (128.0 + (pair ? bn / 2 : bn)) * 128.0 / 80.0);
-    for (int splits = 1; splits <= kMaxSplits && splits <= k_blocks; ++splits) {
-      if (splits > 1 && (k_blocks / splits < 2 || tiles * (splits - 1) >= 4 * workers)) break;
-      const int64_t waves = (tiles * splits + workers - 1) / workers;
-      const double depth = static_cast<double>((k_blocks + splits - 1) / splits);
-      const double epilogue = 11.0 * bn;
-      double cycles = 1500.0 + waves * fmax(depth * slice, epilogue) + epilogue;
-      if (splits > 1) {
-        cycles += 5000.0 + 8.0 * splits * static_cast<double>(m) * n / 3000.0;  // about 3 KB a cycle to L2
-      }
+  double least = 1e300;
+  for (const Cost& c : kCosts) {
+    const int64_t rows = c.pair ? 2 * kBM : kBM;
+    const int64_t tiles = ((m + rows - 1) / rows) * ((n + c.bn - 1) / c.bn);
+    const int64_t workers = c.pair ? sms / 2 : sms;
+    for (int splits = 1; splits <= kMaxSplits; ++splits) {
+      if (splits > 1 && (k_blocks / splits < kLeastSlices || tiles * (splits - 1) >= 4 * workers)) break;
+      const double waves = static_cast<double>((tiles * splits + workers - 1) / workers);
+      double cycles = c.start + waves * (c.tile + (k_blocks + splits - 1) / splits * c.slice);
+      if (splits > 1) cycles += kSecondKernel + 8.0 * splits * static_cast<double>(m) * n / kPartBytesPerCycle;
       if (cycles < least) {
         least = cycles;
-        best = Cut{bn, pair, splits};
+        best = Cut{c.bn, c.pair, splits};
       }
     }
   }
@@ -971,7 +1101,7 @@ extern "C" int64_t rfm_linear_forward_workspace_bytes(int64_t rows, int in_featu
   using namespace rfm;
   const int rc = check_sizes(rows, in_features, out_features, RFM_DTYPE_BF16);
   if (rc != RFM_OK) return -rc;
-  return partial_bytes(rows, out_features, in_features);
+  return rows <= kFewRows ? 0 : partial_bytes(rows, out_features, in_features);
 }
 
 extern "C" int rfm_linear_forward(const rfm_linear* p, void* stream) {
@@ -987,6 +1117,15 @@ extern "C" int rfm_linear_forward(const rfm_linear* p, void* stream) {
     return RFM_ERR_INVALID_ARGUMENT;
   }
   if (p->residual != nullptr && p->rows > 1 && p->ld_residual < p->out_features) return RFM_ERR_INVALID_ARGUMENT;
+  if (p->rows <= kFewRows) {
+    FewArgs f{p->x,     p->weight,      p->bias,
+              p->residual, p->out,      p->pre,
+              p->ld_x,  p->ld_weight,   p->ld_residual,
+              static_cast<int32_t>(p->rows), p->out_features, p->in_features,
+              p->bias_dtype, p->activation};
+    return p->dtype == RFM_DTYPE_BF16 ? launch_few_rows<__nv_bfloat16>(f, as_stream(stream))
+                                      : launch_few_rows<__half>(f, as_stream(stream));
+  }
   const int64_t need = partial_bytes(p->rows, p->out_features, p->in_features);
   if (need > 0 && (p->workspace == nullptr || !aligned16(p->workspace) || p->workspace_bytes < need)) {
     return RFM_ERR_INVALID_ARGUMENT;
@@ -1042,7 +1181,7 @@ extern "C" int rfm_linear_backward(const rfm_linear_grad* p, void* stream) {
       return RFM_ERR_LAUNCH;
     }
     if (p->grad_bias != nullptr) {
-      bias_sum_kernel<<<(out + 31) / 32, 256, 0, s>>>(nullptr, 0, out, p->grad_bias, p->bias_dtype);
+      bias_sum_kernel<<<(out + 31) / 32, 1024, 0, s>>>(nullptr, 0, out, p->grad_bias, p->bias_dtype);
     }
     return launch_status();
   }
@@ -1071,26 +1210,21 @@ extern "C" int rfm_linear_backward(const rfm_linear_grad* p, void* stream) {
     a.partial = p->grad_bias != nullptr ? static_cast<float*>(p->workspace) : nullptr;
     a.rows = rows;
     a.n = out;
-    a.activation = p->activation;
     const bool vec = out % 8 == 0 && a.ld_dy % 8 == 0 && aligned16(a.dy) && aligned16(a.saved);
     const int width = 32 * (vec ? 8 : 1);
     const int slabs = bias_slabs(rows, out, vec ? 8 : 1);
     const dim3 grid((out + width - 1) / width, slabs);
+    int done;
     if (p->dtype == RFM_DTYPE_BF16) {
-      if (vec) {
-        grad_pre_kernel<__nv_bfloat16, 8><<<grid, 256, 0, s>>>(a);
-      } else {
-        grad_pre_kernel<__nv_bfloat16, 1><<<grid, 256, 0, s>>>(a);
-      }
-    } else if (vec) {
-      grad_pre_kernel<__half, 8><<<grid, 256, 0, s>>>(a);
+      done = vec ? launch_grad_pre<__nv_bfloat16, 8>(a, p->activation, grid, s)
+                 : launch_grad_pre<__nv_bfloat16, 1>(a, p->activation, grid, s);
     } else {
-      grad_pre_kernel<__half, 1><<<grid, 256, 0, s>>>(a);
+      done = vec ? launch_grad_pre<__half, 8>(a, p->activation, grid, s)
+                 : launch_grad_pre<__half, 1>(a, p->activation, grid, s);
     }
-    int done = launch_status();
     if (done != RFM_OK) return done;
     if (p->grad_bias != nullptr) {
-      bias_sum_kernel<<<(out + 31) / 32, 256, 0, s>>>(a.partial, slabs, out, p->grad_bias, p->bias_dtype);
+      bias_sum_kernel<<<(out + 31) / 32, 1024, 0, s>>>(a.partial, slabs, out, p->grad_bias, p->bias_dtype);
       done = launch_status();
       if (done != RFM_OK) return done;
     }
