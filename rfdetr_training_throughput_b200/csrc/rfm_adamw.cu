@@ -161,8 +161,6 @@ __device__ __forceinline__ void store_codes(uint32_t w, uint8_t* p, int64_t left
 constexpr float kInv127 = static_cast<float>(1.0 / 127.0);
 constexpr float kInv255 = static_cast<float>(1.0 / 255.0);
 
-__device__ __forceinline__ Pair both(float x) { return pair(x, x); }
-
 // a + b where both are products: ptxas contracts a packed product and a packed
 // sum into a multiply-add even with explicit rounding, which the codes'
 // definition does not have; scalar sums stay as they are.

@@ -100,55 +100,63 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return r;
 }
 
-// The normal distribution's cdf at v: its tail q(|v|) as 2 to a polynomial.
+// The normal distribution's cdf at two values: its tail q(|v|) as 2 to a polynomial.
 // log2 q is smooth where q itself falls over many orders; the coefficients are a
 // least-maximum fit of degree 8 on [0, 6]: q is off by at most 2.5e-6 of itself
 // up to 3 and 1.2e-5 up to 6 (below 2^-30 there), |v| q by 3e-7, far under half a
 // step of the 16-bit results (2^-12).  Beyond, the polynomial keeps falling and q
-// underflows to 0 (at an infinity too; a NaN stays one).  14 instructions, against
-// some 25 of erff and a division less than the usual rational forms.
-__device__ __forceinline__ float normal_cdf(float v) {
-  const float z = fabsf(v);
-  float p = -1.2245089919815655e-07f;
-  p = fmaf(p, z, 8.983980137600156e-07f);
-  p = fmaf(p, z, 3.7126268580323085e-05f);
-  p = fmaf(p, z, -8.181885350495577e-04f);
-  p = fmaf(p, z, 8.22749175131321e-03f);
-  p = fmaf(p, z, -5.3588107228279114e-02f);
-  p = fmaf(p, z, -4.587007761001587e-01f);
-  p = fmaf(p, z, -1.1511954069137573f);
-  p = fmaf(p, z, -9.999973773956299e-01f);
-  const float q = exp2_fast(p);
-  return v > 0.f ? 1.f - q : q;
+// underflows to 0 (at an infinity too; a NaN stays one).  Seven instructions a
+// value and one of the special-function unit, against some 25 of erff.
+__device__ __forceinline__ Pair normal_cdf(Pair v) {
+  const float2 f = split(v);
+  const Pair z = pair(fabsf(f.x), fabsf(f.y));
+  Pair p = fma(both(-1.2245089919815655e-07f), z, both(8.983980137600156e-07f));
+  p = fma(p, z, both(3.7126268580323085e-05f));
+  p = fma(p, z, both(-8.181885350495577e-04f));
+  p = fma(p, z, both(8.22749175131321e-03f));
+  p = fma(p, z, both(-5.3588107228279114e-02f));
+  p = fma(p, z, both(-4.587007761001587e-01f));
+  p = fma(p, z, both(-1.1511954069137573f));
+  p = fma(p, z, both(-9.999973773956299e-01f));
+  const float2 e = split(p);
+  const float qx = exp2_fast(e.x), qy = exp2_fast(e.y);
+  return pair(f.x > 0.f ? 1.f - qx : qx, f.y > 0.f ? 1.f - qy : qy);
 }
 
-__device__ __forceinline__ float activate(float v, int act) {
-  if (act == RFM_ACT_RELU) {  // a NaN stays one
-    float r;
-    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(v));
-    return r;
+__device__ __forceinline__ float relu(float v) {  // a NaN stays one
+  float r;
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+__device__ __forceinline__ Pair activate(Pair v, int act) {
+  if (act == RFM_ACT_RELU) {
+    const float2 f = split(v);
+    return pair(relu(f.x), relu(f.y));
   }
-  if (act == RFM_ACT_GELU) return v * normal_cdf(v);
-  return v;
+  return act == RFM_ACT_GELU ? v * normal_cdf(v) : v;
 }
 
-// act'(v): 0 at relu's border; gelu: cdf(v) + v pdf(v).
-__device__ __forceinline__ float activate_grad(float v, int act) {
-  if (act == RFM_ACT_RELU) return v > 0.f ? 1.f : 0.f;
+__device__ __forceinline__ float activate(float v, int act) { return split(activate(both(v), act)).x; }
+
+// dy act'(v): act' is 0 at relu's border, and cdf(v) + v pdf(v) for gelu.
+__device__ __forceinline__ Pair times_activate_grad(Pair dy, Pair v, int act) {
+  const float2 f = split(v);
+  if (act == RFM_ACT_RELU) return dy * pair(f.x > 0.f ? 1.f : 0.f, f.y > 0.f ? 1.f : 0.f);
   if (act == RFM_ACT_GELU) {
     // pdf(v) = 2^(-v^2 log2(e) / 2) / sqrt(2 pi)
-    return fmaf(v * 0.39894228040143268f, exp2_fast(v * v * -0.72134752044448170f), normal_cdf(v));
+    const float2 e = split(v * v * both(-0.72134752044448170f));
+    const Pair pdf = pair(exp2_fast(e.x), exp2_fast(e.y));
+    return dy * fma(v * both(0.39894228040143268f), pdf, normal_cdf(v));
   }
-  return 1.f;
+  return dy;
 }
 
-// Two fp32 sums in one instruction.
+// Adds two values to two registers that hold floats.
 __device__ __forceinline__ void add2(uint32_t& a, uint32_t& b, float x, float y) {
-  uint64_t s = static_cast<uint64_t>(b) << 32 | a;
-  const uint64_t t = static_cast<uint64_t>(__float_as_uint(y)) << 32 | __float_as_uint(x);
-  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s) : "l"(t));
-  a = static_cast<uint32_t>(s);
-  b = static_cast<uint32_t>(s >> 32);
+  const float2 s = split(pair(__uint_as_float(a), __uint_as_float(b)) + pair(x, y));
+  a = __float_as_uint(s.x);
+  b = __float_as_uint(s.y);
 }
 
 template <typename T>
@@ -556,7 +564,11 @@ __global__ void __launch_bounds__(Shape<BN, CG>::kThreads, 1)
           }
           if (ACT != RFM_ACT_NONE) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(activate(__uint_as_float(v[j]), ACT));
+            for (int j = 0; j < 32; j += 2) {
+              const float2 f = split(activate(pair(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), ACT));
+              v[j] = __float_as_uint(f.x);
+              v[j + 1] = __float_as_uint(f.y);
+            }
           }
           if (has_res) {
 #pragma unroll
@@ -665,23 +677,24 @@ constexpr int kPreWarps = 8;
 // A CTA owns 32 * VEC columns and every gridDim.y-th group of 8 rows (a row a
 // warp); the sums of its warps are added in their order at the end.
 template <typename T, int VEC, int ACT>
-__global__ void __launch_bounds__(32 * kPreWarps) grad_pre_kernel(const GradPreArgs a) {
+__global__ void __launch_bounds__(32 * kPreWarps, 3) grad_pre_kernel(const GradPreArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = (static_cast<int>(blockIdx.x) * 32 + lane) * VEC;
   const bool in = col < a.n;
-  float sum[VEC];
+  constexpr int kPairs = (VEC + 1) / 2;
+  Pair sum[kPairs];
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
+  for (int j = 0; j < kPairs; ++j) sum[j] = both(0.f);
   const int64_t stride = static_cast<int64_t>(gridDim.y) * kPreWarps;
   if (in) {
     // four rows' loads go out before the first row is used
-    constexpr int kRows = VEC > 1 ? 4 : 8;
+    constexpr int kRows = 4;
     for (int64_t row = static_cast<int64_t>(blockIdx.y) * kPreWarps + warp; row < a.rows; row += kRows * stride) {
       Pack<T, VEC> g[kRows], p[kRows];
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
-        const int64_t at = row + r * stride;
-        if (at >= a.rows) continue;
+        // rows past the end: the last one again, not counted and not stored
+        const int64_t at = min(row + r * stride, a.rows - 1);
         g[r] = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.dy) + at * a.ld_dy + col);
         if (ACT != RFM_ACT_NONE) {
           p[r] = *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(a.saved) + at * a.n + col);
@@ -690,18 +703,22 @@ __global__ void __launch_bounds__(32 * kPreWarps) grad_pre_kernel(const GradPreA
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
         const int64_t at = row + r * stride;
-        if (at >= a.rows) continue;
-        float v[VEC];
+        const bool valid = at < a.rows;
+        Pack<T, VEC> o;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          v[j] = to_float(g[r].v[j]);
-          if (ACT != RFM_ACT_NONE) v[j] *= activate_grad(to_float(p[r].v[j]), ACT);
-          sum[j] += v[j];
+        for (int j = 0; j < kPairs; ++j) {
+          Pair v;
+          if constexpr (VEC == 1) {
+            v = times_activate_grad(both(to_float(g[r].v[0])), both(ACT != RFM_ACT_NONE ? to_float(p[r].v[0]) : 0.f), ACT);
+            o.v[0] = from_float<T>(split(v).x);
+          } else {
+            v = load_pair(g[r], j);
+            if (ACT != RFM_ACT_NONE) v = times_activate_grad(v, load_pair(p[r], j), ACT);
+            store_pair(o, j, v);
+          }
+          if (valid) sum[j] = sum[j] + v;
         }
-        if (a.dp != nullptr) {
-          Pack<T, VEC> o;
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) o.v[j] = from_float<T>(v[j]);
+        if (valid && a.dp != nullptr) {
           *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.dp) + at * a.ld_dp + col) = o;
         }
       }
@@ -710,7 +727,7 @@ __global__ void __launch_bounds__(32 * kPreWarps) grad_pre_kernel(const GradPreA
   if (a.partial == nullptr) return;
   __shared__ float sums[kPreWarps][32 * VEC];
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) sums[warp][j * 32 + lane] = sum[j];
+  for (int j = 0; j < VEC; ++j) sums[warp][j * 32 + lane] = j % 2 == 0 ? split(sum[j / 2]).x : split(sum[j / 2]).y;
   __syncthreads();
   if (warp == 0 && in) {
 #pragma unroll

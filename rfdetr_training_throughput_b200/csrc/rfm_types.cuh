@@ -70,6 +70,8 @@ __device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
   return r;
 }
 
+__device__ __forceinline__ Pair both(float x) { return pair(x, x); }
+
 // Elements 2 i and 2 i + 1 of a pack.
 template <typename T, int VEC>
 __device__ __forceinline__ Pair load_pair(const Pack<T, VEC>& p, int i) {
