@@ -241,6 +241,7 @@ __global__ void __launch_bounds__(Shape<BN, CG>::kThreads, 1)
   // of a pair, CTA 0 issues the products and counts both CTAs' loads
   const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
 
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) {
     *dead = 0;
     if ((base & 1023u) != 0) {  // the swizzles count on it; never expected
@@ -268,6 +269,7 @@ __global__ void __launch_bounds__(Shape<BN, CG>::kThreads, 1)
     __syncthreads();
   }
   tc_fence_after();
+  grid_dependency_wait();  // the set-up above touches nothing that the kernel before writes
   const uint32_t tmem = *reinterpret_cast<const volatile uint32_t*>(smem + S::kFlags + 4);
   const uint32_t items = static_cast<uint32_t>(a.tiles_m) * a.tiles_n * a.splits;  // below 2^31
   const uint32_t first = blockIdx.x / CG, stride = gridDim.x / CG;
@@ -624,6 +626,7 @@ struct FinishArgs {
 
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) finish_kernel(const FinishArgs a) {
+  chain_start();
   const int64_t per_row = a.n / VEC;
   const int64_t total = a.m * per_row;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
@@ -678,6 +681,7 @@ constexpr int kPreWarps = 8;
 // warp); the sums of its warps are added in their order at the end.
 template <typename T, int VEC, int ACT>
 __global__ void __launch_bounds__(32 * kPreWarps, 3) grad_pre_kernel(const GradPreArgs a) {
+  chain_start();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = (static_cast<int>(blockIdx.x) * 32 + lane) * VEC;
   const bool in = col < a.n;
@@ -743,6 +747,7 @@ __global__ void __launch_bounds__(32 * kPreWarps, 3) grad_pre_kernel(const GradP
 // The slabs' sums per column, in a fixed order: 32 columns per CTA, each of 32
 // warps every 32nd slab, then the 32 sums.
 __global__ void __launch_bounds__(1024) bias_sum_kernel(const float* partial, int slabs, int n, void* out, int dtype) {
+  chain_start();
   __shared__ float sums[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = static_cast<int>(blockIdx.x) * 32 + lane;
@@ -763,14 +768,10 @@ __global__ void __launch_bounds__(1024) bias_sum_kernel(const float* partial, in
 
 template <typename T, int VEC>
 int launch_grad_pre(const GradPreArgs& a, int activation, const dim3& grid, cudaStream_t s) {
-  if (activation == RFM_ACT_RELU) {
-    grad_pre_kernel<T, VEC, RFM_ACT_RELU><<<grid, 32 * kPreWarps, 0, s>>>(a);
-  } else if (activation == RFM_ACT_GELU) {
-    grad_pre_kernel<T, VEC, RFM_ACT_GELU><<<grid, 32 * kPreWarps, 0, s>>>(a);
-  } else {
-    grad_pre_kernel<T, VEC, RFM_ACT_NONE><<<grid, 32 * kPreWarps, 0, s>>>(a);
-  }
-  return launch_status();
+  const auto kernel = activation == RFM_ACT_RELU   ? grad_pre_kernel<T, VEC, RFM_ACT_RELU>
+                      : activation == RFM_ACT_GELU ? grad_pre_kernel<T, VEC, RFM_ACT_GELU>
+                                                   : grad_pre_kernel<T, VEC, RFM_ACT_NONE>;
+  return launch_chained(true, kernel, grid, 32 * kPreWarps, 0, 1, s, a);
 }
 
 // ---- a few rows: the weight is read once and nothing is tiled
@@ -965,6 +966,7 @@ struct Product {
   int n;
   int64_t k;
   int dtype;
+  bool first;     // of the call's kernels
   GemmArgs args;  // epilogue fields filled in by the caller
 };
 
@@ -1009,22 +1011,8 @@ int launch_gemm(const Product& p, GemmArgs& g, float* partial, cudaStream_t stre
   if (items >= (int64_t(1) << 31) - (1 << 16)) return RFM_ERR_UNSUPPORTED;
   const int sms = device_sm_count();
   const int64_t workers = sms / CG;
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>((items < workers ? items : workers) * CG));
-  config.blockDim = dim3(S::kThreads);
-  config.dynamicSmemBytes = S::kBytes;
-  config.stream = stream;
-  cudaLaunchAttribute cluster{};
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = CG;
-  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-  config.attrs = &cluster;
-  config.numAttrs = CG == 2 ? 1 : 0;
-  if (cudaLaunchKernelEx(&config, kernel, maps, g) != cudaSuccess) {
-    cudaGetLastError();
-    return RFM_ERR_LAUNCH;
-  }
-  return launch_status();
+  const unsigned grid = static_cast<unsigned>((items < workers ? items : workers) * CG);
+  return launch_chained(p.first, kernel, dim3(grid), S::kThreads, S::kBytes, CG, stream, maps, g);
 }
 
 template <typename T, int BN, int CG, bool A_MN, bool B_MN>
@@ -1067,11 +1055,9 @@ int run_product(const Product& p, void* workspace, cudaStream_t stream) {
   const int64_t ctas = (cells + 255) / 256;
   const unsigned grid = static_cast<unsigned>(ctas < most ? ctas : most);
   if (quads) {
-    finish_kernel<T, 4><<<grid, 256, 0, stream>>>(f);
-  } else {
-    finish_kernel<T, 1><<<grid, 256, 0, stream>>>(f);
+    return launch_chained(false, finish_kernel<T, 4>, dim3(grid), 256, 0, 1, stream, f);
   }
-  return launch_status();
+  return launch_chained(false, finish_kernel<T, 1>, dim3(grid), 256, 0, 1, stream, f);
 }
 
 template <bool A_MN, bool B_MN>
@@ -1156,6 +1142,7 @@ extern "C" int rfm_linear_forward(const rfm_linear* p, void* stream) {
   g.n = p->out_features;
   g.k = p->in_features;
   g.dtype = p->dtype;
+  g.first = true;
   g.args.activation = p->activation;
   g.args.bias = p->bias;
   g.args.bias_dtype = p->bias_dtype;
@@ -1241,11 +1228,12 @@ extern "C" int rfm_linear_backward(const rfm_linear_grad* p, void* stream) {
     }
     if (done != RFM_OK) return done;
     if (p->grad_bias != nullptr) {
-      bias_sum_kernel<<<(out + 31) / 32, 1024, 0, s>>>(a.partial, slabs, out, p->grad_bias, p->bias_dtype);
-      done = launch_status();
+      done = launch_chained(false, bias_sum_kernel, dim3((out + 31) / 32), 1024, 0, 1, s, a.partial, slabs, out,
+                            p->grad_bias, p->bias_dtype);
       if (done != RFM_OK) return done;
     }
   }
+  bool first = !own && p->grad_bias == nullptr;  // of the call's kernels: the next product
   const void* dp = own ? p->grad_pre : p->grad_out;
   const int64_t ld_dp = own ? p->ld_grad_pre : p->ld_grad;
   if (p->grad_x != nullptr) {
@@ -1258,9 +1246,11 @@ extern "C" int rfm_linear_backward(const rfm_linear_grad* p, void* stream) {
     g.n = in;
     g.k = out;
     g.dtype = p->dtype;
+    g.first = first;
     g.args.out = p->grad_x;
     const int done = run_typed<false, true>(g, p->workspace, s);
     if (done != RFM_OK) return done;
+    first = false;
   }
   if (p->grad_weight != nullptr) {
     Product g{};
@@ -1272,6 +1262,7 @@ extern "C" int rfm_linear_backward(const rfm_linear_grad* p, void* stream) {
     g.n = in;
     g.k = rows;
     g.dtype = p->dtype;
+    g.first = first;
     g.args.out = p->grad_weight;
     return run_typed<true, true>(g, p->workspace, s);
   }

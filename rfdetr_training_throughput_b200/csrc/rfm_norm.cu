@@ -322,6 +322,7 @@ __global__ void __launch_bounds__(cta_threads(TEAM, CH* VEC)) norm_bwd_kernel(co
   int64_t row = static_cast<int64_t>(blockIdx.x) * kTeams + team;
   int64_t lead = TEAM >= 32 ? row : static_cast<int64_t>(blockIdx.x) * kTeams + (threadIdx.x & ~31u) / TEAM;
 
+  if (PARAMS) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the sums' kernel waits for this one
   Rows xs(a.x, a.ld_x, a.dim, lane, ring);
   Rows dys(a.dy, a.ld_dy, a.dim, lane, ring + Rows::kBytes);
   float mean_ahead[kDepth], rstd_ahead[kDepth];
@@ -520,6 +521,7 @@ __global__ void __launch_bounds__(kThreads) norm_wide_params_kernel(const NormAr
 // of 32 warps every 32nd partial, then the 32 sums.  blockIdx.y picks dw or db.
 __global__ void __launch_bounds__(1024) norm_param_sum_kernel(const float* partial, int parts, int dim,
                                                               void* dweight, void* dbias, int param_dtype) {
+  chain_start();
   __shared__ float sums[32][33];
   void* out = blockIdx.y == 0 ? dweight : dbias;
   if (out == nullptr) return;
@@ -725,7 +727,6 @@ extern "C" int rfm_layer_norm_backward(const void* x, int64_t ld_x, const void* 
   }
   if (!params) return RFM_OK;
   // with no rows the sums are empty: zeros
-  norm_param_sum_kernel<<<dim3((dim + 31) / 32, 2), 1024, 0, as_stream(stream)>>>(
-      a.partial, ctas, dim, grad_weight, grad_bias, param_dtype);
-  return launch_status();
+  return launch_chained(rows == 0, norm_param_sum_kernel, dim3((dim + 31) / 32, 2), 1024, 0, 1, as_stream(stream),
+                        a.partial, ctas, dim, grad_weight, grad_bias, param_dtype);
 }

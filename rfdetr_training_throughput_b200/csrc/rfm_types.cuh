@@ -9,6 +9,46 @@
 
 namespace rfm {
 
+// The kernels of one call follow each other with programmatic stream
+// serialization: a kernel's CTAs may start while the one before it drains (about
+// 2 us a boundary otherwise), and wait here before they touch what it wrote.
+// The call's first kernel is an ordinary launch.  Every kernel of such a chain
+// calls it, at its start.
+__device__ __forceinline__ void chain_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  grid_dependency_wait();
+}
+
+template <typename... Params, typename... Args>
+int launch_chained(bool first, void (*kernel)(Params...), dim3 grid, int threads, int smem, int cluster,
+                   cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = dim3(static_cast<unsigned>(threads));
+  config.dynamicSmemBytes = static_cast<size_t>(smem);
+  config.stream = stream;
+  cudaLaunchAttribute attrs[2];
+  unsigned n = 0;
+  if (cluster > 1) {
+    attrs[n].id = cudaLaunchAttributeClusterDimension;
+    attrs[n].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attrs[n].val.clusterDim.y = attrs[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (!first) {
+    attrs[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  config.attrs = attrs;
+  config.numAttrs = n;
+  if (cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...) != cudaSuccess) {
+    cudaGetLastError();
+    return RFM_ERR_LAUNCH;
+  }
+  return RFM_OK;
+}
+
 inline int dtype_bytes(int dtype) { return dtype == RFM_DTYPE_F32 ? 4 : 2; }
 inline bool dtype_known(int dtype) {
   return dtype == RFM_DTYPE_F32 || dtype == RFM_DTYPE_BF16 || dtype == RFM_DTYPE_F16;
