@@ -156,21 +156,21 @@ __device__ __forceinline__ float2 team_sum(float2 s, float2* slots, int parity) 
   return s;
 }
 
-// Weight (or bias) of a thread's columns as pairs: in registers up to 16 columns,
-// read from shared memory beyond (where every thread of a warp-team's lane needs
-// the same columns for each of its rows, and registers are short).
-template <int VEC, int TEAM, int CH>
+// Weight (or bias) of a thread's columns as pairs: in registers, or (SHARE, beyond
+// 16 columns) in shared memory.  The forward has the registers: reading them from
+// shared memory for every row took its bandwidth (65536 x 1024 fp16: 57 us, 50
+// with registers).  The backward needs its registers for the sums.
+template <int VEC, int TEAM, int CH, bool SHARE>
 struct Params {
   static constexpr int kCols = CH * VEC, kStep = TEAM * VEC;
-  static constexpr bool kShared = kCols > 16;
-  static constexpr int kFloats = kShared ? TEAM * kCols : 0;
+  static constexpr bool kShared = SHARE && kCols > 16;
   Pair reg[kShared ? 1 : kCols / 2];
   const float* smem;
 
   __device__ __forceinline__ void load(const void* p, int dtype, int dim, float missing, int lane, float* shared) {
     smem = shared;
     if constexpr (kShared) {
-      for (int i = threadIdx.x; i < kFloats; i += blockDim.x)
+      for (int i = threadIdx.x; i < kStep * CH; i += blockDim.x)
         shared[i] = i < dim && p != nullptr ? load_param(p, dtype, i) : missing;
     } else {
 #pragma unroll
@@ -212,10 +212,9 @@ __device__ __forceinline__ Pair element_pair(const Pack<T, VEC> (&r)[CH], int i)
 template <typename T, int VEC, int TEAM, int CH>
 __global__ void __launch_bounds__(cta_threads(TEAM, CH* VEC)) norm_fwd_kernel(const NormArgs a) {
   using Rows = Ahead<T, VEC, TEAM, CH>;
-  using P = Params<VEC, TEAM, CH>;
+  using P = Params<VEC, TEAM, CH, false>;
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ float2 slots[2 * Rows::kThreadsCta / 32];
-  __shared__ __align__(16) float params[P::kShared ? 2 * P::kFloats : 1];
   constexpr int kTeams = Rows::kThreadsCta / TEAM;
   constexpr int kStep = TEAM * VEC;
   constexpr int kPairs = CH * VEC / 2;
@@ -235,9 +234,8 @@ __global__ void __launch_bounds__(cta_threads(TEAM, CH* VEC)) norm_fwd_kernel(co
     ring_commit<Rows::kDepth>();
   }
   P w, b;
-  w.load(a.weight, a.param_dtype, a.dim, 1.f, lane, params);
-  b.load(a.bias, a.param_dtype, a.dim, 0.f, lane, params + P::kFloats);
-  if (P::kShared) __syncthreads();
+  w.load(a.weight, a.param_dtype, a.dim, 1.f, lane, nullptr);
+  b.load(a.bias, a.param_dtype, a.dim, 0.f, lane, nullptr);
 
   int slot = 0;
   for (; lead < a.rows; row += stride, lead += stride) {
@@ -307,12 +305,12 @@ __global__ void __launch_bounds__(cta_threads(TEAM, CH* VEC)) norm_fwd_kernel(co
 template <typename T, int VEC, int TEAM, int CH, bool PARAMS>
 __global__ void __launch_bounds__(cta_threads(TEAM, CH* VEC)) norm_bwd_kernel(const NormArgs a) {
   using Rows = Ahead<T, VEC, TEAM, CH>;
-  using P = Params<VEC, TEAM, CH>;
+  using P = Params<VEC, TEAM, CH, true>;
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ float2 slots[2 * Rows::kThreadsCta / 32];
-  __shared__ __align__(16) float params[P::kShared ? P::kFloats : 1];
-  constexpr int kTeams = Rows::kThreadsCta / TEAM;
   constexpr int kStep = TEAM * VEC;
+  __shared__ __align__(16) float params[P::kShared ? kStep * CH : 1];
+  constexpr int kTeams = Rows::kThreadsCta / TEAM;
   constexpr int kPairs = CH * VEC / 2;
   constexpr int kDepth = Rows::kDepth > 0 ? Rows::kDepth : 1;
   const int lane = static_cast<int>(threadIdx.x) % TEAM;
@@ -618,10 +616,10 @@ int dispatch_norm(const NormArgs& a, bool vectors, bool backward, int* ctas, cud
     }
     return launch_status();
   }
-  // a warp a row up to 1024 columns (32 a lane): a team of several warps pays its
-  // shuffles in each of them and a barrier twice a row (16384 x 1024 and longer:
-  // four warps a row 67 and 98 us at 65536 rows of fp16, forward and backward,
-  // see the table beside launch_norm's callers for one warp)
+  // A warp a row up to 1024 columns (32 a lane): a team of several warps pays its
+  // shuffles in each of them and a barrier twice a row (65536 x 1024 fp16, four
+  // warps a row: 67 and 98 us, forward and backward; one warp: 50 and 80 us, 5.4
+  // and 5.0 TB/s).
   if (vectors) {
     if (d <= 8 * V) return launch_norm<T, V, 8, 1>(a, backward, ctas, s);
     if (d <= 32 * V) return launch_norm<T, V, 32, 1>(a, backward, ctas, s);
