@@ -944,6 +944,7 @@ Cut choose_cut(int64_t m, int n, int k_blocks) {
     const int64_t rows = c.pair ? 2 * kBM : kBM;
     const int64_t tiles = ((m + rows - 1) / rows) * ((n + c.bn - 1) / c.bn);
     const int64_t workers = c.pair ? sms / 2 : sms;
+    if (workers == 0) continue;  // no device: sizes are still asked for
     for (int splits = 1; splits <= kMaxSplits; ++splits) {
       if (splits > 1 && (k_blocks / splits < kLeastSlices || tiles * (splits - 1) >= 4 * workers)) break;
       const double waves = static_cast<double>((tiles * splits + workers - 1) / workers);

@@ -35,6 +35,16 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     return host().linear(x, weight, bias, code, residual)
 
 
+def project(layer: torch.nn.Linear, x: torch.Tensor) -> torch.Tensor:
+    """``layer(x)`` through ``linear`` where the product runs in 16 bits (under a 16-bit autocast, or on
+    16-bit tensors); a float32 or host product stays with the layer."""
+    autocast = x.is_cuda and torch.is_autocast_enabled("cuda")
+    dtype = torch.get_autocast_dtype("cuda") if autocast else x.dtype
+    if x.is_cuda and dtype in (torch.bfloat16, torch.float16):
+        return linear(x, layer.weight, layer.bias)
+    return layer(x)
+
+
 def check_faults(device: torch.device | int | None = None) -> None:
     """Raise if a product on ``device`` (the current one) ever gave up a bounded wait, which leaves its
     output incomplete.  Never expected; synchronises the device."""

@@ -10,7 +10,8 @@ three entry points, on this library's sm_100a kernel:
 ``deformable_attention``  rf-detr's core contract, value ``[B, M, D, S]`` (``value_by_head``); one
                           layout copy, as the ``fused_msda`` patch makes
 ``module_forward``        ``MSDeformAttn.forward``'s eager branch with value kept in the native
-                          layout (no copy), as the ``fused_msda_native`` patch does
+                          layout (no copy), as the ``fused_msda_native`` patch does; its projections
+                          may run on this library's ``linear`` (patch ``fused_msda_linear``)
 
 Everything runs in fp32, the precision the replaced ``grid_sample`` path runs at under autocast.
 """
@@ -18,7 +19,7 @@ Everything runs in fp32, the precision the replaced ``grid_sample`` path runs at
 from __future__ import annotations
 
 import ctypes
-from typing import Any
+from typing import Any, Callable
 
 import torch
 import torch.nn.functional as F
@@ -103,19 +104,25 @@ def deformable_attention(value_by_head: torch.Tensor, spatial_shapes: torch.Tens
 
 def module_forward(module: Any, query: torch.Tensor, reference_points: torch.Tensor, input_flatten: torch.Tensor,
                    input_spatial_shapes: torch.Tensor, input_level_start_index: torch.Tensor,
-                   input_padding_mask: torch.Tensor | None = None, input_spatial_shapes_hw: Any = None) -> torch.Tensor:
+                   input_padding_mask: torch.Tensor | None = None, input_spatial_shapes_hw: Any = None, *,
+                   project: Callable[[Any, torch.Tensor], torch.Tensor] | None = None) -> torch.Tensor:
     """``MSDeformAttn.forward`` (Deformable DETR's module: value/offset/weight projections, softmax over
     levels x points, sampling locations from 2-d or 4-d reference points, output projection) with the
-    value kept in the kernel's ``[B, S, M, D]`` layout, a free view of ``value_proj``'s output."""
+    value kept in the kernel's ``[B, S, M, D]`` layout, a free view of ``value_proj``'s output.
+    ``project(layer, x)`` computes the four projections (``linear.project`` on the tensor cores under a
+    16-bit autocast); by default the layers themselves do."""
+    if project is None:
+        def project(layer, x):
+            return layer(x)
     batch, len_q, _ = query.shape
     _, len_in, _ = input_flatten.shape
     heads, levels, points = module.n_heads, module.n_levels, module.n_points
-    value = module.value_proj(input_flatten)
+    value = project(module.value_proj, input_flatten)
     if input_padding_mask is not None:
         value = value.masked_fill(input_padding_mask[..., None], 0.0)
     value = value.view(batch, len_in, heads, module.d_model // heads)
-    offsets = module.sampling_offsets(query).view(batch, len_q, heads, levels, points, 2)
-    weights = module.attention_weights(query).view(batch, len_q, heads, levels * points)
+    offsets = project(module.sampling_offsets, query).view(batch, len_q, heads, levels, points, 2)
+    weights = project(module.attention_weights, query).view(batch, len_q, heads, levels * points)
     weights = F.softmax(weights, -1)
     if reference_points.shape[-1] == 2:
         normalizer = torch.stack([input_spatial_shapes[..., 1], input_spatial_shapes[..., 0]], -1)
@@ -126,4 +133,4 @@ def module_forward(module: Any, query: torch.Tensor, reference_points: torch.Ten
     else:
         raise ValueError(f"last dim of reference_points must be 2 or 4, got {reference_points.shape[-1]}")
     out = ms_deform_attn(value, input_spatial_shapes, input_level_start_index, locations, weights)
-    return module.output_proj(out.to(query.dtype))
+    return project(module.output_proj, out.to(query.dtype))

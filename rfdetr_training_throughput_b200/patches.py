@@ -28,6 +28,13 @@ which applies them in order, returns one description per patch and raises
                     BCE when the criterion has ``ia_bce_loss`` set, else the sigmoid focal
                     loss; the varifocal and position-supervised variants raise)
 
+``fused_msda_linear`` ``MSDeformAttn.forward`` as ``fused_msda_native``, and its four projections on
+                    ``rfm_linear_*`` where they run in 16 bits (new)
+``fused_layer_norm`` ``torch.nn.LayerNorm.forward`` for CUDA inputs normalised over their last
+                    dimension -> ``rfm_layer_norm_*`` (new); other calls keep torch's
+``fused_adamw``     ``torch.optim.AdamW`` -> ``optim.AdamW``, one ``rfm_adamw`` launch per parameter
+                    group (new)
+
 Unlike the reference there is no fallback to the original implementation for
 CPU tensors or out-of-envelope inputs: the patched functions raise instead.
 """
@@ -151,6 +158,58 @@ def _apply_fused_msda_native() -> str:
     return "fused_msda_native: MSDeformAttn.forward reaches the rfm_msda kernels without a layout copy"
 
 
+def _apply_fused_msda_linear() -> str:
+    cls = _module("rfdetr.models.ops.modules.ms_deform_attn").MSDeformAttn
+    from .linear import project
+    from .msda import module_forward
+
+    original = cls.forward
+
+    def forward(self, *args, **kwargs):
+        if getattr(self, "_export", False):
+            return original(self, *args, **kwargs)
+        return module_forward(self, *args, project=project, **kwargs)
+
+    cls.forward = forward
+    return "fused_msda_linear: MSDeformAttn.forward on the rfm_msda kernels, its 16-bit projections on rfm_linear"
+
+
+def _apply_fused_layer_norm() -> str:
+    import torch
+
+    from .norm import layer_norm
+
+    cls = torch.nn.LayerNorm
+    original = cls.forward
+    types = (torch.float32, torch.bfloat16, torch.float16)
+
+    def forward(self, x):
+        if not x.is_cuda or len(self.normalized_shape) != 1 or x.dtype not in types:
+            return original(self, x)
+        weight, bias = self.weight, self.bias
+        if torch.is_autocast_enabled("cuda"):  # torch's autocast runs layer norms in float32
+            x = x.float()
+            weight = weight if weight is None else weight.float()
+            bias = bias if bias is None else bias.float()
+        elif weight is not None and weight.dtype not in (x.dtype, torch.float32):
+            return original(self, x)
+        if x.shape[-1:] != tuple(self.normalized_shape):
+            return original(self, x)  # torch's own error
+        return layer_norm(x, weight, bias, self.eps)
+
+    cls.forward = forward
+    return "fused_layer_norm: torch.nn.LayerNorm on the sm_100a layer norm kernels"
+
+
+def _apply_fused_adamw() -> str:
+    import torch
+
+    from .optim import AdamW
+
+    torch.optim.AdamW = AdamW
+    return "fused_adamw: torch.optim.AdamW steps in one sm_100a launch per parameter group"
+
+
 PATCHES: dict[str, Callable[[], str]] = {
     "triton_matcher": _apply_triton_matcher,
     "cuda_lap": _apply_cuda_lap,
@@ -161,6 +220,9 @@ PATCHES: dict[str, Callable[[], str]] = {
     "label_loss": _apply_label_loss,
     "fused_msda": _apply_fused_msda,
     "fused_msda_native": _apply_fused_msda_native,
+    "fused_msda_linear": _apply_fused_msda_linear,
+    "fused_layer_norm": _apply_fused_layer_norm,
+    "fused_adamw": _apply_fused_adamw,
 }
 
 

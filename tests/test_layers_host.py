@@ -10,6 +10,7 @@ import pytest
 import torch
 
 from rfdetr_training_throughput_b200 import _lib
+from rfdetr_training_throughput_b200.linear import linear
 from rfdetr_training_throughput_b200.norm import layer_norm
 from rfdetr_training_throughput_b200.optim import AdamW, adamw_step, dequantize_moments, quantize_moments
 
@@ -21,6 +22,10 @@ def test_host_tensors_are_refused():
     x = torch.zeros(3, 8)
     with pytest.raises(ValueError, match="CUDA"):
         layer_norm(x)
+    with pytest.raises(ValueError, match="CUDA"):
+        linear(x, x)
+    with pytest.raises(ValueError, match="activation"):
+        linear(x, x, activation="tanh")
     with pytest.raises(ValueError, match="CUDA"):
         adamw_step([x], [x], [x], [x], 1)
     with pytest.raises(ValueError, match="CUDA"):
@@ -119,3 +124,62 @@ def test_adamw_abi_refusals():
 
     assert moments(n=-1) == 1 and moments(a=None) == 1 and moments(n=0) == 0 and moments(n=1 << 42) == 2
     assert ctypes.sizeof(ctypes.c_int64) * _lib.ADAMW_TENSOR_WORDS == 64
+
+
+def test_linear_structs_match_header(tmp_path):
+    """ctypes mirrors of rfm_linear / rfm_linear_grad against the header, compiled with gcc."""
+    import shutil
+    import subprocess
+
+    if shutil.which("gcc") is None:
+        pytest.skip("no gcc")
+    names = [("rfm_linear", _lib.Linear, "ld_residual"), ("rfm_linear", _lib.Linear, "reserved"),
+             ("rfm_linear_grad", _lib.LinearGrad, "ld_grad_pre"), ("rfm_linear_grad", _lib.LinearGrad, "reserved")]
+    src = tmp_path / "sz.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "rfm.h"\nint main(void) {\n'
+                   + "".join(f'  printf("%zu %zu ", sizeof({s}), offsetof({s}, {f}));\n' for s, _, f in names)
+                   + "  return 0;\n}\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe = tmp_path / "sz"
+    subprocess.run(["gcc", "-I", os.path.join(root, "include"), str(src), "-o", str(exe)], check=True)
+    got = [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    assert got == [v for _, c, f in names for v in (ctypes.sizeof(c), getattr(c, f).offset)]
+    for name, value in _lib.ACTIVATIONS.items():
+        assert f"#define RFM_ACT_{name.upper()} {value}\n" in HEADER
+
+
+def test_linear_abi_refusals():
+    lib = _lib.load()
+
+    def forward(**bad):
+        args = dict(x=FAKE, weight=FAKE, out=FAKE, rows=3, ld_x=16, ld_weight=16, in_features=16, out_features=8,
+                    dtype=_lib.DTYPE_BF16, bias_dtype=_lib.DTYPE_BF16)
+        return lib.rfm_linear_forward(ctypes.byref(_lib.Linear(**{**args, **bad})), None)
+
+    for bad in (dict(x=None), dict(weight=None), dict(out=None), dict(rows=-1), dict(in_features=0),
+                dict(out_features=0), dict(dtype=_lib.DTYPE_F32), dict(x=FAKE + 2), dict(weight=FAKE + 8),
+                dict(ld_x=12), dict(ld_x=8), dict(ld_weight=20), dict(ld_weight=0), dict(activation=3),
+                dict(activation=-1), dict(reserved=1), dict(bias=FAKE, bias_dtype=_lib.DTYPE_F16),
+                dict(residual=FAKE, ld_residual=7)):
+        assert forward(**bad) == 1, bad
+    assert forward(rows=1 << 31) == 2 and forward(in_features=(1 << 30) + 1) == 2
+    assert forward(rows=0, x=None, weight=None, out=None) == 0
+    assert lib.rfm_linear_forward(None, None) == 1
+
+    def backward(**bad):
+        args = dict(x=FAKE, weight=FAKE, grad_out=FAKE, grad_x=FAKE, grad_weight=FAKE, grad_bias=FAKE, rows=3, ld_x=16,
+                    ld_weight=16, ld_grad=8, in_features=16, out_features=8, dtype=_lib.DTYPE_BF16,
+                    bias_dtype=_lib.DTYPE_BF16, workspace=FAKE, workspace_bytes=1 << 30)
+        return lib.rfm_linear_backward(ctypes.byref(_lib.LinearGrad(**{**args, **bad})), None)
+
+    for bad in (dict(x=None), dict(weight=None), dict(grad_out=None), dict(rows=-1), dict(ld_grad=7), dict(ld_x=8),
+                dict(workspace=None), dict(workspace=FAKE + 4), dict(workspace_bytes=4), dict(reserved=2),
+                dict(activation=1), dict(activation=1, saved=FAKE), dict(bias_dtype=_lib.DTYPE_F16),
+                dict(activation=1, saved=FAKE, grad_pre=FAKE, ld_grad_pre=4),
+                dict(grad_out=FAKE + 2)):  # dP needs a place of its own
+        assert backward(**bad) == 1, bad
+    assert backward(grad_x=None, grad_weight=None, grad_bias=None) == 0
+    assert lib.rfm_linear_backward(None, None) == 1
+    assert lib.rfm_linear_forward_workspace_bytes(-1, 8, 8) < 0 and lib.rfm_linear_forward_workspace_bytes(1, 8, 8) == 0
+    assert lib.rfm_linear_backward_workspace_bytes(4, 0, 8) < 0
+    assert lib.rfm_linear_faults(None) == 1
