@@ -83,6 +83,15 @@ void adamw_step(const TensorList& params, const TensorList& grads, const TensorL
     RFM_REQUIRE(written[i].first >= written[i - 1].second,
                 "a tensor is given twice: params, moments and scales must not share memory");
   }
+  for (size_t i = 0; i < count; ++i) {
+    const uintptr_t from = reinterpret_cast<uintptr_t>(table[i].grad);
+    const uintptr_t past = from + static_cast<uintptr_t>(table[i].numel * grads[i].element_size());
+    // the first written piece that ends behind the gradient's start
+    const auto it = std::upper_bound(written.begin(), written.end(), from,
+                                     [](uintptr_t at, const std::pair<uintptr_t, uintptr_t>& w) { return at < w.second; });
+    RFM_REQUIRE(from == past || it == written.end() || it->first >= past,
+                "gradients must not share memory with params, moments or scales");
+  }
   void* at_step = device_step ? scalar_pointer("step", *device_step, at::kLong, device) : nullptr;
   void* at_lr = device_lr ? scalar_pointer("lr", *device_lr, at::kFloat, device) : nullptr;
   void* at_scale = grad_scale ? scalar_pointer("grad_scale", *grad_scale, at::kFloat, device) : nullptr;

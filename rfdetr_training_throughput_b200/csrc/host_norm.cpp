@@ -88,7 +88,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 Tensor layer_norm(const Tensor& x, const MaybeTensor& maybe_weight, const MaybeTensor& maybe_bias, double eps) {
   RFM_REQUIRE(x.is_cuda(), "x must be a CUDA tensor (layer_norm has no CPU path)");
   RFM_REQUIRE(dtype_code(x.scalar_type()) >= 0, "x must be float32, bfloat16 or float16, got ", x.scalar_type());
-  RFM_REQUIRE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 0x7fffffff,
+  RFM_REQUIRE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= (1 << 30),
               "x needs a last dimension of at least one element");
   RFM_REQUIRE(eps >= 0.0, "eps must not be negative, got ", eps);
   Tensor weight = or_undefined(maybe_weight), bias = or_undefined(maybe_bias);

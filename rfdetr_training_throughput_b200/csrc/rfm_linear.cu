@@ -40,7 +40,8 @@ namespace {
 constexpr int kBM = 128;
 constexpr int kBK = 64;  // one 128-byte row of 16-bit elements
 constexpr int kMaxSplits = 32;
-constexpr uint32_t kWaitTries = 1u << 22;
+constexpr uint32_t kWaitTries = 1u << 22;       // of a wait for what is in flight after a failure
+constexpr long long kWaitCycles = 1ll << 35;    // of any other wait: some 18 s, the deepest product takes less than 10
 
 __device__ int g_linear_faults = 0;
 
@@ -152,6 +153,15 @@ __device__ __forceinline__ Pair times_activate_grad(Pair dy, Pair v, int act) {
   return dy;
 }
 
+// `pre` is kept finite where it is: a value beyond the type's range would come back
+// as an infinity, whose gelu gradient is NaN, where the value's is 0 or 1.  An
+// infinity stays one.
+template <typename T>
+__device__ __forceinline__ float keep_finite(float v) {
+  const float most = std::is_same<T, __half>::value ? 65504.f : 3.3895313892515355e38f;
+  return fabsf(v) > most && !isinf(v) ? copysignf(most, v) : v;
+}
+
 // Adds two values to two registers that hold floats.
 __device__ __forceinline__ void add2(uint32_t& a, uint32_t& b, float x, float y) {
   const float2 s = split(pair(__uint_as_float(a), __uint_as_float(b)) + pair(x, y));
@@ -182,13 +192,16 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
   return __half22float2(reinterpret_cast<const __half2&>(v));
 }
 
-// A wait that gives up after kWaitTries polls (each of which the hardware
-// suspends for a while), or as soon as another role has given up.
+// A wait that gives up after kWaitCycles, or as soon as another role has given up.
 __device__ __forceinline__ bool bounded_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
-  for (uint32_t i = 0; i < kWaitTries; ++i) {
-    if (mbar_try(bar, parity)) return true;
-    if ((i & 255u) == 255u && *dead) return false;
-  }
+  if (mbar_try(bar, parity)) return true;
+  const long long start = clock64();
+  do {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try(bar, parity)) return true;
+    if (*dead) return false;
+  } while (clock64() - start < kWaitCycles);
   *dead = 1;
   atomicExch(&g_linear_faults, 1);
   return false;
@@ -527,6 +540,8 @@ __global__ void __launch_bounds__(Shape<BN, CG>::kThreads, 1)
           for (int s = 0; s < kTurns; ++s) {
             uint32_t v[32];
             take(v, s);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(keep_finite<T>(__uint_as_float(v[j])));
             if (s == 0) box_free();
             put(v, s);
           }
@@ -649,7 +664,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const FinishArgs a) {
     }
     if (a.pre != nullptr) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) o.v[j] = from_float<T>(v[j]);
+      for (int j = 0; j < VEC; ++j) o.v[j] = from_float<T>(keep_finite<T>(v[j]));
       *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.pre) + row * a.n + col) = o;
     }
 #pragma unroll
@@ -854,7 +869,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_rows_kernel(const FewArgs 
   if (lane >= R * W || row >= a.rows || col >= a.n) return;
   if (a.bias != nullptr) mine += load_param(a.bias, a.bias_dtype, col);
   const int64_t at = static_cast<int64_t>(row) * a.n + col;
-  if (a.pre != nullptr) static_cast<T*>(a.pre)[at] = from_float<T>(mine);
+  if (a.pre != nullptr) static_cast<T*>(a.pre)[at] = from_float<T>(keep_finite<T>(mine));
   mine = activate(mine, a.activation);
   if (a.residual != nullptr) mine += to_float(static_cast<const T*>(a.residual)[row * a.ld_res + col]);
   static_cast<T*>(a.out)[at] = from_float<T>(mine);

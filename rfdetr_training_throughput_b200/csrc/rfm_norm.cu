@@ -654,7 +654,7 @@ int norm_args(NormArgs& a, const void* x, int64_t ld_x, const void* weight, int6
       (ld_x < dim && rows > 1) || ld_x < 0) {
     return RFM_ERR_INVALID_ARGUMENT;
   }
-  if (rows > (int64_t(1) << 40) || ld_x > (int64_t(1) << 40)) return RFM_ERR_UNSUPPORTED;
+  if (rows > (int64_t(1) << 40) || ld_x > (int64_t(1) << 40) || dim > (1 << 30)) return RFM_ERR_UNSUPPORTED;
   if (rows > 0 && x == nullptr) return RFM_ERR_INVALID_ARGUMENT;
   a = NormArgs{};
   a.x = x;

@@ -196,6 +196,66 @@ def test_missing_parts():
     assert out.shape == (0, 40) and gx.shape == (0, 48) and not gw.any() and not gb.any()
 
 
+def test_a_vector_and_one_tensor_twice():
+    d = make(1, 72, 40, torch.bfloat16, residual=False, seed=21)
+    out = linear(d["x"][0], d["weight"], d["bias"], activation="gelu")
+    assert out.shape == (40,)
+    close("out", out[None], reference(d, "gelu", torch.bfloat16)["out"])
+    w = make(48, 48, 48, torch.bfloat16, residual=False, seed=22)
+    both = w["weight"].clone().requires_grad_(True)
+    (g,) = torch.autograd.grad(linear(both, both), [both], w["dy"])
+    ref = reference({**w, "x": w["weight"], "bias": torch.zeros_like(w["bias"])}, "none", torch.bfloat16)
+    want, bound = (a + b for a, b in zip(ref["x"], ref["weight"]))
+    # autograd adds the two gradients in 16 bits
+    close("grad", g, (want, bound + torch.finfo(torch.bfloat16).eps * (want.abs() + bound)))
+
+
+def test_products_beyond_the_type_s_range():
+    """fp16 values beyond 65504 before the activation: the output follows the rounding (infinite, or 0 on
+    gelu's other side), and the gradient is that of a far value, 1 or 0."""
+    x = torch.full((130, 64), 200.0, device=DEV, dtype=torch.float16, requires_grad=True)
+    w = torch.full((64, 64), 20.0, device=DEV, dtype=torch.float16)
+    w[1::2] *= -1
+    for rows in (1, 130):
+        part = x[:rows]
+        out = linear(part, w, activation="gelu")
+        assert bool((out[:, ::2] == float("inf")).all()) and not out[:, 1::2].any()
+        (g,) = torch.autograd.grad(out, x, torch.full_like(out, 1 / 64))
+        # dP = dy on the even columns: 32 of them times 20 / 64
+        assert torch.equal(g[:rows], torch.full_like(g[:rows], 10.0))
+
+
+def test_offsets_beyond_32_bits():
+    """An output of 2.2e9 elements: the last rows and the first, forward and backward."""
+    rows, inner, outer = 1_073_000, 16, 2056
+    g = torch.Generator(device="cuda").manual_seed(23)
+    x = torch.randn(rows, inner, device=DEV, generator=g).to(torch.bfloat16).requires_grad_(True)
+    w = torch.randn(outer, inner, device=DEV, generator=g).to(torch.bfloat16)
+    b = torch.randn(outer, device=DEV, generator=g).to(torch.bfloat16)
+    out = linear(x, w, b, activation="relu")
+    assert out.numel() > 2 ** 31
+    dy = torch.zeros_like(out)
+    ends = torch.cat([torch.arange(300), torch.arange(rows - 300, rows)]).to(DEV)
+    d = dict(x=x.detach()[ends], weight=w, bias=b, residual=None,
+             dy=torch.randn(600, outer, device=DEV, generator=g).to(torch.bfloat16))
+    dy[ends] = d["dy"]
+    gx, = torch.autograd.grad(out, [x], dy)
+    ref = reference(d, "relu", torch.bfloat16)
+    close("out", out.detach()[ends], ref["out"])
+    close("grad x", gx[ends], ref["x"])
+    assert not gx[300:-300].any()
+    check_faults()
+
+
+def test_a_changed_output_is_noticed():
+    d = make(8, 16, 16, torch.bfloat16, residual=False, seed=24)
+    x = d["x"].clone().requires_grad_(True)
+    out = linear(x, d["weight"], activation="relu")
+    out.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        out.sum().backward()
+
+
 def test_special_values_stay_in_their_rows():
     d = make(200, 72, 136, torch.bfloat16, residual=False, seed=4)
     clean = linear(d["x"], d["weight"], d["bias"], activation="relu")

@@ -158,6 +158,25 @@ def test_layouts_and_missing_parameters():
     close(bias.grad, ref["db"], ref["db_size"], 24 + 64, torch.float32)
 
 
+@pytest.mark.parametrize("rows,dim", [(2_100_000, 1032), (262_200, 8200)])
+def test_offsets_beyond_32_bits(rows, dim):
+    """2.2e9 elements, rows in registers and re-read: the last rows, forward and backward."""
+    x = torch.zeros(rows, dim, device=DEV, dtype=torch.bfloat16)
+    tail, w, b, dy_tail = make(40, dim, torch.bfloat16, seed=31)
+    assert x.numel() > 2 ** 31
+    x[-40:] = tail
+    x.requires_grad_(True)
+    out = layer_norm(x, w, b)
+    dy = torch.zeros_like(out)
+    dy[-40:] = dy_tail
+    (g,) = torch.autograd.grad(out, [x], dy)
+    ref = reference(tail, w, b, dy_tail, 1e-5)
+    k = 4 * (40 + dim / 256)
+    close(out[-40:].detach(), ref["out"], ref["out_size"], k, torch.bfloat16)
+    close(g[-40:], ref["dx"], ref["dx_size"], 3 * k, torch.bfloat16)
+    assert not g[:-40].any()
+
+
 def test_empty_rows_and_special_values():
     w = torch.ones(16, device=DEV, requires_grad=True)
     x = torch.zeros((0, 16), device=DEV, requires_grad=True)

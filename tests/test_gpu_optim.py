@@ -330,6 +330,10 @@ def test_gpu_refusals():
     p, g, m, v = (values([64, 32], torch.float32, k, 0.1) for k in range(4))
     with pytest.raises(ValueError, match="twice"):
         adamw_step([p[0], p[0]], [g[0], g[0]], [m[0], m[0]], [v[0], v[0]], 1)
+    with pytest.raises(ValueError, match="share memory"):
+        adamw_step([p[0]], [g[0]], [p[0]], [v[0]], 1)
+    with pytest.raises(ValueError, match="gradients"):
+        adamw_step([p[0][:32]], [p[0][16:48]], [m[1]], [v[1]], 1)
     with pytest.raises(ValueError, match="grads"):
         adamw_step(p, [g[0], g[1].half()], m, v, 1)
     with pytest.raises(ValueError, match="exp_avg"):
