@@ -8,11 +8,12 @@
 
 namespace rfm_host {
 
-using TensorList = std::vector<Tensor>;
+// Tensors that somebody else holds.
+using TensorRefs = std::vector<const Tensor*>;
 
-void adamw_step(const TensorList& params, const TensorList& grads, const TensorList& exp_avg,
-                const TensorList& exp_avg_sq, const std::optional<TensorList>& exp_avg_scale,
-                const std::optional<TensorList>& exp_avg_sq_scale, int64_t step, const MaybeTensor& device_step,
+void adamw_step(const TensorRefs& params, const TensorRefs& grads, const TensorRefs& exp_avg,
+                const TensorRefs& exp_avg_sq, const std::optional<TensorRefs>& exp_avg_scale,
+                const std::optional<TensorRefs>& exp_avg_sq_scale, int64_t step, const MaybeTensor& device_step,
                 double lr, const MaybeTensor& device_lr, double beta1, double beta2, double eps, double weight_decay,
                 const MaybeTensor& grad_scale);
 

@@ -10,12 +10,14 @@ less than half a code a step would stand still.
 
 from __future__ import annotations
 
-from typing import Any, Iterable, Sequence
+from typing import Any, Iterable
 
 import torch
 
 from . import _lib
 from ._native import host
+
+TensorList = list[torch.Tensor] | tuple[torch.Tensor, ...]
 
 #: Elements that share one scale of the 8-bit moments.
 MOMENT_BLOCK = _lib.MOMENT_BLOCK
@@ -26,17 +28,17 @@ def moment_scales(numel: int) -> int:
     return -(-numel // MOMENT_BLOCK)
 
 
-def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avg: Sequence[torch.Tensor],
-               exp_avg_sq: Sequence[torch.Tensor], step: int | torch.Tensor, *,
-               scales: tuple[Sequence[torch.Tensor], Sequence[torch.Tensor]] | None = None,
-               lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
-               weight_decay: float = 1e-2, grad_scale: torch.Tensor | None = None) -> None:
+def adamw_step(params: TensorList, grads: TensorList, exp_avg: TensorList, exp_avg_sq: TensorList,
+               step: int | torch.Tensor, *, scales: tuple[TensorList, TensorList] | None = None, lr: float | torch.Tensor = 1e-3,
+               betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
+               grad_scale: torch.Tensor | None = None) -> None:
     """One AdamW step in place on ``params`` and their moments.
 
-    ``params`` and ``grads`` contiguous CUDA tensors of one type (float32, bfloat16 or float16) on one
-    device, pairwise of one size and all distinct.  Without ``scales``, ``exp_avg`` and ``exp_avg_sq`` are
-    float32 tensors of the params' sizes.  With ``scales`` (two lists of float32 tensors, of
-    ``moment_scales(numel)`` elements each) they hold int8 and uint8 codes (see ``rfm_adamw``).
+    ``params`` and ``grads``: contiguous CUDA tensors of one type (float32, bfloat16 or float16) on one
+    device, pairwise of one size; nothing that is written may share memory with anything else.  Without
+    ``scales``, ``exp_avg`` and ``exp_avg_sq`` are float32 tensors of the params' sizes.  With ``scales``
+    (two lists of float32 tensors, of ``moment_scales(numel)`` elements each) they hold int8 and uint8
+    codes (see ``rfm_adamw``).
 
     ``step`` is the number of this update, from 1; an int64 tensor of one element on the device, and for
     ``lr`` a float32 one, are read by the kernels, so that a captured step follows them.  ``grad_scale``
@@ -165,12 +167,12 @@ class AdamW(torch.optim.Optimizer):
             step.add_(1)
         params, grads, avg, avg_sq = [], [], [], []
         for p, s in zip(members, states):
-            data, g, m, v = p.detach(), p.grad.detach(), s["exp_avg"], s["exp_avg_sq"]
-            if not data.is_contiguous():
-                data, g, m, v = _flat_alike(data, g, m, v)
+            g, m, v = p.grad, s["exp_avg"], s["exp_avg_sq"]
+            if not p.is_contiguous():
+                p, g, m, v = _flat_alike(p, g, m, v)
             elif not g.is_contiguous():
                 g = g.contiguous()
-            params.append(data)
+            params.append(p)
             grads.append(g)
             avg.append(m)
             avg_sq.append(v)
