@@ -330,6 +330,16 @@ __global__ void __launch_bounds__(Shape<BN, CG>::kThreads, 1)
           }
         }
       }
+      // Every arrival on this CTA's `empty` barriers has come before it leaves: of a
+      // pair, CTA 0's products signal CTA 1's too, and nothing else waits for the
+      // last of them there.
+      for (int i = 0; ok && i < S::kStages; ++i) {
+        ok = bounded_wait(empty + 8 * stage, phase ^ 1u, dead);
+        if (ok && ++stage == S::kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
       if (!ok && rank == 0) {
         // the copies in flight (a pair's: of both) land before the shared memory is given up
         for (uint32_t i = 0; i < issued; ++i) {
@@ -1098,6 +1108,14 @@ int bias_slabs(int64_t rows, int n, int vec) {
   return static_cast<int>(slabs < 1 ? 1 : (slabs > 4096 ? 4096 : slabs));
 }
 
+// The sums' bytes whichever way the columns are read: wider strips are fewer, and
+// their rows are cut into more slabs.
+int64_t bias_bytes(int64_t rows, int n) {
+  const int slabs = bias_slabs(rows, n, 8);
+  const int narrow = bias_slabs(rows, n, 1);
+  return (static_cast<int64_t>(slabs > narrow ? slabs : narrow) * n * 4 + 15) & ~int64_t(15);
+}
+
 int check_sizes(int64_t rows, int in_features, int out_features, int dtype) {
   if (rows < 0 || in_features < 1 || out_features < 1 || (dtype != RFM_DTYPE_BF16 && dtype != RFM_DTYPE_F16)) {
     return RFM_ERR_INVALID_ARGUMENT;
@@ -1177,7 +1195,7 @@ extern "C" int64_t rfm_linear_backward_workspace_bytes(int64_t rows, int in_feat
   int64_t most = partial_bytes(rows, in_features, out_features);
   const int64_t dw = rows == 0 ? 0 : partial_bytes(out_features, in_features, rows);
   most = dw > most ? dw : most;
-  const int64_t bias = (static_cast<int64_t>(bias_slabs(rows, out_features, 1)) * out_features * 4 + 15) & ~int64_t(15);
+  const int64_t bias = bias_bytes(rows, out_features);
   return bias > most ? bias : most;
 }
 
