@@ -582,11 +582,12 @@ int launch_bwd(const NormArgs& a, int* ctas, cudaStream_t stream) {
   return launch_status();
 }
 
-template <typename T, int VEC, int TEAM, int CH>
+// The backward may have another team (BTEAM, BCH) than the forward.
+template <typename T, int VEC, int TEAM, int CH, int BTEAM = TEAM, int BCH = CH>
 int launch_norm(const NormArgs& a, bool backward, int* ctas, cudaStream_t stream) {
   if (backward) {
-    return a.partial != nullptr ? launch_bwd<T, VEC, TEAM, CH, true>(a, ctas, stream)
-                                : launch_bwd<T, VEC, TEAM, CH, false>(a, ctas, stream);
+    return a.partial != nullptr ? launch_bwd<T, VEC, BTEAM, BCH, true>(a, ctas, stream)
+                                : launch_bwd<T, VEC, BTEAM, BCH, false>(a, ctas, stream);
   }
   constexpr int threads = cta_threads(TEAM, CH * VEC), bytes = Ahead<T, VEC, TEAM, CH>::kBytes;
   static thread_local unsigned long long ready = 0;
@@ -618,13 +619,14 @@ int dispatch_norm(const NormArgs& a, bool vectors, bool backward, int* ctas, cud
   }
   // A warp a row up to 1024 columns (32 a lane): a team of several warps pays its
   // shuffles in each of them and a barrier twice a row (65536 x 1024 fp16, four
-  // warps a row: 67 and 98 us, forward and backward; one warp: 50 and 80 us, 5.4
-  // and 5.0 TB/s).
+  // warps a row: 67 and 98 us, forward and backward; one warp: 49 and 80 us).  The
+  // backward of 16-bit rows takes two warps, for the registers: 71 us.  That is 5.5
+  // and 5.7 TB/s.
   if (vectors) {
     if (d <= 8 * V) return launch_norm<T, V, 8, 1>(a, backward, ctas, s);
     if (d <= 32 * V) return launch_norm<T, V, 32, 1>(a, backward, ctas, s);
     if (d <= 64 * V) return launch_norm<T, V, 32, 2>(a, backward, ctas, s);
-    if (d <= 128 * V) return launch_norm<T, V, 32, 4>(a, backward, ctas, s);
+    if (d <= 128 * V) return launch_norm<T, V, 32, 4, V == 8 ? 64 : 32, V == 8 ? 2 : 4>(a, backward, ctas, s);
     if constexpr (V == 4) {
       if (d <= 1024) return launch_norm<T, V, 32, 8>(a, backward, ctas, s);
     }
