@@ -510,11 +510,13 @@ __global__ void __launch_bounds__(Shape<BN, CG>::kThreads, 1)
           }
         } else {
           __syncwarp();
-          for (int r = 0; r < 32 && live; ++r) {
-            const int64_t row = row0 + r;
+          const int rows = live ? static_cast<int>(min(a.m - row0, static_cast<int64_t>(32))) : 0;
+          T* dst = static_cast<T*>(to) + row0 * a.n + col0;
+#pragma unroll 8
+          for (int r = 0; r < rows; ++r) {
 #pragma unroll
             for (int c = lane; c < kCols; c += 32)
-              if (row < a.m && col0 + c < a.n) static_cast<T*>(to)[row * a.n + col0 + c] = *cell(r, c);
+              if (col0 + c < a.n) dst[static_cast<int64_t>(r) * a.n + c] = *cell(r, c);
           }
           __syncwarp();
         }
@@ -563,12 +565,12 @@ __global__ void __launch_bounds__(Shape<BN, CG>::kThreads, 1)
         } else if (has_res && !straight) {
           // residual rows that do not start on 16 bytes: element by element, a lane a column
           box_free();
-          const T* res = static_cast<const T*>(a.residual);
+          const T* res = static_cast<const T*>(a.residual) + row0 * a.ld_res + col0;
+#pragma unroll 8
           for (int r = 0; r < 32; ++r) {
-            const int64_t row = row0 + r;
 #pragma unroll
             for (int c = lane; c < kCols; c += 32)
-              *cell(r, c) = row < a.m && col0 + c < a.n ? res[row * a.ld_res + col0 + c] : from_float<T>(0.f);
+              *cell(r, c) = row0 + r < a.m && col0 + c < a.n ? res[r * a.ld_res + c] : from_float<T>(0.f);
           }
           __syncwarp();
         }
