@@ -96,7 +96,7 @@ def parse() -> argparse.Namespace:
     ap.add_argument("--no-configs", action="store_true", help="skip the per-configuration table (N = 1)")
     ap.add_argument("--config-cpu-seconds", type=float, default=2.0,
                     help="CPU time budget of each CPU leg of the per-configuration table")
-    ap.add_argument("--kernel", choices=["cost", "cost_qm", "lsap", "lsap_push", "label", "box", "msda"],
+    ap.add_argument("--kernel", choices=["cost", "cost_qm", "lsap", "lsap_push", "label", "box", "msda", "linear", "norm", "adamw"],
                     default=None,
                     help="profiling mode: run only this kernel's workload a few times (for an ncu capture) and exit")
     return ap.parse_args()
@@ -1128,7 +1128,8 @@ def run_kernel(name: str, workload: str = "sweep", images: int | None = None) ->
     cost / lsap (the workload's step, issued as two calls), cost_qm (the drop-in query-major cost
     matrix, ``compute_compact_detection_cost_matrix``), label / box (the classification or the
     matched-box loss, forward and backward, on the workload's pairs), msda (deformable attention
-    forward and backward, decoder geometry), lsap_push (the sharded step with the pushed exchange on
+    forward and backward, decoder geometry), linear (8192 x 2048 -> 2048 bf16 with gelu), norm (65536 x
+    1024 fp16) and adamw (25 M fp32 parameters, 8-bit moments), forward and backward where there is one, lsap_push (the sharded step with the pushed exchange on
     a one-rank group: the solver with its push epilogue, replayed as a graph)."""
     from rfdetr_training_throughput_b200 import matcher, workloads
 
@@ -1197,6 +1198,30 @@ def run_kernel(name: str, workload: str = "sweep", images: int | None = None) ->
                 loss, _c = matched_label_losses(x, bx, pk, res, mode="ia_bce")
                 loss.sum().backward()
                 flush.zero_()
+    elif name in ("linear", "norm"):
+        from rfdetr_training_throughput_b200.linear import linear
+        from rfdetr_training_throughput_b200.norm import layer_norm
+
+        g = torch.Generator(device="cuda").manual_seed(7)
+        rows, inner, dtype = (8192, 2048, torch.bfloat16) if name == "linear" else (65536, 1024, torch.float16)
+        x = torch.randn((rows, inner), device=dev, generator=g).to(dtype).requires_grad_(True)
+        shape = (2048, inner) if name == "linear" else (inner,)
+        w = (torch.randn(shape, device=dev, generator=g) * inner ** -0.5).to(dtype).requires_grad_(True)
+        b = torch.zeros(shape[0], device=dev, dtype=dtype).requires_grad_(True)
+        for _ in range(3):
+            y = linear(x, w, b, activation="gelu") if name == "linear" else layer_norm(x, w, b)
+            y.backward(y.detach())
+            flush.zero_()
+    elif name == "adamw":
+        from rfdetr_training_throughput_b200.optim import AdamW
+
+        ps = [torch.nn.Parameter(torch.randn(1024, 1024, device=dev)) for _ in range(24)]
+        opt = AdamW(ps, moment_bits=8)
+        for p in ps:
+            p.grad = torch.randn_like(p)
+        for _ in range(4):
+            opt.step()
+            flush.zero_()
     else:
         from rfdetr_training_throughput_b200.msda import ms_deform_attn
 
