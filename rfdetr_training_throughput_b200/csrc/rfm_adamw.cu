@@ -103,6 +103,7 @@ __host__ __device__ inline AdamScalars adam_scalars(double lr, double b1, double
 
 __global__ void adam_scalars_kernel(const float* device_lr, const int64_t* device_step, double lr, double b1,
                                     double b2, double wd, int64_t step, AdamScalars* out) {
+  chain_start();
   *out = adam_scalars(device_lr != nullptr ? static_cast<double>(*device_lr) : lr, b1, b2, wd,
                       device_step != nullptr ? *device_step : step);
 }
@@ -383,6 +384,7 @@ __device__ __forceinline__ void adam_block(const AdamTensor& t, const AdamCommon
 
 template <typename T, bool EIGHT, int N>
 __global__ void __launch_bounds__(kThreads, 9) adamw_kernel(const __grid_constant__ AdamArgs<N> a) {
+  chain_start();
   // the tensor of this CTA: the last whose first chunk is not after it
   int lo = 0, hi = a.c.count - 1;
   const int chunk = static_cast<int>(blockIdx.x);
@@ -427,6 +429,7 @@ __device__ __forceinline__ void decode_block(const uint8_t* m, const uint8_t* v,
 __global__ void __launch_bounds__(kThreads) adam_moments_kernel(const uint8_t* m, const uint8_t* v,
                                                                const float* m_scale, const float* v_scale, int64_t n,
                                                                float* out_m, float* out_v) {
+  chain_start();
   const int64_t block = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
   if (block * kBlock >= n) return;
   const uintptr_t at = reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v);
@@ -459,8 +462,8 @@ int launch_adamw(const AdamCommon& common, const rfm_adamw_tensor* tensors, int 
   }
   if (k == 0) return RFM_OK;
   a.c.count = k;
-  adamw_kernel<T, EIGHT, N><<<static_cast<unsigned>(chunks), kThreads, 0, s>>>(a);
-  return launch_status();
+  return launch_chained(first == 0 && common.device_s == nullptr, adamw_kernel<T, EIGHT, N>,
+                        dim3(static_cast<unsigned>(chunks)), kThreads, 0, 1, s, a);
 }
 
 template <typename T, bool EIGHT>
@@ -526,8 +529,8 @@ extern "C" int rfm_adamw(const rfm_adamw_tensor* tensors, int count, int dtype, 
   cudaStream_t s = as_stream(stream);
   if (on_device) {
     AdamScalars* out = static_cast<AdamScalars*>(workspace);
-    adam_scalars_kernel<<<1, 1, 0, s>>>(device_lr, device_step, lr, beta1, beta2, weight_decay, step, out);
-    const int rc = launch_status();
+    const int rc = launch_chained(true, adam_scalars_kernel, dim3(1), 1, 0, 1, s, device_lr, device_step, lr, beta1,
+                                  beta2, weight_decay, step, out);
     if (rc != RFM_OK) return rc;
     c.device_s = out;
   } else {
@@ -555,8 +558,8 @@ extern "C" int rfm_adamw_moments(const void* exp_avg, const void* exp_avg_sq, co
     return RFM_ERR_INVALID_ARGUMENT;
   }
   const int64_t per = static_cast<int64_t>(kThreads / 32) * kBlock;
-  adam_moments_kernel<<<static_cast<unsigned>((numel + per - 1) / per), kThreads, 0, as_stream(stream)>>>(
-      static_cast<const uint8_t*>(exp_avg), static_cast<const uint8_t*>(exp_avg_sq), exp_avg_scale, exp_avg_sq_scale,
-      numel, out_avg, out_avg_sq);
-  return launch_status();
+  return launch_chained(true, adam_moments_kernel, dim3(static_cast<unsigned>((numel + per - 1) / per)), kThreads, 0, 1,
+                        as_stream(stream), static_cast<const uint8_t*>(exp_avg),
+                        static_cast<const uint8_t*>(exp_avg_sq), exp_avg_scale, exp_avg_sq_scale, numel, out_avg,
+                        out_avg_sq);
 }

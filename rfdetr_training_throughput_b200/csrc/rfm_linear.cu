@@ -836,6 +836,7 @@ __device__ __forceinline__ Pack<T, 8> load_piece(const T* row, int k, int depth)
 
 template <typename T, int R, int W, int UNROLL>
 __global__ void __launch_bounds__(32 * kFewWarps) few_rows_kernel(const FewArgs a) {
+  chain_start();
   const int lane = threadIdx.x & 31;
   const int n0 = (static_cast<int>(blockIdx.x) * kFewWarps + (threadIdx.x >> 5)) * W;
   if (n0 >= a.n) return;
@@ -893,12 +894,9 @@ template <typename T>
 int launch_few_rows(const FewArgs& a, cudaStream_t s) {
   constexpr int kColumns = 2;  // of a warp
   const unsigned grid = static_cast<unsigned>((a.n + kFewWarps * kColumns - 1) / (kFewWarps * kColumns));
-  if (a.rows == 1) {
-    few_rows_kernel<T, 1, kColumns, 4><<<grid, 32 * kFewWarps, 0, s>>>(a);
-  } else {
-    few_rows_kernel<T, 2, kColumns, 4><<<grid, 32 * kFewWarps, 0, s>>>(a);
-  }
-  return launch_status();
+  return a.rows == 1
+             ? launch_chained(true, few_rows_kernel<T, 1, kColumns, 4>, dim3(grid), 32 * kFewWarps, 0, 1, s, a)
+             : launch_chained(true, few_rows_kernel<T, 2, kColumns, 4>, dim3(grid), 32 * kFewWarps, 0, 1, s, a);
 }
 
 // ---- host side
@@ -1221,9 +1219,10 @@ extern "C" int rfm_linear_backward(const rfm_linear_grad* p, void* stream) {
       return RFM_ERR_LAUNCH;
     }
     if (p->grad_bias != nullptr) {
-      bias_sum_kernel<<<(out + 31) / 32, 1024, 0, s>>>(nullptr, 0, out, p->grad_bias, p->bias_dtype);
+      return launch_chained(true, bias_sum_kernel, dim3((out + 31) / 32), 1024, 0, 1, s,
+                            static_cast<const float*>(nullptr), 0, out, p->grad_bias, p->bias_dtype);
     }
-    return launch_status();
+    return RFM_OK;
   }
   const bool acts = p->activation != RFM_ACT_NONE;
   if (p->grad_out == nullptr || (rows > 1 && p->ld_grad < out) || (acts && p->saved == nullptr)) {

@@ -227,6 +227,7 @@ __global__ void __launch_bounds__(cta_threads(TEAM, CH* VEC)) norm_fwd_kernel(co
   // the loop runs on the row of the warp's first team, so that a warp stays whole
   int64_t lead = TEAM >= 32 ? row : static_cast<int64_t>(blockIdx.x) * kTeams + (threadIdx.x & ~31u) / TEAM;
 
+  chain_start();
   Rows rows(a.x, a.ld_x, a.dim, lane, ring);
 #pragma unroll
   for (int d = 0; d < kDepth; ++d) {
@@ -320,7 +321,7 @@ __global__ void __launch_bounds__(cta_threads(TEAM, CH* VEC)) norm_bwd_kernel(co
   int64_t row = static_cast<int64_t>(blockIdx.x) * kTeams + team;
   int64_t lead = TEAM >= 32 ? row : static_cast<int64_t>(blockIdx.x) * kTeams + (threadIdx.x & ~31u) / TEAM;
 
-  if (PARAMS) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the sums' kernel waits for this one
+  chain_start();
   Rows xs(a.x, a.ld_x, a.dim, lane, ring);
   Rows dys(a.dy, a.ld_dy, a.dim, lane, ring + Rows::kBytes);
   float mean_ahead[kDepth], rstd_ahead[kDepth];
@@ -446,6 +447,7 @@ __global__ void __launch_bounds__(cta_threads(TEAM, CH* VEC)) norm_bwd_kernel(co
 // L2) for each sum.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) norm_fwd_wide_kernel(const NormArgs a) {
+  chain_start();
   __shared__ float2 slots[2 * kWarps];
   T* out = static_cast<T*>(a.out);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -473,6 +475,7 @@ __global__ void __launch_bounds__(kThreads) norm_fwd_wide_kernel(const NormArgs 
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) norm_bwd_wide_kernel(const NormArgs a) {
+  chain_start();
   __shared__ float2 slots[2 * kWarps];
   T* out = static_cast<T*>(a.out);
   int parity = 0;
@@ -501,6 +504,7 @@ __global__ void __launch_bounds__(kThreads) norm_bwd_wide_kernel(const NormArgs 
 // rows (blockIdx.y).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) norm_wide_params_kernel(const NormArgs a) {
+  chain_start();
   const int col = static_cast<int>(blockIdx.x) * kThreads + static_cast<int>(threadIdx.x);
   if (col >= a.dim) return;
   float dw = 0.f, db = 0.f;
@@ -578,8 +582,7 @@ int launch_bwd(const NormArgs& a, int* ctas, cudaStream_t stream) {
   const int fit = resident(kernel, threads, bytes, &ready, &per_sm);
   if (fit == 0) return RFM_ERR_LAUNCH;
   *ctas = norm_ctas(a.rows, threads / TEAM, fit < kBwdPerSm ? fit : kBwdPerSm);
-  kernel<<<*ctas, threads, bytes, stream>>>(a);
-  return launch_status();
+  return launch_chained(true, kernel, dim3(*ctas), threads, bytes, 1, stream, a);
 }
 
 // The backward may have another team (BTEAM, BCH) than the forward.
@@ -595,8 +598,7 @@ int launch_norm(const NormArgs& a, bool backward, int* ctas, cudaStream_t stream
   const auto kernel = norm_fwd_kernel<T, VEC, TEAM, CH>;
   const int fit = resident(kernel, threads, bytes, &ready, &per_sm);
   if (fit == 0) return RFM_ERR_LAUNCH;
-  kernel<<<norm_ctas(a.rows, threads / TEAM, fit), threads, bytes, stream>>>(a);
-  return launch_status();
+  return launch_chained(true, kernel, dim3(norm_ctas(a.rows, threads / TEAM, fit)), threads, bytes, 1, stream, a);
 }
 
 // The smallest team and register count that hold a row.
@@ -606,16 +608,15 @@ int dispatch_norm(const NormArgs& a, bool vectors, bool backward, int* ctas, cud
   const int d = a.dim;
   if (d > kWideDim) {
     const int grid = norm_ctas(a.rows, 1, 8);
-    if (!backward) {
-      norm_fwd_wide_kernel<T><<<grid, kThreads, 0, s>>>(a);
-      return launch_status();
+    if (!backward) return launch_chained(true, norm_fwd_wide_kernel<T>, dim3(grid), kThreads, 0, 1, s, a);
+    if (a.out != nullptr) {
+      const int rc = launch_chained(true, norm_bwd_wide_kernel<T>, dim3(grid), kThreads, 0, 1, s, a);
+      if (rc != RFM_OK) return rc;
     }
-    if (a.out != nullptr) norm_bwd_wide_kernel<T><<<grid, kThreads, 0, s>>>(a);
-    if (a.partial != nullptr) {
-      *ctas = static_cast<int>(a.rows < kWideSlabs ? a.rows : kWideSlabs);
-      norm_wide_params_kernel<T><<<dim3((d + kThreads - 1) / kThreads, *ctas), kThreads, 0, s>>>(a);
-    }
-    return launch_status();
+    if (a.partial == nullptr) return RFM_OK;
+    *ctas = static_cast<int>(a.rows < kWideSlabs ? a.rows : kWideSlabs);
+    return launch_chained(a.out == nullptr, norm_wide_params_kernel<T>, dim3((d + kThreads - 1) / kThreads, *ctas),
+                          kThreads, 0, 1, s, a);
   }
   // A warp a row up to 1024 columns (32 a lane): a team of several warps pays its
   // shuffles in each of them and a barrier twice a row (65536 x 1024 fp16, four
