@@ -435,7 +435,8 @@ int rfm_layer_norm_backward(const void* x, int64_t ld_x, const void* weight, con
  *                codes are rounded at random by a hash of (t, the tensor's number, the element's index).
  *                A NaN or infinite gradient leaves no finite value in its block.
  *   step         t >= 1 of this update; device_step (int64, not NULL) replaces it, device_lr (float32)
- *                replaces lr, for steps captured in a graph.  With either, `workspace` is 16 bytes,
+ *                replaces lr, for steps captured in a graph; both are the caller's to keep in range (t = 0
+ *                divides by 0: NaN parameters).  With either, `workspace` is 16 bytes,
  *                16-byte aligned, used by this call's kernels alone.
  *   grad_scale   float32 on the device, or NULL for 1 (a clipping or loss-scaling factor)
  *

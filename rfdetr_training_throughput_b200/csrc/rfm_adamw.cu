@@ -444,7 +444,8 @@ __global__ void __launch_bounds__(kThreads) adam_moments_kernel(const uint8_t* m
 }
 
 template <typename T, bool EIGHT, int N>
-int launch_adamw(const AdamCommon& common, const rfm_adamw_tensor* tensors, int first, int last, cudaStream_t s) {
+int launch_adamw(const AdamCommon& common, const rfm_adamw_tensor* tensors, int first, int last, bool& started,
+                 cudaStream_t s) {
   AdamArgs<N> a;
   a.c = common;
   int64_t chunks = 0;
@@ -462,16 +463,19 @@ int launch_adamw(const AdamCommon& common, const rfm_adamw_tensor* tensors, int 
   }
   if (k == 0) return RFM_OK;
   a.c.count = k;
-  return launch_chained(first == 0 && common.device_s == nullptr, adamw_kernel<T, EIGHT, N>,
-                        dim3(static_cast<unsigned>(chunks)), kThreads, 0, 1, s, a);
+  const bool first_of_call = !started;
+  started = true;
+  return launch_chained(first_of_call, adamw_kernel<T, EIGHT, N>, dim3(static_cast<unsigned>(chunks)), kThreads, 0, 1,
+                        s, a);
 }
 
 template <typename T, bool EIGHT>
 int run_adamw(const AdamCommon& c, const rfm_adamw_tensor* tensors, int count, cudaStream_t s) {
-  if (count <= kSmallTable) return launch_adamw<T, EIGHT, kSmallTable>(c, tensors, 0, count, s);
+  bool started = c.device_s != nullptr;  // one of the call's kernels has been launched
+  if (count <= kSmallTable) return launch_adamw<T, EIGHT, kSmallTable>(c, tensors, 0, count, started, s);
   for (int first = 0; first < count; first += kLargeTable) {
     const int last = count - first < kLargeTable ? count : first + kLargeTable;
-    const int rc = launch_adamw<T, EIGHT, kLargeTable>(c, tensors, first, last, s);
+    const int rc = launch_adamw<T, EIGHT, kLargeTable>(c, tensors, first, last, started, s);
     if (rc != RFM_OK) return rc;
   }
   return RFM_OK;

@@ -140,10 +140,15 @@ __device__ __forceinline__ Pair activate(Pair v, int act) {
 
 __device__ __forceinline__ float activate(float v, int act) { return split(activate(both(v), act)).x; }
 
-// dy act'(v): act' is 0 at relu's border, and cdf(v) + v pdf(v) for gelu.
+// dy act'(v): act' is 0 at relu's border, and cdf(v) + v pdf(v) for gelu.  What
+// relu cut leaves a 0 whatever dy is there (an infinity times 0 would be NaN), and
+// a NaN that it kept passes dy on.
 __device__ __forceinline__ Pair times_activate_grad(Pair dy, Pair v, int act) {
   const float2 f = split(v);
-  if (act == RFM_ACT_RELU) return dy * pair(f.x > 0.f ? 1.f : 0.f, f.y > 0.f ? 1.f : 0.f);
+  if (act == RFM_ACT_RELU) {
+    const float2 d = split(dy);
+    return pair(f.x <= 0.f ? 0.f : d.x, f.y <= 0.f ? 0.f : d.y);
+  }
   if (act == RFM_ACT_GELU) {
     // pdf(v) = 2^(-v^2 log2(e) / 2) / sqrt(2 pi)
     const float2 e = split(v * v * both(-0.72134752044448170f));

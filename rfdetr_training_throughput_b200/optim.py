@@ -41,7 +41,8 @@ def adamw_step(params: TensorList, grads: TensorList, exp_avg: TensorList, exp_a
     codes (see ``rfm_adamw``).
 
     ``step`` is the number of this update, from 1; an int64 tensor of one element on the device, and for
-    ``lr`` a float32 one, are read by the kernels, so that a captured step follows them.  ``grad_scale``
+    ``lr`` a float32 one, are read by the kernels, so that a captured step follows them (unchecked: a counter
+    of 0 gives NaN).  ``grad_scale``
     (float32, one element, on the device) multiplies the gradients: a clipping factor or the inverse of a
     loss scale, without a host synchronisation.
     """

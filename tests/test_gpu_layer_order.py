@@ -85,3 +85,26 @@ def test_steps_in_a_row(bits):
 
     for a, b in zip(run(lambda: None), run(torch.cuda.synchronize)):
         assert torch.equal(a, b)
+
+
+def test_captured_step_whose_first_launch_is_empty():
+    """More tensors than one launch takes, the first of them all empty, captured behind another kernel."""
+    count = 700
+    p = [torch.randn(0 if i < 600 else 100 + i, device=DEV) for i in range(count)]
+    other = [x.clone() for x in p]
+    state = [[torch.zeros_like(x) for x in p] for _ in range(4)]
+    g = [torch.empty_like(x) for x in p]
+
+    def one(t, params, m, v):
+        torch._foreach_copy_(g[600:], [torch.sin(x) for x in params[600:]])
+        adamw_step(params, g, m, v, t, lr=1e-2)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        one(1, p, *state[:2])
+    for t in range(3):
+        graph.replay()
+        one(1, other, *state[2:])
+    torch.cuda.synchronize()
+    for a, b in zip(p, other):
+        assert torch.equal(a, b)

@@ -422,3 +422,26 @@ def test_a_feed_forward_block_trains():
     for k, p in ps.items():
         assert bool(p.isfinite().all()) and not torch.equal(p, before[k])
     check_faults()
+
+
+def test_relu_cuts_infinite_gradients():
+    """Where relu cut, an infinite or undefined incoming gradient does not come through; where it kept a NaN
+    the gradient passes, as torch's relu has it.  Rows of the identity's product, so that each element of
+    dX is one of dP."""
+    bad = [float("inf"), -float("inf"), float("nan"), 1.0]
+    for outer, residual in ((64, False), (64, True), (51, False)):
+        x = torch.zeros(8, outer, device=DEV, dtype=torch.bfloat16)
+        x[:4] = -1
+        x[4:] = 1
+        x[7] = float("nan")
+        bias = torch.zeros(outer, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+        leaf = x.clone().requires_grad_(True)
+        res = torch.ones_like(x) if residual else None
+        out = linear(leaf, torch.eye(outer, device=DEV, dtype=torch.bfloat16), bias, activation="relu", residual=res)
+        dy = torch.ones_like(x)
+        dy[:4, 0] = torch.tensor(bad, device=DEV, dtype=torch.bfloat16)
+        out.backward(dy)
+        want = torch.zeros_like(x)
+        want[4:] = 1
+        assert torch.equal(leaf.grad, want)
+        assert torch.equal(bias.grad, torch.full_like(bias, 4.0))
