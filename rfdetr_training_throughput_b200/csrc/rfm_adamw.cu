@@ -463,9 +463,9 @@ int launch_adamw(const AdamCommon& common, const rfm_adamw_tensor* tensors, int 
   }
   if (k == 0) return RFM_OK;
   a.c.count = k;
-  const bool first_of_call = !started;
+  const Chain chain = started ? Chain::kNext : Chain::kFirst;
   started = true;
-  return launch_chained(first_of_call, adamw_kernel<T, EIGHT, N>, dim3(static_cast<unsigned>(chunks)), kThreads, 0, 1,
+  return launch_chained(chain, adamw_kernel<T, EIGHT, N>, dim3(static_cast<unsigned>(chunks)), kThreads, 0, 1,
                         s, a);
 }
 
@@ -533,8 +533,8 @@ extern "C" int rfm_adamw(const rfm_adamw_tensor* tensors, int count, int dtype, 
   cudaStream_t s = as_stream(stream);
   if (on_device) {
     AdamScalars* out = static_cast<AdamScalars*>(workspace);
-    const int rc = launch_chained(true, adam_scalars_kernel, dim3(1), 1, 0, 1, s, device_lr, device_step, lr, beta1,
-                                  beta2, weight_decay, step, out);
+    const int rc = launch_chained(Chain::kFirst, adam_scalars_kernel, dim3(1), 1, 0, 1, s, device_lr, device_step, lr,
+                                  beta1, beta2, weight_decay, step, out);
     if (rc != RFM_OK) return rc;
     c.device_s = out;
   } else {
@@ -562,8 +562,8 @@ extern "C" int rfm_adamw_moments(const void* exp_avg, const void* exp_avg_sq, co
     return RFM_ERR_INVALID_ARGUMENT;
   }
   const int64_t per = static_cast<int64_t>(kThreads / 32) * kBlock;
-  return launch_chained(true, adam_moments_kernel, dim3(static_cast<unsigned>((numel + per - 1) / per)), kThreads, 0, 1,
-                        as_stream(stream), static_cast<const uint8_t*>(exp_avg),
-                        static_cast<const uint8_t*>(exp_avg_sq), exp_avg_scale, exp_avg_sq_scale, numel, out_avg,
-                        out_avg_sq);
+  const dim3 grid(static_cast<unsigned>((numel + per - 1) / per));
+  return launch_chained(Chain::kFirst, adam_moments_kernel, grid, kThreads, 0, 1, as_stream(stream),
+                        static_cast<const uint8_t*>(exp_avg), static_cast<const uint8_t*>(exp_avg_sq), exp_avg_scale,
+                        exp_avg_sq_scale, numel, out_avg, out_avg_sq);
 }

@@ -803,7 +803,9 @@ int launch_grad_pre(const GradPreArgs& a, int activation, const dim3& grid, cuda
   const auto kernel = activation == RFM_ACT_RELU   ? grad_pre_kernel<T, VEC, RFM_ACT_RELU>
                       : activation == RFM_ACT_GELU ? grad_pre_kernel<T, VEC, RFM_ACT_GELU>
                                                    : grad_pre_kernel<T, VEC, RFM_ACT_NONE>;
-  return launch_chained(true, kernel, grid, 32 * kPreWarps, 0, 1, s, a);
+  // an ordinary launch: CTAs that start one by one as the forward's leave find the
+  // SMs unevenly filled (31200 x 2048, relu: a training pass of 213 us, 199 so)
+  return launch_chained(Chain::kNone, kernel, grid, 32 * kPreWarps, 0, 1, s, a);
 }
 
 // ---- a few rows: the weight is read once and nothing is tiled
@@ -899,9 +901,8 @@ template <typename T>
 int launch_few_rows(const FewArgs& a, cudaStream_t s) {
   constexpr int kColumns = 2;  // of a warp
   const unsigned grid = static_cast<unsigned>((a.n + kFewWarps * kColumns - 1) / (kFewWarps * kColumns));
-  return a.rows == 1
-             ? launch_chained(true, few_rows_kernel<T, 1, kColumns, 4>, dim3(grid), 32 * kFewWarps, 0, 1, s, a)
-             : launch_chained(true, few_rows_kernel<T, 2, kColumns, 4>, dim3(grid), 32 * kFewWarps, 0, 1, s, a);
+  const auto kernel = a.rows == 1 ? few_rows_kernel<T, 1, kColumns, 4> : few_rows_kernel<T, 2, kColumns, 4>;
+  return launch_chained(Chain::kFirst, kernel, dim3(grid), 32 * kFewWarps, 0, 1, s, a);
 }
 
 // ---- host side
@@ -997,7 +998,7 @@ struct Product {
   int n;
   int64_t k;
   int dtype;
-  bool first;     // of the call's kernels
+  Chain chain;
   GemmArgs args;  // epilogue fields filled in by the caller
 };
 
@@ -1043,7 +1044,7 @@ int launch_gemm(const Product& p, GemmArgs& g, float* partial, cudaStream_t stre
   const int sms = device_sm_count();
   const int64_t workers = sms / CG;
   const unsigned grid = static_cast<unsigned>((items < workers ? items : workers) * CG);
-  return launch_chained(p.first, kernel, dim3(grid), S::kThreads, S::kBytes, CG, stream, maps, g);
+  return launch_chained(p.chain, kernel, dim3(grid), S::kThreads, S::kBytes, CG, stream, maps, g);
 }
 
 template <typename T, int BN, int CG, bool A_MN, bool B_MN>
@@ -1086,9 +1087,9 @@ int run_product(const Product& p, void* workspace, cudaStream_t stream) {
   const int64_t ctas = (cells + 255) / 256;
   const unsigned grid = static_cast<unsigned>(ctas < most ? ctas : most);
   if (quads) {
-    return launch_chained(false, finish_kernel<T, 4>, dim3(grid), 256, 0, 1, stream, f);
+    return launch_chained(Chain::kNext, finish_kernel<T, 4>, dim3(grid), 256, 0, 1, stream, f);
   }
-  return launch_chained(false, finish_kernel<T, 1>, dim3(grid), 256, 0, 1, stream, f);
+  return launch_chained(Chain::kNext, finish_kernel<T, 1>, dim3(grid), 256, 0, 1, stream, f);
 }
 
 template <bool A_MN, bool B_MN>
@@ -1181,7 +1182,7 @@ extern "C" int rfm_linear_forward(const rfm_linear* p, void* stream) {
   g.n = p->out_features;
   g.k = p->in_features;
   g.dtype = p->dtype;
-  g.first = true;
+  g.chain = Chain::kFirst;
   g.args.activation = p->activation;
   g.args.bias = p->bias;
   g.args.bias_dtype = p->bias_dtype;
@@ -1224,7 +1225,7 @@ extern "C" int rfm_linear_backward(const rfm_linear_grad* p, void* stream) {
       return RFM_ERR_LAUNCH;
     }
     if (p->grad_bias != nullptr) {
-      return launch_chained(true, bias_sum_kernel, dim3((out + 31) / 32), 1024, 0, 1, s,
+      return launch_chained(Chain::kFirst, bias_sum_kernel, dim3((out + 31) / 32), 1024, 0, 1, s,
                             static_cast<const float*>(nullptr), 0, out, p->grad_bias, p->bias_dtype);
     }
     return RFM_OK;
@@ -1268,12 +1269,12 @@ extern "C" int rfm_linear_backward(const rfm_linear_grad* p, void* stream) {
     }
     if (done != RFM_OK) return done;
     if (p->grad_bias != nullptr) {
-      done = launch_chained(false, bias_sum_kernel, dim3((out + 31) / 32), 1024, 0, 1, s, a.partial, slabs, out,
+      done = launch_chained(Chain::kNext, bias_sum_kernel, dim3((out + 31) / 32), 1024, 0, 1, s, a.partial, slabs, out,
                             p->grad_bias, p->bias_dtype);
       if (done != RFM_OK) return done;
     }
   }
-  bool first = !own && p->grad_bias == nullptr;  // of the call's kernels: the next product
+  Chain chain = own || p->grad_bias != nullptr ? Chain::kNext : Chain::kFirst;  // of the next product
   const void* dp = own ? p->grad_pre : p->grad_out;
   const int64_t ld_dp = own ? p->ld_grad_pre : p->ld_grad;
   if (p->grad_x != nullptr) {
@@ -1286,11 +1287,11 @@ extern "C" int rfm_linear_backward(const rfm_linear_grad* p, void* stream) {
     g.n = in;
     g.k = out;
     g.dtype = p->dtype;
-    g.first = first;
+    g.chain = chain;
     g.args.out = p->grad_x;
     const int done = run_typed<false, true>(g, p->workspace, s);
     if (done != RFM_OK) return done;
-    first = false;
+    chain = Chain::kNext;
   }
   if (p->grad_weight != nullptr) {
     Product g{};
@@ -1302,7 +1303,7 @@ extern "C" int rfm_linear_backward(const rfm_linear_grad* p, void* stream) {
     g.n = in;
     g.k = rows;
     g.dtype = p->dtype;
-    g.first = first;
+    g.chain = chain;
     g.args.out = p->grad_weight;
     return run_typed<true, true>(g, p->workspace, s);
   }

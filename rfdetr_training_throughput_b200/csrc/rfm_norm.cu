@@ -582,7 +582,7 @@ int launch_bwd(const NormArgs& a, int* ctas, cudaStream_t stream) {
   const int fit = resident(kernel, threads, bytes, &ready, &per_sm);
   if (fit == 0) return RFM_ERR_LAUNCH;
   *ctas = norm_ctas(a.rows, threads / TEAM, fit < kBwdPerSm ? fit : kBwdPerSm);
-  return launch_chained(true, kernel, dim3(*ctas), threads, bytes, 1, stream, a);
+  return launch_chained(Chain::kFirst, kernel, dim3(*ctas), threads, bytes, 1, stream, a);
 }
 
 // The backward may have another team (BTEAM, BCH) than the forward.
@@ -598,7 +598,8 @@ int launch_norm(const NormArgs& a, bool backward, int* ctas, cudaStream_t stream
   const auto kernel = norm_fwd_kernel<T, VEC, TEAM, CH>;
   const int fit = resident(kernel, threads, bytes, &ready, &per_sm);
   if (fit == 0) return RFM_ERR_LAUNCH;
-  return launch_chained(true, kernel, dim3(norm_ctas(a.rows, threads / TEAM, fit)), threads, bytes, 1, stream, a);
+  const dim3 grid(norm_ctas(a.rows, threads / TEAM, fit));
+  return launch_chained(Chain::kFirst, kernel, grid, threads, bytes, 1, stream, a);
 }
 
 // The smallest team and register count that hold a row.
@@ -608,15 +609,15 @@ int dispatch_norm(const NormArgs& a, bool vectors, bool backward, int* ctas, cud
   const int d = a.dim;
   if (d > kWideDim) {
     const int grid = norm_ctas(a.rows, 1, 8);
-    if (!backward) return launch_chained(true, norm_fwd_wide_kernel<T>, dim3(grid), kThreads, 0, 1, s, a);
+    if (!backward) return launch_chained(Chain::kFirst, norm_fwd_wide_kernel<T>, dim3(grid), kThreads, 0, 1, s, a);
     if (a.out != nullptr) {
-      const int rc = launch_chained(true, norm_bwd_wide_kernel<T>, dim3(grid), kThreads, 0, 1, s, a);
+      const int rc = launch_chained(Chain::kFirst, norm_bwd_wide_kernel<T>, dim3(grid), kThreads, 0, 1, s, a);
       if (rc != RFM_OK) return rc;
     }
     if (a.partial == nullptr) return RFM_OK;
     *ctas = static_cast<int>(a.rows < kWideSlabs ? a.rows : kWideSlabs);
-    return launch_chained(a.out == nullptr, norm_wide_params_kernel<T>, dim3((d + kThreads - 1) / kThreads, *ctas),
-                          kThreads, 0, 1, s, a);
+    return launch_chained(a.out == nullptr ? Chain::kFirst : Chain::kNext, norm_wide_params_kernel<T>,
+                          dim3((d + kThreads - 1) / kThreads, *ctas), kThreads, 0, 1, s, a);
   }
   // A warp a row up to 1024 columns (32 a lane): a team of several warps pays its
   // shuffles in each of them and a barrier twice a row (65536 x 1024 fp16, four
@@ -728,6 +729,6 @@ extern "C" int rfm_layer_norm_backward(const void* x, int64_t ld_x, const void* 
   }
   if (!params) return RFM_OK;
   // with no rows the sums are empty: zeros
-  return launch_chained(rows == 0, norm_param_sum_kernel, dim3((dim + 31) / 32, 2), 1024, 0, 1, as_stream(stream),
-                        a.partial, ctas, dim, grad_weight, grad_bias, param_dtype);
+  return launch_chained(rows == 0 ? Chain::kFirst : Chain::kNext, norm_param_sum_kernel, dim3((dim + 31) / 32, 2), 1024,
+                        0, 1, as_stream(stream), a.partial, ctas, dim, grad_weight, grad_bias, param_dtype);
 }

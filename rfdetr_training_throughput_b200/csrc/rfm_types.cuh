@@ -14,16 +14,20 @@ namespace rfm {
 // wait in chain_start before they touch memory, until that kernel has completed
 // (and so, as it waited in its turn, everything before it).  About 2 us a launch
 // where kernels are short (300 x 256 -> 91: 8.2 us a call without, 6.0 with).
-// Every kernel that launch_chained starts calls chain_start first.  The call's
-// first kernel is an ordinary launch inside a stream capture, where the node
-// before it may be anything.
+// Every kernel that launch_chained starts calls chain_start first.
+enum class Chain {
+  kNext,   // behind another kernel of the same call
+  kFirst,  // the call's first: an ordinary launch inside a stream capture, where the node before may be anything
+  kNone,   // an ordinary launch
+};
+
 __device__ __forceinline__ void chain_start() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   grid_dependency_wait();
 }
 
 template <typename... Params, typename... Args>
-int launch_chained(bool first_of_call, void (*kernel)(Params...), dim3 grid, int threads, int smem, int cluster,
+int launch_chained(Chain chain, void (*kernel)(Params...), dim3 grid, int threads, int smem, int cluster,
                    cudaStream_t stream, const Args&... args) {
   cudaLaunchConfig_t config{};
   config.gridDim = grid;
@@ -39,11 +43,11 @@ int launch_chained(bool first_of_call, void (*kernel)(Params...), dim3 grid, int
     ++n;
   }
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-  if (first_of_call && cudaStreamIsCapturing(stream, &capture) != cudaSuccess) {
+  if (chain == Chain::kFirst && cudaStreamIsCapturing(stream, &capture) != cudaSuccess) {
     cudaGetLastError();
     capture = cudaStreamCaptureStatusInvalidated;  // an ordinary launch, which reports the stream's error
   }
-  if (capture == cudaStreamCaptureStatusNone) {
+  if (chain != Chain::kNone && capture == cudaStreamCaptureStatusNone) {
     attrs[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attrs[n].val.programmaticStreamSerializationAllowed = 1;
     ++n;
