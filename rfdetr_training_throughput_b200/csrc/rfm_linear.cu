@@ -1005,6 +1005,19 @@ struct Product {
 template <typename T, int BN, int CG, bool A_MN, bool B_MN, int ACT>
 int launch_gemm(const Product& p, GemmArgs& g, float* partial, cudaStream_t stream) {
   using S = Shape<BN, CG>;
+  // The context whose shared-memory limit is raised.  Before the maps: in a thread
+  // that has made no CUDA call yet (autograd's, in a process's first backward) this
+  // makes the context current, which encoding a map needs.
+  static thread_local unsigned long long ready = 0;
+  const auto kernel = gemm_kernel<T, BN, CG, A_MN, B_MN, ACT>;
+  const unsigned long long context = current_context_id();
+  if (ready != context || context == 0) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess) {
+      cudaGetLastError();
+      return RFM_ERR_LAUNCH;
+    }
+    ready = context;
+  }
   GemmMaps maps;
   const bool ok_a = A_MN ? make_map(&maps.a, p.dtype, p.a, p.m, p.k, p.ld_a, 64, kBK, CU_TENSOR_MAP_SWIZZLE_128B)
                          : make_map(&maps.a, p.dtype, p.a, p.k, p.m, p.ld_a, kBK, kBM, CU_TENSOR_MAP_SWIZZLE_128B);
@@ -1028,16 +1041,6 @@ int launch_gemm(const Product& p, GemmArgs& g, float* partial, cudaStream_t stre
   if (g.tma_res &&
       !make_map(&maps.res, p.dtype, g.residual, p.n, p.m, g.ld_res, S::kBoxCols, 32, swizzle)) {
     return RFM_ERR_LAUNCH;
-  }
-  static thread_local unsigned long long ready = 0;  // the context whose shared-memory limit is raised
-  const auto kernel = gemm_kernel<T, BN, CG, A_MN, B_MN, ACT>;
-  const unsigned long long context = current_context_id();
-  if (ready != context || context == 0) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess) {
-      cudaGetLastError();
-      return RFM_ERR_LAUNCH;
-    }
-    ready = context;
   }
   const int64_t items = static_cast<int64_t>(g.tiles_m) * g.tiles_n * g.splits;
   if (items >= (int64_t(1) << 31) - (1 << 16)) return RFM_ERR_UNSUPPORTED;

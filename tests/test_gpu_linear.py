@@ -8,6 +8,10 @@ was `saved`: gelu'' is at most 0.8, so act' is off by 0.8 eps/2 |pre|; relu's bo
 within its own error of 0, where dP is off by |dY|.  What is off in dP comes into the sums of the
 backward products with the magnitudes of the other operand."""
 
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -445,3 +449,15 @@ def test_relu_cuts_infinite_gradients():
         want[4:] = 1
         assert torch.equal(leaf.grad, want)
         assert torch.equal(bias.grad, torch.full_like(bias, 4.0))
+
+
+@pytest.mark.parametrize("act,rows", [("none", 40), ("relu", 10000)])
+def test_first_backward_of_a_process(act, rows):
+    """Autograd's thread has made no CUDA call when the first backward of a process reaches the product."""
+    code = ("import torch; from rfdetr_training_throughput_b200.linear import linear\n"
+            f"x = torch.ones({rows}, 64, device='cuda', dtype=torch.bfloat16, requires_grad=True)\n"
+            "w = torch.ones(32, 64, device='cuda', dtype=torch.bfloat16)\n"
+            f"out = linear(x, w, activation='{act}')\n"
+            "(g,) = torch.autograd.grad(out, x, torch.ones_like(out))\n"
+            "assert bool((g == 32).all())\n")
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300, cwd=Path(__file__).resolve().parents[1])
