@@ -808,6 +808,364 @@ int launch_grad_pre(const GradPreArgs& a, int activation, const dim3& grid, cuda
   return launch_chained(Chain::kNone, kernel, grid, 32 * kPreWarps, 0, 1, s, a);
 }
 
+// ---- dP and dX = dP W in one pass, where a row of dX fits one tile
+
+// Up to 384 columns of dX an activation's gradient needs no pass of its own: dY
+// and `saved` come by TMA into the ring of the product's A operand, eight warps
+// turn dY into dP in place (element by element, so the swizzle does not matter),
+// and from there the tensor cores read it and TMA stores it for dW.  A warp owns
+// 8 columns of every slice, so the bias sums need no other warp: over a lane's
+// four rows, over the lanes by shuffles, and over the CTA's tiles in shared
+// memory, in a fixed order.
+//
+// HBM-bound: dY, `saved` and dP, 6 bytes an element, where the dP pass and dX
+// apart move 8.
+template <int BN>
+struct GradShape {
+  static constexpr int kPreparers = 8;  // a warp 8 of a slice's 64 columns
+  static constexpr int kEpiWarps = 4;
+  static constexpr int kEpi = kPreparers, kLoadWarp = kEpi + kEpiWarps, kWeightWarp = kLoadWarp + 1;
+  static constexpr int kMmaWarp = kWeightWarp + 1, kStoreWarp = kMmaWarp + 1;
+  static constexpr int kThreads = 32 * (kStoreWarp + 1);
+  // three rings: dY (then dP), saved, the weight; the first two hide HBM's latency
+  static constexpr int kA = 4, kS = BN == 384 ? 3 : 4, kW = BN == 128 ? 4 : 2;
+  static constexpr int kSliceBytes = kBM * kBK * 2, kWeightBytes = BN * kBK * 2;
+  static constexpr int kMostOut = BN == 384 ? 2048 : 4096;  // columns of bias sums
+  static constexpr int kAccs = BN == 384 ? 1 : 2;
+  static constexpr int kTmemColumns = BN == 128 ? 256 : 512;
+  static constexpr int kMmaN = BN == 384 ? 192 : BN;
+  static constexpr int kBoxBytes = 32 * 32 * 2;
+  static constexpr int kSaved = kA * kSliceBytes, kWeight = kSaved + kS * kSliceBytes;
+  static constexpr int kBoxes = kWeight + kW * kWeightBytes;
+  static constexpr int kSums = kBoxes + kEpiWarps * kBoxBytes;
+  static constexpr int kBars = kSums + kMostOut * 4;
+  static constexpr int kNumBars = 3 * kA + 2 * kS + 2 * kW + 2 * kAccs;
+  static constexpr int kFlags = kBars + kNumBars * 8;
+  static constexpr int kBytes = kFlags + 16;
+  static_assert(kBytes <= 232448, "shared memory of one CTA");
+};
+
+struct GradXArgs {
+  int64_t m;
+  int32_t n;         // columns of dX
+  int32_t out;       // columns of dP
+  int32_t tiles, k_blocks;
+  int32_t store;     // dP is stored
+  float* partial;    // [CTAs][out] column sums, null: not wanted
+};
+
+struct GradXMaps {
+  CUtensorMap dy, saved, dp, weight, dx;
+};
+
+// A place in a ring of N stages.
+template <int N>
+struct Ring {
+  uint32_t stage = 0, phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == N) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+  // every stage has been given back
+  __device__ __forceinline__ bool drained(uint32_t empty, volatile int* dead) {
+    for (int i = 0; i < N; ++i) {
+      if (!bounded_wait(empty + 8 * stage, phase ^ 1u, dead)) return false;
+      next();
+    }
+    return true;
+  }
+  // after a failure: the copies of the last `issued` slices land before the shared memory is given up
+  __device__ __forceinline__ void settle(uint32_t full, uint32_t issued) {
+    for (uint32_t i = 0; i < (issued < N ? issued : N); ++i) {
+      if (stage == 0) {
+        stage = N;
+        phase ^= 1u;
+      }
+      --stage;
+      for (uint32_t k = 0; k < kWaitTries && !mbar_try(full + 8 * stage, phase); ++k) {
+      }
+    }
+  }
+};
+
+template <typename T, int BN, int ACT>
+__global__ void __launch_bounds__(GradShape<BN>::kThreads, 1)
+    grad_x_kernel(const __grid_constant__ GradXMaps maps, const __grid_constant__ GradXArgs a) {
+  using S = GradShape<BN>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = smem_u32(smem);
+  const uint32_t a_full = base + S::kBars, a_ready = a_full + 8 * S::kA, a_empty = a_ready + 8 * S::kA;
+  const uint32_t s_full = a_empty + 8 * S::kA, s_empty = s_full + 8 * S::kS;
+  const uint32_t w_full = s_empty + 8 * S::kS, w_empty = w_full + 8 * S::kW;
+  const uint32_t acc_full = w_empty + 8 * S::kW, acc_empty = acc_full + 8 * S::kAccs;
+  volatile int* dead = reinterpret_cast<volatile int*>(smem + S::kFlags);
+  const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x == 0) {
+    *dead = 0;
+    if ((base & 1023u) != 0) {  // the swizzles count on it; never expected
+      *dead = 1;
+      atomicExch(&g_linear_faults, 1);
+    }
+    for (int i = 0; i < S::kA; ++i) {
+      mbar_init(a_full + 8 * i, 1);
+      mbar_init(a_ready + 8 * i, S::kPreparers);
+      mbar_init(a_empty + 8 * i, a.store ? 2 : 1);  // the products, the store
+    }
+    for (int i = 0; i < S::kS; ++i) {
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(s_empty + 8 * i, S::kPreparers);
+    }
+    for (int i = 0; i < S::kW; ++i) {
+      mbar_init(w_full + 8 * i, 1);
+      mbar_init(w_empty + 8 * i, 1);
+    }
+    for (int i = 0; i < S::kAccs; ++i) {
+      mbar_init(acc_full + 8 * i, 1);
+      mbar_init(acc_empty + 8 * i, S::kEpiWarps);
+    }
+    mbar_init_fence();
+    tma_prefetch_map(&maps.dy);
+    tma_prefetch_map(&maps.saved);
+    tma_prefetch_map(&maps.weight);
+  }
+  if (warp == S::kMmaWarp) tmem_alloc<1>(base + S::kFlags + 4, S::kTmemColumns);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  grid_dependency_wait();  // the set-up above touches nothing that the kernel before writes
+  const uint32_t tmem = *reinterpret_cast<const volatile uint32_t*>(smem + S::kFlags + 4);
+
+  if (warp < S::kPreparers) {
+    Ring<S::kA> ra;
+    Ring<S::kS> rs;
+    // this lane's 16-byte piece of rows lane, lane + 32, ..: the warp's 8 columns under the swizzle
+    const int at = lane * 128 + ((warp ^ (lane & 7)) << 4);
+    float* sums = reinterpret_cast<float*>(smem + S::kSums) + warp * 8;
+    // after the shuffles lane l holds the sum of column l / 4
+    if (a.partial != nullptr && (lane & 3) == 0) {
+      for (int kb = 0; kb < a.k_blocks; ++kb) sums[kb * kBK + (lane >> 2)] = 0.f;
+    }
+    bool ok = true;
+    for (int t = static_cast<int>(blockIdx.x); ok && t < a.tiles; t += static_cast<int>(gridDim.x)) {
+      for (int kb = 0; kb < a.k_blocks; ++kb) {
+        ok = bounded_wait(a_full + 8 * ra.stage, ra.phase, dead) && bounded_wait(s_full + 8 * rs.stage, rs.phase, dead);
+        ok = __all_sync(kFullMask, ok);
+        if (!ok) break;
+        uint8_t* dy = smem + ra.stage * S::kSliceBytes + at;
+        const uint8_t* saved = smem + S::kSaved + rs.stage * S::kSliceBytes + at;
+        Pack<T, 8> g[4], p[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          g[r] = *reinterpret_cast<const Pack<T, 8>*>(dy + r * 4096);
+          p[r] = *reinterpret_cast<const Pack<T, 8>*>(saved + r * 4096);
+        }
+        Pair sum[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          Pack<T, 8> o;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const Pair v = times_activate_grad(load_pair(g[r], j), load_pair(p[r], j), ACT);
+            store_pair(o, j, v);
+            sum[j] = r == 0 ? v : sum[j] + v;
+          }
+          *reinterpret_cast<Pack<T, 8>*>(dy + r * 4096) = o;
+        }
+        proxy_fence();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(a_ready + 8 * ra.stage);
+          mbar_arrive(s_empty + 8 * rs.stage);
+        }
+        if (a.partial != nullptr) {
+          // each step halves the columns a lane still sums
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = split(sum[j]);
+            v[2 * j] = f.x;
+            v[2 * j + 1] = f.y;
+          }
+#pragma unroll
+          for (int half = 4, o = 16; half > 0; half >>= 1, o >>= 1) {
+            const bool upper = (lane & o) != 0;
+#pragma unroll
+            for (int j = 0; j < half; ++j) {
+              const float give = upper ? v[j] : v[j + half], keep = upper ? v[j + half] : v[j];
+              v[j] = keep + __shfl_xor_sync(kFullMask, give, o);
+            }
+          }
+          v[0] += __shfl_xor_sync(kFullMask, v[0], 2);
+          v[0] += __shfl_xor_sync(kFullMask, v[0], 1);
+          if ((lane & 3) == 0) sums[kb * kBK + (lane >> 2)] += v[0];
+        }
+        ra.next();
+        rs.next();
+      }
+    }
+    if (a.partial != nullptr && (lane & 3) == 0) {
+      for (int kb = 0; kb < a.k_blocks; ++kb) {
+        const int col = kb * kBK + warp * 8 + (lane >> 2);
+        if (col < a.out) a.partial[static_cast<int64_t>(blockIdx.x) * a.out + col] = sums[kb * kBK + (lane >> 2)];
+      }
+    }
+  } else if (warp < S::kEpi + S::kEpiWarps) {
+    const int quarter = warp & 3;
+    const uint32_t box = base + S::kBoxes + quarter * S::kBoxBytes;
+    uint8_t* row_ptr = smem + S::kBoxes + quarter * S::kBoxBytes + lane * 64;
+    const int swz = (lane >> 1) & 3;
+    Ring<S::kAccs> acc;
+    for (int t = static_cast<int>(blockIdx.x); t < a.tiles; t += static_cast<int>(gridDim.x)) {
+      const int64_t row0 = static_cast<int64_t>(t) * kBM + quarter * 32;
+      if (!__all_sync(kFullMask, bounded_wait(acc_full + 8 * acc.stage, acc.phase, dead))) break;
+      tc_fence_after();
+      if (row0 < a.m) {
+#pragma unroll 1
+        for (int c = 0; c < BN && c < a.n; c += 32) {
+          uint32_t v[32];
+          tmem_load_32(v, tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc.stage * BN + c);
+          if (lane == 0) tma_wait_read<0>();  // the box's last store has been read
+          __syncwarp();
+          tmem_wait_load(v);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t q[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              q[i] = pack2<T>(__uint_as_float(v[8 * j + 2 * i]), __uint_as_float(v[8 * j + 2 * i + 1]));
+            *reinterpret_cast<uint4*>(row_ptr + ((j ^ swz) << 4)) = make_uint4(q[0], q[1], q[2], q[3]);
+          }
+          proxy_fence();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&maps.dx, c, static_cast<int>(row0), box);
+            tma_commit();
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty + 8 * acc.stage);
+      acc.next();
+    }
+    if (lane == 0) tma_wait_read<0>();
+  } else if (warp == S::kLoadWarp) {
+    if (lane == 0) {
+      Ring<S::kA> ra;
+      Ring<S::kS> rs;
+      uint32_t issued_a = 0, issued_s = 0;
+      bool ok = true;
+      for (int t = static_cast<int>(blockIdx.x); ok && t < a.tiles; t += static_cast<int>(gridDim.x)) {
+        for (int kb = 0; kb < a.k_blocks; ++kb) {
+          ok = bounded_wait(a_empty + 8 * ra.stage, ra.phase ^ 1u, dead);
+          if (!ok) break;
+          mbar_expect(a_full + 8 * ra.stage, S::kSliceBytes);
+          tma_load_2d(base + ra.stage * S::kSliceBytes, &maps.dy, kb * kBK, t * kBM, a_full + 8 * ra.stage);
+          ra.next();
+          ++issued_a;
+          ok = bounded_wait(s_empty + 8 * rs.stage, rs.phase ^ 1u, dead);
+          if (!ok) break;
+          mbar_expect(s_full + 8 * rs.stage, S::kSliceBytes);
+          tma_load_2d(base + S::kSaved + rs.stage * S::kSliceBytes, &maps.saved, kb * kBK, t * kBM,
+                      s_full + 8 * rs.stage);
+          rs.next();
+          ++issued_s;
+        }
+      }
+      if (!ok || !ra.drained(a_empty, dead) || !rs.drained(s_empty, dead)) {
+        ra.settle(a_full, issued_a);
+        rs.settle(s_full, issued_s);
+      }
+    }
+  } else if (warp == S::kWeightWarp) {
+    if (lane == 0) {
+      Ring<S::kW> rw;
+      uint32_t issued = 0;
+      bool ok = true;
+      for (int t = static_cast<int>(blockIdx.x); ok && t < a.tiles; t += static_cast<int>(gridDim.x)) {
+        for (int kb = 0; kb < a.k_blocks; ++kb) {
+          ok = bounded_wait(w_empty + 8 * rw.stage, rw.phase ^ 1u, dead);
+          if (!ok) break;
+          const uint32_t bar = w_full + 8 * rw.stage, to = base + S::kWeight + rw.stage * S::kWeightBytes;
+          mbar_expect(bar, S::kWeightBytes);
+#pragma unroll
+          for (int j = 0; j < BN / 64; ++j) tma_load_2d(to + j * 8192, &maps.weight, j * 64, kb * kBK, bar);
+          rw.next();
+          ++issued;
+        }
+      }
+      if (!ok || !rw.drained(w_empty, dead)) rw.settle(w_full, issued);
+    }
+  } else if (warp == S::kMmaWarp) {
+    if (lane == 0) {
+      constexpr int kType = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+      constexpr uint32_t kInstr = mma_instr(kType, false, true, kBM, S::kMmaN);
+      Ring<S::kA> ra;
+      Ring<S::kW> rw;
+      Ring<S::kAccs> acc;
+      bool ok = true;
+      for (int t = static_cast<int>(blockIdx.x); ok && t < a.tiles; t += static_cast<int>(gridDim.x)) {
+        if (!bounded_wait(acc_empty + 8 * acc.stage, acc.phase ^ 1u, dead)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + acc.stage * BN;
+        for (int kb = 0; kb < a.k_blocks; ++kb) {
+          ok = bounded_wait(w_full + 8 * rw.stage, rw.phase, dead) && bounded_wait(a_ready + 8 * ra.stage, ra.phase, dead);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sa = base + ra.stage * S::kSliceBytes, sb = base + S::kWeight + rw.stage * S::kWeightBytes;
+#pragma unroll
+          for (int k = 0; k < kBK / 16; ++k) {
+#pragma unroll
+            for (int part = 0; part < BN / S::kMmaN; ++part) {
+              tc_mma_f16<1>(d + part * S::kMmaN, operand_desc(sa + k * 32, 16, 1024),
+                            operand_desc(sb + part * (S::kMmaN / 64) * 8192 + k * 2048, 8192, 1024), kInstr,
+                            kb > 0 || k > 0);
+            }
+          }
+          tc_commit<1>(a_empty + 8 * ra.stage);
+          tc_commit<1>(w_empty + 8 * rw.stage);
+          ra.next();
+          rw.next();
+        }
+        if (!ok) break;
+        tc_commit<1>(acc_full + 8 * acc.stage);
+        acc.next();
+      }
+      // as in gemm_kernel: products in flight end before the tensor memory is given up
+      if (*dead) {
+        tc_commit<1>(acc_full + 8 * acc.stage);
+        for (uint32_t k = 0; k < kWaitTries && !mbar_try(acc_full + 8 * acc.stage, acc.phase); ++k) {
+        }
+      }
+    }
+  } else if (lane == 0 && a.store) {
+    Ring<S::kA> ra;
+    bool ok = true;
+    for (int t = static_cast<int>(blockIdx.x); ok && t < a.tiles; t += static_cast<int>(gridDim.x)) {
+      for (int kb = 0; kb < a.k_blocks; ++kb) {
+        ok = bounded_wait(a_ready + 8 * ra.stage, ra.phase, dead);
+        if (!ok) break;
+        tma_store_2d(&maps.dp, kb * kBK, t * kBM, base + ra.stage * S::kSliceBytes);
+        tma_commit();
+        tma_wait_read<0>();
+        mbar_arrive(a_empty + 8 * ra.stage);
+        ra.next();
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == S::kMmaWarp) {
+    tc_fence_after();
+    tmem_free<1>(tmem, S::kTmemColumns);
+  }
+}
+
 // ---- a few rows: the weight is read once and nothing is tiled
 
 // One warp computes W columns of the output for R rows: lane l holds the 16-byte
@@ -1118,11 +1476,75 @@ int bias_slabs(int64_t rows, int n, int vec) {
 }
 
 // The sums' bytes whichever way the columns are read: wider strips are fewer, and
-// their rows are cut into more slabs.
+// their rows are cut into more slabs; grad_x_kernel leaves one row of sums a CTA.
 int64_t bias_bytes(int64_t rows, int n) {
-  const int slabs = bias_slabs(rows, n, 8);
-  const int narrow = bias_slabs(rows, n, 1);
-  return (static_cast<int64_t>(slabs > narrow ? slabs : narrow) * n * 4 + 15) & ~int64_t(15);
+  int64_t slabs = bias_slabs(rows, n, 8);
+  const int64_t narrow = bias_slabs(rows, n, 1), tiles = (rows + kBM - 1) / kBM, sms = device_sm_count();
+  const int64_t ctas = tiles < sms ? tiles : sms;
+  slabs = narrow > slabs ? narrow : slabs;
+  slabs = ctas > slabs ? ctas : slabs;
+  return (slabs * n * 4 + 15) & ~int64_t(15);
+}
+
+// dP and dX in one kernel: an activation, a row of dX in one tile, rows that TMA
+// reads, and enough tiles to occupy most SMs.
+bool grad_x_fused(const rfm_linear_grad* p) {
+  const int in = p->in_features, out = p->out_features;
+  return p->activation != RFM_ACT_NONE && p->grad_x != nullptr && in % 8 == 0 && out % 8 == 0 && in <= 384 &&
+         (p->grad_bias == nullptr || out <= (in > 256 ? GradShape<384>::kMostOut : GradShape<256>::kMostOut)) &&
+         tma_rows(p->grad_out, p->ld_grad) && aligned16(p->saved) && aligned16(p->grad_x) &&
+         (p->rows + kBM - 1) / kBM * 2 >= device_sm_count();
+}
+
+template <typename T, int BN, int ACT>
+int launch_grad_x(const rfm_linear_grad* p, int* ctas, cudaStream_t stream) {
+  using S = GradShape<BN>;
+  const int in = p->in_features, out = p->out_features;
+  GradXArgs a{};
+  a.m = p->rows;
+  a.n = in;
+  a.out = out;
+  a.tiles = static_cast<int>((p->rows + kBM - 1) / kBM);
+  a.k_blocks = (out + kBK - 1) / kBK;
+  a.store = p->grad_weight != nullptr;
+  a.partial = p->grad_bias != nullptr ? static_cast<float*>(p->workspace) : nullptr;
+  static thread_local unsigned long long ready = 0;  // as in launch_gemm: before the maps
+  const auto kernel = grad_x_kernel<T, BN, ACT>;
+  const unsigned long long context = current_context_id();
+  if (ready != context || context == 0) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) != cudaSuccess) {
+      cudaGetLastError();
+      return RFM_ERR_LAUNCH;
+    }
+    ready = context;
+  }
+  GradXMaps maps;
+  if (!make_map(&maps.dy, p->dtype, p->grad_out, out, p->rows, p->ld_grad, kBK, kBM, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_map(&maps.saved, p->dtype, p->saved, out, p->rows, out, kBK, kBM, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_map(&maps.dp, p->dtype, p->grad_pre, out, p->rows, p->ld_grad_pre, kBK, kBM, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_map(&maps.weight, p->dtype, p->weight, in, out, p->ld_weight, 64, kBK, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_map(&maps.dx, p->dtype, p->grad_x, in, p->rows, in, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B)) {
+    return RFM_ERR_LAUNCH;
+  }
+  const int sms = device_sm_count();
+  *ctas = a.tiles < sms ? a.tiles : sms;
+  return launch_chained(Chain::kFirst, kernel, dim3(*ctas), S::kThreads, S::kBytes, 1, stream, maps, a);
+}
+
+template <typename T, int ACT>
+int launch_grad_x(const rfm_linear_grad* p, int* ctas, cudaStream_t stream) {
+  if (p->in_features <= 128) return launch_grad_x<T, 128, ACT>(p, ctas, stream);
+  if (p->in_features <= 256) return launch_grad_x<T, 256, ACT>(p, ctas, stream);
+  return launch_grad_x<T, 384, ACT>(p, ctas, stream);
+}
+
+int run_grad_x(const rfm_linear_grad* p, int* ctas, cudaStream_t stream) {
+  if (p->dtype == RFM_DTYPE_BF16) {
+    return p->activation == RFM_ACT_RELU ? launch_grad_x<__nv_bfloat16, RFM_ACT_RELU>(p, ctas, stream)
+                                         : launch_grad_x<__nv_bfloat16, RFM_ACT_GELU>(p, ctas, stream);
+  }
+  return p->activation == RFM_ACT_RELU ? launch_grad_x<__half, RFM_ACT_RELU>(p, ctas, stream)
+                                       : launch_grad_x<__half, RFM_ACT_GELU>(p, ctas, stream);
 }
 
 int check_sizes(int64_t rows, int in_features, int out_features, int dtype) {
@@ -1248,7 +1670,16 @@ extern "C" int rfm_linear_backward(const rfm_linear_grad* p, void* stream) {
     return RFM_ERR_INVALID_ARGUMENT;
   }
 
-  if (own || p->grad_bias != nullptr) {
+  const bool fused = grad_x_fused(p);
+  if (fused) {
+    int ctas = 0;
+    int done = run_grad_x(p, &ctas, s);
+    if (done == RFM_OK && p->grad_bias != nullptr) {
+      done = launch_chained(Chain::kNext, bias_sum_kernel, dim3((out + 31) / 32), 1024, 0, 1, s,
+                            static_cast<const float*>(p->workspace), ctas, out, p->grad_bias, p->bias_dtype);
+    }
+    if (done != RFM_OK) return done;
+  } else if (own || p->grad_bias != nullptr) {
     GradPreArgs a{};
     a.dy = p->grad_out;
     a.ld_dy = rows > 1 ? p->ld_grad : out;
@@ -1280,7 +1711,7 @@ extern "C" int rfm_linear_backward(const rfm_linear_grad* p, void* stream) {
   Chain chain = own || p->grad_bias != nullptr ? Chain::kNext : Chain::kFirst;  // of the next product
   const void* dp = own ? p->grad_pre : p->grad_out;
   const int64_t ld_dp = own ? p->ld_grad_pre : p->ld_grad;
-  if (p->grad_x != nullptr) {
+  if (p->grad_x != nullptr && !fused) {
     Product g{};
     g.a = dp;
     g.ld_a = ld_dp;

@@ -451,6 +451,74 @@ def test_relu_cuts_infinite_gradients():
         assert torch.equal(bias.grad, torch.full_like(bias, 4.0))
 
 
+# enough rows that dP and dX come from one kernel: columns of dX around 128, 256 and 384, slices of dP that
+# end inside 64 columns, more slices than stages, CTAs with one, two and three tiles, a last tile of one row
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("act", ["relu", "gelu"])
+@pytest.mark.parametrize("rows,inner,outer", [(9473, 8, 8), (9600, 128, 72), (9729, 136, 1000), (18944, 256, 64),
+                                              (19073, 264, 520), (20001, 384, 2048), (38017, 40, 200),
+                                              (10000, 256, 4096), (10000, 384, 2056), (10000, 392, 96)])
+def test_gradients_of_many_rows(rows, inner, outer, act, dtype):
+    check(make(rows, inner, outer, dtype, residual=outer == 72, seed=31 + inner), act, dtype)
+    check_faults()
+
+
+def test_gradients_of_many_rows_in_parts():
+    """dX alone, without a bias, from gradients whose rows lie apart; the same bits alone, together with the
+    others, and on another stream at once."""
+    dtype = torch.bfloat16
+    rows, inner, outer = 12345, 256, 328
+    d = make(rows, inner, outer, dtype, residual=False, seed=33)
+    ref = reference(d, "gelu", dtype)
+    wide = torch.full((rows, outer + 24), float("nan"), device=DEV, dtype=dtype)
+    wide[:, 8:8 + outer] = d["dy"]
+    leaves = [d[k].clone().requires_grad_(True) for k in ("x", "weight", "bias")]
+    out = linear(*leaves, activation="gelu")
+    whole = torch.autograd.grad(out, leaves, d["dy"], retain_graph=True)
+    apart = torch.autograd.grad(out, leaves, wide[:, 8:8 + outer], retain_graph=True)
+    (alone,) = torch.autograd.grad(out, leaves[:1], d["dy"], retain_graph=True)
+    for name, a, b in zip(("x", "weight", "bias"), whole, apart):
+        close(f"grad {name}", a, ref[name])
+        assert torch.equal(a, b)
+    assert torch.equal(alone, whole[0])
+    x = d["x"].clone().requires_grad_(True)
+    (frozen,) = torch.autograd.grad(linear(x, d["weight"], d["bias"], activation="gelu"), x, d["dy"])
+    assert torch.equal(frozen, whole[0])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    results = []
+    for stream in streams:
+        with torch.cuda.stream(stream):
+            mine = [t.detach().clone().requires_grad_(True) for t in leaves]
+            results.append(torch.autograd.grad(linear(*mine, activation="gelu"), mine, d["dy"]))
+    torch.cuda.synchronize()
+    for grads in results:
+        for a, b in zip(grads, whole):
+            assert torch.equal(a, b)
+    check_faults()
+
+
+def test_gradients_of_many_rows_with_special_values():
+    """A NaN and infinities in the gradient stay in their rows of dX; the rows behind the last one are not
+    read as values."""
+    dtype = torch.float16
+    d = make(9501, 256, 136, dtype, residual=False, seed=34)
+    x = d["x"].clone().requires_grad_(True)
+    out = linear(x, d["weight"], d["bias"], activation="relu")
+    (clean,) = torch.autograd.grad(out, x, d["dy"], retain_graph=True)
+    dy = d["dy"].clone()
+    live, cut = (out[9500] > 0).nonzero()[0, 0], (out[9500] == 0).nonzero()[0, 0]
+    dy[9500, live] = float("nan")
+    dy[77, (out[77] == 0).nonzero()[0, 0]] = float("inf")
+    dy[9500, cut] = float("inf")
+    (g,) = torch.autograd.grad(out, x, dy)
+    assert bool(g[9500].isnan().all())
+    assert bool(g[77].isfinite().all())
+    keep = torch.ones(9501, dtype=torch.bool, device=DEV)
+    keep[[77, 9500]] = False
+    assert torch.equal(g[keep], clean[keep])
+
+
 @pytest.mark.parametrize("act,rows", [("none", 40), ("relu", 10000)])
 def test_first_backward_of_a_process(act, rows):
     """Autograd's thread has made no CUDA call when the first backward of a process reaches the product."""
