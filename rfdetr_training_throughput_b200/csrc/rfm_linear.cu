@@ -25,6 +25,9 @@
 // workspace, and a second kernel adds the parts in their order and applies the
 // epilogue.  No atomics: the same bits on every run.
 //
+// The gradient of an activation and dX come from one kernel where a row of dX is
+// short (grad_x_kernel); else dP has a pass of its own.
+//
 // Every wait on a barrier is bounded.  One that runs out marks the call as
 // failed (rfm_linear_faults) and every role leaves its loop.
 #include <math.h>
@@ -811,26 +814,43 @@ int launch_grad_pre(const GradPreArgs& a, int activation, const dim3& grid, cuda
 // ---- dP and dX = dP W in one pass, where a row of dX fits one tile
 
 // Up to 384 columns of dX an activation's gradient needs no pass of its own: dY
-// and `saved` come by TMA into the ring of the product's A operand, eight warps
-// turn dY into dP in place (element by element, so the swizzle does not matter),
-// and from there the tensor cores read it and TMA stores it for dW.  A warp owns
-// 8 columns of every slice, so the bias sums need no other warp: over a lane's
-// four rows, over the lanes by shuffles, and over the CTA's tiles in shared
-// memory, in a fixed order.
+// and `saved` come by TMA into the ring of the product's A operand, warps turn dY
+// into dP in place (element by element, so the swizzle does not matter), and from
+// there the tensor cores read it and TMA stores it for dW.  A warp owns 8 columns
+// of a slice, so its bias sums need no other warp: over a lane's rows, over the
+// lanes by shuffles, and over the CTA's tiles in shared memory, in a fixed order.
+// Two groups of eight warps take the slices in turn: with one, gelu's gradient
+// (some 30 instructions a pair) left the issue slots half idle.
 //
 // HBM-bound: dY, `saved` and dP, 6 bytes an element, where the dP pass and dX
-// apart move 8.
+// apart move 8.  Rows are dealt out in units of 32, up to four a tile, so that the
+// last wave occupies every SM (31200 rows: 244 tiles of 128 on 148 SMs).  A lane
+// takes its rows one after the other: all four at once spilled, and spills go to
+// L2 where shared memory leaves no L1 (31200 x 256 -> 2048 bf16: 109 us, 74 so).
+// Measured, the whole backward with relu: 31200 x 256 -> 2048 bf16 118 us (with
+// the dP pass 138), dX alone 61 (92); 13608 x 384 -> 1536 fp16 with gelu 68 (85)
+// and 34 (53).  Fewer than some 64 tiles of 128 rows go the other way: 4800 x 256
+// -> 2048 47.5 and 47.6, 2400 43.7 and 40, 300 28.1 and 18.8.
 template <int BN>
 struct GradShape {
-  static constexpr int kPreparers = 8;  // a warp 8 of a slice's 64 columns
+  static constexpr int kUnit = 32;      // rows
+  static constexpr int kPreparers = 8;  // of a slice: a warp 8 of its 64 columns
+  static constexpr int kGroups = 2;     // of preparers
   static constexpr int kEpiWarps = 4;
-  static constexpr int kEpi = kPreparers, kLoadWarp = kEpi + kEpiWarps, kWeightWarp = kLoadWarp + 1;
+  static constexpr int kEpi = kGroups * kPreparers, kLoadWarp = kEpi + kEpiWarps, kWeightWarp = kLoadWarp + 1;
   static constexpr int kMmaWarp = kWeightWarp + 1, kStoreWarp = kMmaWarp + 1;
   static constexpr int kThreads = 32 * (kStoreWarp + 1);
-  // three rings: dY (then dP), saved, the weight; the first two hide HBM's latency
-  static constexpr int kA = 4, kS = BN == 384 ? 3 : 4, kW = BN == 128 ? 4 : 2;
-  static constexpr int kSliceBytes = kBM * kBK * 2, kWeightBytes = BN * kBK * 2;
-  static constexpr int kMostOut = BN == 384 ? 2048 : 4096;  // columns of bias sums
+  // Three rings: dY (then dP), saved, and the weight (384 columns: three half
+  // slices, where only two whole ones had room).  A group waits for a stage's next
+  // phase only after it has seen the phase before, or the wait would end at once:
+  // so the first two rings have an even number of stages, and a stage's uses are
+  // all one group's.
+  static constexpr int kA = 4, kS = 4, kW = BN == 384 ? 3 : BN == 256 ? 2 : 8;
+  static_assert(kA % kGroups == 0 && kS % kGroups == 0, "a group's stages are its own");
+  static constexpr int kUnitBytes = kUnit * kBK * 2, kSliceBytes = kBM * kBK * 2;
+  static constexpr int kWeightParts = BN == 256 ? 1 : 2;  // of a slice
+  static constexpr int kWeightRows = kBK / kWeightParts, kWeightBytes = BN * kWeightRows * 2;
+  static constexpr int kMostOut = 2048;  // columns of bias sums
   static constexpr int kAccs = BN == 384 ? 1 : 2;
   static constexpr int kTmemColumns = BN == 128 ? 256 : 512;
   static constexpr int kMmaN = BN == 384 ? 192 : BN;
@@ -838,7 +858,7 @@ struct GradShape {
   static constexpr int kSaved = kA * kSliceBytes, kWeight = kSaved + kS * kSliceBytes;
   static constexpr int kBoxes = kWeight + kW * kWeightBytes;
   static constexpr int kSums = kBoxes + kEpiWarps * kBoxBytes;
-  static constexpr int kBars = kSums + kMostOut * 4;
+  static constexpr int kBars = kSums + kGroups * kMostOut * 4;
   static constexpr int kNumBars = 3 * kA + 2 * kS + 2 * kW + 2 * kAccs;
   static constexpr int kFlags = kBars + kNumBars * 8;
   static constexpr int kBytes = kFlags + 16;
@@ -849,13 +869,16 @@ struct GradXArgs {
   int64_t m;
   int32_t n;         // columns of dX
   int32_t out;       // columns of dP
-  int32_t tiles, k_blocks;
+  int32_t units;     // of 32 rows
+  int32_t k_blocks;
   int32_t store;     // dP is stored
   float* partial;    // [CTAs][out] column sums, null: not wanted
 };
 
 struct GradXMaps {
-  CUtensorMap dy, saved, dp, weight, dx;
+  CUtensorMap dy, saved, dp;                 // boxes of a tile's rows
+  CUtensorMap dy_unit, saved_unit, dp_unit;  // of a unit's
+  CUtensorMap weight, dx;
 };
 
 // A place in a ring of N stages.
@@ -938,42 +961,57 @@ __global__ void __launch_bounds__(GradShape<BN>::kThreads, 1)
   tc_fence_after();
   grid_dependency_wait();  // the set-up above touches nothing that the kernel before writes
   const uint32_t tmem = *reinterpret_cast<const volatile uint32_t*>(smem + S::kFlags + 4);
+  // This CTA's tiles: in every wave but the last the CTAs take four units each, one
+  // behind the other; what is left is dealt out evenly.
+  constexpr int kTile = kBM / S::kUnit;
+  const int ctas = static_cast<int>(gridDim.x), waves = a.units / (kTile * ctas);
+  const int left = a.units - waves * kTile * ctas;
+  const int last0 = static_cast<int>(static_cast<int64_t>(left) * blockIdx.x / ctas);
+  const int last1 = static_cast<int>(static_cast<int64_t>(left) * (blockIdx.x + 1) / ctas);
+  const int tiles = waves + (last1 > last0 ? 1 : 0);
+  const auto tile_units = [&](int t) { return t < waves ? kTile : last1 - last0; };
+  const auto tile_first = [&](int t) {
+    return t < waves ? (t * ctas + static_cast<int>(blockIdx.x)) * kTile : waves * kTile * ctas + last0;
+  };
 
-  if (warp < S::kPreparers) {
+  if (warp < S::kEpi) {
+    const int group = warp / S::kPreparers, chunk = warp % S::kPreparers;
     Ring<S::kA> ra;
     Ring<S::kS> rs;
     // this lane's 16-byte piece of rows lane, lane + 32, ..: the warp's 8 columns under the swizzle
-    const int at = lane * 128 + ((warp ^ (lane & 7)) << 4);
-    float* sums = reinterpret_cast<float*>(smem + S::kSums) + warp * 8;
+    const int at = lane * 128 + ((chunk ^ (lane & 7)) << 4);
+    float* all_sums = reinterpret_cast<float*>(smem + S::kSums);
+    float* sums = all_sums + group * S::kMostOut + chunk * 8;
     // after the shuffles lane l holds the sum of column l / 4
     if (a.partial != nullptr && (lane & 3) == 0) {
       for (int kb = 0; kb < a.k_blocks; ++kb) sums[kb * kBK + (lane >> 2)] = 0.f;
     }
     bool ok = true;
-    for (int t = static_cast<int>(blockIdx.x); ok && t < a.tiles; t += static_cast<int>(gridDim.x)) {
-      for (int kb = 0; kb < a.k_blocks; ++kb) {
+    int turn = 0;  // the group whose slice it is
+    for (int t = 0; ok && t < tiles; ++t) {
+      const int units = tile_units(t);
+      for (int kb = 0; kb < a.k_blocks; ++kb, ra.next(), rs.next(), turn = (turn + 1) % S::kGroups) {
+        if (turn != group) continue;
         ok = bounded_wait(a_full + 8 * ra.stage, ra.phase, dead) && bounded_wait(s_full + 8 * rs.stage, rs.phase, dead);
         ok = __all_sync(kFullMask, ok);
         if (!ok) break;
         uint8_t* dy = smem + ra.stage * S::kSliceBytes + at;
         const uint8_t* saved = smem + S::kSaved + rs.stage * S::kSliceBytes + at;
-        Pack<T, 8> g[4], p[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          g[r] = *reinterpret_cast<const Pack<T, 8>*>(dy + r * 4096);
-          p[r] = *reinterpret_cast<const Pack<T, 8>*>(saved + r * 4096);
-        }
         Pair sum[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
+        for (int j = 0; j < 4; ++j) sum[j] = both(0.f);
+#pragma unroll 1
+        for (int r = 0; r < units; ++r) {
+          const Pack<T, 8> g = *reinterpret_cast<const Pack<T, 8>*>(dy + r * S::kUnitBytes);
+          const Pack<T, 8> p = *reinterpret_cast<const Pack<T, 8>*>(saved + r * S::kUnitBytes);
           Pack<T, 8> o;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const Pair v = times_activate_grad(load_pair(g[r], j), load_pair(p[r], j), ACT);
+            const Pair v = times_activate_grad(load_pair(g, j), load_pair(p, j), ACT);
             store_pair(o, j, v);
-            sum[j] = r == 0 ? v : sum[j] + v;
+            sum[j] = sum[j] + v;
           }
-          *reinterpret_cast<Pack<T, 8>*>(dy + r * 4096) = o;
+          *reinterpret_cast<Pack<T, 8>*>(dy + r * S::kUnitBytes) = o;
         }
         proxy_fence();
         __syncwarp();
@@ -1003,15 +1041,14 @@ __global__ void __launch_bounds__(GradShape<BN>::kThreads, 1)
           v[0] += __shfl_xor_sync(kFullMask, v[0], 1);
           if ((lane & 3) == 0) sums[kb * kBK + (lane >> 2)] += v[0];
         }
-        ra.next();
-        rs.next();
       }
     }
-    if (a.partial != nullptr && (lane & 3) == 0) {
-      for (int kb = 0; kb < a.k_blocks; ++kb) {
-        const int col = kb * kBK + warp * 8 + (lane >> 2);
-        if (col < a.out) a.partial[static_cast<int64_t>(blockIdx.x) * a.out + col] = sums[kb * kBK + (lane >> 2)];
-      }
+    if (a.partial != nullptr) {
+      // the groups' sums, in their order
+      static_assert(S::kGroups == 2, "two sums");
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * S::kEpi) : "memory");
+      for (int col = static_cast<int>(threadIdx.x); col < a.out; col += 32 * S::kEpi)
+        a.partial[static_cast<int64_t>(blockIdx.x) * a.out + col] = all_sums[col] + all_sums[S::kMostOut + col];
     }
   } else if (warp < S::kEpi + S::kEpiWarps) {
     const int quarter = warp & 3;
@@ -1019,11 +1056,11 @@ __global__ void __launch_bounds__(GradShape<BN>::kThreads, 1)
     uint8_t* row_ptr = smem + S::kBoxes + quarter * S::kBoxBytes + lane * 64;
     const int swz = (lane >> 1) & 3;
     Ring<S::kAccs> acc;
-    for (int t = static_cast<int>(blockIdx.x); t < a.tiles; t += static_cast<int>(gridDim.x)) {
-      const int64_t row0 = static_cast<int64_t>(t) * kBM + quarter * 32;
+    for (int t = 0; t < tiles; ++t) {
+      const int64_t row0 = static_cast<int64_t>(tile_first(t) + quarter) * S::kUnit;
       if (!__all_sync(kFullMask, bounded_wait(acc_full + 8 * acc.stage, acc.phase, dead))) break;
       tc_fence_after();
-      if (row0 < a.m) {
+      if (quarter < tile_units(t)) {
 #pragma unroll 1
         for (int c = 0; c < BN && c < a.n; c += 32) {
           uint32_t v[32];
@@ -1059,19 +1096,26 @@ __global__ void __launch_bounds__(GradShape<BN>::kThreads, 1)
       Ring<S::kS> rs;
       uint32_t issued_a = 0, issued_s = 0;
       bool ok = true;
-      for (int t = static_cast<int>(blockIdx.x); ok && t < a.tiles; t += static_cast<int>(gridDim.x)) {
+      for (int t = 0; ok && t < tiles; ++t) {
+        const int u = tile_first(t), units = tile_units(t);
+        const auto load = [&](uint32_t to, const CUtensorMap* tile, const CUtensorMap* unit, int kb, uint32_t bar) {
+          mbar_expect(bar, units * S::kUnitBytes);
+          if (units == kTile) {
+            tma_load_2d(to, tile, kb * kBK, u * S::kUnit, bar);
+          } else {
+            for (int r = 0; r < units; ++r)
+              tma_load_2d(to + r * S::kUnitBytes, unit, kb * kBK, (u + r) * S::kUnit, bar);
+          }
+        };
         for (int kb = 0; kb < a.k_blocks; ++kb) {
           ok = bounded_wait(a_empty + 8 * ra.stage, ra.phase ^ 1u, dead);
           if (!ok) break;
-          mbar_expect(a_full + 8 * ra.stage, S::kSliceBytes);
-          tma_load_2d(base + ra.stage * S::kSliceBytes, &maps.dy, kb * kBK, t * kBM, a_full + 8 * ra.stage);
+          load(base + ra.stage * S::kSliceBytes, &maps.dy, &maps.dy_unit, kb, a_full + 8 * ra.stage);
           ra.next();
           ++issued_a;
           ok = bounded_wait(s_empty + 8 * rs.stage, rs.phase ^ 1u, dead);
           if (!ok) break;
-          mbar_expect(s_full + 8 * rs.stage, S::kSliceBytes);
-          tma_load_2d(base + S::kSaved + rs.stage * S::kSliceBytes, &maps.saved, kb * kBK, t * kBM,
-                      s_full + 8 * rs.stage);
+          load(base + S::kSaved + rs.stage * S::kSliceBytes, &maps.saved, &maps.saved_unit, kb, s_full + 8 * rs.stage);
           rs.next();
           ++issued_s;
         }
@@ -1086,14 +1130,15 @@ __global__ void __launch_bounds__(GradShape<BN>::kThreads, 1)
       Ring<S::kW> rw;
       uint32_t issued = 0;
       bool ok = true;
-      for (int t = static_cast<int>(blockIdx.x); ok && t < a.tiles; t += static_cast<int>(gridDim.x)) {
-        for (int kb = 0; kb < a.k_blocks; ++kb) {
+      for (int t = 0; ok && t < tiles; ++t) {
+        for (int kb = 0; kb < S::kWeightParts * a.k_blocks; ++kb) {
           ok = bounded_wait(w_empty + 8 * rw.stage, rw.phase ^ 1u, dead);
           if (!ok) break;
           const uint32_t bar = w_full + 8 * rw.stage, to = base + S::kWeight + rw.stage * S::kWeightBytes;
           mbar_expect(bar, S::kWeightBytes);
 #pragma unroll
-          for (int j = 0; j < BN / 64; ++j) tma_load_2d(to + j * 8192, &maps.weight, j * 64, kb * kBK, bar);
+          for (int j = 0; j < BN / 64; ++j)
+            tma_load_2d(to + j * 128 * S::kWeightRows, &maps.weight, j * 64, kb * S::kWeightRows, bar);
           rw.next();
           ++issued;
         }
@@ -1104,32 +1149,39 @@ __global__ void __launch_bounds__(GradShape<BN>::kThreads, 1)
     if (lane == 0) {
       constexpr int kType = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
       constexpr uint32_t kInstr = mma_instr(kType, false, true, kBM, S::kMmaN);
+      constexpr uint32_t kGroup = 128 * S::kWeightRows;  // bytes of 64 columns of the weight
       Ring<S::kA> ra;
       Ring<S::kW> rw;
       Ring<S::kAccs> acc;
       bool ok = true;
-      for (int t = static_cast<int>(blockIdx.x); ok && t < a.tiles; t += static_cast<int>(gridDim.x)) {
+      for (int t = 0; ok && t < tiles; ++t) {
         if (!bounded_wait(acc_empty + 8 * acc.stage, acc.phase ^ 1u, dead)) break;
         tc_fence_after();
         const uint32_t d = tmem + acc.stage * BN;
-        for (int kb = 0; kb < a.k_blocks; ++kb) {
-          ok = bounded_wait(w_full + 8 * rw.stage, rw.phase, dead) && bounded_wait(a_ready + 8 * ra.stage, ra.phase, dead);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t sa = base + ra.stage * S::kSliceBytes, sb = base + S::kWeight + rw.stage * S::kWeightBytes;
+        for (int kb = 0; ok && kb < a.k_blocks; ++kb) {
+          // rows past the tile's units hold what was there before: their products are not stored
+          const uint32_t sa = base + ra.stage * S::kSliceBytes;
+          for (int half = 0; half < S::kWeightParts; ++half) {
+            ok = bounded_wait(w_full + 8 * rw.stage, rw.phase, dead) &&
+                 (half > 0 || bounded_wait(a_ready + 8 * ra.stage, ra.phase, dead));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t sb = base + S::kWeight + rw.stage * S::kWeightBytes;
 #pragma unroll
-          for (int k = 0; k < kBK / 16; ++k) {
+            for (int k = 0; k < S::kWeightRows / 16; ++k) {
 #pragma unroll
-            for (int part = 0; part < BN / S::kMmaN; ++part) {
-              tc_mma_f16<1>(d + part * S::kMmaN, operand_desc(sa + k * 32, 16, 1024),
-                            operand_desc(sb + part * (S::kMmaN / 64) * 8192 + k * 2048, 8192, 1024), kInstr,
-                            kb > 0 || k > 0);
+              for (int part = 0; part < BN / S::kMmaN; ++part) {
+                tc_mma_f16<1>(d + part * S::kMmaN, operand_desc(sa + half * S::kWeightRows * 2 + k * 32, 16, 1024),
+                              operand_desc(sb + part * (S::kMmaN / 64) * kGroup + k * 2048, kGroup, 1024), kInstr,
+                              kb > 0 || half > 0 || k > 0);
+              }
             }
+            tc_commit<1>(w_empty + 8 * rw.stage);
+            rw.next();
           }
+          if (!ok) break;
           tc_commit<1>(a_empty + 8 * ra.stage);
-          tc_commit<1>(w_empty + 8 * rw.stage);
           ra.next();
-          rw.next();
         }
         if (!ok) break;
         tc_commit<1>(acc_full + 8 * acc.stage);
@@ -1145,11 +1197,18 @@ __global__ void __launch_bounds__(GradShape<BN>::kThreads, 1)
   } else if (lane == 0 && a.store) {
     Ring<S::kA> ra;
     bool ok = true;
-    for (int t = static_cast<int>(blockIdx.x); ok && t < a.tiles; t += static_cast<int>(gridDim.x)) {
+    for (int t = 0; ok && t < tiles; ++t) {
+      const int u = tile_first(t), units = tile_units(t);
       for (int kb = 0; kb < a.k_blocks; ++kb) {
         ok = bounded_wait(a_ready + 8 * ra.stage, ra.phase, dead);
         if (!ok) break;
-        tma_store_2d(&maps.dp, kb * kBK, t * kBM, base + ra.stage * S::kSliceBytes);
+        const uint32_t from = base + ra.stage * S::kSliceBytes;
+        if (units == kTile) {
+          tma_store_2d(&maps.dp, kb * kBK, u * S::kUnit, from);
+        } else {
+          for (int r = 0; r < units; ++r)
+            tma_store_2d(&maps.dp_unit, kb * kBK, (u + r) * S::kUnit, from + r * S::kUnitBytes);
+        }
         tma_commit();
         tma_wait_read<0>();
         mbar_arrive(a_empty + 8 * ra.stage);
@@ -1479,8 +1538,8 @@ int bias_slabs(int64_t rows, int n, int vec) {
 // their rows are cut into more slabs; grad_x_kernel leaves one row of sums a CTA.
 int64_t bias_bytes(int64_t rows, int n) {
   int64_t slabs = bias_slabs(rows, n, 8);
-  const int64_t narrow = bias_slabs(rows, n, 1), tiles = (rows + kBM - 1) / kBM, sms = device_sm_count();
-  const int64_t ctas = tiles < sms ? tiles : sms;
+  const int64_t narrow = bias_slabs(rows, n, 1), units = (rows + 31) / 32, sms = device_sm_count();
+  const int64_t ctas = units < sms ? units : sms;
   slabs = narrow > slabs ? narrow : slabs;
   slabs = ctas > slabs ? ctas : slabs;
   return (slabs * n * 4 + 15) & ~int64_t(15);
@@ -1491,7 +1550,7 @@ int64_t bias_bytes(int64_t rows, int n) {
 bool grad_x_fused(const rfm_linear_grad* p) {
   const int in = p->in_features, out = p->out_features;
   return p->activation != RFM_ACT_NONE && p->grad_x != nullptr && in % 8 == 0 && out % 8 == 0 && in <= 384 &&
-         (p->grad_bias == nullptr || out <= (in > 256 ? GradShape<384>::kMostOut : GradShape<256>::kMostOut)) &&
+         (p->grad_bias == nullptr || out <= GradShape<384>::kMostOut) &&
          tma_rows(p->grad_out, p->ld_grad) && aligned16(p->saved) && aligned16(p->grad_x) &&
          (p->rows + kBM - 1) / kBM * 2 >= device_sm_count();
 }
@@ -1504,7 +1563,7 @@ int launch_grad_x(const rfm_linear_grad* p, int* ctas, cudaStream_t stream) {
   a.m = p->rows;
   a.n = in;
   a.out = out;
-  a.tiles = static_cast<int>((p->rows + kBM - 1) / kBM);
+  a.units = static_cast<int>((p->rows + S::kUnit - 1) / S::kUnit);
   a.k_blocks = (out + kBK - 1) / kBK;
   a.store = p->grad_weight != nullptr;
   a.partial = p->grad_bias != nullptr ? static_cast<float*>(p->workspace) : nullptr;
@@ -1519,15 +1578,20 @@ int launch_grad_x(const rfm_linear_grad* p, int* ctas, cudaStream_t stream) {
     ready = context;
   }
   GradXMaps maps;
-  if (!make_map(&maps.dy, p->dtype, p->grad_out, out, p->rows, p->ld_grad, kBK, kBM, CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !make_map(&maps.saved, p->dtype, p->saved, out, p->rows, out, kBK, kBM, CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !make_map(&maps.dp, p->dtype, p->grad_pre, out, p->rows, p->ld_grad_pre, kBK, kBM, CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !make_map(&maps.weight, p->dtype, p->weight, in, out, p->ld_weight, 64, kBK, CU_TENSOR_MAP_SWIZZLE_128B) ||
+  const auto slices = [&](CUtensorMap* tile, CUtensorMap* unit, const void* at, int64_t ld) {
+    return make_map(tile, p->dtype, at, out, p->rows, ld, kBK, kBM, CU_TENSOR_MAP_SWIZZLE_128B) &&
+           make_map(unit, p->dtype, at, out, p->rows, ld, kBK, S::kUnit, CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  if (!slices(&maps.dy, &maps.dy_unit, p->grad_out, p->ld_grad) ||
+      !slices(&maps.saved, &maps.saved_unit, p->saved, out) ||
+      !slices(&maps.dp, &maps.dp_unit, p->grad_pre, p->ld_grad_pre) ||
+      !make_map(&maps.weight, p->dtype, p->weight, in, out, p->ld_weight, 64, S::kWeightRows,
+                CU_TENSOR_MAP_SWIZZLE_128B) ||
       !make_map(&maps.dx, p->dtype, p->grad_x, in, p->rows, in, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B)) {
     return RFM_ERR_LAUNCH;
   }
   const int sms = device_sm_count();
-  *ctas = a.tiles < sms ? a.tiles : sms;
+  *ctas = a.units < sms ? a.units : sms;
   return launch_chained(Chain::kFirst, kernel, dim3(*ctas), S::kThreads, S::kBytes, 1, stream, maps, a);
 }
 
