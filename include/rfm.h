@@ -484,7 +484,8 @@ int rfm_adamw_moments(const void* exp_avg, const void* exp_avg_sq, const float* 
  * RFM_ACT_RELU without a residual the forward's `out` does as well; NULL without an activation.
  * grad_pre [rows, out_features] with stride ld_grad_pre (16-byte aligned, a multiple of 8) receives dP
  * rounded to `dtype`, the products' operand; it is needed with an activation, and where grad_out is not
- * 16-byte aligned with a stride that is a multiple of 8.  Sums over rows are in fixed order (deterministic).
+ * 16-byte aligned with a stride that is a multiple of 8 (without grad_weight it may stay unwritten).  Sums
+ * over rows are in fixed order (deterministic).
  */
 #define RFM_ACT_NONE 0
 #define RFM_ACT_RELU 1
