@@ -27,6 +27,7 @@ int64_t operand_stride(const Tensor& y) { return y.size(0) > 1 ? y.stride(0) : p
 
 struct Outputs {
   Tensor out, pre;
+  Tensor x, weight;  // as the product read them
 };
 
 Outputs forward_rows(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t activation,
@@ -37,6 +38,8 @@ Outputs forward_rows(const Tensor& x, const Tensor& weight, const Tensor& bias, 
   o.out = at::empty(shape, x.options().memory_format(at::MemoryFormat::Contiguous));
   const Tensor xs = operand(x), ws = operand(weight);
   const int64_t rows = xs.size(0);
+  o.x = xs;
+  o.weight = ws;
   if (keep_pre) o.pre = at::empty({rows, weight.size(0)}, x.options().memory_format(at::MemoryFormat::Contiguous));
   if (rows == 0) return o;
   const Tensor res = residual.defined() ? rows_of(residual) : Tensor();
@@ -76,7 +79,15 @@ struct Linear : torch::autograd::Function<Linear> {
     const bool from_out = activation == RFM_ACT_RELU && !residual.defined();
     const Outputs o =
         forward_rows(x, weight, bias, activation, residual, activation != RFM_ACT_NONE && !from_out);
-    ctx->save_for_backward({x, weight, from_out ? o.out : o.pre});
+    // operands that had to be copied are kept for the backward, beside the tensors that it checks for changes
+    const Tensor x_copy = weight.requires_grad() && !o.x.is_alias_of(x) ? o.x : Tensor();
+    const Tensor weight_copy = x.requires_grad() && !o.weight.is_alias_of(weight) ? o.weight : Tensor();
+    variable_list kept{x, weight, from_out ? o.out : o.pre};
+    if (x_copy.defined() || weight_copy.defined()) {
+      kept.push_back(x_copy);
+      kept.push_back(weight_copy);
+    }
+    ctx->save_for_backward(std::move(kept));
     ctx->saved_data["activation"] = activation;
     // places among the tensors given (-1: not given), which number the gradients asked for
     ctx->saved_data["bias"] = static_cast<int64_t>(bias.defined() ? 2 : -1);
@@ -100,10 +111,12 @@ struct Linear : torch::autograd::Function<Linear> {
       if (at_res > 0 && ctx->needs_input_grad(at_res)) result[4] = dy;
       if (need_x || need_w || need_bias) {
         const Tensor g = rows_of(dy);
-        const Tensor xs = need_w ? operand(x) : rows_of(x), ws = operand(weight);
+        const bool copies = saved.size() > 3;
+        const Tensor xs = !need_w ? Tensor() : copies && saved[3].defined() ? saved[3] : operand(x);
+        const Tensor ws = !need_x ? Tensor() : copies && saved[4].defined() ? saved[4] : operand(weight);
         const auto options = x.options().memory_format(at::MemoryFormat::Contiguous);
         rfm_linear_grad a{};
-        a.rows = xs.size(0);
+        a.rows = g.size(0);
         a.in_features = static_cast<int32_t>(weight.size(1));
         a.out_features = static_cast<int32_t>(weight.size(0));
         a.dtype = dtype_code(x.scalar_type());
@@ -113,12 +126,12 @@ struct Linear : torch::autograd::Function<Linear> {
         if (need_x) result[0] = at::empty(x.sizes(), options);
         if (need_w) result[1] = at::empty(weight.sizes(), options);
         if (need_bias) result[2] = at::empty({weight.size(0)}, options.dtype(bias_type));
-        a.x = xs.data_ptr();
-        a.weight = ws.data_ptr();
+        a.x = data_or_null(xs);
+        a.weight = data_or_null(ws);
         a.saved = data_or_null(kept);
         a.grad_out = g.data_ptr();
-        a.ld_x = operand_stride(xs);
-        a.ld_weight = operand_stride(ws);
+        a.ld_x = need_w ? operand_stride(xs) : 0;
+        a.ld_weight = need_x ? operand_stride(ws) : 0;
         a.ld_grad = operand_stride(g);
         a.grad_x = data_or_null(result[0]);
         a.grad_weight = data_or_null(result[1]);

@@ -529,3 +529,55 @@ def test_first_backward_of_a_process(act, rows):
             "(g,) = torch.autograd.grad(out, x, torch.ones_like(out))\n"
             "assert bool((g == 32).all())\n")
     subprocess.run([sys.executable, "-c", code], check=True, timeout=300, cwd=Path(__file__).resolve().parents[1])
+
+
+def test_many_rows_captured_and_replayed():
+    """The backward that takes dP and dX from one kernel, captured behind the kernel that makes its input."""
+    d = make(10017, 256, 264, torch.bfloat16, residual=False, seed=35)
+    leaves = [d[k].clone().requires_grad_(True) for k in ("x", "weight", "bias")]
+
+    def both():
+        out = linear(*leaves, activation="gelu")
+        return [out.detach(), *torch.autograd.grad(out, leaves, d["dy"].neg())]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = both()
+    with torch.no_grad():
+        leaves[0].copy_(make(10017, 256, 264, torch.bfloat16, seed=36)["x"])
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(captured, both()):
+        assert torch.equal(a, b)
+    check_faults()
+
+
+def test_copied_operands_serve_the_backward():
+    """Operands that TMA cannot read are copied once, and a change of the originals is still noticed; a frozen
+    weight's or input's gradient needs neither."""
+    dtype = torch.bfloat16
+    d = make(37, 45, 51, dtype, residual=False, seed=37)
+    ref = reference(d, "gelu", dtype)
+    wide = torch.zeros(45, 37, device=DEV, dtype=dtype)
+    wide.copy_(d["x"].t())
+    x = wide.t().requires_grad_(True)  # columns apart
+    w = d["weight"].clone().requires_grad_(True)
+    out = linear(x, w, d["bias"], activation="gelu")
+    gx, gw = torch.autograd.grad(out, [x, w], d["dy"], retain_graph=True)
+    close("grad x", gx, ref["x"])
+    close("grad weight", gw, ref["weight"])
+    again = torch.autograd.grad(out, [x, w], d["dy"], retain_graph=True)
+    assert torch.equal(again[0], gx) and torch.equal(again[1], gw)
+    (only_w,) = torch.autograd.grad(linear(x.detach(), w, d["bias"], activation="gelu"), w, d["dy"])
+    (only_x,) = torch.autograd.grad(linear(x, w.detach(), d["bias"], activation="gelu"), x, d["dy"])
+    assert torch.equal(only_w, gw) and torch.equal(only_x, gx)
+    with torch.no_grad():
+        w.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        out.sum().backward()
