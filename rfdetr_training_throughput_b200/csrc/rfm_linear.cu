@@ -806,9 +806,10 @@ int launch_grad_pre(const GradPreArgs& a, int activation, const dim3& grid, cuda
   const auto kernel = activation == RFM_ACT_RELU   ? grad_pre_kernel<T, VEC, RFM_ACT_RELU>
                       : activation == RFM_ACT_GELU ? grad_pre_kernel<T, VEC, RFM_ACT_GELU>
                                                    : grad_pre_kernel<T, VEC, RFM_ACT_NONE>;
-  // an ordinary launch: CTAs that start one by one as the forward's leave find the
-  // SMs unevenly filled (31200 x 2048, relu: a training pass of 213 us, 199 so)
-  return launch_chained(Chain::kNone, kernel, grid, 32 * kPreWarps, 0, 1, s, a);
+  // Where dP is stored an ordinary launch: CTAs that start one by one as the forward's
+  // leave find the SMs unevenly filled (31200 x 2048, relu, a training pass: 213 us,
+  // 199 so).
+  return launch_chained(a.dp != nullptr ? Chain::kNone : Chain::kFirst, kernel, grid, 32 * kPreWarps, 0, 1, s, a);
 }
 
 // ---- dP and dX = dP W in one pass, where a row of dX fits one tile
