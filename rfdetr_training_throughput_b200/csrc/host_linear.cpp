@@ -100,7 +100,9 @@ struct Linear : torch::autograd::Function<Linear> {
     variable_list result(5);
     if (!grads[0].defined()) return result;
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &weight = saved[1], &kept = saved[2];
+    const Tensor &x = saved[0], &weight = saved[1];
+    // saved-tensor hooks may have given everything other strides
+    const Tensor kept = saved[2].defined() ? saved[2].contiguous() : Tensor();
     const c10::cuda::CUDAGuard guard(x.device());
     {
       at::AutoGradMode off(false);
@@ -112,8 +114,8 @@ struct Linear : torch::autograd::Function<Linear> {
       if (need_x || need_w || need_bias) {
         const Tensor g = rows_of(dy);
         const bool copies = saved.size() > 3;
-        const Tensor xs = !need_w ? Tensor() : copies && saved[3].defined() ? saved[3] : operand(x);
-        const Tensor ws = !need_x ? Tensor() : copies && saved[4].defined() ? saved[4] : operand(weight);
+        const Tensor xs = !need_w ? Tensor() : operand(copies && saved[3].defined() ? saved[3] : x);
+        const Tensor ws = !need_x ? Tensor() : operand(copies && saved[4].defined() ? saved[4] : weight);
         const auto options = x.options().memory_format(at::MemoryFormat::Contiguous);
         rfm_linear_grad a{};
         a.rows = g.size(0);

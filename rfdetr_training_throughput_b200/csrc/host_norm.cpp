@@ -47,8 +47,10 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &weight = saved[1], &stats = saved[2];
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    const Tensor& x = saved[0];
+    // saved-tensor hooks may have given everything other strides
+    const Tensor weight = saved[1].defined() ? saved[1].contiguous() : Tensor(), stats = saved[2].contiguous();
     const c10::cuda::CUDAGuard guard(x.device());
     variable_list result(4);
     {

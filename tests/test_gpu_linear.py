@@ -581,3 +581,26 @@ def test_copied_operands_serve_the_backward():
         w.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         out.sum().backward()
+
+
+@pytest.mark.parametrize("sizes", [(37, 45, 51), (64, 64, 64)])
+def test_saved_tensor_hooks(sizes):
+    """What the backward needs may be packed and come back elsewhere with other strides."""
+    d = make(*sizes, torch.bfloat16, residual=False, seed=38)
+    norm = torch.ones(sizes[2], device=DEV, dtype=torch.bfloat16)
+
+    def grads():
+        leaves = [d[k].clone().requires_grad_(True) for k in ("x", "weight", "bias")]
+        out = layer_norm(linear(*leaves, activation="gelu"), norm)
+        return torch.autograd.grad(out, leaves, d["dy"])
+
+    def turned(t):
+        return t.t().contiguous().t() if t.dim() == 2 else t.clone()
+
+    want = grads()
+    with torch.autograd.graph.save_on_cpu():
+        off = grads()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, turned):
+        other = grads()
+    for a, b, c in zip(want, off, other):
+        assert torch.equal(a, b) and torch.equal(a, c)
