@@ -136,7 +136,7 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         for group in self.param_groups:
             buckets: dict[tuple, list] = {}
-            fresh: dict[torch.device, torch.Tensor] = {}
+            fresh: dict[tuple, torch.Tensor] = {}
             for p in group["params"]:
                 if p.grad is None:
                     continue
@@ -145,8 +145,8 @@ class AdamW(torch.optim.Optimizer):
                 state = self.state[p]
                 if not state:
                     state.update(self._new_state(p, group))
-                    if group["capturable"]:  # parameters that start together share one counter
-                        state["step"] = fresh.setdefault(p.device, state["step"])
+                    if group["capturable"]:  # parameters of a launch that start together share one counter
+                        state["step"] = fresh.setdefault((p.device, p.dtype), state["step"])
                 if group["capturable"]:
                     key = (p.dtype, p.device, id(state["step"]))
                 else:
@@ -202,7 +202,7 @@ class AdamW(torch.optim.Optimizer):
                 _adopt(state, saved, bits)
                 count = int(saved["step"])
                 if capturable:
-                    state["step"] = shared.setdefault((p.device, count), state["step"].fill_(count))
+                    state["step"] = shared.setdefault((p.device, p.dtype, count), state["step"].fill_(count))
                 else:
                     state["step"] = count
                 self.state[p] = state

@@ -1,0 +1,81 @@
+"""AdamW's bookkeeping: which parameters share a step counter, when counters and states move, and what a
+capture may hold.  The host tests put the step itself in plain torch in the place of the kernel."""
+
+import copy
+
+import pytest
+import torch
+
+from rfdetr_training_throughput_b200 import optim
+from rfdetr_training_throughput_b200.optim import AdamW
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def plain_step(params, grads, exp_avg, exp_avg_sq, step, *, scales=None, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
+               weight_decay=1e-2, grad_scale=None):
+    t, (b1, b2) = int(step), betas
+    if any(p.dtype != g.dtype for p, g in zip(params, grads)):
+        raise ValueError("grads must be of the params' type")
+    for p, g, m, v in zip(params, grads, exp_avg, exp_avg_sq):
+        m.mul_(b1).add_(g.float(), alpha=1 - b1)
+        v.mul_(b2).addcmul_(g.float(), g.float(), value=1 - b2)
+        p.copy_(p.float() * (1 - lr * weight_decay) - lr / (1 - b1 ** t) * m / ((v / (1 - b2 ** t)).sqrt() + eps))
+
+
+@pytest.fixture(autouse=True)
+def host_step(request, monkeypatch):
+    if request.node.callspec.params.get("device") == "cpu":
+        monkeypatch.setattr(optim, "adamw_step", plain_step)
+
+
+def parameters(device, types, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.nn.Parameter(torch.randn(40 + 3 * i, generator=g).to(device, t)) for i, t in enumerate(types)]
+
+
+def set_grads(params, t, skip=()):
+    for i, p in enumerate(params):
+        g = torch.randn(p.shape, generator=torch.Generator().manual_seed(100 * t + i))
+        p.grad = None if i in skip else g.to(p.device, p.dtype)
+
+
+def counts(opt, params):
+    return [int(opt.state[p]["step"]) if opt.state.get(p) else 0 for p in params]
+
+
+def check_alike(a, pa, b, pb):
+    """Parameters, moments and counts of two optimisers, bit for bit."""
+    for p, q in zip(pa, pb):
+        assert torch.equal(p, q)
+        assert bool(a.state.get(p)) == bool(b.state.get(q))
+        for k, x in a.state.get(p, {}).items():
+            y = b.state[q][k]
+            assert int(x) == int(y) if k == "step" else torch.equal(x, y), k
+
+
+MIXED = [torch.float32, torch.bfloat16, torch.float32, torch.float16]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_capturable_group_of_mixed_types(device):
+    """One counter advances once a step whatever the types; the same bits as with host counters."""
+    ours, ref = parameters(device, MIXED), parameters(device, MIXED)
+    a, b = AdamW(ours, lr=1e-2, capturable=True), AdamW(ref, lr=1e-2)
+    for t in range(3):
+        set_grads(ours, t)
+        set_grads(ref, t)
+        a.step()
+        b.step()
+        assert counts(a, ours) == [t + 1] * 4
+    check_alike(a, ours, b, ref)
+    # through a state dict, in both directions
+    again = [torch.nn.Parameter(p.detach().clone()) for p in ours]
+    c = AdamW(again, lr=1e-2, capturable=True)
+    c.load_state_dict(copy.deepcopy(a.state_dict()))
+    for t in range(3, 5):
+        set_grads(again, t)
+        set_grads(ref, t)
+        c.step()
+        b.step()
+    check_alike(c, again, b, ref)
