@@ -162,9 +162,7 @@ class AdamW(torch.optim.Optimizer):
         eight = group["moment_bits"] == 8
         step = states[0]["step"]
         if group["capturable"]:
-            sharing = sum(1 for p in group["params"] if self.state.get(p, {}).get("step") is step)
-            if sharing != len(members):
-                raise ValueError("a capturable step needs a gradient for every parameter that shares a step counter")
+            step = self._own_counter(group, members)
             step.add_(1)
         params, grads, avg, avg_sq = [], [], [], []
         for p, s in zip(members, states):
@@ -180,6 +178,23 @@ class AdamW(torch.optim.Optimizer):
         scales = tuple([s[k] for s in states] for k in ("exp_avg_scale", "exp_avg_sq_scale")) if eight else None
         adamw_step(params, grads, avg, avg_sq, step, scales=scales, lr=group["lr"], betas=group["betas"],
                    eps=group["eps"], weight_decay=group["weight_decay"])
+
+    def _own_counter(self, group: dict, members: list) -> torch.Tensor:
+        """The step counter of a launch's parameters: one of their own where others, of another type or
+        without a gradient this time, stay at its present count."""
+        counter, capturing = self.state[members[0]]["step"], _capturing()
+        mine = {id(p) for p in members}
+        if all(id(p) in mine or self.state.get(p, {}).get("step") is not counter for p in group["params"]):
+            if capturing:
+                counter.in_a_graph = True
+            return counter
+        if capturing or getattr(counter, "in_a_graph", False):
+            raise RuntimeError("a captured step counts for all parameters that share its step counter, and some of them "
+                               "have no gradient now: before the capture, take a step with the same gradients")
+        counter = counter.clone()
+        for p in members:
+            self.state[p]["step"] = counter
+        return counter
 
     def load_state_dict(self, state_dict: dict) -> None:
         """Load a state dict of this class or of ``torch.optim.AdamW``.  ``moment_bits`` and ``capturable``
@@ -206,6 +221,11 @@ class AdamW(torch.optim.Optimizer):
                 else:
                     state["step"] = count
                 self.state[p] = state
+
+
+def _capturing() -> bool:
+    """Whether the current stream's work goes into a graph."""
+    return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
 
 
 def _flat_alike(data, g, m, v):

@@ -79,3 +79,82 @@ def test_capturable_group_of_mixed_types(device):
         c.step()
         b.step()
     check_alike(c, again, b, ref)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_capturable_after_a_change_of_type(device):
+    """Parameters that shared a counter and no longer have one type."""
+    ours, ref = parameters(device, [torch.float32] * 3), parameters(device, [torch.float32] * 3)
+    a, b = AdamW(ours, lr=1e-2, capturable=True), AdamW(ref, lr=1e-2)
+    for t in range(4):
+        if t == 2:
+            for p in (ours[1], ref[1]):
+                p.grad = None
+                p.data = p.data.bfloat16()
+        set_grads(ours, t)
+        set_grads(ref, t)
+        a.step()
+        b.step()
+    assert counts(a, ours) == [4] * 3
+    check_alike(a, ours, b, ref)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_capturable_with_absent_gradients(device):
+    """A parameter without a gradient is passed over and its count stands, as with torch's AdamW."""
+    ours, ref = parameters(device, MIXED), parameters(device, MIXED)
+    a, b = AdamW(ours, lr=1e-2, capturable=True), AdamW(ref, lr=1e-2)
+    absent = [(), (0,), (0, 1), (), (2,), (0, 1, 2, 3), ()]
+    for t, skip in enumerate(absent):
+        set_grads(ours, t, skip)
+        set_grads(ref, t, skip)
+        a.step()
+        b.step()
+    assert counts(a, ours) == [sum(i not in s for s in absent) for i in range(4)]
+    check_alike(a, ours, b, ref)
+
+
+@pytest.mark.parametrize("device", ["cpu"])
+def test_no_new_counter_inside_a_capture(device, monkeypatch):
+    """A replay would set it back every time."""
+    params = parameters(device, [torch.float32] * 2)
+    opt = AdamW(params, lr=1e-2, capturable=True)
+    set_grads(params, 0)
+    opt.step()
+    monkeypatch.setattr(optim, "_capturing", lambda: True)
+    opt.step()
+    assert counts(opt, params) == [2, 2]
+    set_grads(params, 1, skip=(0,))
+    with pytest.raises(RuntimeError, match="captured"):
+        opt.step()
+    # nor later: the graph would go on counting for the parameter that left its counter
+    monkeypatch.setattr(optim, "_capturing", lambda: False)
+    with pytest.raises(RuntimeError, match="captured"):
+        opt.step()
+    assert counts(opt, params) == [2, 2]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("device", ["cuda"])
+def test_captured_with_absent_gradients(device):
+    """Mixed types, and a parameter that stopped having gradients before the capture."""
+    ours, ref = parameters(device, MIXED), parameters(device, MIXED)
+    a, b = AdamW(ours, lr=1e-2, capturable=True), AdamW(ref, lr=1e-2)
+    for t, skip in enumerate([(), (2,)]):
+        set_grads(ours, t, skip)
+        set_grads(ref, t, skip)
+        a.step()
+        b.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step()
+    grads = [p.grad for p in ours]
+    for t in range(2, 5):
+        set_grads(ref, t, (2,))
+        for g, q in zip(grads, ref):
+            if g is not None:
+                g.copy_(q.grad)
+        graph.replay()
+        b.step()
+    torch.cuda.synchronize()
+    check_alike(a, ours, b, ref)
