@@ -135,37 +135,34 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for group in self.param_groups:
-            buckets: dict[tuple, list] = {}
-            fresh: dict[tuple, torch.Tensor] = {}
-            for p in group["params"]:
-                if p.grad is None:
-                    continue
-                if p.grad.is_sparse:
-                    raise ValueError("AdamW does not take sparse gradients")
-                state = self.state[p]
-                if not state:
-                    state.update(self._new_state(p, group))
-                    if group["capturable"]:  # parameters of a launch that start together share one counter
-                        state["step"] = fresh.setdefault((p.device, p.dtype), state["step"])
-                if group["capturable"]:
-                    key = (p.dtype, p.device, id(state["step"]))
-                else:
-                    state["step"] += 1
-                    key = (p.dtype, p.device, state["step"])
-                buckets.setdefault(key, []).append(p)
-            for members in buckets.values():
+            for members in self._buckets(group):
                 self._step_bucket(group, members)
         return loss
 
+    def _buckets(self, group: dict) -> list[list]:
+        """The parameters that have a gradient, with their states (new ones are not the optimiser's yet), a
+        list for each launch: of one type and device, with one step count."""
+        buckets: dict[tuple, list] = {}
+        fresh: dict[tuple, torch.Tensor] = {}
+        capturable = group["capturable"]
+        for p in group["params"]:
+            if p.grad is None:
+                continue
+            if p.grad.is_sparse:
+                raise ValueError("AdamW does not take sparse gradients")
+            state = self.state.get(p)
+            if not state:
+                state = self._new_state(p, group)
+                if capturable:  # parameters of a launch that start together share one counter
+                    state["step"] = fresh.setdefault((p.device, p.dtype), state["step"])
+            count = id(state["step"]) if capturable else state["step"]
+            buckets.setdefault((p.dtype, p.device, count), []).append((p, state))
+        return list(buckets.values())
+
     def _step_bucket(self, group: dict, members: list) -> None:
-        states = [self.state[p] for p in members]
-        eight = group["moment_bits"] == 8
-        step = states[0]["step"]
-        if group["capturable"]:
-            step = self._own_counter(group, members)
-            step.add_(1)
+        """One launch.  Counters and new states are the optimiser's once it has been accepted."""
         params, grads, avg, avg_sq = [], [], [], []
-        for p, s in zip(members, states):
+        for p, s in members:
             g, m, v = p.grad, s["exp_avg"], s["exp_avg_sq"]
             if not p.is_contiguous():
                 p, g, m, v = _flat_alike(p, g, m, v)
@@ -175,16 +172,30 @@ class AdamW(torch.optim.Optimizer):
             grads.append(g)
             avg.append(m)
             avg_sq.append(v)
-        scales = tuple([s[k] for s in states] for k in ("exp_avg_scale", "exp_avg_sq_scale")) if eight else None
-        adamw_step(params, grads, avg, avg_sq, step, scales=scales, lr=group["lr"], betas=group["betas"],
-                   eps=group["eps"], weight_decay=group["weight_decay"])
+        scales = None
+        if group["moment_bits"] == 8:
+            scales = tuple([s[k] for _, s in members] for k in ("exp_avg_scale", "exp_avg_sq_scale"))
+        if group["capturable"]:
+            step = self._own_counter(group, members).add_(1)
+        else:
+            step = members[0][1]["step"] + 1
+        try:
+            adamw_step(params, grads, avg, avg_sq, step, scales=scales, lr=group["lr"], betas=group["betas"],
+                       eps=group["eps"], weight_decay=group["weight_decay"])
+        except Exception:
+            if group["capturable"]:
+                step.sub_(1)
+            raise
+        for p, s in members:
+            s["step"] = step
+            self.state[p] = s
 
     def _own_counter(self, group: dict, members: list) -> torch.Tensor:
         """The step counter of a launch's parameters: one of their own where others, of another type or
         without a gradient this time, stay at its present count."""
-        counter, capturing = self.state[members[0]]["step"], _capturing()
-        mine = {id(p) for p in members}
-        if all(id(p) in mine or self.state.get(p, {}).get("step") is not counter for p in group["params"]):
+        counter, capturing = members[0][1]["step"], _capturing()
+        mine = {id(s) for _, s in members}
+        if all(s.get("step") is not counter or id(s) in mine for s in map(self.state.get, group["params"]) if s):
             if capturing:
                 counter.in_a_graph = True
             return counter
@@ -192,8 +203,8 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("a captured step counts for all parameters that share its step counter, and some of them "
                                "have no gradient now: before the capture, take a step with the same gradients")
         counter = counter.clone()
-        for p in members:
-            self.state[p]["step"] = counter
+        for _, s in members:
+            s["step"] = counter
         return counter
 
     def load_state_dict(self, state_dict: dict) -> None:

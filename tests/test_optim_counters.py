@@ -114,6 +114,50 @@ def test_capturable_with_absent_gradients(device):
     check_alike(a, ours, b, ref)
 
 
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_refused_step_leaves_everything(device, capturable, monkeypatch):
+    """A step that is refused moves no counter and makes no state, whether it is the first or a later one."""
+    params = parameters(device, [torch.float32] * 2)
+    opt = AdamW(params, lr=1e-2, capturable=capturable)
+    step = optim.adamw_step
+
+    def refuse(*args, **kwargs):
+        raise ValueError("refused")
+
+    set_grads(params, 0)
+    for done in (0, 1):
+        monkeypatch.setattr(optim, "adamw_step", refuse)
+        for _ in range(2):
+            with pytest.raises(ValueError, match="refused"):
+                opt.step()
+        assert counts(opt, params) == [done] * 2 and (done or not opt.state)
+        monkeypatch.setattr(optim, "adamw_step", step)
+        opt.step()
+        assert counts(opt, params) == [done + 1] * 2
+    ref = parameters(device, [torch.float32] * 2)
+    other = AdamW(ref, lr=1e-2)
+    set_grads(ref, 0)
+    other.step()
+    other.step()
+    check_alike(opt, params, other, ref)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_refusal_among_buckets(device):
+    """Two types, two launches: what was launched has counted, what was refused has not."""
+    params = parameters(device, [torch.float32, torch.bfloat16])
+    opt = AdamW(params, lr=1e-2)
+    set_grads(params, 0)
+    wrong = params[1].grad
+    params[1].grad = None
+    opt.step()
+    params[1].grad = wrong.to_sparse()
+    with pytest.raises(ValueError, match="sparse"):
+        opt.step()
+    assert counts(opt, params) == [1, 0]  # seen before anything is launched
+
+
 @pytest.mark.parametrize("device", ["cpu"])
 def test_no_new_counter_inside_a_capture(device, monkeypatch):
     """A replay would set it back every time."""
