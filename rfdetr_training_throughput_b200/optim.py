@@ -130,6 +130,9 @@ class AdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def step(self, closure=None):
         """One update of every parameter that has a gradient."""
+        if _capturing() and not all(group["capturable"] for group in self.param_groups):
+            raise RuntimeError("a captured step needs capturable=True: a host counter would stay at this step's number "
+                               "in every replay")
         loss = None
         if closure is not None:
             with torch.enable_grad():

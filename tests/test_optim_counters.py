@@ -178,6 +178,35 @@ def test_no_new_counter_inside_a_capture(device, monkeypatch):
     assert counts(opt, params) == [2, 2]
 
 
+@pytest.mark.parametrize("device", ["cpu"])
+def test_no_host_counter_inside_a_capture(device, monkeypatch):
+    """It would stay at the captured step's number in every replay."""
+    params = parameters(device, [torch.float32] * 2)
+    opt = AdamW(params, lr=1e-2)
+    set_grads(params, 0)
+    opt.step()
+    before = [p.detach().clone() for p in params]
+    monkeypatch.setattr(optim, "_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="capturable"):
+        opt.step()
+    assert counts(opt, params) == [1, 1] and all(torch.equal(p, q) for p, q in zip(params, before))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("device", ["cuda"])
+def test_host_counter_in_a_real_capture(device):
+    params = parameters(device, MIXED)
+    opt = AdamW(params, lr=1e-2)
+    set_grads(params, 0)
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="capturable"):
+        with torch.cuda.graph(graph):
+            opt.step()
+    torch.cuda.synchronize()
+    assert counts(opt, params) == [1] * 4
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("device", ["cuda"])
 def test_captured_with_absent_gradients(device):
