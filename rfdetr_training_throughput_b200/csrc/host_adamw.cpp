@@ -94,6 +94,7 @@ void adamw_step(const TensorRefs& params, const TensorRefs& grads, const TensorR
                 const std::optional<TensorRefs>& exp_avg_sq_scale, int64_t step, const MaybeTensor& device_step,
                 double lr, const MaybeTensor& device_lr, double beta1, double beta2, double eps, double weight_decay,
                 const MaybeTensor& grad_scale) {
+  refuse_traced("adamw_step");
   RFM_REQUIRE(device_step.has_value() || step >= 1, "step counts from 1, got ", step);
   RFM_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0 && lr >= 0.0 &&
                   weight_decay >= 0.0,
@@ -150,6 +151,7 @@ void adamw_step(const TensorRefs& params, const TensorRefs& grads, const TensorR
 
 std::tuple<Tensor, Tensor> dequantize_moments(const Tensor& exp_avg, const Tensor& exp_avg_sq,
                                               const Tensor& exp_avg_scale, const Tensor& exp_avg_sq_scale) {
+  refuse_traced("dequantize_moments");
   RFM_REQUIRE(exp_avg.is_cuda(), "exp_avg must be a CUDA tensor (dequantize_moments has no CPU path)");
   const at::Device device = exp_avg.device();
   const TensorRefs like{&exp_avg};

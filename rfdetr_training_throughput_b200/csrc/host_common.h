@@ -4,6 +4,8 @@
 #pragma once
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -46,6 +48,21 @@ inline Tensor or_undefined(const MaybeTensor& t) { return t.has_value() ? *t : T
 inline MaybeTensor maybe(const Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); }
 
 inline bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+// Whether this thread's operators are being recorded, or run without data.  A
+// recorder sees what goes through torch's dispatcher, and of the calls here that
+// is the output's allocation alone: what it records would return memory that
+// nobody wrote.
+inline bool traced() {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  return at::tracer::impl::is_dispatch_enabled() || Modes::get_mode(Key::PROXY).has_value() ||
+         Modes::get_mode(Key::FAKE).has_value() || Modes::get_mode(Key::FUNCTIONAL).has_value();
+}
+
+inline void refuse_traced(const char* op) {
+  TORCH_CHECK(!traced(), op, " cannot be traced: its kernels are launched past torch's dispatcher");
+}
 
 // `x` as [rows, last] with a unit stride along the rows' elements and rows that
 // do not overlap: a view where the layout allows, else a copy.

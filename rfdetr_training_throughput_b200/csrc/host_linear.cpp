@@ -168,6 +168,7 @@ Tensor lowered(const Tensor& t, at::ScalarType type) {
 
 Tensor linear(const Tensor& x_in, const Tensor& weight_in, const MaybeTensor& maybe_bias, int64_t activation,
               const MaybeTensor& maybe_residual) {
+  refuse_traced("linear");
   Tensor x = x_in, weight = weight_in, bias = or_undefined(maybe_bias), residual = or_undefined(maybe_residual);
   RFM_REQUIRE(x.is_cuda(), "x must be a CUDA tensor (linear has no CPU path)");
   RFM_REQUIRE(activation >= RFM_ACT_NONE && activation <= RFM_ACT_GELU, "unknown activation ", activation);

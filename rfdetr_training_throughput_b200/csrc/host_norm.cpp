@@ -88,6 +88,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 }  // namespace
 
 Tensor layer_norm(const Tensor& x, const MaybeTensor& maybe_weight, const MaybeTensor& maybe_bias, double eps) {
+  refuse_traced("layer_norm");
   RFM_REQUIRE(x.is_cuda(), "x must be a CUDA tensor (layer_norm has no CPU path)");
   RFM_REQUIRE(dtype_code(x.scalar_type()) >= 0, "x must be float32, bfloat16 or float16, got ", x.scalar_type());
   RFM_REQUIRE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= (1 << 30),
