@@ -11,6 +11,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include <initializer_list>
 #include <string>
 
 #include "rfm.h"
@@ -62,6 +63,14 @@ inline bool traced() {
 
 inline void refuse_traced(const char* op) {
   TORCH_CHECK(!traced(), op, " cannot be traced: its kernels are launched past torch's dispatcher");
+}
+
+// Forward-mode derivatives: an output made here has no tangent, which would read
+// as one of zero.
+inline void refuse_tangents(const char* op, std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors) {
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), op, " has no forward-mode derivative");
+  }
 }
 
 // `x` as [rows, last] with a unit stride along the rows' elements and rows that

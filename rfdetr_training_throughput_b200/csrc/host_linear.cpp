@@ -99,6 +99,7 @@ struct Linear : torch::autograd::Function<Linear> {
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     variable_list result(5);
     if (!grads[0].defined()) return result;
+    refuse_tangents("linear's gradient", {&grads[0]});
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1];
     // saved-tensor hooks may have given everything other strides
@@ -170,6 +171,7 @@ Tensor linear(const Tensor& x_in, const Tensor& weight_in, const MaybeTensor& ma
               const MaybeTensor& maybe_residual) {
   refuse_traced("linear");
   Tensor x = x_in, weight = weight_in, bias = or_undefined(maybe_bias), residual = or_undefined(maybe_residual);
+  refuse_tangents("linear", {&x, &weight, &bias, &residual});
   RFM_REQUIRE(x.is_cuda(), "x must be a CUDA tensor (linear has no CPU path)");
   RFM_REQUIRE(activation >= RFM_ACT_NONE && activation <= RFM_ACT_GELU, "unknown activation ", activation);
   RFM_REQUIRE(weight.dim() == 2 && weight.device() == x.device(), "weight must be a matrix on x's device");

@@ -48,6 +48,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const variable_list saved = ctx->get_saved_variables();
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    refuse_tangents("layer_norm's gradient", {&grads[0]});
     const Tensor& x = saved[0];
     // saved-tensor hooks may have given everything other strides
     const Tensor weight = saved[1].defined() ? saved[1].contiguous() : Tensor(), stats = saved[2].contiguous();
@@ -89,12 +90,13 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 Tensor layer_norm(const Tensor& x, const MaybeTensor& maybe_weight, const MaybeTensor& maybe_bias, double eps) {
   refuse_traced("layer_norm");
+  Tensor weight = or_undefined(maybe_weight), bias = or_undefined(maybe_bias);
+  refuse_tangents("layer_norm", {&x, &weight, &bias});
   RFM_REQUIRE(x.is_cuda(), "x must be a CUDA tensor (layer_norm has no CPU path)");
   RFM_REQUIRE(dtype_code(x.scalar_type()) >= 0, "x must be float32, bfloat16 or float16, got ", x.scalar_type());
   RFM_REQUIRE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= (1 << 30),
               "x needs a last dimension of at least one element");
   RFM_REQUIRE(eps >= 0.0, "eps must not be negative, got ", eps);
-  Tensor weight = or_undefined(maybe_weight), bias = or_undefined(maybe_bias);
   for (const Tensor* p : {&weight, &bias}) {
     if (!p->defined()) continue;
     const char* name = p == &weight ? "weight" : "bias";

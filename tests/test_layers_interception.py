@@ -49,3 +49,53 @@ def test_traced_steps_are_refused(device):
             torch.jit.trace(call, (torch.ones(7, device=device),), check_trace=False)
         with pytest.raises(RuntimeError, match="traced"):
             make_fx(call)(torch.ones(7, device=device))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("which", ["x", "weight", "bias", "residual"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_are_refused(device, which, grad):
+    shapes = dict(x=(4, 8), weight=(8, 8), bias=(8,), residual=(4, 8))
+    tensors = {k: torch.randn(s).bfloat16().to(device).requires_grad_(grad) for k, s in shapes.items()}
+    with forward_ad.dual_level():
+        tensors[which] = forward_ad.make_dual(tensors[which], torch.ones_like(tensors[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            linear(tensors["x"], tensors["weight"], tensors["bias"], residual=tensors["residual"])
+        if which != "residual":
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                layer_norm(tensors["x"], tensors["weight"][0], tensors["bias"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("call", [product, square])
+def test_tangents_of_a_gradient_are_refused(call):
+    """Forward over reverse: the tangent comes in behind the operator, with the gradient of its output."""
+    x = torch.randn(4, 8, device="cuda").bfloat16().requires_grad_(True)
+    with forward_ad.dual_level():
+        out = call(x)
+        dy = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(out, x, dy)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("call", [product, square])
+def test_other_tensors_inside_a_dual_level(call):
+    """A dual level by itself refuses nothing."""
+    x = torch.randn(4, 8, device="cuda").bfloat16()
+    want = call(x)
+    with forward_ad.dual_level():
+        assert torch.equal(call(x), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("call", [product, square])
+def test_function_transforms_are_refused(call):
+    """vmap, jvp and grad of torch.func wrap what they pass in: no storage, no kernel."""
+    x = torch.randn(2, 4, 8, device="cuda").bfloat16()
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(call)(x)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(call, (x,), (torch.ones_like(x),))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: call(t).float().sum())(x)
