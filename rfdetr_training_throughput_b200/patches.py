@@ -183,7 +183,8 @@ def _apply_fused_layer_norm() -> str:
     original = cls.forward
     types = (torch.float32, torch.bfloat16, torch.float16)
 
-    def forward(self, x):
+    def forward(self, input):  # torch's name: it may come as a keyword
+        x = input
         if not x.is_cuda or len(self.normalized_shape) != 1 or x.dtype not in types:
             return original(self, x)
         weight, bias = self.weight, self.bias

@@ -1,0 +1,122 @@
+"""What the patches of the layer operators leave to torch: arguments by torch's names, modules that do more
+than their weight says, and calls that a tracer, a compiler or a transform has to see."""
+
+import sys
+import types
+
+import pytest
+import torch
+import torch.nn.functional as F
+from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.nn.utils import parametrize
+
+from rfdetr_training_throughput_b200 import linear as products
+from rfdetr_training_throughput_b200 import patches
+from rfdetr_training_throughput_b200.linear import project
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+@pytest.fixture()
+def norms(monkeypatch):
+    """torch.nn.LayerNorm with the patch applied, torch's own forward back after the test."""
+    monkeypatch.setattr(torch.nn.LayerNorm, "forward", torch.nn.LayerNorm.forward)
+    patches.apply_patches("fused_layer_norm")
+
+
+def norm_layer(device, dtype=torch.float32):
+    torch.manual_seed(3)
+    layer = torch.nn.LayerNorm(16).to(device, dtype)
+    with torch.no_grad():
+        layer.weight.uniform_(0.5, 1.5)
+        layer.bias.uniform_(-1, 1)
+    return layer, torch.randn(5, 16, device=device, dtype=dtype)
+
+
+def own(layer, x):
+    return F.layer_norm(x, layer.normalized_shape, layer.weight, layer.bias, layer.eps)
+
+
+def near(got, want):
+    """Two float32 layer norms of 16 values: 100 roundings of values of order 4."""
+    return bool(((got - want).abs() <= 400 * 2.0 ** -24).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_layer_norm_by_torch_s_argument_name(norms, device):
+    layer, x = norm_layer(device)
+    assert near(layer(input=x), own(layer, x))
+
+
+# ------------------------------------------------------------------ projections
+
+class Twice(torch.nn.Linear):
+    """A subclass whose forward adds a term of its own, as adapters do."""
+
+    def forward(self, x):
+        return super().forward(x) + 1
+
+
+class Halved(torch.nn.Module):
+    def forward(self, w):
+        return w / 2
+
+
+def plain(device):
+    torch.manual_seed(4)
+    return torch.nn.Linear(16, 8).to(device, torch.bfloat16)
+
+
+def hooked(kind):
+    def make(device):
+        layer = plain(device)
+        getattr(layer, f"register_{kind}")(HOOKS[kind])
+        return layer
+    return make
+
+
+HOOKS = {"forward_hook": lambda m, a, out: out + 1, "forward_pre_hook": lambda m, a: (a[0] * 2,),
+         "full_backward_hook": lambda m, gi, go: tuple(None if g is None else g * 3 for g in gi),
+         "full_backward_pre_hook": lambda m, go: tuple(g * 3 for g in go)}
+
+
+def subclass(device):
+    torch.manual_seed(4)
+    return Twice(16, 8).to(device, torch.bfloat16)
+
+
+def parametrized(device):
+    layer = plain(device)
+    parametrize.register_parametrization(layer, "weight", Halved())
+    return layer
+
+
+def rebound(device):
+    layer = plain(device)
+    layer.forward = lambda x: F.linear(x, layer.weight, layer.bias) - 1
+    return layer
+
+
+def wrapper(device):
+    class Adapter(torch.nn.Module):
+        def __init__(self, base):
+            super().__init__()
+            self.base = base
+
+        weight = property(lambda self: self.base.weight)
+        bias = property(lambda self: self.base.bias)
+
+        def forward(self, x):
+            return self.base(x) + x[..., :8]
+
+    return Adapter(plain(device))
+
+
+class Projecting(torch.nn.Module):
+    def __init__(self, layer):
+        super().__init__()
+        self.layer = layer
+
+    def forward(self, x):
+        return project(self.layer, x)
