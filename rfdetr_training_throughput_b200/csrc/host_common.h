@@ -5,6 +5,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/TracerMode.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -59,6 +60,12 @@ inline bool traced() {
   using Key = c10::impl::TorchDispatchModeKey;
   return at::tracer::impl::is_dispatch_enabled() || Modes::get_mode(Key::PROXY).has_value() ||
          Modes::get_mode(Key::FAKE).has_value() || Modes::get_mode(Key::FUNCTIONAL).has_value();
+}
+
+// The same, or a function transform (torch.func's) that may have wrapped the
+// tensors of a call: what a patched module asks before it leaves torch's path.
+inline bool intercepted() {
+  return traced() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode);
 }
 
 inline void refuse_traced(const char* op) {

@@ -55,4 +55,5 @@ PYBIND11_MODULE(_host, m) {
   m.def("linear", &rfm_host::linear, release);
   m.def("adamw_step", &adamw_step);
   m.def("dequantize_moments", &rfm_host::dequantize_moments, release);
+  m.def("intercepted", &rfm_host::intercepted);
 }

@@ -177,6 +177,7 @@ def _apply_fused_msda_linear() -> str:
 def _apply_fused_layer_norm() -> str:
     import torch
 
+    from ._native import reaches_kernels
     from .norm import layer_norm
 
     cls = torch.nn.LayerNorm
@@ -184,10 +185,9 @@ def _apply_fused_layer_norm() -> str:
     types = (torch.float32, torch.bfloat16, torch.float16)
 
     def forward(self, input):  # torch's name: it may come as a keyword
-        x = input
-        if not x.is_cuda or len(self.normalized_shape) != 1 or x.dtype not in types:
+        x, weight, bias = input, self.weight, self.bias
+        if not reaches_kernels(x, weight, bias) or len(self.normalized_shape) != 1 or x.dtype not in types:
             return original(self, x)
-        weight, bias = self.weight, self.bias
         if torch.is_autocast_enabled("cuda"):  # torch's autocast runs layer norms in float32
             x = x.float()
             weight = weight if weight is None else weight.float()

@@ -49,6 +49,42 @@ def test_layer_norm_by_torch_s_argument_name(norms, device):
     assert near(layer(input=x), own(layer, x))
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_layer_norm_traced(norms, device):
+    """A trace holds torch's layer norm: it computes, also on other inputs."""
+    layer, x = norm_layer(device)
+    other = x * 2 + 1
+    graph = torch.jit.trace(layer, (x,))
+    assert "layer_norm" in str(graph.graph) and torch.equal(graph(other), own(layer, other))
+    fx = make_fx(layer)(x)
+    assert near(fx(other), own(layer, other))
+    exported = torch.export.export(layer, (x,)).module()
+    assert near(exported(other), own(layer, other))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_layer_norm_compiled(norms, device):
+    layer, x = norm_layer(device)
+    assert near(torch.compile(layer, backend="eager", fullgraph=True)(x), own(layer, x))
+    torch._dynamo.reset()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_layer_norm_under_transforms(norms, device):
+    """vmap, jvp, forward-mode and a second derivative by functorch, as torch's module has them."""
+    layer, x = norm_layer(device)
+    t = torch.ones_like(x).cumsum(0)
+    want, tangent = torch.func.jvp(lambda v: own(layer, v), (x,), (t,))
+    got = torch.func.jvp(layer, (x,), (t,))
+    assert near(got[0], want) and near(got[1], tangent)
+    with forward_ad.dual_level():
+        out = forward_ad.unpack_dual(layer(forward_ad.make_dual(x, t)))
+    assert near(out.primal, want) and near(out.tangent, tangent)
+    assert near(torch.func.vmap(layer)(x[:, None]), want[:, None])
+    grad = torch.func.grad(lambda v: own(layer, v).square().sum())(x)
+    assert near(torch.func.grad(lambda v: layer(v).square().sum())(x) / 16, grad / 16)
+
+
 # ------------------------------------------------------------------ projections
 
 class Twice(torch.nn.Linear):
