@@ -35,9 +35,23 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     return host().linear(x, weight, bias, code, residual)
 
 
-def project(layer: torch.nn.Linear, x: torch.Tensor) -> torch.Tensor:
-    """``layer(x)`` through ``linear`` where the product runs in 16 bits (under a 16-bit autocast, or on
-    16-bit tensors); a float32 or host product stays with the layer."""
+_LAYER_FORWARD = torch.nn.Linear.forward
+_HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
+
+
+def _only_a_product(layer: torch.nn.Module) -> bool:
+    """Whether calling ``layer`` is ``x W^T + b`` on its parameters and nothing else: no subclass, adapter,
+    parametrisation or forward of its own, and no hooks."""
+    return (type(layer) is torch.nn.Linear and torch.nn.Linear.forward is _LAYER_FORWARD
+            and "forward" not in layer.__dict__ and layer._compiled_call_impl is None
+            and not any(getattr(layer, k) for k in _HOOKS) and not torch.nn.modules.module._has_any_global_hook())
+
+
+def project(layer: torch.nn.Module, x: torch.Tensor) -> torch.Tensor:
+    """``layer(x)`` through ``linear`` where the layer is a plain ``torch.nn.Linear`` whose product runs in 16
+    bits (under a 16-bit autocast, or on 16-bit tensors); any other call stays with the layer."""
+    if not _only_a_product(layer):
+        return layer(x)
     autocast = x.is_cuda and torch.is_autocast_enabled("cuda")
     dtype = torch.get_autocast_dtype("cuda") if autocast else x.dtype
     if x.is_cuda and dtype in (torch.bfloat16, torch.float16):

@@ -149,6 +149,29 @@ def wrapper(device):
     return Adapter(plain(device))
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("make", [*(pytest.param(hooked(k), id=k) for k in HOOKS), subclass, parametrized, rebound,
+                                  wrapper])
+def test_layers_that_do_more_are_called(make, device):
+    layer = make(device)
+    x = torch.randn(5, 16, device=device).bfloat16().requires_grad_(True)
+    want, got = layer(x), project(layer, x)
+    assert torch.equal(got, want)
+    (a,) = torch.autograd.grad(want.float().sum(), x)
+    (b,) = torch.autograd.grad(got.float().sum(), x)
+    assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_global_hooks_are_called():
+    layer, x = plain("cuda"), torch.randn(5, 16, device="cuda").bfloat16()
+    hook = torch.nn.modules.module.register_module_forward_hook(lambda m, a, out: out * 2)
+    try:
+        assert torch.equal(project(layer, x), layer(x))
+    finally:
+        hook.remove()
+
+
 class Projecting(torch.nn.Module):
     def __init__(self, layer):
         super().__init__()
