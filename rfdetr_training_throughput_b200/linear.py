@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._native import host
+from ._native import host, reaches_kernels
 
 #: ``activation`` values.
 ACTIVATIONS = _lib.ACTIVATIONS
@@ -35,6 +35,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     return host().linear(x, weight, bias, code, residual)
 
 
+_TYPES = {torch.bfloat16, torch.float16}
 _LAYER_FORWARD = torch.nn.Linear.forward
 _HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
 
@@ -50,13 +51,18 @@ def _only_a_product(layer: torch.nn.Module) -> bool:
 def project(layer: torch.nn.Module, x: torch.Tensor) -> torch.Tensor:
     """``layer(x)`` through ``linear`` where the layer is a plain ``torch.nn.Linear`` whose product runs in 16
     bits (under a 16-bit autocast, or on 16-bit tensors); any other call stays with the layer."""
-    if not _only_a_product(layer):
+    if not _only_a_product(layer) or not reaches_kernels(x, layer.weight, layer.bias):
         return layer(x)
-    autocast = x.is_cuda and torch.is_autocast_enabled("cuda")
-    dtype = torch.get_autocast_dtype("cuda") if autocast else x.dtype
-    if x.is_cuda and dtype in (torch.bfloat16, torch.float16):
-        return linear(x, layer.weight, layer.bias)
-    return layer(x)
+    weight, bias = layer.weight, layer.bias
+    if torch.is_autocast_enabled("cuda"):
+        # autocast leaves float64 operands alone, and so the product stays in 64 bits
+        lowered = {torch.float32, *_TYPES}
+        kernels = (torch.get_autocast_dtype("cuda") in _TYPES
+                   and all(t is None or t.dtype in lowered for t in (x, weight, bias)))
+    else:
+        kernels = (x.dtype in _TYPES and weight.dtype == x.dtype
+                   and (bias is None or bias.dtype in (x.dtype, torch.float32)))
+    return linear(x, weight, bias) if kernels else layer(x)
 
 
 def check_faults(device: torch.device | int | None = None) -> None:

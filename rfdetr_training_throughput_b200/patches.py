@@ -160,13 +160,14 @@ def _apply_fused_msda_native() -> str:
 
 def _apply_fused_msda_linear() -> str:
     cls = _module("rfdetr.models.ops.modules.ms_deform_attn").MSDeformAttn
+    from ._native import host
     from .linear import project
     from .msda import module_forward
 
     original = cls.forward
 
     def forward(self, *args, **kwargs):
-        if getattr(self, "_export", False):
+        if getattr(self, "_export", False) or host().intercepted():
             return original(self, *args, **kwargs)
         return module_forward(self, *args, project=project, **kwargs)
 

@@ -172,6 +172,24 @@ def test_global_hooks_are_called():
         hook.remove()
 
 
+@pytest.mark.gpu
+def test_a_plain_layer_runs_on_the_kernels(monkeypatch):
+    """... and a float64 input under autocast, which torch's autocast leaves alone, on torch."""
+    calls = []
+    kernel = products.linear
+    monkeypatch.setattr(products, "linear", lambda *a, **k: calls.append(1) or kernel(*a, **k))
+    layer = torch.nn.Linear(16, 8).cuda()
+    x = torch.randn(5, 16, device="cuda")
+    project(plain("cuda"), x.bfloat16())
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        project(layer, x)
+    assert len(calls) == 2
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        wide = layer.double()
+        assert project(wide, x.double()).dtype == torch.float64
+    assert len(calls) == 2
+
+
 class Projecting(torch.nn.Module):
     def __init__(self, layer):
         super().__init__()
@@ -179,3 +197,26 @@ class Projecting(torch.nn.Module):
 
     def forward(self, x):
         return project(self.layer, x)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_traced_projection(device):
+    layer, x = plain(device), torch.randn(5, 16, device=device).bfloat16()
+    graph = torch.jit.trace(Projecting(layer), (x,))
+    assert torch.equal(graph(x * 2), layer(x * 2))
+    out, tangent = torch.func.jvp(Projecting(layer), (x,), (torch.ones_like(x),))
+    assert torch.equal(out, layer(x)) and tangent.shape == out.shape
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_traced_attention_keeps_the_original(device, monkeypatch):
+    name = "rfdetr.models.ops.modules.ms_deform_attn"
+    parts = name.split(".")
+    for i in range(1, len(parts) + 1):
+        monkeypatch.setitem(sys.modules, ".".join(parts[:i]), types.ModuleType(".".join(parts[:i])))
+    cls = type("MSDeformAttn", (), {"forward": lambda self, x: x * 3, "_export": False})
+    sys.modules[name].MSDeformAttn = cls
+    patches.apply_patches("fused_msda_linear")
+    attn, x = cls(), torch.ones(2, device=device)
+    # the check would call the stand-in untraced, with arguments that the module does not take
+    assert torch.equal(torch.jit.trace(attn.forward, (x,), check_trace=False)(x * 2), x * 6)
