@@ -71,28 +71,40 @@ Outputs forward_rows(const Tensor& x, const Tensor& weight, const Tensor& bias, 
 }
 
 struct Linear : torch::autograd::Function<Linear> {
+  // what the backward knows about the call beside the saved tensors
+  enum { kActivation, kInFeatures, kType, kBiasType, kBias, kResidual, kCallSize };
+
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const MaybeTensor& maybe_bias,
                         int64_t activation, const MaybeTensor& maybe_residual) {
     at::AutoDispatchBelowADInplaceOrView guard;
     const Tensor bias = or_undefined(maybe_bias), residual = or_undefined(maybe_residual);
-    // relu's gradient only asks for the sign, which the output has where nothing was added to it
+    // what the wanted gradients read, and nothing else: x for the weight's, the weight for x's, the
+    // pre-activation for any that passes the activation.  relu's gradient only asks for its sign, which the
+    // output has where nothing was added to it
+    const bool for_x = x.requires_grad(), for_w = weight.requires_grad();
+    const bool acts =
+        activation != RFM_ACT_NONE && (for_x || for_w || (bias.defined() && bias.requires_grad()));
     const bool from_out = activation == RFM_ACT_RELU && !residual.defined();
-    const Outputs o =
-        forward_rows(x, weight, bias, activation, residual, activation != RFM_ACT_NONE && !from_out);
+    const Outputs o = forward_rows(x, weight, bias, activation, residual, acts && !from_out);
+    variable_list kept{for_w ? x : Tensor(), for_x ? weight : Tensor(),
+                       !acts ? Tensor() : from_out ? o.out : o.pre};
     // operands that had to be copied are kept for the backward, beside the tensors that it checks for changes
-    const Tensor x_copy = weight.requires_grad() && !o.x.is_alias_of(x) ? o.x : Tensor();
-    const Tensor weight_copy = x.requires_grad() && !o.weight.is_alias_of(weight) ? o.weight : Tensor();
-    variable_list kept{x, weight, from_out ? o.out : o.pre};
+    const Tensor x_copy = for_w && !o.x.is_alias_of(x) ? o.x : Tensor();
+    const Tensor weight_copy = for_x && !o.weight.is_alias_of(weight) ? o.weight : Tensor();
     if (x_copy.defined() || weight_copy.defined()) {
       kept.push_back(x_copy);
       kept.push_back(weight_copy);
     }
     ctx->save_for_backward(std::move(kept));
-    ctx->saved_data["activation"] = activation;
+    std::vector<int64_t> call(kCallSize);
+    call[kActivation] = activation;
+    call[kInFeatures] = weight.size(1);
+    call[kType] = static_cast<int64_t>(x.scalar_type());
+    call[kBiasType] = static_cast<int64_t>(bias.defined() ? bias.scalar_type() : x.scalar_type());
     // places among the tensors given (-1: not given), which number the gradients asked for
-    ctx->saved_data["bias"] = static_cast<int64_t>(bias.defined() ? 2 : -1);
-    ctx->saved_data["residual"] = static_cast<int64_t>(residual.defined() ? (bias.defined() ? 3 : 2) : -1);
-    ctx->saved_data["bias_type"] = static_cast<int64_t>(bias.defined() ? bias.scalar_type() : x.scalar_type());
+    call[kBias] = bias.defined() ? 2 : -1;
+    call[kResidual] = residual.defined() ? (bias.defined() ? 3 : 2) : -1;
+    ctx->saved_data["call"] = std::move(call);
     return o.out;
   }
 
@@ -101,34 +113,39 @@ struct Linear : torch::autograd::Function<Linear> {
     if (!grads[0].defined()) return result;
     refuse_tangents("linear's gradient", {&grads[0]});
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &weight = saved[1];
+    const std::vector<int64_t> call = ctx->saved_data["call"].toIntVector();
     // saved-tensor hooks may have given everything other strides
     const Tensor kept = saved[2].defined() ? saved[2].contiguous() : Tensor();
-    const c10::cuda::CUDAGuard guard(x.device());
+    const c10::cuda::CUDAGuard guard(grads[0].device());
     {
       at::AutoGradMode off(false);
-      const int64_t at_bias = ctx->saved_data["bias"].toInt(), at_res = ctx->saved_data["residual"].toInt();
-      const bool need_bias = at_bias > 0 && ctx->needs_input_grad(at_bias);
+      const bool need_bias = call[kBias] > 0 && ctx->needs_input_grad(call[kBias]);
       const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
-      const Tensor dy = grads[0].scalar_type() == x.scalar_type() ? grads[0] : grads[0].to(x.scalar_type());
+      const int64_t at_res = call[kResidual], in = call[kInFeatures], out = grads[0].size(-1);
+      const auto type = static_cast<at::ScalarType>(call[kType]);
+      const Tensor dy = grads[0].scalar_type() == type ? grads[0] : grads[0].to(type);
       if (at_res > 0 && ctx->needs_input_grad(at_res)) result[4] = dy;
       if (need_x || need_w || need_bias) {
         const Tensor g = rows_of(dy);
         const bool copies = saved.size() > 3;
-        const Tensor xs = !need_w ? Tensor() : operand(copies && saved[3].defined() ? saved[3] : x);
-        const Tensor ws = !need_x ? Tensor() : operand(copies && saved[4].defined() ? saved[4] : weight);
-        const auto options = x.options().memory_format(at::MemoryFormat::Contiguous);
+        const Tensor xs = !need_w ? Tensor() : operand(copies && saved[3].defined() ? saved[3] : saved[0]);
+        const Tensor ws = !need_x ? Tensor() : operand(copies && saved[4].defined() ? saved[4] : saved[1]);
+        const auto options = dy.options().memory_format(at::MemoryFormat::Contiguous);
         rfm_linear_grad a{};
         a.rows = g.size(0);
-        a.in_features = static_cast<int32_t>(weight.size(1));
-        a.out_features = static_cast<int32_t>(weight.size(0));
-        a.dtype = dtype_code(x.scalar_type());
-        a.activation = static_cast<int32_t>(ctx->saved_data["activation"].toInt());
-        const auto bias_type = static_cast<at::ScalarType>(ctx->saved_data["bias_type"].toInt());
+        a.in_features = static_cast<int32_t>(in);
+        a.out_features = static_cast<int32_t>(out);
+        a.dtype = dtype_code(type);
+        a.activation = static_cast<int32_t>(call[kActivation]);
+        const auto bias_type = static_cast<at::ScalarType>(call[kBiasType]);
         a.bias_dtype = dtype_code(bias_type);
-        if (need_x) result[0] = at::empty(x.sizes(), options);
-        if (need_w) result[1] = at::empty(weight.sizes(), options);
-        if (need_bias) result[2] = at::empty({weight.size(0)}, options.dtype(bias_type));
+        if (need_x) {
+          std::vector<int64_t> shape = dy.sizes().vec();
+          shape.back() = in;
+          result[0] = at::empty(shape, options);
+        }
+        if (need_w) result[1] = at::empty({out, in}, options);
+        if (need_bias) result[2] = at::empty({out}, options.dtype(bias_type));
         a.x = data_or_null(xs);
         a.weight = data_or_null(ws);
         a.saved = data_or_null(kept);
@@ -141,7 +158,7 @@ struct Linear : torch::autograd::Function<Linear> {
         a.grad_bias = data_or_null(result[2]);
         Tensor dp, work;
         if ((need_x || need_w) && a.rows > 0 && (a.activation != RFM_ACT_NONE || !tma_rows(g))) {
-          a.ld_grad_pre = pad8(weight.size(0));
+          a.ld_grad_pre = pad8(out);
           dp = at::empty({a.rows, a.ld_grad_pre}, options);
           a.grad_pre = dp.data_ptr();
         }
@@ -151,7 +168,7 @@ struct Linear : torch::autograd::Function<Linear> {
           a.workspace = work.data_ptr();
           a.workspace_bytes = size;
         }
-        check_call("rfm_linear_backward", rfm_linear_backward(&a, current_stream(x.device())));
+        check_call("rfm_linear_backward", rfm_linear_backward(&a, current_stream(dy.device())));
       }
     }
     return once(std::move(result), "linear");

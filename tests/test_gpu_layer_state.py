@@ -1,0 +1,69 @@
+"""What the layer operators hold between a forward and its backward, what counts as written, and when their
+fault mark can be read."""
+
+import pytest
+import torch
+
+from rfdetr_training_throughput_b200.linear import check_faults, linear
+from rfdetr_training_throughput_b200.optim import adamw_step, quantize_moments
+
+pytestmark = pytest.mark.gpu
+
+DEV = torch.device("cuda", 0)
+
+
+def operands(rows=64, inner=48, outer=40):
+    g = torch.Generator(device="cuda").manual_seed(0)
+
+    def normal(*shape):
+        return torch.randn(*shape, device=DEV, generator=g).bfloat16()
+
+    return dict(x=normal(rows, inner), weight=normal(outer, inner), bias=normal(outer), residual=normal(rows, outer),
+                dy=normal(rows, outer))
+
+
+@pytest.mark.parametrize("inner", [48, 45])  # 45: operands that have to be copied
+@pytest.mark.parametrize("act", ["none", "relu", "gelu"])
+@pytest.mark.parametrize("wanted", [("x",), ("weight",), ("bias",), ("residual",), ("x", "bias"),
+                                    ("weight", "residual")])
+def test_only_what_the_gradients_need_is_kept(wanted, act, inner):
+    """Operands that no wanted gradient reads may change before the backward: the bits stay those of an
+    unchanged one.  Those that one reads may not."""
+    d = operands(inner=inner)
+    needed = {"weight"} if "x" in wanted else {"x"} if "weight" in wanted else set()
+
+    def grads(change):
+        t = {k: d[k].clone() for k in ("x", "weight", "bias", "residual")}
+        for k in wanted:
+            t[k].requires_grad_(True)
+        out = linear(t["x"], t["weight"], t["bias"], activation=act, residual=t["residual"])
+        with torch.no_grad():
+            for k in change:
+                t[k].add_(1)
+        return torch.autograd.grad(out, [t[k] for k in wanted], d["dy"])
+
+    free = [k for k in ("x", "weight", "bias", "residual") if k not in needed]
+    for a, b in zip(grads([]), grads(free)):
+        assert torch.equal(a, b)
+    for k in needed:
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            grads([k])
+
+
+@pytest.mark.parametrize("leaf", ["x", "weight", "residual"])
+def test_memory_between_forward_and_backward(leaf):
+    """An operand that no wanted gradient reads is freed with its last reference."""
+    rows, inner, outer = (64, 512, 65536) if leaf == "weight" else (65536, 512, 64)
+    sizes = dict(x=(rows, inner), weight=(outer, inner), residual=(rows, outer))
+    leaves = {k: torch.zeros(s, device=DEV, dtype=torch.bfloat16, requires_grad=k == leaf) for k, s in sizes.items()}
+    passing = {k: t * 1 for k, t in leaves.items()}
+    out = linear(passing["x"], passing["weight"], activation="gelu", residual=passing["residual"])
+    passing.clear()
+    before = torch.cuda.memory_allocated()
+    del out
+    freed = before - torch.cuda.memory_allocated()
+    # the output; the pre-activation and the one operand that the gradient reads, where it reads any
+    values = rows * outer
+    if leaf != "residual":
+        values += rows * outer + (outer * inner if leaf == "x" else rows * inner)
+    assert freed <= 2 * values + 4096
