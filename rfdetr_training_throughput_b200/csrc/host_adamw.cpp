@@ -81,6 +81,10 @@ void check_memory(const std::vector<Spans>& written, const Spans& grads) {
   }
 }
 
+void bump_versions(const TensorRefs& list) {
+  for (const Tensor* t : list) t->unsafeGetTensorImpl()->bump_version();
+}
+
 void* scalar_pointer(const char* name, const Tensor& t, at::ScalarType type, const at::Device& device) {
   RFM_REQUIRE(t.scalar_type() == type && t.numel() == 1 && t.device() == device, name, " must be one ", type,
               " element on the params' device");
@@ -146,7 +150,13 @@ void adamw_step(const TensorRefs& params, const TensorRefs& grads, const TensorR
                        weight_decay, step, static_cast<const float*>(at_lr), static_cast<const int64_t*>(at_step),
                        static_cast<const float*>(at_scale), data_or_null(work), current_stream(device)));
   // the in-place updates count as writes for autograd's saved tensors
-  for (const Tensor* p : params) p->unsafeGetTensorImpl()->bump_version();
+  bump_versions(params);
+  bump_versions(exp_avg);
+  bump_versions(exp_avg_sq);
+  if (eight) {
+    bump_versions(*exp_avg_scale);
+    bump_versions(*exp_avg_sq_scale);
+  }
 }
 
 std::tuple<Tensor, Tensor> dequantize_moments(const Tensor& exp_avg, const Tensor& exp_avg_sq,

@@ -67,3 +67,20 @@ def test_memory_between_forward_and_backward(leaf):
     if leaf != "residual":
         values += rows * outer + (outer * inner if leaf == "x" else rows * inner)
     assert freed <= 2 * values + 4096
+
+
+@pytest.mark.parametrize("which", ["param", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"])
+def test_written_tensors_count_as_changed(which):
+    """A graph that saved something the step writes says so instead of using the new values."""
+    p, g, m, v = (torch.rand(600, device=DEV) for _ in range(4))
+    eight = "scale" in which
+    cm, cv, sm, sv = quantize_moments(m, v)
+    saved = dict(param=p, exp_avg=m, exp_avg_sq=v, exp_avg_scale=sm, exp_avg_sq_scale=sv)[which]
+    w = torch.ones_like(saved, requires_grad=True)
+    loss = (w * saved).sum()
+    if eight:
+        adamw_step([p], [g], [cm], [cv], 1, scales=([sm], [sv]))
+    else:
+        adamw_step([p], [g], [m], [v], 1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.backward()
