@@ -142,14 +142,8 @@ void adamw_step(const TensorRefs& params, const TensorRefs& grads, const TensorR
   void* at_step = device_step ? scalar_pointer("step", *device_step, at::kLong, device) : nullptr;
   void* at_lr = device_lr ? scalar_pointer("lr", *device_lr, at::kFloat, device) : nullptr;
   void* at_scale = grad_scale ? scalar_pointer("grad_scale", *grad_scale, at::kFloat, device) : nullptr;
-  const c10::cuda::CUDAGuard guard(device);
-  Tensor work;
-  if (at_step != nullptr || at_lr != nullptr) work = at::empty({4}, params[0]->options().dtype(at::kFloat));
-  check_call("rfm_adamw",
-             rfm_adamw(table.data(), static_cast<int>(count), dtype_code(type), eight ? 8 : 32, lr, beta1, beta2, eps,
-                       weight_decay, step, static_cast<const float*>(at_lr), static_cast<const int64_t*>(at_step),
-                       static_cast<const float*>(at_scale), data_or_null(work), current_stream(device)));
-  // the in-place updates count as writes for autograd's saved tensors
+  // The in-place updates count as writes for autograd's saved tensors.  Before the launch: a tensor that may
+  // not be written (of inference mode, outside it) raises here.
   bump_versions(params);
   bump_versions(exp_avg);
   bump_versions(exp_avg_sq);
@@ -157,6 +151,13 @@ void adamw_step(const TensorRefs& params, const TensorRefs& grads, const TensorR
     bump_versions(*exp_avg_scale);
     bump_versions(*exp_avg_sq_scale);
   }
+  const c10::cuda::CUDAGuard guard(device);
+  Tensor work;
+  if (at_step != nullptr || at_lr != nullptr) work = at::empty({4}, params[0]->options().dtype(at::kFloat));
+  check_call("rfm_adamw",
+             rfm_adamw(table.data(), static_cast<int>(count), dtype_code(type), eight ? 8 : 32, lr, beta1, beta2, eps,
+                       weight_decay, step, static_cast<const float*>(at_lr), static_cast<const int64_t*>(at_step),
+                       static_cast<const float*>(at_scale), data_or_null(work), current_stream(device)));
 }
 
 std::tuple<Tensor, Tensor> dequantize_moments(const Tensor& exp_avg, const Tensor& exp_avg_sq,

@@ -84,3 +84,17 @@ def test_written_tensors_count_as_changed(which):
         adamw_step([p], [g], [m], [v], 1)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         loss.backward()
+
+
+def test_inference_tensors_are_not_written_outside_inference_mode():
+    """... as torch's in-place operations: refused before anything is written."""
+    with torch.inference_mode():
+        p = torch.rand(600, device=DEV)
+    g, m, v = (torch.rand(600, device=DEV) for _ in range(3))
+    before = [t.clone() for t in (p, m, v)]
+    with pytest.raises(RuntimeError, match="[Ii]nference"):
+        adamw_step([p], [g], [m], [v], 1)
+    assert all(torch.equal(a, b) for a, b in zip((p, m, v), before))
+    with torch.inference_mode():
+        adamw_step([p], [g], [m], [v], 1)
+    assert not torch.equal(p, before[0])
