@@ -81,6 +81,17 @@ void check_memory(const std::vector<Spans>& written, const Spans& grads) {
   }
 }
 
+// A scalar that kernels of the call read lies in nothing that they write.
+void check_apart(const std::vector<Spans>& written, const Tensor& scalar) {
+  const Span read = span_of(scalar);
+  for (const Spans& list : written) {
+    if (list.all.empty() || apart(list.hull, read)) continue;
+    for (const Span& s : list.all) {
+      RFM_REQUIRE(apart(s, read), "step, lr and grad_scale must not share memory with params, moments or scales");
+    }
+  }
+}
+
 void bump_versions(const TensorRefs& list) {
   for (const Tensor* t : list) t->unsafeGetTensorImpl()->bump_version();
 }
@@ -124,6 +135,9 @@ void adamw_step(const TensorRefs& params, const TensorRefs& grads, const TensorR
     written.emplace_back(*exp_avg_sq_scale);
   }
   check_memory(written, Spans(grads));
+  for (const MaybeTensor* scalar : {&device_step, &device_lr, &grad_scale}) {
+    if (scalar->has_value()) check_apart(written, **scalar);
+  }
   const size_t count = params.size();
   std::vector<rfm_adamw_tensor> table(count);
   for (size_t i = 0; i < count; ++i) {

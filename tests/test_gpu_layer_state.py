@@ -98,3 +98,19 @@ def test_inference_tensors_are_not_written_outside_inference_mode():
     with torch.inference_mode():
         adamw_step([p], [g], [m], [v], 1)
     assert not torch.equal(p, before[0])
+
+
+def test_device_scalars_apart_from_what_is_written():
+    """A scalar inside a written tensor would be read by some blocks before and by some after its update."""
+    p, g, m, v = (torch.rand(5000, device=DEV) for _ in range(4))
+    one = torch.ones(1, device=DEV)
+    for bad in (p[10:11], m[-1:], v[:1]):
+        with pytest.raises(ValueError, match="share memory"):
+            adamw_step([p], [g], [m], [v], 1, grad_scale=bad)
+        with pytest.raises(ValueError, match="share memory"):
+            adamw_step([p], [g], [m], [v], 1, lr=bad)
+    step = torch.ones(1, dtype=torch.int64, device=DEV)
+    with pytest.raises(ValueError, match="share memory"):
+        adamw_step([step.view(torch.float32)], [one.repeat(2)], [torch.zeros(2, device=DEV)],
+                   [torch.zeros(2, device=DEV)], step)
+    adamw_step([p], [g], [m], [v], 1, grad_scale=g[:1], lr=one)  # a gradient's element is only read
