@@ -540,7 +540,8 @@ int rfm_linear_forward(const rfm_linear* args, void* stream);
 int64_t rfm_linear_backward_workspace_bytes(int64_t rows, int in_features, int out_features);
 int rfm_linear_backward(const rfm_linear_grad* args, void* stream);
 /* Whether a product on the current device ever gave up one of its bounded waits (never expected; its
- * output is then incomplete): *faults 0 or 1.  Synchronises the device. */
+ * output is then incomplete): *faults 0 or 1.  Waits for all of the device's streams.  Once 1 it stays 1 for
+ * the process: which call it was is not known, and nothing else reports it. */
 int rfm_linear_faults(int* faults);
 
 /*

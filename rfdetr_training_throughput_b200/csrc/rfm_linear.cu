@@ -1812,7 +1812,9 @@ extern "C" int rfm_linear_backward(const rfm_linear_grad* p, void* stream) {
 extern "C" int rfm_linear_faults(int* faults) {
   using namespace rfm;
   if (faults == nullptr) return RFM_ERR_INVALID_ARGUMENT;
-  const cudaError_t err = cudaMemcpyFromSymbol(faults, g_linear_faults, sizeof(int));
+  // the copy alone waits for streams that synchronise with the default one; torch's own do not
+  cudaError_t err = cudaDeviceSynchronize();
+  if (err == cudaSuccess) err = cudaMemcpyFromSymbol(faults, g_linear_faults, sizeof(int));
   if (err == cudaSuccess) return RFM_OK;
   const int rc = launch_status();
   return rc == RFM_OK ? RFM_ERR_LAUNCH : rc;

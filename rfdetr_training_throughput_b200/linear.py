@@ -67,7 +67,8 @@ def project(layer: torch.nn.Module, x: torch.Tensor) -> torch.Tensor:
 
 def check_faults(device: torch.device | int | None = None) -> None:
     """Raise if a product on ``device`` (the current one) ever gave up a bounded wait, which leaves its
-    output incomplete.  Never expected; synchronises the device."""
+    output incomplete.  Never expected, and reported here only: a program that wants to know asks, between
+    steps.  Waits for all of the device's streams; the mark stays for the rest of the process."""
     faults = ctypes.c_int(0)
     with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
         _lib.check("rfm_linear_faults", _lib.load().rfm_linear_faults(ctypes.byref(faults)))

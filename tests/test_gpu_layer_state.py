@@ -69,6 +69,20 @@ def test_memory_between_forward_and_backward(leaf):
     assert freed <= 2 * values + 4096
 
 
+def test_faults_are_read_after_everything():
+    """check_faults waits for streams that do not synchronise with the default one."""
+    side = torch.cuda.Stream()
+    x = torch.zeros(128, 64, device=DEV, dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    done = torch.cuda.Event()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # some 100 ms
+        linear(x, x)
+        done.record()
+    check_faults()
+    assert done.query()
+
+
 @pytest.mark.parametrize("which", ["param", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"])
 def test_written_tensors_count_as_changed(which):
     """A graph that saved something the step writes says so instead of using the new values."""
