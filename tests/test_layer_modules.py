@@ -70,6 +70,21 @@ def test_layer_norm_compiled(norms, device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_layer_norm_scripted(norms, device):
+    """A scripted module holds torch's layer norm."""
+    class Block(torch.nn.Module):
+        def __init__(self, norm):
+            super().__init__()
+            self.norm = norm
+
+        def forward(self, x):
+            return self.norm(x) * 2
+
+    layer, x = norm_layer(device)
+    assert near(torch.jit.script(Block(layer))(x) / 2, own(layer, x))
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_layer_norm_under_transforms(norms, device):
     """vmap, jvp, forward-mode and a second derivative by functorch, as torch's module has them."""
     layer, x = norm_layer(device)
