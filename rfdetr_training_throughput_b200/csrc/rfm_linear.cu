@@ -107,10 +107,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // The normal distribution's cdf at two values: its tail q(|v|) as 2 to a polynomial.
 // log2 q is smooth where q itself falls over many orders; the coefficients are a
 // least-maximum fit of degree 8 on [0, 6]: q is off by at most 2.5e-6 of itself
-// up to 3 and 1.2e-5 up to 6 (below 2^-30 there), |v| q by 3e-7, far under half a
-// step of the 16-bit results (2^-12).  Beyond, the polynomial keeps falling and q
-// underflows to 0 (at an infinity too; a NaN stays one).  Seven instructions a
-// value and one of the special-function unit, against some 25 of erff.
+// up to 3 and 1.2e-5 up to 6 (below 2^-30 there), |v| q by 3e-7: far under half a
+// step of fp16 anywhere, and of bf16 down to v = -6.9.  Below that, where |v| q is
+// 1.4e-11 and less, bf16 still has steps: there q is off by more than half of one
+// (2.6 % of itself at -8, 45 % at -10), in values that 1 + erf in fp32 gives as 0
+// from -5.6 on.  Beyond 6 the polynomial keeps falling and q underflows to 0 (at an
+// infinity too; a NaN stays one).  Seven instructions a value and one of the
+// special-function unit, against some 25 of erff.
 __device__ __forceinline__ Pair normal_cdf(Pair v) {
   const float2 f = split(v);
   const Pair z = pair(fabsf(f.x), fabsf(f.y));
@@ -161,7 +164,11 @@ __device__ __forceinline__ Pair times_activate_grad(Pair dy, Pair v, int act) {
   return dy;
 }
 
-// `pre` is kept finite where it is: a value beyond the type's range would come back
+// `pre` is kept in the operands' 16 bits, half the bytes of fp32 both ways: the
+// derivative of gelu is then taken at a value half a step off (as where a product
+// and a gelu are two 16-bit operations).  With dP's rounding this puts the gradients
+// of 13608 x 384 -> 1536 fp16 3.0e-4 from 64 bits, 2.1e-4 with both in fp32.
+// It is kept finite where it is: a value beyond the type's range would come back
 // as an infinity, whose gelu gradient is NaN, where the value's is 0 or 1.  An
 // infinity stays one.
 template <typename T>
@@ -699,6 +706,11 @@ __global__ void __launch_bounds__(256) finish_kernel(const FinishArgs a) {
 
 // ---- dP = dY act'(saved) and its column sums
 
+// dP is rounded to 16 bits once, here: it is an operand of the tensor cores, which
+// take no fp32 one (tf32 would run at half the rate on twice the bytes).  The
+// column sums take it before that rounding, in fp32: a lane its rows, then the
+// warps, then the slabs, each in order.
+
 struct GradPreArgs {
   const void* dy;
   const void* saved;  // pre, or (relu without a residual) out; not read without an activation
@@ -851,7 +863,11 @@ struct GradShape {
   static constexpr int kUnitBytes = kUnit * kBK * 2, kSliceBytes = kBM * kBK * 2;
   static constexpr int kWeightParts = BN == 256 ? 1 : 2;  // of a slice
   static constexpr int kWeightRows = kBK / kWeightParts, kWeightBytes = BN * kWeightRows * 2;
-  static constexpr int kMostOut = 2048;  // columns of bias sums
+  // Columns of bias sums, 4 bytes each for every group: sized for 256 -> 2048, the
+  // decoder's feed-forward block.  Beside the rings there is room for 350 more with
+  // 384 columns of dX and for 1,370 with fewer; beyond the limit (256 -> 2056) dP has
+  // its pass of its own.
+  static constexpr int kMostOut = 2048;
   static constexpr int kAccs = BN == 384 ? 1 : 2;
   static constexpr int kTmemColumns = BN == 128 ? 256 : 512;
   static constexpr int kMmaN = BN == 384 ? 192 : BN;
@@ -1233,8 +1249,9 @@ __global__ void __launch_bounds__(GradShape<BN>::kThreads, 1)
 // one shuffle tree at the end.  With a tile of 128 rows the tensor cores would
 // work on zeros, and the contraction would be split to occupy the SMs: two
 // launches.  Here the weight's bytes in flight are all that counts.  Measured
-// (4096 -> 4096, fp16): 1 row 8.4 us (4.0 TB/s with its launch), tiles 20.6; 2
-// rows 10.4 and 23.9; 4 rows 18.6 and 16.5, so two rows are the most.
+// (4096 -> 4096, fp16, the kernels' own time): 1 row 8.4 us (4.0 TB/s), tiles 20.6;
+// 2 rows 10.4 and 23.9; 4 rows 18.6 and 16.5, so two rows are the most.  A whole
+// call of one row takes 9.5 us among others.
 struct FewArgs {
   const void* x;
   const void* weight;

@@ -13,7 +13,9 @@
 // HBM-bound: the forward moves 2 and the backward 3 arrays of rows x D.  A team
 // of TEAM threads keeps one row in registers (TEAM * VEC * CH >= D), so every
 // element is read once.  Teams of 8 lanes for short rows, a warp (no barrier) up to
-// 512 columns, 128 to 512 threads up to 8192; longer rows are re-read from L2.
+// 1024 columns (512 where rows are read element by element; the backward of 16-bit
+// rows has two warps beyond 512), 128 to 512 threads up to 8192; longer rows are
+// re-read from L2.
 // Each thread copies its own 16-byte pieces of the next DEPTH rows into shared
 // memory ahead of time (cp.async; nobody else reads them, so no barrier is
 // needed): bytes in flight, some 100 KB an SM, are what the bandwidth hangs on,
@@ -187,7 +189,7 @@ struct Params {
     }
   }
 
-  // columns 4 q .. 4 q + 3 of the thread (VEC >= 4) or 2 q, 2 q + 1
+  // the thread's columns 2 i and 2 i + 1
   __device__ __forceinline__ Pair at(int i, int lane) const {
     if constexpr (kShared) {
       const int c = (2 * i) / VEC, j = (2 * i) % VEC;
