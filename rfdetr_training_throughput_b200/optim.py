@@ -85,8 +85,9 @@ class AdamW(torch.optim.Optimizer):
     """AdamW with torch's arguments, one launch per parameter group and type.
 
     ``moment_bits`` 32 keeps float32 moments, 8 the codes and scales of ``adamw_step``.  With
-    ``capturable`` the step counter of a group lies on the device and advances inside ``step()``, so that
-    a captured step can be replayed; ``lr`` may then be a float32 device tensor.  ``amsgrad`` and
+    ``capturable`` step counters lie on the device, one for the parameters of a launch, and advance inside
+    ``step()``, so that a captured step can be replayed (without it a capture raises); ``lr`` may then be a
+    float32 device tensor.  ``amsgrad`` and
     ``maximize`` are not offered and raise.  A parameter's state is ``exp_avg``, ``exp_avg_sq`` (and
     ``exp_avg_scale``, ``exp_avg_sq_scale``) with ``step``; a float32 state dict loads into either form.
     """
